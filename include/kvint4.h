@@ -322,10 +322,90 @@ int kv4_prefill_attention(const kv4_tensor *q, const kv4_tensor *k_packed,
                           const kv4_tensor *v_scales, const kv4_tensor *out, int group_size,
                           int is_causal, float sm_scale, void *stream);
 
+/*
+ * Tree attention (speculative decoding; no counterpart in the reference):
+ * q [B, Hq, N, d] (bf16/f16/f32) holds N drafted nodes per sequence whose K/V
+ * rows are in a draft buffer dk/dv [B, Hkv, N, ...] in the cache's format
+ * (kv4_append_kv at pos 0 fills it).  Node i attends to the context rows
+ * [0, context_lens[b]) of the cache [B, Hkv, S, ...] and to the drafted rows j
+ * with mask[b, i, j] != 0: mask is uint8 [1, B or 1, N, N] (any strides).
+ * context_lens: device int32 [B], or NULL for S rows everywhere; an entry
+ * outside [0, S] sets bit 16 of kv4_device_error and reads as 0.  out
+ * [B, Hq, N, d] in the dtype of q; a node that sees nothing gives 0.  lse
+ * (f32 [B, Hq, N, 1], natural log) may be NULL.  d <= 512, any group size and
+ * strides; all four scale tensors have one dtype.  `workspace` holds at least
+ * kv4_tree_workspace() bytes (device, 16-byte aligned, any contents; a
+ * negative result of that function is minus a status).
+ */
+int64_t kv4_tree_workspace(const kv4_tensor *q, const kv4_tensor *k_packed,
+                           const kv4_tensor *k_scales, const kv4_tensor *v_packed,
+                           const kv4_tensor *v_scales, const kv4_tensor *dk_packed,
+                           const kv4_tensor *dk_scales, const kv4_tensor *dv_packed,
+                           const kv4_tensor *dv_scales, int group_size);
+int kv4_tree_attention(const kv4_tensor *q, const kv4_tensor *k_packed, const kv4_tensor *k_scales,
+                       const kv4_tensor *v_packed, const kv4_tensor *v_scales,
+                       const kv4_tensor *dk_packed, const kv4_tensor *dk_scales,
+                       const kv4_tensor *dv_packed, const kv4_tensor *dv_scales,
+                       const kv4_tensor *mask, const int32_t *context_lens, const kv4_tensor *out,
+                       const kv4_tensor *lse, int group_size, float sm_scale, void *workspace,
+                       size_t workspace_bytes, void *stream);
+
+/*
+ * Commit of an accepted path: for j < accepted[b], row context_lens[b] + j of
+ * every cache tensor [B, Hkv, cap, ...] becomes drafted row
+ * path[b * path_stride + j]; lens_out[b] = context_lens[b] + accepted[b]
+ * (lens_out may be context_lens only when Hkv == 1; pass another buffer).
+ * path, accepted, context_lens, lens_out: device int32; path_width bounds
+ * accepted.  A sequence whose length, count or capacity does not fit is left
+ * as it was (lens_out = context_lens), a node outside the draft is skipped;
+ * both set bit 16 of kv4_device_error.  Unit stride in the last dimension.
+ */
+int kv4_commit_rows(const kv4_tensor *k_packed, const kv4_tensor *k_scales,
+                    const kv4_tensor *v_packed, const kv4_tensor *v_scales,
+                    const kv4_tensor *dk_packed, const kv4_tensor *dk_scales,
+                    const kv4_tensor *dv_packed, const kv4_tensor *dv_scales, const int32_t *path,
+                    int64_t path_stride, int64_t path_width, const int32_t *accepted,
+                    const int32_t *context_lens, int32_t *lens_out, void *stream);
+
+/*
+ * Attention that scores the cached tokens (eviction policies; no counterpart
+ * in the reference): out as kv4_attention, and
+ *   score_out[b, g, t] = decay * score_in[b, g, t] + the softmax weight that
+ *   token t received, summed over the queries and over the q heads of KV head g.
+ * score_in, score_out: f32 [1, B, Hkv, S] (any strides; they may be the same
+ * tensor).  Shapes, dtypes and workspace as for kv4_tree_attention, with
+ * kv4_scored_workspace() bytes.
+ */
+int64_t kv4_scored_workspace(const kv4_tensor *q, const kv4_tensor *k_packed,
+                             const kv4_tensor *k_scales, const kv4_tensor *v_packed,
+                             const kv4_tensor *v_scales, int group_size, int is_causal);
+int kv4_scored_attention(const kv4_tensor *q, const kv4_tensor *k_packed,
+                         const kv4_tensor *k_scales, const kv4_tensor *v_packed,
+                         const kv4_tensor *v_scales, const kv4_tensor *score_in,
+                         const kv4_tensor *score_out, const kv4_tensor *out, int group_size,
+                         int is_causal, float decay, float sm_scale, void *workspace,
+                         size_t workspace_bytes, void *stream);
+
+/*
+ * Eviction: each (sequence, KV head) keeps `keep` = out_k_packed->shape[2]
+ * tokens, in token order: the first `sinks`, the last `recent` and, of the
+ * rest, those with the highest score (f32 [1, B, Hkv, S]; equal scores: the
+ * earlier token; NaN below everything).  Writes the kept rows of the four
+ * cache tensors and of the scores into the out_* tensors (which may not
+ * overlap the inputs) and the kept token numbers into index (device int32
+ * [B, Hkv, keep], contiguous).  recent + sinks <= keep <= S.
+ */
+int kv4_evict(const kv4_tensor *k_packed, const kv4_tensor *k_scales, const kv4_tensor *v_packed,
+              const kv4_tensor *v_scales, const kv4_tensor *score, const kv4_tensor *out_k_packed,
+              const kv4_tensor *out_k_scales, const kv4_tensor *out_v_packed,
+              const kv4_tensor *out_v_scales, const kv4_tensor *out_score, int32_t *index,
+              int64_t recent, int64_t sinks, void *stream);
+
 /* Read-and-clear the device error word (synchronizes the stream): bit 1 a
    bounded mbarrier wait expired, bit 2 a page id outside the pool, bit 4 a
    peer exchange wait expired, bit 8 kv4_prefill_attention met K/V values
-   outside the f16 range. */
+   outside the f16 range, bit 16 a context length, accepted count or path node
+   out of range (kv4_tree_attention, kv4_commit_rows). */
 int kv4_device_error(void *stream, int *flag_out);
 
 #ifdef __cplusplus

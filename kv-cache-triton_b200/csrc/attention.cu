@@ -2410,6 +2410,7 @@ extern "C" int kv4_lse_combine(const float *parts_o, const float *parts_lse, int
 
 namespace kv4 {
 int prefill_take_device_error(int *v);  // prefill.cu
+int branch_take_device_error(int *v);   // branch.cu
 }
 
 extern "C" int kv4_device_error(void *stream, int *flag_out) {
@@ -2422,9 +2423,10 @@ extern "C" int kv4_device_error(void *stream, int *flag_out) {
   if (rc) return rc;
   rc = cuda_status(cudaMemcpyToSymbol(g_device_error, &zero, sizeof(int)));
   if (rc) return rc;
-  int pv = 0;
+  int pv = 0, bv = 0;
   rc = prefill_take_device_error(&pv);
-  *flag_out = v | pv;
+  if (!rc) rc = branch_take_device_error(&bv);
+  *flag_out = v | pv | bv;
   return rc;
 }
 

@@ -1,0 +1,507 @@
+// Tree attention over the INT4 cache, and the commit of an accepted path.
+//
+// Speculative decoding drafts a tree of N nodes per sequence.  Their K/V rows
+// are quantized into a draft buffer; verification is one attention call in
+// which node i (of every q head) sees the whole committed context and the
+// drafted nodes that a boolean mask lets it see (its ancestors and itself):
+//
+//   x[t]  = q . K[t] * sm_scale        t < len_b, and drafted rows j with mask[b, i, j]
+//   out   = sum_t softmax(x)[t] V[t]   (0 where the row sees nothing)
+//
+// Rows that share a KV head share one read of it: row r of a (sequence, KV
+// head) unit is node r / R of q head kvh * R + r % R, R = Hq / Hkv.
+//
+// tree_generic: any head size up to 512, group size, strides and float types,
+// in fp32 FFMA.  A warp owns RW rows and a range of keys: 32 keys at a time it
+// dequantizes K into its own shared memory (lane = key for the scores), then V
+// over it (lane = column for the output), with the running maximum and sum of
+// the softmax per row.  Warps never wait for one another; ranges of one unit
+// meet in tree_merge through the workspace.
+#include <algorithm>
+
+#include "branch.cuh"
+
+namespace kv4 {
+
+// device error word of this file (folded into kv4_device_error)
+__device__ int g_branch_error = 0;
+
+namespace {
+
+template <int RW>
+__device__ __forceinline__ float warp_max(float v) {
+#pragma unroll
+  for (int o = 16; o; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+  return v;
+}
+
+struct GenPlan {
+  int64_t units, tasks;  // units = B * Hkv; tasks = units * row_tiles * parts
+  int rows, row_tiles, parts, warps, ld;
+  size_t smem;
+};
+
+template <int DC, int RW>
+__global__ void tree_generic(const TreeParams P, const GenPlan L) {
+  extern __shared__ __align__(16) float gsm[];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t task = static_cast<int64_t>(blockIdx.x) * L.warps + warp;
+  if (task >= L.tasks) return;
+  float *sT = gsm + warp * (32 * L.ld + RW * L.ld + 32 * RW);  // K or V tile
+  float *sQ = sT + 32 * L.ld, *sP = sQ + RW * L.ld;            // rows of q; weights [key][RW]
+  const int part = static_cast<int>(task % L.parts);
+  const int64_t ur = task / L.parts;
+  const int rt = static_cast<int>(ur % L.row_tiles);
+  const int64_t unit = ur / L.row_tiles, b = unit / P.Hkv;
+  const int kvh = static_cast<int>(unit - b * P.Hkv);
+  const int64_t len = context_len(P, b, part == 0 && rt == 0 && lane == 0 ? &g_branch_error : nullptr);
+  const int64_t total = len + P.ndraft, tiles = (total + 31) >> 5;
+  const int64_t per = (tiles + L.parts - 1) / L.parts;
+  const int64_t k0 = part * per * 32, k1 = min(total, k0 + per * 32);
+  const int r0 = rt * RW, d8 = (P.d + 7) >> 3;
+
+  for (int r = 0; r < RW; ++r) {
+    const int row = r0 + r, i = row / P.R, h = kvh * P.R + row - i * P.R;
+    for (int c = lane; c < 8 * d8; c += 32)
+      sQ[r * L.ld + c] = row < L.rows && c < P.d
+                             ? load_as_f32(P.q, P.q_dtype,
+                                           b * P.qs[0] + h * P.qs[1] + i * P.qs[2] + c * P.qs[3])
+                             : 0.0f;
+  }
+  float m[RW], l[RW], acc[RW][DC];
+#pragma unroll
+  for (int r = 0; r < RW; ++r) {
+    m[r] = -INFINITY;
+    l[r] = 0.0f;
+#pragma unroll
+    for (int k = 0; k < DC; ++k) acc[r][k] = 0.0f;
+  }
+
+  for (int64_t t0 = k0; t0 < k1; t0 += 32) {
+    __syncwarp();
+    warp_dequant_tile(P, false, b, kvh, len, t0, k1, sT, L.ld, lane);
+    __syncwarp();
+    float s[RW];
+#pragma unroll
+    for (int r = 0; r < RW; ++r) s[r] = 0.0f;
+    for (int c = 0; c < 2 * d8; ++c) {
+      const float4 k4 = *reinterpret_cast<const float4 *>(sT + lane * L.ld + 4 * c);
+#pragma unroll
+      for (int r = 0; r < RW; ++r) {
+        const float4 q4 = *reinterpret_cast<const float4 *>(sQ + r * L.ld + 4 * c);
+        s[r] = fmaf(q4.x, k4.x, s[r]);
+        s[r] = fmaf(q4.y, k4.y, s[r]);
+        s[r] = fmaf(q4.z, k4.z, s[r]);
+        s[r] = fmaf(q4.w, k4.w, s[r]);
+      }
+    }
+    const int64_t t = t0 + lane;
+#pragma unroll
+    for (int r = 0; r < RW; ++r) {
+      const int row = r0 + r;
+      bool see = t < k1 && row < L.rows;
+      if (see && t >= len) see = draft_visible(P, b, row / P.R, static_cast<int>(t - len));
+      const float x = see ? s[r] * P.scale_log2 : -INFINITY;
+      const float mn = fmaxf(m[r], warp_max<RW>(x));
+      const float base = mn == -INFINITY ? 0.0f : mn;
+      const float a = exp2f(m[r] - base), p = exp2f(x - base);
+      m[r] = mn;
+      l[r] = l[r] * a + p;  // this lane's keys; the lanes meet at the end
+#pragma unroll
+      for (int k = 0; k < DC; ++k) acc[r][k] *= a;
+      sP[lane * RW + r] = p;
+    }
+    __syncwarp();
+    warp_dequant_tile(P, true, b, kvh, len, t0, k1, sT, L.ld, lane);
+    __syncwarp();
+#pragma unroll 4
+    for (int j = 0; j < 32; ++j) {
+      float v[DC], p[RW];
+#pragma unroll
+      for (int k = 0; k < DC; ++k) v[k] = lane + 32 * k < 8 * d8 ? sT[j * L.ld + lane + 32 * k] : 0.0f;
+#pragma unroll
+      for (int r = 0; r < RW; ++r) p[r] = sP[j * RW + r];
+#pragma unroll
+      for (int r = 0; r < RW; ++r)
+#pragma unroll
+        for (int k = 0; k < DC; ++k) acc[r][k] = fmaf(p[r], v[k], acc[r][k]);
+    }
+  }
+#pragma unroll
+  for (int r = 0; r < RW; ++r) {
+#pragma unroll
+    for (int o = 16; o; o >>= 1) l[r] += __shfl_xor_sync(0xffffffffu, l[r], o);
+    const int row = r0 + r;
+    if (row >= L.rows) continue;
+    const int64_t at = unit * L.rows + row;
+    if (L.parts == 1) {
+      const int i = row / P.R, h = kvh * P.R + row - i * P.R;
+      const float inv = l[r] > 0.0f ? 1.0f / l[r] : 0.0f;
+#pragma unroll
+      for (int k = 0; k < DC; ++k)
+        if (lane + 32 * k < P.d)
+          store_from_f32(P.out, P.q_dtype,
+                         b * P.os[0] + h * P.os[1] + i * P.os[2] + (lane + 32 * k) * P.os[3],
+                         acc[r][k] * inv);
+      if (lane == 0) {
+        if (P.stats) P.stats[at] = make_float2(m[r], inv);
+        if (P.lse)
+          P.lse[b * P.ls[0] + h * P.ls[1] + i * P.ls[2]] =
+              l[r] > 0.0f ? (m[r] + log2f(l[r])) * kBrLn2 : -INFINITY;
+      }
+    } else {
+      const int64_t slot = static_cast<int64_t>(part) * L.units * L.rows + at;
+#pragma unroll
+      for (int k = 0; k < DC; ++k)
+        if (lane + 32 * k < P.d) P.ws_o[slot * P.d + lane + 32 * k] = acc[r][k];
+      if (lane == 0) P.ws_ml[slot] = make_float2(m[r], l[r]);
+    }
+  }
+}
+
+// One warp joins the partial rows of `parts` key ranges: ws_o [parts][rows][d]
+// unnormalised, ws_ml [parts][rows] (base-2 maximum, sum).
+template <int DC>
+__global__ void tree_merge(const TreeParams P, const GenPlan L) {
+  const int lane = threadIdx.x & 31;
+  const int64_t n = L.units * L.rows;
+  const int64_t at = static_cast<int64_t>(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5);
+  if (at >= n) return;
+  float m = -INFINITY;
+  for (int p = lane; p < L.parts; p += 32) m = fmaxf(m, P.ws_ml[p * n + at].x);
+  m = warp_max<1>(m);
+  const float base = m == -INFINITY ? 0.0f : m;
+  float l = 0.0f, acc[DC];
+#pragma unroll
+  for (int k = 0; k < DC; ++k) acc[k] = 0.0f;
+#pragma unroll 4
+  for (int p = 0; p < L.parts; ++p) {
+    const float2 ml = P.ws_ml[p * n + at];
+    const float f = exp2f(ml.x - base);
+    l = fmaf(f, ml.y, l);
+#pragma unroll
+    for (int k = 0; k < DC; ++k)
+      if (lane + 32 * k < P.d) acc[k] = fmaf(f, P.ws_o[(p * n + at) * P.d + lane + 32 * k], acc[k]);
+  }
+  const int64_t unit = at / L.rows, b = unit / P.Hkv;
+  const int row = static_cast<int>(at - unit * L.rows), i = row / P.R;
+  const int h = static_cast<int>(unit - b * P.Hkv) * P.R + row - i * P.R;
+  const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+#pragma unroll
+  for (int k = 0; k < DC; ++k)
+    if (lane + 32 * k < P.d)
+      store_from_f32(P.out, P.q_dtype,
+                     b * P.os[0] + h * P.os[1] + i * P.os[2] + (lane + 32 * k) * P.os[3],
+                     acc[k] * inv);
+  if (lane == 0) {
+    if (P.stats) P.stats[at] = make_float2(m, inv);
+    if (P.lse)
+      P.lse[b * P.ls[0] + h * P.ls[1] + i * P.ls[2]] =
+          l > 0.0f ? (m + log2f(l)) * kBrLn2 : -INFINITY;
+  }
+}
+
+constexpr int kSms = 148;
+
+GenPlan gen_plan(const TreeParams &P) {
+  GenPlan L{};
+  L.rows = P.R * P.nodes;
+  const int rw = L.rows <= 2 ? 2 : 8;
+  L.row_tiles = (L.rows + rw - 1) / rw;
+  L.units = P.B * P.Hkv;
+  L.ld = row_ld(P.d);
+  const size_t per_warp = sizeof(float) * (32 * L.ld + rw * L.ld + 32 * rw);
+  L.warps = static_cast<int>(std::max<size_t>(1, std::min<size_t>(4, 100 * 1024 / per_warp)));
+  L.smem = per_warp * L.warps;
+  // ranges of at least 32 keys, enough of them for about eight warps per SM
+  const int64_t tiles = (P.S + P.ndraft + 31) / 32, have = L.units * L.row_tiles;
+  const int64_t want = (8 * kSms + have - 1) / have;
+  L.parts = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({want, tiles, 256})));
+  L.tasks = have * L.parts;
+  return L;
+}
+
+int64_t gen_workspace(const TreeParams &P, const GenPlan &L) {
+  if (L.parts == 1) return 0;
+  return L.parts * L.units * L.rows * (static_cast<int64_t>(P.d) * 4 + 8);
+}
+
+template <int DC, int RW>
+int launch_gen(const TreeParams &P, const GenPlan &L, cudaStream_t st) {
+  const int64_t blocks = (L.tasks + L.warps - 1) / L.warps;
+  if (blocks > 0x7fffffff) return KV4_ERR_UNSUPPORTED;
+  if (L.smem > 48 * 1024) {
+    const int rc = cuda_status(cudaFuncSetAttribute(
+        tree_generic<DC, RW>, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024));
+    if (rc) return rc;
+  }
+  tree_generic<DC, RW><<<static_cast<unsigned>(blocks), 32 * L.warps, L.smem, st>>>(P, L);
+  int rc = cuda_status(cudaGetLastError());
+  if (rc || L.parts == 1) return rc;
+  const int64_t n = L.units * L.rows;
+  tree_merge<DC><<<static_cast<unsigned>((n + 3) / 4), 128, 0, st>>>(P, L);
+  return cuda_status(cudaGetLastError());
+}
+
+template <int DC>
+int launch_gen_rw(const TreeParams &P, const GenPlan &L, cudaStream_t st) {
+  return L.rows <= 2 ? launch_gen<DC, 2>(P, L, st) : launch_gen<DC, 8>(P, L, st);
+}
+
+bool is_float(int dt) { return dt == KV4_F32 || dt == KV4_F16 || dt == KV4_BF16; }
+
+// strides of one K/V source with its shapes checked: rows [B, Hkv, T, ...]
+int fill_source(RowSource &S, const kv4_tensor *const t[4], int64_t B, int64_t Hkv, int64_t T,
+                int64_t pw, int64_t ng, int s_dtype) {
+  for (int k = 0; k < 4; ++k) {
+    const kv4_tensor *x = t[k];
+    if (!x) return KV4_ERR_INVALID;
+    const bool scales = k & 1;
+    if (scales ? x->dtype != s_dtype : x->dtype != KV4_U8) return KV4_ERR_DTYPE;
+    if (x->shape[0] != B || x->shape[1] != Hkv || x->shape[2] != T ||
+        x->shape[3] < (scales ? ng : pw))
+      return KV4_ERR_SHAPE;
+    if (x->shape[3] != t[k & 1]->shape[3]) return KV4_ERR_SHAPE;
+    int64_t *st = k == 0 ? S.kps : k == 1 ? S.kss : k == 2 ? S.vps : S.vss;
+    for (int i = 0; i < 4; ++i) st[i] = x->stride[i];
+    if (T > 0 && !x->data) return KV4_ERR_INVALID;
+  }
+  S.kp = static_cast<const uint8_t *>(t[0]->data);
+  S.ks = t[1]->data;
+  S.vp = static_cast<const uint8_t *>(t[2]->data);
+  S.vs = t[3]->data;
+  return KV4_OK;
+}
+
+}  // namespace
+
+int tree_fill(TreeParams &P, const kv4_tensor *q, const kv4_tensor *const cache[4],
+              const kv4_tensor *const draft[4], const kv4_tensor *out, int G, float sm_scale) {
+  if (!q || !out || !cache[0] || !cache[1] || G <= 0) return KV4_ERR_INVALID;
+  if (!is_float(q->dtype) || out->dtype != q->dtype || !is_float(cache[1]->dtype))
+    return KV4_ERR_DTYPE;
+  const int64_t B = q->shape[0], Hq = q->shape[1], N = q->shape[2], d = q->shape[3];
+  const int64_t Hkv = cache[0]->shape[1], S = cache[0]->shape[2];
+  for (int i = 0; i < 4; ++i)
+    if (out->shape[i] != q->shape[i]) return KV4_ERR_SHAPE;
+  if (Hkv <= 0 || Hq <= 0 || Hq % Hkv) return KV4_ERR_INVALID;
+  if (B < 0 || N < 0 || d <= 0) return KV4_ERR_SHAPE;
+  if (d > 512 || B * Hkv > (int64_t(1) << 24) || S >= (int64_t(1) << 30) ||
+      N * (Hq / Hkv) >= (int64_t(1) << 24))
+    return KV4_ERR_UNSUPPORTED;
+  const int64_t ng = (d + G - 1) / G, pw = ng * ((G + 1) / 2);
+  P.s_dtype = cache[1]->dtype;
+  int rc = fill_source(P.cache, cache, B, Hkv, S, pw, ng, P.s_dtype);
+  if (rc) return rc;
+  P.ndraft = 0;
+  if (draft && draft[0]) {
+    const int64_t nd = draft[0]->shape[2];
+    if (nd >= (int64_t(1) << 24)) return KV4_ERR_UNSUPPORTED;
+    rc = fill_source(P.draft, draft, B, Hkv, nd, pw, ng, P.s_dtype);
+    if (rc) return rc;
+    P.ndraft = static_cast<int>(nd);
+  }
+  P.q = q->data;
+  P.out = out->data;
+  P.q_dtype = q->dtype;
+  for (int i = 0; i < 4; ++i) {
+    P.qs[i] = q->stride[i];
+    P.os[i] = out->stride[i];
+  }
+  P.B = B;
+  P.Hkv = static_cast<int>(Hkv);
+  P.R = static_cast<int>(Hq / Hkv);
+  P.nodes = static_cast<int>(N);
+  P.d = static_cast<int>(d);
+  P.G = G;
+  P.S = S;
+  P.scale_log2 = (sm_scale > 0.0f ? sm_scale : 1.0f / sqrtf(static_cast<float>(d))) * kBrLog2e;
+  return KV4_OK;
+}
+
+int64_t tree_workspace(const TreeParams &P) { return gen_workspace(P, gen_plan(P)); }
+
+int tree_run(TreeParams &P, void *workspace, int64_t bytes, cudaStream_t st) {
+  if (P.B == 0 || P.nodes == 0) return KV4_OK;
+  const GenPlan L = gen_plan(P);
+  if (gen_workspace(P, L) > 0) {
+    if (!workspace || bytes < gen_workspace(P, L)) return KV4_ERR_WORKSPACE;
+    const int64_t n = L.parts * L.units * L.rows;
+    P.ws_ml = static_cast<float2 *>(workspace);
+    P.ws_o = static_cast<float *>(workspace) + 2 * n;
+  }
+  if (P.d <= 64) return launch_gen_rw<2>(P, L, st);
+  if (P.d <= 128) return launch_gen_rw<4>(P, L, st);
+  if (P.d <= 256) return launch_gen_rw<8>(P, L, st);
+  return launch_gen_rw<16>(P, L, st);
+}
+
+// ---------------------------------------------------------------------------
+// commit: the accepted rows of the draft buffer move behind the context
+// ---------------------------------------------------------------------------
+namespace {
+
+struct CommitParams {
+  uint8_t *dst[4];
+  const uint8_t *src[4];
+  int64_t ds[4][3], ss[4][3];  // batch, head, token strides (bytes)
+  int bytes[4];                // of a row
+  const int32_t *path, *accepted, *lens;
+  int32_t *lens_out;
+  int64_t path_stride;
+  int64_t cap;
+  int B, Hkv, nodes, width;
+};
+
+// A block per (sequence, KV head) moves its rows; the block of head 0 writes
+// the new length.  Rows are at most some tens of KB per block: the launch is
+// what such a call costs.
+__global__ void __launch_bounds__(128) commit_rows(const CommitParams P) {
+  const int b = blockIdx.x / P.Hkv, h = blockIdx.x - b * P.Hkv;
+  const int64_t len = P.lens[b], n = P.accepted[b];
+  if (len < 0 || n < 0 || n > P.width || len + n > P.cap) {  // left as it was, and reported
+    if (h == 0 && threadIdx.x == 0) {
+      atomicOr(&g_branch_error, DEV_ERR_BAD_LENGTH);
+      P.lens_out[b] = static_cast<int32_t>(len);
+    }
+    return;
+  }
+  if (h == 0 && threadIdx.x == 0) P.lens_out[b] = static_cast<int32_t>(len + n);
+  for (int k = 0; k < 4; ++k) {
+    uint8_t *dst = P.dst[k] + b * P.ds[k][0] + h * P.ds[k][1] + len * P.ds[k][2];
+    const uint8_t *src = P.src[k] + b * P.ss[k][0] + h * P.ss[k][1];
+    const int nb = P.bytes[k];
+    for (int64_t e = threadIdx.x; e < n * nb; e += blockDim.x) {
+      const int j = static_cast<int>(e / nb), c = static_cast<int>(e - static_cast<int64_t>(j) * nb);
+      const int node = P.path[b * P.path_stride + j];
+      if (node < 0 || node >= P.nodes) {
+        atomicOr(&g_branch_error, DEV_ERR_BAD_LENGTH);
+        continue;
+      }
+      dst[j * P.ds[k][2] + c] = src[node * P.ss[k][2] + c];
+    }
+  }
+}
+
+}  // namespace
+
+// read-and-clear of this file's device error word
+int branch_take_device_error(int *v) {
+  int zero = 0;
+  int rc = cuda_status(cudaMemcpyFromSymbol(v, g_branch_error, sizeof(int)));
+  if (rc) return rc;
+  return cuda_status(cudaMemcpyToSymbol(g_branch_error, &zero, sizeof(int)));
+}
+
+namespace {
+
+int tree_args(TreeParams &P, const kv4_tensor *q, const kv4_tensor *const cache[4],
+              const kv4_tensor *const draft[4], const kv4_tensor *mask, const int32_t *lens,
+              const kv4_tensor *out, const kv4_tensor *lse, int group_size, float sm_scale) {
+  for (int k = 0; k < 4; ++k)
+    if (!cache[k] || !draft[k]) return KV4_ERR_INVALID;
+  int rc = tree_fill(P, q, cache, draft, out, group_size, sm_scale);
+  if (rc) return rc;
+  if (!mask) return KV4_ERR_INVALID;
+  if (mask->dtype != KV4_U8) return KV4_ERR_DTYPE;
+  if (mask->shape[0] != 1 || (mask->shape[1] != 1 && mask->shape[1] != P.B) ||
+      mask->shape[2] != P.nodes || mask->shape[3] != P.ndraft)
+    return KV4_ERR_SHAPE;
+  P.mask = static_cast<const uint8_t *>(mask->data);
+  P.ms[0] = mask->shape[1] == 1 ? 0 : mask->stride[1];
+  P.ms[1] = mask->stride[2];
+  P.ms[2] = mask->stride[3];
+  P.lens = lens;
+  if (lse) {
+    if (lse->dtype != KV4_F32) return KV4_ERR_DTYPE;
+    for (int i = 0; i < 3; ++i) {
+      if (lse->shape[i] != q->shape[i]) return KV4_ERR_SHAPE;
+      P.ls[i] = lse->stride[i];
+    }
+    P.lse = static_cast<float *>(lse->data);
+  }
+  return KV4_OK;
+}
+
+}  // namespace
+}  // namespace kv4
+
+using namespace kv4;
+
+extern "C" int64_t kv4_tree_workspace(const kv4_tensor *q, const kv4_tensor *k_packed,
+                                      const kv4_tensor *k_scales, const kv4_tensor *v_packed,
+                                      const kv4_tensor *v_scales, const kv4_tensor *dk_packed,
+                                      const kv4_tensor *dk_scales, const kv4_tensor *dv_packed,
+                                      const kv4_tensor *dv_scales, int group_size) {
+  const kv4_tensor *cache[4] = {k_packed, k_scales, v_packed, v_scales};
+  const kv4_tensor *draft[4] = {dk_packed, dk_scales, dv_packed, dv_scales};
+  TreeParams P{};
+  const int rc = tree_fill(P, q, cache, draft, q, group_size, 0.0f);
+  return rc ? -rc : tree_workspace(P);
+}
+
+extern "C" int kv4_tree_attention(const kv4_tensor *q, const kv4_tensor *k_packed,
+                                  const kv4_tensor *k_scales, const kv4_tensor *v_packed,
+                                  const kv4_tensor *v_scales, const kv4_tensor *dk_packed,
+                                  const kv4_tensor *dk_scales, const kv4_tensor *dv_packed,
+                                  const kv4_tensor *dv_scales, const kv4_tensor *mask,
+                                  const int32_t *context_lens, const kv4_tensor *out,
+                                  const kv4_tensor *lse, int group_size, float sm_scale,
+                                  void *workspace, size_t workspace_bytes, void *stream) {
+  const kv4_tensor *cache[4] = {k_packed, k_scales, v_packed, v_scales};
+  const kv4_tensor *draft[4] = {dk_packed, dk_scales, dv_packed, dv_scales};
+  TreeParams P{};
+  const int rc = tree_args(P, q, cache, draft, mask, context_lens, out, lse, group_size, sm_scale);
+  if (rc) return rc;
+  return tree_run(P, workspace, static_cast<int64_t>(workspace_bytes),
+                  static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int kv4_commit_rows(const kv4_tensor *k_packed, const kv4_tensor *k_scales,
+                               const kv4_tensor *v_packed, const kv4_tensor *v_scales,
+                               const kv4_tensor *dk_packed, const kv4_tensor *dk_scales,
+                               const kv4_tensor *dv_packed, const kv4_tensor *dv_scales,
+                               const int32_t *path, int64_t path_stride, int64_t path_width,
+                               const int32_t *accepted, const int32_t *context_lens,
+                               int32_t *lens_out, void *stream) {
+  const kv4_tensor *dst[4] = {k_packed, k_scales, v_packed, v_scales};
+  const kv4_tensor *src[4] = {dk_packed, dk_scales, dv_packed, dv_scales};
+  CommitParams P{};
+  for (int k = 0; k < 4; ++k) {
+    const kv4_tensor *c = dst[k], *s = src[k];
+    if (!c || !s) return KV4_ERR_INVALID;
+    if ((k & 1) ? !is_float(c->dtype) : c->dtype != KV4_U8) return KV4_ERR_DTYPE;
+    if (c->dtype != s->dtype) return KV4_ERR_DTYPE;
+    if (c->shape[0] != s->shape[0] || c->shape[1] != s->shape[1] || c->shape[3] != s->shape[3] ||
+        c->shape[0] != dst[0]->shape[0] || c->shape[1] != dst[0]->shape[1] ||
+        c->shape[2] != dst[0]->shape[2] || s->shape[2] != src[0]->shape[2])
+      return KV4_ERR_SHAPE;
+    if ((c->shape[3] > 1 && c->stride[3] != 1) || (s->shape[3] > 1 && s->stride[3] != 1))
+      return KV4_ERR_LAYOUT;
+    const int e = dtype_size(c->dtype);
+    P.bytes[k] = static_cast<int>(c->shape[3] * e);
+    P.dst[k] = static_cast<uint8_t *>(c->data);
+    P.src[k] = static_cast<const uint8_t *>(s->data);
+    for (int i = 0; i < 3; ++i) {
+      P.ds[k][i] = c->stride[i] * e;
+      P.ss[k][i] = s->stride[i] * e;
+    }
+  }
+  if (!path || !accepted || !context_lens || !lens_out || path_width < 0) return KV4_ERR_INVALID;
+  const int64_t B = dst[0]->shape[0], Hkv = dst[0]->shape[1], n = src[0]->shape[2];
+  if (B == 0 || Hkv == 0) return KV4_OK;
+  if (B * Hkv > 0x7fffffff || n >= (int64_t(1) << 30) || path_width >= (int64_t(1) << 30))
+    return KV4_ERR_UNSUPPORTED;
+  P.path = path;
+  P.path_stride = path_stride;
+  P.accepted = accepted;
+  P.lens = context_lens;
+  P.lens_out = lens_out;
+  P.cap = dst[0]->shape[2];
+  P.B = static_cast<int>(B);
+  P.Hkv = static_cast<int>(Hkv);
+  P.nodes = static_cast<int>(n);
+  P.width = static_cast<int>(path_width);
+  commit_rows<<<static_cast<unsigned>(B * Hkv), 128, 0, static_cast<cudaStream_t>(stream)>>>(P);
+  return cuda_status(cudaGetLastError());
+}

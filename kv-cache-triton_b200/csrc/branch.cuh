@@ -1,0 +1,132 @@
+// Shared declarations of the operators that branch and trim the INT4 cache
+// (branch.cu: tree attention and the commit of an accepted path; trim.cu:
+// attention that scores the cached tokens, and eviction).
+#pragma once
+
+#include "common.cuh"
+
+namespace kv4 {
+
+constexpr float kBrLog2e = 1.4426950408889634f;
+constexpr float kBrLn2 = 0.6931471805599453f;
+
+// Packed K and V rows and their scales: [B, Hkv, T, ...], strides in bytes
+// for the codes and in elements for the scales (batch, head, token, column).
+struct RowSource {
+  const uint8_t *kp, *vp;
+  const void *ks, *vs;
+  int64_t kps[4], vps[4], kss[4], vss[4];
+};
+
+// Attention of `nodes` query rows per sequence over the cache's context rows
+// [0, len_b) followed by `ndraft` rows of `draft`.  Node i sees every context
+// row and draft row j iff mask[b, i, j] (when given), or j <= i + shift (when
+// causal), or always.
+struct TreeParams {
+  const void *q;
+  void *out;
+  float *lse;  // natural log, or null
+  int q_dtype, s_dtype;
+  int64_t qs[4], os[4], ls[3];
+  RowSource cache, draft;
+  const uint8_t *mask;
+  int64_t ms[3];  // batch, node, draft strides (bytes)
+  const int32_t *lens;  // context rows of each sequence, or null: all of them
+  int64_t B;
+  int Hkv, R, nodes, ndraft, d, G, causal, shift;
+  int64_t S;           // context rows in the cache views
+  float scale_log2;    // sm_scale * log2(e)
+  float2 *stats;       // per (unit, row): base-2 maximum and 1 / sum; or null
+  float *ws_o;         // split partials, see the kernels
+  float2 *ws_ml;
+};
+
+// context rows of sequence b; an entry outside [0, S] is reported and read as 0
+__device__ __forceinline__ int64_t context_len(const TreeParams &P, int64_t b, int *err) {
+  if (!P.lens) return P.S;
+  const int n = __ldg(P.lens + b);
+  if (n < 0 || n > P.S) {
+    if (err) atomicOr(err, DEV_ERR_BAD_LENGTH);
+    return 0;
+  }
+  return n;
+}
+
+__device__ __forceinline__ bool draft_visible(const TreeParams &P, int64_t b, int i, int j) {
+  if (P.mask) return P.mask[b * P.ms[0] + i * P.ms[1] + j * P.ms[2]] != 0;
+  return !P.causal || j <= i + P.shift;
+}
+
+// Fill everything of P that comes from the arguments; KV4_OK or the reason.
+// draft tensors null: no drafted rows.
+int tree_fill(TreeParams &P, const kv4_tensor *q, const kv4_tensor *const cache[4],
+              const kv4_tensor *const draft[4], const kv4_tensor *out, int group_size,
+              float sm_scale);
+// Workspace bytes of tree_run and the run itself (branch.cu).
+int64_t tree_workspace(const TreeParams &P);
+int tree_run(TreeParams &P, void *workspace, int64_t bytes, cudaStream_t st);
+
+// one score row set of 8 elements: codes of columns [8c, 8c+8) of a packed row
+// as floats times their scale; columns at or past d are 0
+__device__ __forceinline__ void dequant8(const uint8_t *row, int64_t cs, const void *srow,
+                                         int64_t scs, int sdt, int G, int pb, int d, int c,
+                                         float (&v)[8]) {
+  const int e0 = 8 * c;
+  if ((G & 7) == 0 && cs == 1 && e0 + 8 <= d &&
+      ((reinterpret_cast<uintptr_t>(row) + (e0 >> 1)) & 3) == 0) {
+    const uint32_t w = __ldg(reinterpret_cast<const uint32_t *>(row + (e0 >> 1)));
+    const float s = load_as_f32(srow, sdt, (e0 / G) * scs);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = static_cast<float>(static_cast<int>((w >> (4 * k)) & 15u) - 8) * s;
+  } else {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const int e = e0 + k;
+      v[k] = 0.0f;
+      if (e < d) {
+        const int g = e / G, nib = g * 2 * pb + (e - g * G);
+        const uint32_t byte = row[(nib >> 1) * cs];
+        const int code = (nib & 1) ? byte >> 4 : byte & 15;
+        v[k] = static_cast<float>(code - 8) * load_as_f32(srow, sdt, g * scs);
+      }
+    }
+  }
+}
+
+// 32 rows (keys t0 .. t0+31 of `len` context rows then draft rows) of K or V
+// as floats in shared memory, ld floats apart, by one warp; rows at or past
+// `end` are 0.  d is padded with zeros to a multiple of 8.
+__device__ __forceinline__ void warp_dequant_tile(const TreeParams &P, bool is_v, int64_t b, int h,
+                                                  int64_t len, int64_t t0, int64_t end, float *dst,
+                                                  int ld, int lane) {
+  const int d8 = (P.d + 7) >> 3, pb = (P.G + 1) >> 1;
+  for (int idx = lane; idx < 32 * d8; idx += 32) {
+    const int r = idx / d8, c = idx - r * d8;
+    const int64_t t = t0 + r;
+    float v[8];
+    if (t < end) {
+      const bool ctx = t < len;
+      const RowSource &S = ctx ? P.cache : P.draft;
+      const int64_t row = ctx ? t : t - len;
+      const uint8_t *p = is_v ? S.vp : S.kp;
+      const int64_t *ps = is_v ? S.vps : S.kps, *ss = is_v ? S.vss : S.kss;
+      const int64_t so = b * ss[0] + h * ss[1] + row * ss[2];
+      const char *sp = static_cast<const char *>(is_v ? S.vs : S.ks) +
+                       so * (P.s_dtype == KV4_F32 ? 4 : 2);
+      dequant8(p + b * ps[0] + h * ps[1] + row * ps[2], ps[3], sp, ss[3], P.s_dtype, P.G, pb, P.d,
+               c, v);
+    } else {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] = 0.0f;
+    }
+    float4 *o = reinterpret_cast<float4 *>(dst + r * ld + 8 * c);
+    o[0] = make_float4(v[0], v[1], v[2], v[3]);
+    o[1] = make_float4(v[4], v[5], v[6], v[7]);
+  }
+}
+
+// shared-memory row length of a d-wide row: float4 steps, an odd number of
+// them, so that 32 rows read in step fall into different banks
+__host__ __device__ constexpr int row_ld(int d) { return 4 * (((d + 7) / 8 * 2) | 1); }
+
+}  // namespace kv4

@@ -20,7 +20,8 @@ enum DeviceErr : int {
   DEV_ERR_MBAR_TIMEOUT = 1,
   DEV_ERR_BAD_PAGE = 2,
   DEV_ERR_PEER_TIMEOUT = 4,  // a peer exchange wait expired
-  DEV_ERR_F16_RANGE = 8       // prefill: K/V values outside the f16 operand range
+  DEV_ERR_F16_RANGE = 8,      // prefill, tree: K/V values outside the f16 operand range
+  DEV_ERR_BAD_LENGTH = 16     // a context length, accepted count or path node out of range
 };
 
 // ---------------------------------------------------------------------------

@@ -28,6 +28,8 @@ EXPORTED = (
     "kv4_lse_combine", "kv4_device_error", "kv4_attention_noalloc", "kv4_append_attention",
     "kv4_attention_paged", "kv4_attention_paged_plan", "kv4_append_kv_paged",
     "kv4_lse_exchange_bytes", "kv4_lse_exchange", "kv4_prefill_attention",
+    "kv4_tree_workspace", "kv4_tree_attention", "kv4_commit_rows", "kv4_scored_workspace",
+    "kv4_scored_attention", "kv4_evict",
 )
 
 
@@ -110,12 +112,19 @@ def lib() -> ctypes.CDLL:
     L.kv4_attention_paged_plan.argtypes = [T, T, T, T, T, i64, i64, i32, P(AttnOpts),
                                            P(AttnPlan)]
     L.kv4_append_kv_paged.argtypes = [T, T, T, T, T, T, vp, i32, i32, vp]
-    L.kv4_lse_exchange_bytes.restype = i64
     L.kv4_lse_exchange_bytes.argtypes = [i64, i32, i32]
     L.kv4_lse_exchange.argtypes = [vp, vp, i64, i32, vp, i32, i32, vp, T, vp]
+    L.kv4_tree_workspace.argtypes = [T] * 9 + [i32]
+    L.kv4_tree_attention.argtypes = [T] * 10 + [vp, T, T, i32, f32, vp, sz, vp]
+    L.kv4_commit_rows.argtypes = [T] * 8 + [vp, i64, i64, vp, vp, vp, vp]
+    L.kv4_scored_workspace.argtypes = [T] * 5 + [i32, i32]
+    L.kv4_scored_attention.argtypes = [T] * 8 + [i32, i32, f32, f32, vp, sz, vp]
+    L.kv4_evict.argtypes = [T] * 10 + [vp, i64, i64, vp]
     for name in EXPORTED:
         if name not in ("kv4_version", "kv4_strerror", "kv4_last_cuda_error"):
             getattr(L, name).restype = i32
+    for name in ("kv4_tree_workspace", "kv4_scored_workspace", "kv4_lse_exchange_bytes"):
+        getattr(L, name).restype = i64
     _lib = L
     return L
 

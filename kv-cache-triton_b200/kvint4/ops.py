@@ -371,6 +371,73 @@ def lse_combine_into(parts_o: torch.Tensor, parts_lse: torch.Tensor, out: torch.
                                                _stream(out.device)))
 
 
+# --------------------------------------------------------------------------
+# branching and trimming the cache
+# --------------------------------------------------------------------------
+def _scratch(fn: str, nbytes: int, dev: torch.device) -> torch.Tensor | None:
+    """Workspace of one call, from the caching allocator (a negative size is
+    minus a status)."""
+    if nbytes < 0:
+        check(fn, -nbytes)
+    return torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+
+
+@_on_device
+def tree_attention_into(q, cache, draft, mask, out, group_size: int, *, context_lens=None,
+                        lse=None, sm_scale: float = 0.0) -> None:
+    """``kv4_tree_attention``: ``cache`` and ``draft`` are (k_packed, k_scales,
+    v_packed, v_scales); ``mask`` bool or uint8 [N, N] or [B, N, N];
+    ``context_lens`` int32 [B] on the device, or None."""
+    L = lib()
+    ds = [desc(t) for t in (q, *cache, *draft)]
+    refs = [ctypes.byref(d) for d in ds]
+    dm, do = desc(mask.view(torch.uint8)), desc(out)
+    dl = desc(lse.unsqueeze(-1)) if lse is not None else None
+    ws = _scratch("kv4_tree_workspace", L.kv4_tree_workspace(*refs, int(group_size)), q.device)
+    check("kv4_tree_attention", L.kv4_tree_attention(
+        *refs, ctypes.byref(dm), context_lens.data_ptr() if context_lens is not None else None,
+        ctypes.byref(do), ctypes.byref(dl) if dl is not None else None, int(group_size),
+        float(sm_scale), ws.data_ptr() if ws is not None else None,
+        ws.numel() if ws is not None else 0, _stream(q.device)))
+
+
+@_on_device
+def commit_rows(k_packed, cache, draft, path, accepted, context_lens, lens_out) -> None:
+    """``kv4_commit_rows``; ``k_packed`` (the first of ``cache``) names the device."""
+    L = lib()
+    ds = [desc(t) for t in (*cache, *draft)]
+    check("kv4_commit_rows", L.kv4_commit_rows(
+        *[ctypes.byref(d) for d in ds], path.data_ptr(), path.stride(0), path.shape[1],
+        accepted.data_ptr(), context_lens.data_ptr(), lens_out.data_ptr(),
+        _stream(k_packed.device)))
+
+
+@_on_device
+def scored_attention_into(q, cache, score_in, score_out, out, group_size: int,
+                          is_causal: bool = False, decay: float = 1.0,
+                          sm_scale: float = 0.0) -> None:
+    """``kv4_scored_attention``: scores f32 [B, Hkv, S]; ``score_out`` may be ``score_in``."""
+    L = lib()
+    ds = [desc(t) for t in (q, *cache)]
+    refs = [ctypes.byref(d) for d in ds]
+    tail = [ctypes.byref(desc(t)) for t in (score_in, score_out, out)]
+    ws = _scratch("kv4_scored_workspace",
+                  L.kv4_scored_workspace(*refs, int(group_size), int(is_causal)), q.device)
+    check("kv4_scored_attention", L.kv4_scored_attention(
+        *refs, *tail, int(group_size), int(is_causal), float(decay), float(sm_scale),
+        ws.data_ptr() if ws is not None else None, ws.numel() if ws is not None else 0,
+        _stream(q.device)))
+
+
+@_on_device
+def evict_into(score, cache, out_cache, out_score, index, recent: int, sinks: int) -> None:
+    """``kv4_evict``: cut ``cache`` to the shapes of ``out_cache``."""
+    L = lib()
+    ds = [desc(t) for t in (*cache, score, *out_cache, out_score)]
+    check("kv4_evict", L.kv4_evict(*[ctypes.byref(d) for d in ds], index.data_ptr(),
+                                   int(recent), int(sinks), _stream(score.device)))
+
+
 def device_error(dev: torch.device | None = None) -> int:
     """Read and clear the device error word set by bounded waits."""
     L = lib()
