@@ -16,7 +16,8 @@
 // dequantizes K into its own shared memory (lane = key for the scores), then V
 // over it (lane = column for the output), with the running maximum and sum of
 // the softmax per row.  Warps never wait for one another; ranges of one unit
-// meet in tree_merge through the workspace.
+// meet in tree_merge through the workspace.  bf16 queries over bf16 scales
+// take branch_tc.cu's kernel where the layout allows.
 #include <algorithm>
 
 #include "branch.cuh"
@@ -114,6 +115,9 @@ __global__ void tree_generic(const TreeParams P, const GenPlan L) {
     __syncwarp();
     warp_dequant_tile(P, true, b, kvh, len, t0, k1, sT, L.ld, lane);
     __syncwarp();
+    // a drafted row may hold anything where a node does not see it: there a
+    // weight of zero leaves it out instead of multiplying it
+    const bool guard = t0 + 32 > len;
 #pragma unroll 4
     for (int j = 0; j < 32; ++j) {
       float v[DC], p[RW];
@@ -122,9 +126,11 @@ __global__ void tree_generic(const TreeParams P, const GenPlan L) {
 #pragma unroll
       for (int r = 0; r < RW; ++r) p[r] = sP[j * RW + r];
 #pragma unroll
-      for (int r = 0; r < RW; ++r)
+      for (int r = 0; r < RW; ++r) {
+        if (guard && p[r] == 0.0f) continue;
 #pragma unroll
         for (int k = 0; k < DC; ++k) acc[r][k] = fmaf(p[r], v[k], acc[r][k]);
+      }
     }
   }
 #pragma unroll
@@ -319,10 +325,18 @@ int tree_fill(TreeParams &P, const kv4_tensor *q, const kv4_tensor *const cache[
   return KV4_OK;
 }
 
-int64_t tree_workspace(const TreeParams &P) { return gen_workspace(P, gen_plan(P)); }
+bool tree_tc_takes(const TreeParams &P);  // branch_tc.cu
+int64_t tree_tc_workspace(const TreeParams &P);
+int tree_tc_run(TreeParams &P, void *workspace, int64_t bytes, cudaStream_t st);
+int branch_tc_take_device_error(int *v);
+
+int64_t tree_workspace(const TreeParams &P) {
+  return tree_tc_takes(P) ? tree_tc_workspace(P) : gen_workspace(P, gen_plan(P));
+}
 
 int tree_run(TreeParams &P, void *workspace, int64_t bytes, cudaStream_t st) {
   if (P.B == 0 || P.nodes == 0) return KV4_OK;
+  if (tree_tc_takes(P)) return tree_tc_run(P, workspace, bytes, st);
   const GenPlan L = gen_plan(P);
   if (gen_workspace(P, L) > 0) {
     if (!workspace || bytes < gen_workspace(P, L)) return KV4_ERR_WORKSPACE;
@@ -387,10 +401,14 @@ __global__ void __launch_bounds__(128) commit_rows(const CommitParams P) {
 
 // read-and-clear of this file's device error word
 int branch_take_device_error(int *v) {
-  int zero = 0;
+  int zero = 0, t = 0;
   int rc = cuda_status(cudaMemcpyFromSymbol(v, g_branch_error, sizeof(int)));
   if (rc) return rc;
-  return cuda_status(cudaMemcpyToSymbol(g_branch_error, &zero, sizeof(int)));
+  rc = cuda_status(cudaMemcpyToSymbol(g_branch_error, &zero, sizeof(int)));
+  if (rc) return rc;
+  rc = branch_tc_take_device_error(&t);
+  *v |= t;
+  return rc;
 }
 
 namespace {

@@ -1,0 +1,1068 @@
+// Tree attention on the 5th-generation tensor cores (tcgen05), for bf16
+// queries over caches with bf16 scales and head sizes 64 and 128.
+//
+// The mathematics is branch.cu's.  All rows (node, q head of the group) that
+// read one KV head form the M dimension, 128 at a time, so a tile of 128 keys
+// is dequantized once for up to 256 rows.  One CTA per SM, 20 warps:
+//
+//   warps 0-7    softmax: two streams of 128 threads, a thread per row.  A
+//                stream reads its scores from tensor memory, keeps the running
+//                maximum and sum, writes the weights back as f16 over the
+//                scores, and rescales its output accumulator when the maximum
+//                moved by more than 2^8 (seldom).
+//   warps 8-15   dequantization: 16 bytes (32 codes) a thread and step, loaded
+//                one tile ahead into registers, to f16 tiles in the swizzled
+//                layout of the matrix descriptors; K and V double-buffered.
+//   warp 16      an elected lane issues S = Q K^T and O += P V for both streams.
+//   warps 17-19  turn the mask bytes of drafted tiles into 128 bits per row.
+//
+// With more than 128 rows the streams are two row tiles that share every
+// dequantized key tile; with fewer they are the even and odd key tiles of one
+// row tile, joined at the end through shared memory.  Either way the tensor
+// cores work on one stream while the other is in its softmax.
+//
+// Work is cut evenly: the (unit, key tile) pairs of all sequences lie end to
+// end and CTA c takes pairs [c W / n, (c + 1) W / n).  A unit that falls into
+// several CTAs leaves partial rows in the workspace, column by column (a warp
+// then writes 32 rows of a column in one piece), which tree_tc_merge joins in a
+// fixed order.  Lengths are read on the device.
+//
+// Operands are f16: q times a power of two per row that brings its largest
+// element to [2^13, 2^14) (exact for bf16), K and V values exactly (tc.cuh).
+// Weights enter the second product rounded to f16, times 2^7 (at most 2^15);
+// their sum is taken before that rounding, in fp32.
+#include <algorithm>
+
+#include "branch.cuh"
+#include "tc.cuh"
+
+namespace kv4 {
+
+// device error word of this file (folded into kv4_device_error)
+__device__ int g_branch_error_tc = 0;
+
+namespace {
+
+constexpr int KT = 128;      // keys per tile
+constexpr int THREADS = 640;  // five warpgroups of 96 registers a thread, shared out below
+constexpr float kWeightShift = 7.0f;  // weights are written times 2^7: f16 then resolves 2^-31 of the largest
+constexpr uint32_t kWaitPolls = 1u << 11;  // of at most 1 ms each
+
+struct TcParams {
+  TreeParams t;
+  int rows, blocks;  // rows per KV head; blocks of 256 of them
+  int dtiles;        // tiles of drafted rows
+  int2 *shares;      // workspace, per unit and block: slot of its first share (-1:
+                     // it was whole in one CTA) and CTA of its last
+};
+constexpr int WS_ROWS = 256;  // rows of a partial slot, [column][row]
+
+__device__ __forceinline__ int ctx_tiles(const TcParams &P, int b, int *err = nullptr) {
+  return static_cast<int>((static_cast<uint32_t>(context_len(P.t, b, err)) + KT - 1) / KT);
+}
+__device__ __forceinline__ int unit_tiles(const TcParams &P, int b, int *err = nullptr) {
+  return ctx_tiles(P, b, err) + P.dtiles;
+}
+
+// one CTA's share of one unit
+struct Segment {
+  int b, kvh, row0, nrows;  // rows [row0, row0 + nrows) of KV head kvh of sequence b
+  int tile, ntiles;         // key tiles [tile, tile + ntiles)
+  bool whole, last;         // all of the unit's tiles; its last one among them
+  bool first;               // the CTA's first segment
+};
+
+// walks a CTA's segments; every role walks its own copy
+struct Walk {
+  uint32_t left;            // tiles still to do
+  int b, kvh, blk, t;
+  bool first;
+  __device__ __forceinline__ bool next(const TcParams &P, Segment &s) {
+    if (left == 0) return false;
+    int T = unit_tiles(P, b);
+#pragma unroll 1
+    while (T == 0) T = unit_tiles(P, ++b);  // units without keys have no work
+    s.b = b;
+    s.kvh = kvh;
+    s.row0 = blk * 256;
+    s.nrows = min(256, P.rows - s.row0);
+    s.tile = t;
+    s.ntiles = static_cast<int>(min(static_cast<uint32_t>(T - t), left));
+    s.whole = s.ntiles == T;
+    s.last = t + s.ntiles == T;
+    s.first = first;
+    first = false;
+    left -= s.ntiles;
+    t += s.ntiles;
+    if (t == T) {
+      t = 0;
+      if (++blk == P.blocks) {
+        blk = 0;
+        if (++kvh == P.t.Hkv) {
+          kvh = 0;
+          ++b;
+        }
+      }
+    }
+    return true;
+  }
+};
+
+template <int D>
+struct Smem {
+  static constexpr int TILE = KT * D * 2;  // 128 rows of D 16-bit values
+  static constexpr int Q = 0, K = 2 * TILE, V = 4 * TILE, END = 6 * TILE;
+  static constexpr int ML = END;            // float2 [2][128]
+  static constexpr int MASK = ML + 2048;    // uint4 [2][128]: a row's visible keys of a drafted tile
+  static constexpr int BAD = MASK + 4096;   // uint32 [2][4]: drafted keys without a usable scale
+  static constexpr int BARS = BAD + 32;     // mbarriers
+  static constexpr int MISC = BARS + 160;   // TMEM address, abort flag, walk start
+  static constexpr int BYTES = MISC + 64;
+};
+
+// barriers (pairs: by stage or by stream) and their arrival counts
+enum Bar { KFULL = 0, VFULL = 2, KEMPTY = 4, VEMPTY = 6, SFULL = 8, PREADY = 10, OREADY = 12,
+           MFULL = 14, MEMPTY = 16, QREADY = 18, NBARS = 19 };
+__device__ __forceinline__ int bar_count(int i) {
+  if (i < KEMPTY) return 8;           // dequantizing warps
+  if (i < PREADY) return 1;           // commits
+  if (i < OREADY) return 4;           // a stream's warps
+  if (i < MFULL) return 1;
+  if (i < MEMPTY) return 3;           // mask warps
+  return i < QREADY ? 4 : 8;
+}
+
+struct Waiter {
+  uint32_t bars, flag;
+  __device__ __forceinline__ uint32_t at(int i) const { return bars + 8 * i; }
+  // wait for phase number n of barrier i; after a time-out nobody waits any
+  // more: the CTA runs through its loops, reports, and its output is not valid
+  __device__ __forceinline__ void wait(int i, uint32_t n) const {
+    const uint32_t bar = at(i), parity = n & 1u;
+#pragma unroll 1
+    for (uint32_t k = 0; k < kWaitPolls; ++k) {
+      if (mbar_try_wait(bar, parity)) return;
+      uint32_t off;
+      asm volatile("ld.volatile.shared.u32 %0, [%1];" : "=r"(off) : "r"(flag) : "memory");
+      if (off) return;
+    }
+    asm volatile("st.volatile.shared.u32 [%0], %1;" ::"r"(flag), "r"(1u) : "memory");
+    atomicOr(&g_branch_error_tc, DEV_ERR_MBAR_TIMEOUT);
+  }
+};
+
+// 16 bytes global -> shared, zeros instead of the source bytes past `n`
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, uint32_t n) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
+__device__ __forceinline__ void cp_async_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+
+__device__ __forceinline__ void bar_softmax() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
+
+// ---------------------------------------------------------------------------
+// A thread's place in the rows of K and V: its 16-byte chunk and its scales in
+// one row, and how far (bytes; elements) the row of its next chunk is.
+struct Source {
+  const uint8_t *k, *v;
+  const uint16_t *ks, *vs;
+  int kst, vst, ksst, vsst;
+};
+
+template <int D, int G>
+__device__ __noinline__ Source source_of(const TreeParams &T, bool draft, int b, int h, int row, int c) {
+  constexpr int RSTEP = 256 / (D / 32);
+  const RowSource &S = draft ? T.draft : T.cache;
+  Source o;
+  o.k = S.kp + b * S.kps[0] + h * S.kps[1] + row * S.kps[2] + 16 * c;
+  o.v = S.vp + b * S.vps[0] + h * S.vps[1] + row * S.vps[2] + 16 * c;
+  o.ks = static_cast<const uint16_t *>(S.ks) + b * S.kss[0] + h * S.kss[1] + row * S.kss[2] + c * 32 / G;
+  o.vs = static_cast<const uint16_t *>(S.vs) + b * S.vss[0] + h * S.vss[1] + row * S.vss[2] + c * 32 / G;
+  o.kst = static_cast<int>(S.kps[2]) * RSTEP;
+  o.vst = static_cast<int>(S.vps[2]) * RSTEP;
+  o.ksst = static_cast<int>(S.kss[2]) * RSTEP;
+  o.vsst = static_cast<int>(S.vss[2]) * RSTEP;
+  return o;
+}
+
+template <int D, int G>
+__device__ __forceinline__ void dequant_role(const TcParams &P, Walk walk, const Waiter &W,
+                                             uint32_t smem, int tid) {
+  constexpr int CPR = D / 32;                // 16-byte chunks per row
+  constexpr int RSTEP = 256 / CPR;           // rows between a thread's chunks
+  constexpr int NCH = KT / RSTEP;            // chunks per thread, tensor and tile
+  constexpr int NS = G < 32 ? 2 : 1;         // scales per chunk
+  using SM = Smem<D>;
+  struct Regs {
+    uint4 k[NCH], v[NCH];
+    uint16_t ks[NCH][NS], vs[NCH][NS];
+    bool draft;
+  };
+  const TreeParams &T = P.t;
+  const int r0 = tid / CPR, c = tid % CPR;
+
+  // the tile to load next: its segment, and this thread's first row in it
+  Segment s;
+  bool have = walk.next(P, s);
+  int i = 0, nctx = 0, len = 0, rem = 0;
+  bool draft = false;
+  Source src{};
+
+  auto point = [&](bool fresh) {
+    if (fresh) {
+      len = static_cast<int>(context_len(T, s.b, nullptr));
+      nctx = (len + KT - 1) / KT;
+    }
+    const int tile = s.tile + i;
+    draft = tile >= nctx;
+    const int t0 = (draft ? tile - nctx : tile) * KT + r0;
+    rem = (draft ? T.ndraft : len) - t0;
+    src = source_of<D, G>(T, draft, s.b, s.kvh, t0, c);
+  };
+  auto load = [&](Regs &r) {  // and step to the tile after it
+    r.draft = draft;
+#pragma unroll
+    for (int k = 0; k < NCH; ++k) {
+      r.k[k] = r.v[k] = make_uint4(0, 0, 0, 0);
+#pragma unroll
+      for (int e = 0; e < NS; ++e) r.ks[k][e] = r.vs[k][e] = 0;
+      if (RSTEP * k < rem) {
+        r.k[k] = __ldg(reinterpret_cast<const uint4 *>(src.k + static_cast<int64_t>(k) * src.kst));
+        r.v[k] = __ldg(reinterpret_cast<const uint4 *>(src.v + static_cast<int64_t>(k) * src.vst));
+#pragma unroll
+        for (int e = 0; e < NS; ++e) {
+          r.ks[k][e] = __ldg(src.ks + static_cast<int64_t>(k) * src.ksst + e);
+          r.vs[k][e] = __ldg(src.vs + static_cast<int64_t>(k) * src.vsst + e);
+        }
+      }
+    }
+    bool fresh = false;
+    if (++i == s.ntiles) {
+      i = 0;
+      have = fresh = walk.next(P, s);
+    }
+    if (!fresh && !draft && s.tile + i < nctx) {
+      src.k += static_cast<int64_t>(NCH) * src.kst;
+      src.v += static_cast<int64_t>(NCH) * src.vst;
+      src.ks += static_cast<int64_t>(NCH) * src.ksst;
+      src.vs += static_cast<int64_t>(NCH) * src.vsst;
+      rem -= KT;
+    } else if (have) {
+      point(fresh);
+    }
+  };
+  bool big = false;
+  auto store = [&](uint32_t tile, const uint4 (&w)[NCH], const uint16_t (&sc)[NCH][NS], bool drafted,
+                   uint32_t bad) {
+#pragma unroll
+    for (int k = 0; k < NCH; ++k) {
+      const int row = r0 + RSTEP * k;
+      uint32_t sp[NS];
+#pragma unroll
+      for (int e = 0; e < NS; ++e) {
+        sp[e] = tc::scale_pair(sc[k][e]);
+        const float f = __uint_as_float(static_cast<uint32_t>(sc[k][e]) << 16);
+        if (!(fabsf(f) <= tc::kMaxScale)) {
+          big = true;
+          if (drafted) {  // seen by some rows only: out of the product, those rows are marked
+            sp[e] = 0;
+            asm volatile("red.shared.or.b32 [%0], %1;" ::"r"(bad + 4 * (row >> 5)), "r"(1u << (row & 31))
+                         : "memory");
+          }
+        }
+      }
+      const uint32_t ws[4] = {w[k].x, w[k].y, w[k].z, w[k].w};
+#pragma unroll
+      for (int j0 = 0; j0 < 4; ++j0) {
+        // half of the chunks go in another order: a quarter-warp's stores then
+        // fall into eight different 16-byte columns
+        const bool turn = CPR == 4 && c >= 2;
+        const uint32_t word = turn ? ws[j0 ^ 2] : ws[j0];
+        const uint32_t sj = NS == 2 ? (turn ? sp[(j0 >> 1) ^ (NS - 1)] : sp[(j0 >> 1) & (NS - 1)]) : sp[0];
+        uint32_t v[4];
+        tc::dequant_word(word, sj, v);
+        tc::sts128(tile + tc::tile_off(row, 4 * c + (turn ? j0 ^ 2 : j0)), v[0], v[1], v[2], v[3]);
+      }
+    }
+  };
+
+  uint32_t n = 0;  // tiles so far
+  auto turn_over = [&](Regs &r) {  // a loaded tile to shared memory
+    const uint32_t st = n & 1u, use = n >> 1, bad = smem + SM::BAD + 16 * st;
+    if (r.draft) {  // the marks of the stage's last tile have been read: clear them
+      W.wait(VEMPTY + st, use + 1u);
+      if (tid < 4) asm volatile("st.shared.u32 [%0], %1;" ::"r"(bad + 4 * tid), "r"(0u) : "memory");
+      asm volatile("bar.sync 2, 256;" ::: "memory");
+    }
+#pragma unroll 1
+    for (int t = 0; t < 2; ++t) {  // K, then V, by the same code
+      W.wait((t ? VEMPTY : KEMPTY) + st, use + 1u);  // passes at once for the first use of a stage
+      store(smem + (t ? SM::V : SM::K) + st * SM::TILE, r.k, r.ks, r.draft, bad);
+      tc::fence_smem();
+      __syncwarp();
+      if ((tid & 31) == 0) mbar_arrive(W.at((t ? VFULL : KFULL) + st));
+#pragma unroll
+      for (int k = 0; k < NCH; ++k) {
+        r.k[k] = r.v[k];
+#pragma unroll
+        for (int e = 0; e < NS; ++e) r.ks[k][e] = r.vs[k][e];
+      }
+    }
+    ++n;
+  };
+  // two tiles in flight: each is loaded while the one before it is stored
+  Regs a, b2;
+  bool ha = false, hb = false;
+  if (have) point(true);
+#pragma unroll 1
+  do {
+    if (ha) turn_over(a);
+    ha = have;
+    if (ha) load(a);
+    if (hb) turn_over(b2);
+    hb = have;
+    if (hb) load(b2);
+  } while (ha);
+  if (big) atomicOr(&g_branch_error_tc, DEV_ERR_F16_RANGE);
+}
+
+// ---------------------------------------------------------------------------
+// The whole warp runs this converged; one elected lane issues.
+template <int D>
+__device__ __forceinline__ void mma_role(const TcParams &P, Walk walk, const Waiter &W,
+                                         uint32_t smem, uint32_t tmem) {
+  using SM = Smem<D>;
+  constexpr uint32_t id_s = tc::idesc(128, false), id_o = tc::idesc(D, true);
+  Segment s;
+  uint32_t base = 0, seg = 0;         // tiles before this segment; segments
+  uint32_t np0 = 0, np1 = 0;          // steps of each stream before this segment
+  while (walk.next(P, s)) {
+    const bool two = s.nrows > 128;   // two row tiles, or even and odd key tiles
+    const int nt = s.ntiles;
+    const int s0 = two ? nt : (nt + 1) / 2, s1 = two ? nt : nt / 2;
+    W.wait(QREADY, seg);
+    // S0(0) S1(0) | O0(i) S0(i+1) O1(i) S1(i+1) | ...: scores go out behind the
+    // product that reads the weights they overwrite
+#pragma unroll 1
+    for (int i = -1; i < s0; ++i) {
+#pragma unroll 1
+      for (int x = 0; x < 2; ++x) {
+        const int steps = x ? s1 : s0;
+        const bool last = !two || x == 1;  // stream that uses a tile last
+        if (i >= 0 && i < steps) {
+          const uint32_t n = base + (two ? i : 2 * i + x), st = n & 1u;
+          const uint64_t dv = tc::desc(smem + SM::V + st * SM::TILE, tc::PANEL, 1024);
+          W.wait(VFULL + st, n >> 1);
+          W.wait(PREADY + x, (x ? np1 : np0) + i);
+          tc::fence_after();
+          if (tc::elect()) {
+#pragma unroll
+            for (int j = 0; j < KT / 16; ++j)
+              tc::mma_ts(tmem + 256 + 128 * x, tmem + 128 * x + 8 * j, dv + j * 128, id_o,
+                         (i > 0 || j > 0) ? 1u : 0u);
+            tc::commit(W.at(OREADY + x));
+            if (last) tc::commit(W.at(VEMPTY + st));
+          }
+          __syncwarp();
+        }
+        if (i + 1 < steps) {
+          const uint32_t n = base + (two ? i + 1 : 2 * (i + 1) + x), st = n & 1u;
+          const uint64_t dq = tc::desc(smem + SM::Q + (two ? x : 0) * SM::TILE, 16, 1024);
+          const uint64_t dk = tc::desc(smem + SM::K + st * SM::TILE, 16, 1024);
+          W.wait(KFULL + st, n >> 1);
+          tc::fence_after();
+          if (tc::elect()) {
+#pragma unroll
+            for (int j = 0; j < D / 16; ++j) {
+              const uint64_t off = ((j >> 2) * tc::PANEL + (j & 3) * 32) / 16;
+              tc::mma_ss(tmem + 128 * x, dq + off, dk + off, id_s, j > 0 ? 1u : 0u);
+            }
+            tc::commit(W.at(SFULL + x));
+            if (last) tc::commit(W.at(KEMPTY + st));
+          }
+          __syncwarp();
+        }
+      }
+    }
+    np0 += s0;
+    np1 += s1;
+    base += nt;
+    ++seg;
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Three warps turn the mask of each drafted tile into four words per row; a
+// warp takes every third node, a lane every 32nd key.
+template <int D>
+__device__ __forceinline__ void mask_role(const TcParams &P, Walk walk, const Waiter &W,
+                                          uint32_t smem, int part, int lane) {
+  using SM = Smem<D>;
+  const TreeParams &T = P.t;
+  if (!T.mask || P.dtiles == 0) return;
+  Segment s;
+  uint32_t nm0 = 0, nm1 = 0;  // drafted tiles of each stream so far
+  while (walk.next(P, s)) {
+    const bool two = s.nrows > 128;
+    const int nctx = ctx_tiles(P, s.b);
+#pragma unroll 1
+    for (int j = max(0, nctx - s.tile); j < s.ntiles; ++j) {
+      const int j0 = (s.tile + j - nctx) * KT;
+#pragma unroll 1
+      for (int x = 0; x < 2; ++x) {
+        if (!two && (j & 1) != x) continue;
+        W.wait(MEMPTY + x, (x ? nm1 : nm0) + 1u);
+        const int ra = s.row0 + (two ? 128 * x : 0), rb = min(ra + 128, P.rows);
+#pragma unroll 1
+        for (int nd = ra / T.R + part; nd * T.R < rb; nd += 3) {
+          const uint8_t *m = T.mask + s.b * T.ms[0] + nd * T.ms[1];
+          uint32_t byte[4], word[4];
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const int jj = j0 + 32 * q + lane;
+            byte[q] = jj < T.ndraft ? __ldg(m + jj * T.ms[2]) : 0u;
+          }
+#pragma unroll
+          for (int q = 0; q < 4; ++q) word[q] = __ballot_sync(0xffffffffu, byte[q] != 0u);
+#pragma unroll 1
+          for (int r = max(nd * T.R, ra) + lane; r < min((nd + 1) * T.R, rb); r += 32)
+            tc::sts128(smem + SM::MASK + 16 * (128 * x + r - ra), word[0], word[1], word[2], word[3]);
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(W.at(MFULL + x));
+        if (x) ++nm1;
+        else ++nm0;
+      }
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+__device__ __forceinline__ uint64_t pair(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void unpair(uint64_t v, float &a, float &b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
+// A score, or -infinity where the row does not see its column (bit `e` of `bits`).
+template <bool MASKED>
+__device__ __forceinline__ float seen(uint32_t s, int e, uint32_t bits) {
+  const float f = __uint_as_float(s);
+  return !MASKED || ((bits >> e) & 1u) ? f : -INFINITY;
+}
+
+// largest visible score of 32 columns
+template <bool MASKED>
+__device__ __forceinline__ void max32(const uint32_t (&s)[32], uint32_t bits, float &m0, float &m1) {
+#pragma unroll
+  for (int e = 0; e < 32; e += 4) {
+    m0 = max3(m0, seen<MASKED>(s[e], e, bits), seen<MASKED>(s[e + 1], e + 1, bits));
+    m1 = max3(m1, seen<MASKED>(s[e + 2], e + 2, bits), seen<MASKED>(s[e + 3], e + 3, bits));
+  }
+}
+
+__device__ __forceinline__ uint32_t word_of(const uint4 &v, int i) {
+  return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w;
+}
+
+// Both passes take 32 columns at a time, the next ones on their way from
+// tensor memory, in rolled loops: the kernel's roles run side by side, and the
+// code of all of them has to stay in the instruction cache.
+template <bool MASKED>
+__device__ __forceinline__ float tile_max(uint32_t tS, const uint4 &bits) {
+  float m0 = -INFINITY, m1 = -INFINITY;
+  uint32_t a[32], b[32];
+  tc::ld32(tS, a);
+#pragma unroll 1
+  for (int c = 0; c < 4; c += 2) {
+    tc::wait_ld(a);
+    tc::ld32(tS + 32 * (c + 1), b);
+    max32<MASKED>(a, MASKED ? word_of(bits, c) : 0u, m0, m1);
+    tc::wait_ld(b);
+    if (c == 0) tc::ld32(tS + 64, a);
+    max32<MASKED>(b, MASKED ? word_of(bits, c + 1) : 0u, m0, m1);
+  }
+  return fmaxf(m0, m1);
+}
+
+// weights 2^(s c0 - m) of 32 scores as f16, added to the sums
+template <bool MASKED>
+__device__ __forceinline__ void weights32(const uint32_t (&s)[32], uint32_t bits, uint64_t cc,
+                                          uint64_t mm, uint64_t &l0, uint64_t &l1, uint32_t to) {
+  uint32_t pk[16];
+#pragma unroll
+  for (int e = 0; e < 32; e += 2) {
+    float x0, x1;
+    unpair(fma2(pair(seen<MASKED>(s[e], e, bits), seen<MASKED>(s[e + 1], e + 1, bits)), cc, mm), x0, x1);
+    x0 = fast_exp2(x0);
+    x1 = fast_exp2(x1);
+    if (e & 2) l1 = add2(l1, pair(x0, x1));
+    else l0 = add2(l0, pair(x0, x1));
+    pk[e >> 1] = pack_f16x2(x0, x1);
+  }
+  tc::st16(to, pk);
+}
+
+// ... of a tile, written over its scores; returns their sum
+template <bool MASKED>
+__device__ __forceinline__ float tile_weights(uint32_t tS, float c0, float m, const uint4 &bits) {
+  const uint64_t cc = pair(c0, c0), mm = pair(-m, -m);
+  uint64_t l0 = 0, l1 = 0;
+  uint32_t a[32], b[32];
+  tc::ld32(tS, a);
+#pragma unroll 1
+  for (int c = 0; c < 4; c += 2) {
+    tc::wait_ld(a);
+    tc::ld32(tS + 32 * (c + 1), b);
+    // over columns that have been read: 16 c + 15 < 32 (c + 1)
+    weights32<MASKED>(a, MASKED ? word_of(bits, c) : 0u, cc, mm, l0, l1, tS + 16 * c);
+    tc::wait_ld(b);
+    if (c == 0) tc::ld32(tS + 64, a);
+    weights32<MASKED>(b, MASKED ? word_of(bits, c + 1) : 0u, cc, mm, l0, l1, tS + 16 * c + 16);
+  }
+  float s0, s1;
+  unpair(add2(l0, l1), s0, s1);
+  return s0 + s1;
+}
+
+template <int D>
+__device__ __forceinline__ void softmax_role(const TcParams &P, Walk walk, const Waiter &W,
+                                             uint32_t smem, uint32_t tmem, int tid) {
+  using SM = Smem<D>;
+  const TreeParams &T = P.t;
+  const int x = tid >> 7, r = tid & 127, lane = tid & 31;
+  const uint32_t lanes = static_cast<uint32_t>((tid >> 5) & 3) << 21;  // 32 lanes per warp
+  const uint32_t tS = tmem + 128 * x + lanes, tO = tmem + 256 + 128 * x + lanes;
+  Segment s;
+  uint32_t ns = 0, nm = 0, base = 0;  // steps and drafted tiles of this stream; tiles before this segment
+  while (walk.next(P, s)) {
+    const bool two = s.nrows > 128;
+    const int nt = s.ntiles, steps = two ? nt : (nt + 1 - x) / 2;
+    const int row = s.row0 + (two ? 128 * x : 0) + r;
+    const bool ok = row < P.rows, idle = __all_sync(0xffffffffu, !ok);
+    const int node = row / T.R, head = s.kvh * T.R + row - node * T.R;
+
+    // This row of q as f16, times the power of two that brings its largest
+    // element to [2^13, 2^14): copied as it is to its place in shared memory
+    // (D / 8 lanes a row), then converted there by the row's thread.  The second
+    // stream of a single row tile only needs the factor.
+    float c0;
+    {
+      constexpr int LPR = D / 8, RPI = 32 / LPR;  // lanes per row, rows at a time
+      const uint32_t tile = smem + SM::Q + x * SM::TILE;
+      {
+        const int k = lane % LPR, rl = lane / LPR, first = row - lane;
+        const __nv_bfloat16 *q = static_cast<const __nv_bfloat16 *>(T.q) + s.b * T.qs[0] +
+                                 static_cast<int64_t>(s.kvh * T.R) * T.qs[1] + 8 * k;
+        const int dn = RPI / T.R, dh = RPI - dn * T.R;
+        int qn = (first + rl) / T.R, qh = first + rl - qn * T.R;  // node and head of this lane's row
+#pragma unroll 2
+        for (int g = rl; g < 32; g += RPI) {
+          const bool in = first + g < P.rows;
+          cp_async16(tile + tc::tile_off((r & ~31) + g, k),
+                     in ? q + qh * T.qs[1] + qn * T.qs[2] : static_cast<const __nv_bfloat16 *>(T.q),
+                     in ? 16u : 0u);
+          qn += dn;
+          qh += dh;
+          if (qh >= T.R) {
+            qh -= T.R;
+            ++qn;
+          }
+        }
+        cp_async_wait_all();
+        __syncwarp();
+      }
+      uint32_t top = 0;  // largest |q| as bits: bf16 magnitudes order like integers
+#pragma unroll 4
+      for (int k = 0; k < D / 8; ++k) {
+        const uint4 w = lds128(tile + tc::tile_off(r, k));
+        const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) top = max(top, max(u[e] & 0x7FFFu, (u[e] >> 16) & 0x7FFFu));
+      }
+      int ex = 13 - (static_cast<int>(top >> 7) - 127);
+      ex = top == 0 ? 0 : min(max(ex, -126), 126);
+      c0 = T.scale_log2 * __uint_as_float(static_cast<uint32_t>(127 - ex) << 23);
+      if (two || x == 0) {
+        const float up = __uint_as_float(static_cast<uint32_t>(ex + 127) << 23);
+#pragma unroll 4
+        for (int k = 0; k < D / 8; ++k) {
+          const uint32_t at = tile + tc::tile_off(r, k);
+          const uint4 w = lds128(at);
+          const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+          float f[8];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            f[2 * e] = bf16lo_to_f32(u[e]) * up;
+            f[2 * e + 1] = bf16hi_to_f32(u[e]) * up;
+          }
+          tc::sts128(at, pack_f16x2(f[0], f[4]), pack_f16x2(f[1], f[5]), pack_f16x2(f[2], f[6]),
+                     pack_f16x2(f[3], f[7]));
+        }
+      }
+      tc::fence_smem();
+      tc::fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(W.at(QREADY));
+    }
+    const int len = static_cast<int>(context_len(T, s.b, nullptr)), nctx = (len + KT - 1) / KT;
+
+    float m = -INFINITY, l = 0.0f;
+    bool broken = false;  // saw a key without a usable scale
+    for (int i = 0; i < steps; ++i) {
+      const int j = two ? i : 2 * i + x, tile = s.tile + j;
+      const bool draft = tile >= nctx;
+      uint4 bits;
+      bool whole = false;
+      if (draft && T.mask) {
+        W.wait(MFULL + x, nm++);
+        bits = lds128(smem + SM::MASK + 16 * tid);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(W.at(MEMPTY + x));
+      } else {  // the first `lim` keys of the tile
+        int lim;
+        if (draft) {
+          const int j0 = (tile - nctx) * KT;
+          lim = min(KT, T.ndraft - j0);
+          if (T.causal) lim = min(lim, node + T.shift + 1 - j0);
+        } else {
+          lim = len - tile * KT;
+        }
+        whole = __all_sync(0xffffffffu, lim >= KT);
+        auto below = [&](int q) {
+          const int k = min(max(lim - 32 * q, 0), 32);
+          return k == 32 ? 0xffffffffu : (1u << k) - 1u;
+        };
+        bits = make_uint4(below(0), below(1), below(2), below(3));
+      }
+      W.wait(SFULL + x, ns);
+      tc::fence_after();
+      if (!idle) {  // rows past the last: their weights may be anything
+        const float mx = (whole ? tile_max<false>(tS, bits) : tile_max<true>(tS, bits)) * c0;
+        // the maximum moves only when a score passes it by more than 8, so that
+        // weights stay below 2^8 (2^15 as written): seldom after a row's first tile
+        const bool up = mx > m + 8.0f;
+        if (__any_sync(0xffffffffu, up)) {
+          const float alpha = up && m != -INFINITY ? fast_exp2(m - mx) : up ? 0.0f : 1.0f;
+          if (up) m = mx;
+          l *= alpha;
+          if (i > 0) {
+            W.wait(OREADY + x, ns - 1);
+            tc::fence_after();
+#pragma unroll 1
+            for (int c = 0; c < D; c += 32) {
+              uint32_t o[32];
+              tc::ld32(tO + c, o);
+              tc::wait_ld(o);
+#pragma unroll
+              for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+              tc::st32(tO + c, o);
+            }
+          }
+        }
+        const float me = m == -INFINITY ? 0.0f : m - kWeightShift;
+        l += whole ? tile_weights<false>(tS, c0, me, bits) : tile_weights<true>(tS, c0, me, bits);
+        if (draft) {
+          const uint32_t n = base + j;
+          W.wait(VFULL + (n & 1u), n >> 1);  // both tensors' marks
+          const uint4 bad = lds128(smem + SM::BAD + 16 * (n & 1u));
+          broken |= ((bad.x & bits.x) | (bad.y & bits.y) | (bad.z & bits.z) | (bad.w & bits.w)) != 0u;
+        }
+        tc::wait_st();
+      }
+      tc::fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(W.at(PREADY + x));
+      ++ns;
+    }
+    base += nt;
+    m -= kWeightShift;  // what the sum refers to
+    if (broken) l = __uint_as_float(0x7fc00000u);
+
+    // ---- this row's sum and output ----
+    if (steps > 0) {
+      W.wait(OREADY + x, ns - 1);
+      tc::fence_after();
+    }
+    float2 *ml = reinterpret_cast<float2 *>(__cvta_shared_to_generic(smem + SM::ML));
+    float *xch = reinterpret_cast<float *>(__cvta_shared_to_generic(smem + SM::Q));
+    float mine = 1.0f, other = 0.0f;  // factors of this stream's and the other's output
+    const bool joined = !two && nt > 1;
+    if (!two) {
+      // each stream hands half of its columns to the other: xch [column][row]
+      ml[tid] = make_float2(m, l);
+      tc::fence_before();
+      bar_softmax();  // both streams' products are complete: Q may be overwritten
+      tc::fence_after();
+      const float2 a = ml[r], b = ml[128 + r];
+      const float M = fmaxf(a.x, b.x), Me = M == -INFINITY ? 0.0f : M;
+      const float f0 = exp2f(a.x - Me), f1 = exp2f(b.x - Me);
+      mine = x ? f1 : f0;
+      other = x ? f0 : f1;
+      m = M;
+      l = a.y * f0 + b.y * f1;
+      if (joined && !idle) {
+#pragma unroll
+        for (int c = 0; c < D / 64; ++c) {
+          uint32_t o[32];
+          tc::ld32(tO + 32 * c + (x ? 0 : D / 2), o);
+          tc::wait_ld(o);
+#pragma unroll
+          for (int e = 0; e < 32; ++e)
+            xch[(x * (D / 2) + 32 * c + e) * 128 + r] = __uint_as_float(o[e]);
+        }
+      }
+      bar_softmax();
+    }
+    if (!idle) {
+      const float inv = l > 0.0f ? 1.0f / l : (l == l ? 0.0f : l);
+      const int64_t unit = static_cast<int64_t>(s.b) * T.Hkv + s.kvh;
+      const int64_t slot = 2 * static_cast<int64_t>(blockIdx.x) + (s.first ? 0 : 1);
+      if (tid == 0) {
+        int2 *at = P.shares + unit * P.blocks + (s.row0 >> 8);
+        if (s.tile == 0) at->x = s.whole ? -1 : static_cast<int>(slot);
+        if (s.last) at->y = static_cast<int>(blockIdx.x);
+      }
+      // columns this thread writes: all of its row, or (two streams on one row) its half
+      const int cb = two ? 0 : x * (D / 2), ce = two ? D : cb + D / 2;
+      // a single tile is stream 0's alone, in its accumulator
+      const uint32_t tR = !two && !joined ? tmem + 256 + lanes : tO;
+      if (!joined) mine = 1.0f;
+#pragma unroll 1
+      for (int col = cb; col < ce; col += 32) {
+        uint32_t o[32];
+        float v[32];
+        tc::ld32(tR + col, o);
+        tc::wait_ld(o);
+#pragma unroll
+        for (int e = 0; e < 32; ++e) v[e] = __uint_as_float(o[e]) * mine;
+        if (joined) {
+#pragma unroll
+          for (int e = 0; e < 32; ++e)
+            v[e] = fmaf(xch[((1 - x) * (D / 2) + col - cb + e) * 128 + r], other, v[e]);
+        }
+        if (!ok) continue;
+        // accumulator columns 8a.. hold dims 8a + (0,4,1,5,2,6,3,7)
+        if (s.whole) {
+          __nv_bfloat16 *g = static_cast<__nv_bfloat16 *>(T.out) + s.b * T.os[0] + head * T.os[1] +
+                             node * T.os[2] + col;
+#pragma unroll
+          for (int a = 0; a < 4; ++a) {
+            const float *p = v + 8 * a;
+            uint4 w;
+            w.x = pack_bf16x2(p[0] * inv, p[2] * inv);
+            w.y = pack_bf16x2(p[4] * inv, p[6] * inv);
+            w.z = pack_bf16x2(p[1] * inv, p[3] * inv);
+            w.w = pack_bf16x2(p[5] * inv, p[7] * inv);
+            reinterpret_cast<uint4 *>(g)[a] = w;
+          }
+        } else {
+          float *g = T.ws_o + (slot * D + col) * WS_ROWS + row - s.row0;
+#pragma unroll
+          for (int e = 0; e < 32; ++e) {
+            const int dim = (e & ~7) + ((e & 1) ? 4 : 0) + ((e & 7) >> 1);
+            g[dim * WS_ROWS] = v[e];
+          }
+        }
+      }
+      if (ok && (two || x == 0)) {
+        if (!s.whole) {
+          T.ws_ml[slot * WS_ROWS + row - s.row0] = make_float2(m, l);
+        } else {
+          if (T.stats) T.stats[unit * P.rows + row] = make_float2(m, inv);
+          if (T.lse)
+            T.lse[s.b * T.ls[0] + head * T.ls[1] + node * T.ls[2]] =
+                l == 0.0f ? -INFINITY : (m + log2f(l)) * kBrLn2;
+        }
+      }
+    }
+    tc::fence_before();
+    bar_softmax();  // nobody writes Q or the exchange area of the next segment early
+  }
+}
+
+template <int D, int G>
+__global__ void __launch_bounds__(THREADS, 1) tree_tc(const __grid_constant__ TcParams P) {
+  using SM = Smem<D>;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  const uint32_t smem = smem_u32(smem_raw);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const Waiter W{smem + SM::BARS, smem + SM::MISC + 4};
+  volatile int *start = reinterpret_cast<volatile int *>(smem_raw + SM::MISC + 8);
+  griddep_launch_dependents();  // the merge may be set up: it waits for this grid's end
+  if (smem & 1023u) {  // the swizzled tiles need 1024-byte alignment
+    if (tid == 0) atomicOr(&g_branch_error_tc, DEV_ERR_MBAR_TIMEOUT);
+    return;
+  }
+  if (warp == 9) {
+    if (lane < NBARS) mbar_init(W.at(lane), bar_count(lane));
+    fence_mbar_init();
+    if (lane < 8) reinterpret_cast<uint32_t *>(smem_raw + SM::BAD)[lane] = 0u;
+    if (lane == 0) *reinterpret_cast<volatile uint32_t *>(smem_raw + SM::MISC + 4) = 0u;
+  }
+  if (warp == 16) tc::alloc(smem + SM::MISC, 512);
+  if (warp == 8) {
+    // This CTA's share: all tiles of all units lie end to end, W / n of them for
+    // each CTA and one more for the first W % n.  Sequences 32 at a time, by
+    // prefix sums; work counts fit 31 bits (the host checks).
+    const uint32_t per = static_cast<uint32_t>(P.t.Hkv * P.blocks), n = gridDim.x;
+    uint32_t total = 0;
+#pragma unroll 1
+    for (int g = lane; g < P.t.B; g += 32)
+      total += unit_tiles(P, g, blockIdx.x == 0 ? &g_branch_error_tc : nullptr);
+    total = __reduce_add_sync(0xffffffffu, total) * per;
+    const uint32_t each = total / n, rest = total - each * n;
+    const uint32_t w0 = blockIdx.x * each + min(blockIdx.x, rest);
+    uint32_t left = each + (blockIdx.x < rest ? 1u : 0u), b = 0, before = 0, T = 1;
+    if (left > 0) {
+#pragma unroll 1
+      for (int g = 0;; g += 32) {
+        const uint32_t t = g + lane < P.t.B ? unit_tiles(P, g + lane) : 0u;
+        uint32_t sum = t * per;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const uint32_t y = __shfl_up_sync(0xffffffffu, sum, o);
+          if (lane >= o) sum += y;
+        }
+        const uint32_t past = __ballot_sync(0xffffffffu, before + sum > w0);
+        if (past || g + 32 >= P.t.B) {
+          const int k = past ? __ffs(past) - 1 : 31;
+          b = g + k;
+          T = __shfl_sync(0xffffffffu, t, k);
+          before += __shfl_sync(0xffffffffu, sum, k) - T * per;
+          break;
+        }
+        before += __shfl_sync(0xffffffffu, sum, 31);
+      }
+    }
+    if (lane == 0) {
+      const uint32_t u = (w0 - before) / T, h = u / P.blocks;
+      start[0] = static_cast<int>(left);
+      start[1] = static_cast<int>(b);
+      start[2] = static_cast<int>(h);
+      start[3] = static_cast<int>(u - h * P.blocks);
+      start[4] = static_cast<int>(w0 - before - u * T);
+    }
+  }
+  tc::fence_before();
+  __syncthreads();
+  tc::fence_after();
+  const uint32_t tmem =
+      __shfl_sync(0xffffffffu, *reinterpret_cast<volatile uint32_t *>(smem_raw + SM::MISC), 0);
+  const Walk walk{static_cast<uint32_t>(start[0]), start[1], start[2], start[3], start[4], true};
+  // 128 * (2 * 128 + 2 * 88 + 48) = 640 * 96 registers
+  if (warp < 8) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 128;");
+    softmax_role<D>(P, walk, W, smem, tmem, tid);
+  } else if (warp < 16) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+    dequant_role<D, G>(P, walk, W, smem, tid - 256);
+  } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
+    if (warp == 16) mma_role<D>(P, walk, W, smem, tmem);
+    else mask_role<D>(P, walk, W, smem, warp - 17, lane);
+  }
+  __syncwarp();
+  tc::fence_before();
+  __syncthreads();
+  tc::fence_after();
+  if (warp == 16) tc::dealloc(tmem, 512);
+}
+
+// Joins the partial rows of units that fell into several CTAs; units without
+// any key get zeros.  A block takes 32 rows, a lane a row, a warp D / 8 columns.
+// Kept short: a call of few tiles spends as long fetching this code as running it.
+template <int D>
+__global__ void __launch_bounds__(256) tree_tc_merge(const __grid_constant__ TcParams P) {
+  constexpr int C = D / 8;
+  const TreeParams &T = P.t;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int kvh = blockIdx.y, b = blockIdx.z, row = blockIdx.x * 32 + lane;
+  const int unit = b * T.Hkv + kvh;
+  float m = -INFINITY, l = 0.0f, acc[C];
+#pragma unroll
+  for (int k = 0; k < C; ++k) acc[k] = 0.0f;
+  griddep_wait();
+  if (unit_tiles(P, b) > 0) {
+    const int2 share = P.shares[unit * static_cast<int64_t>(P.blocks) + (blockIdx.x >> 3)];
+    if (share.x < 0) return;  // written by its CTA
+    // the unit is the first segment of every CTA after the one it began in
+    int64_t slot = share.x;
+#pragma unroll 1
+    for (int c = share.x >> 1; c <= share.y; ++c) {
+      // rows past the last read what nobody wrote and are dropped
+      const float2 ml = T.ws_ml[slot * WS_ROWS + (row & 255)];
+      const float *o = T.ws_o + (slot * D + warp * C) * WS_ROWS + (row & 255);
+      float v[C];
+#pragma unroll
+      for (int k = 0; k < C; ++k) v[k] = o[k * WS_ROWS];
+      const float to = fmaxf(m, ml.x), base = to == -INFINITY ? 0.0f : to;
+      const float f = exp2f(m - base), g = exp2f(ml.x - base);
+      m = to;
+      l = fmaf(l, f, g * ml.y);
+#pragma unroll
+      for (int k = 0; k < C; ++k) acc[k] = fmaf(acc[k], f, g * v[k]);
+      slot = 2 * static_cast<int64_t>(c + 1);
+    }
+  }
+  if (row >= P.rows) return;
+  const int node = row / T.R, head = kvh * T.R + row - node * T.R;
+  const float inv = l > 0.0f ? 1.0f / l : (l == l ? 0.0f : l);
+  uint4 *o = reinterpret_cast<uint4 *>(static_cast<__nv_bfloat16 *>(T.out) + b * T.os[0] +
+                                       head * T.os[1] + node * T.os[2] + warp * C);
+#pragma unroll
+  for (int k = 0; k < C; k += 8)
+    o[k / 8] = make_uint4(pack_bf16x2(acc[k] * inv, acc[k + 1] * inv),
+                          pack_bf16x2(acc[k + 2] * inv, acc[k + 3] * inv),
+                          pack_bf16x2(acc[k + 4] * inv, acc[k + 5] * inv),
+                          pack_bf16x2(acc[k + 6] * inv, acc[k + 7] * inv));
+  if (warp == 0) {
+    if (T.stats) T.stats[static_cast<int64_t>(unit) * P.rows + row] = make_float2(m, inv);
+    if (T.lse)
+      T.lse[b * T.ls[0] + head * T.ls[1] + node * T.ls[2]] =
+          l == 0.0f ? -INFINITY : (m + log2f(l)) * kBrLn2;
+  }
+}
+
+bool al16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+bool rows_ok(const RowSource &S, int64_t B, int Hkv, int64_t T) {
+  if (T == 0) return true;
+  if (!al16(S.kp) || !al16(S.vp)) return false;
+  for (const int64_t *st : {S.kps, S.vps}) {
+    if (st[3] != 1 || st[2] % 16 || (Hkv > 1 && st[1] % 16) || (B > 1 && st[0] % 16)) return false;
+    if (st[2] < 0 || st[2] >= (1 << 20)) return false;  // 64 of them fit 32 bits
+  }
+  for (const int64_t *st : {S.kss, S.vss})
+    if (st[3] != 1 || st[2] < 0 || st[2] >= (1 << 20)) return false;
+  return true;
+}
+
+int sm_count() {
+  static int n[64] = {};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 148;
+  if (!n[dev]) {
+    int v = 0;
+    if (cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || v <= 0)
+      v = 148;
+    n[dev] = v;
+  }
+  return n[dev];
+}
+
+TcParams tc_plan(const TreeParams &T) {
+  TcParams P{};
+  P.t = T;
+  P.rows = T.R * T.nodes;
+  P.blocks = (P.rows + 255) / 256;
+  P.dtiles = (T.ndraft + KT - 1) / KT;
+  return P;
+}
+
+int64_t most_tiles(const TcParams &P) {
+  return P.t.B * P.t.Hkv * P.blocks * ((P.t.S + KT - 1) / KT + P.dtiles);
+}
+
+int tc_ctas(const TcParams &P) {
+  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(sm_count(), most_tiles(P))));
+}
+
+template <int D, int G>
+int launch_tc(const TcParams &P, int n, cudaStream_t st) {
+  static bool configured[64] = {};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) dev = 0;
+  if (!configured[dev]) {
+    const int rc = cuda_status(cudaFuncSetAttribute(
+        tree_tc<D, G>, cudaFuncAttributeMaxDynamicSharedMemorySize, Smem<D>::BYTES));
+    if (rc) return rc;
+    configured[dev] = true;
+  }
+  tree_tc<D, G><<<n, THREADS, Smem<D>::BYTES, st>>>(P);
+  int rc = cuda_status(cudaGetLastError());
+  if (rc) return rc;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>((P.rows + 31) / 32), static_cast<unsigned>(P.t.Hkv),
+                     static_cast<unsigned>(P.t.B));
+  cfg.blockDim = dim3(256);
+  cfg.stream = st;
+  cudaLaunchAttribute at{};
+  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &at;
+  cfg.numAttrs = 1;
+  return cuda_status(cudaLaunchKernelEx(&cfg, tree_tc_merge<D>, P));
+}
+
+}  // namespace
+
+// Whether tree_tc takes the call: bf16 queries and scales (their products are
+// exact in f16), the head sizes and groups it is built for, rows that 16-byte
+// loads can read.  Everything else is branch.cu's.
+bool tree_tc_takes(const TreeParams &T) {
+  if (T.q_dtype != KV4_BF16 || T.s_dtype != KV4_BF16) return false;
+  if (T.d != 64 && T.d != 128) return false;
+  if (T.G != 16 && T.G != 32 && T.G != 64 && T.G != 128) return false;
+  if (T.G > T.d) return false;
+  if (!rows_ok(T.cache, T.B, T.Hkv, T.S) || !rows_ok(T.draft, T.B, T.Hkv, T.ndraft)) return false;
+  if (!al16(T.q) || !al16(T.out) || T.qs[3] != 1 || T.os[3] != 1) return false;
+  const int64_t n[3] = {T.B, static_cast<int64_t>(T.Hkv) * T.R, T.nodes};
+  for (int i = 0; i < 3; ++i)
+    if (n[i] > 1 && (T.qs[i] % 8 || T.os[i] % 8)) return false;
+  return T.B < 65536 && T.Hkv < 65536 && most_tiles(tc_plan(T)) < (int64_t(1) << 31);
+}
+
+int64_t tree_tc_workspace(const TreeParams &T) {
+  const TcParams P = tc_plan(T);
+  return 2 * static_cast<int64_t>(tc_ctas(P)) * WS_ROWS * (static_cast<int64_t>(T.d) * 4 + 8) +
+         T.B * T.Hkv * P.blocks * 8;
+}
+
+int tree_tc_run(TreeParams &T, void *workspace, int64_t bytes, cudaStream_t st) {
+  if (!workspace || bytes < tree_tc_workspace(T)) return KV4_ERR_WORKSPACE;
+  TcParams P = tc_plan(T);
+  const int n = tc_ctas(P);
+  P.t.ws_o = static_cast<float *>(workspace);
+  P.t.ws_ml = reinterpret_cast<float2 *>(P.t.ws_o + 2 * static_cast<int64_t>(n) * WS_ROWS * T.d);
+  P.shares = reinterpret_cast<int2 *>(P.t.ws_ml + 2 * static_cast<int64_t>(n) * WS_ROWS);
+  if (T.d == 64) {
+    switch (T.G) {
+      case 16: return launch_tc<64, 16>(P, n, st);
+      case 32: return launch_tc<64, 32>(P, n, st);
+      default: return launch_tc<64, 64>(P, n, st);
+    }
+  }
+  switch (T.G) {
+    case 16: return launch_tc<128, 16>(P, n, st);
+    case 32: return launch_tc<128, 32>(P, n, st);
+    case 64: return launch_tc<128, 64>(P, n, st);
+    default: return launch_tc<128, 128>(P, n, st);
+  }
+}
+
+int branch_tc_take_device_error(int *v) {
+  int zero = 0;
+  int rc = cuda_status(cudaMemcpyFromSymbol(v, g_branch_error_tc, sizeof(int)));
+  if (rc) return rc;
+  return cuda_status(cudaMemcpyToSymbol(g_branch_error_tc, &zero, sizeof(int)));
+}
+
+}  // namespace kv4

@@ -128,7 +128,8 @@ int scored_fill(TreeParams &P, kv4_tensor ctx[4], kv4_tensor tail[4], const kv4_
   const int64_t S = cache[0]->shape[2];
   for (int k = 1; k < 4; ++k)
     if (cache[k]->shape[2] != S) return KV4_ERR_SHAPE;
-  const int64_t n = is_causal ? std::min(q->shape[2], S) : 0;
+  // a single query sees everything either way
+  const int64_t n = is_causal && q->shape[2] > 1 ? std::min(q->shape[2], S) : 0;
   const kv4_tensor *pc[4], *pt[4];
   for (int k = 0; k < 4; ++k) {
     ctx[k] = token_range(cache[k], 0, S - n);

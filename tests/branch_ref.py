@@ -10,12 +10,16 @@ over n visible keys of head size d:
   weight by twice that; the row's sum and output sums add (n + 64) * u32 each
   (the exponential's own error is inside the 64);
 * on the tensor-core path the weights enter the second product as f16, 2**-11
-  relative (one rounding, 2**-12 and the normaliser's share), and the products
+  relative (one rounding), and the products
   accumulate with fp32 inputs aligned to the largest term, counted as one more
   u32 * 2 per term;
+* f16 has an absolute step of 2**-24 below 2**-14, and the largest weight of a
+  row is written as at least 2**7, so a weight is also off by up to 2**-31 of
+  the largest (2**-20 of it times the 2**-11 above);
 * the output is rounded once to its type, u_out relative.
 
-A[c] = sum_t p_t |v_tc| scales the absolute error of output column c.
+A[c] = sum_t (p_t + 2**-20) |v_tc| over the visible keys scales the absolute
+error of output column c.
 """
 
 from __future__ import annotations
@@ -63,7 +67,7 @@ def attend(q, k, v, seen, sm_scale=None):
     p = torch.nan_to_num(torch.softmax(x, -1), nan=0.0)
     big = big.masked_fill(~seen, 0.0)
     X = big.amax(-1) if x.shape[-1] else torch.zeros(hq, n, dtype=torch.float64)
-    return p @ vv, p, X, p @ vv.abs()
+    return p @ vv, p, X, (p + 2.0 ** -20 * seen.double()) @ vv.abs()
 
 
 def weight_bound(X, d, keys):
