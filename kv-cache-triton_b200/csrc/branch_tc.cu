@@ -10,9 +10,9 @@
 //                maximum and sum, writes the weights back as f16 over the
 //                scores, and rescales its output accumulator when the maximum
 //                moved by more than 2^8 (seldom).
-//   warps 8-15   dequantization: 16 bytes (32 codes) a thread and step, loaded
-//                one tile ahead into registers, to f16 tiles in the swizzled
-//                layout of the matrix descriptors; K and V double-buffered.
+//   warps 8-15   dequantization, four warps each for K and V: chunks of 16 bytes
+//                (32 codes), loaded two tiles ahead into registers, to f16 tiles
+//                in the swizzled layout of the matrix descriptors, double-buffered.
 //   warp 16      an elected lane issues S = Q K^T and O += P V for both streams.
 //   warps 17-19  turn the mask bytes of drafted tiles into 128 bits per row.
 //
@@ -114,8 +114,8 @@ struct Smem {
   static constexpr int Q = 0, K = 2 * TILE, V = 4 * TILE, END = 6 * TILE;
   static constexpr int ML = END;            // float2 [2][128]
   static constexpr int MASK = ML + 2048;    // uint4 [2][128]: a row's visible keys of a drafted tile
-  static constexpr int BAD = MASK + 4096;   // uint32 [2][4]: drafted keys without a usable scale
-  static constexpr int BARS = BAD + 32;     // mbarriers
+  static constexpr int BAD = MASK + 4096;   // uint32 [4 + 2][4]: drafted keys without a usable scale in K, V
+  static constexpr int BARS = BAD + 96;     // mbarriers
   static constexpr int MISC = BARS + 160;   // TMEM address, abort flag, walk start
   static constexpr int BYTES = MISC + 64;
 };
@@ -124,7 +124,7 @@ struct Smem {
 enum Bar { KFULL = 0, VFULL = 2, KEMPTY = 4, VEMPTY = 6, SFULL = 8, PREADY = 10, OREADY = 12,
            MFULL = 14, MEMPTY = 16, QREADY = 18, NBARS = 19 };
 __device__ __forceinline__ int bar_count(int i) {
-  if (i < KEMPTY) return 8;           // dequantizing warps
+  if (i < KEMPTY) return 4;           // dequantizing warps of K, of V
   if (i < PREADY) return 1;           // commits
   if (i < OREADY) return 4;           // a stream's warps
   if (i < MFULL) return 1;
@@ -160,41 +160,41 @@ __device__ __forceinline__ void cp_async_wait_all() { asm volatile("cp.async.wai
 __device__ __forceinline__ void bar_softmax() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
 
 // ---------------------------------------------------------------------------
-// A thread's place in the rows of K and V: its 16-byte chunk and its scales in
-// one row, and how far (bytes; elements) the row of its next chunk is.
+// A thread's place in the packed rows of K or V: its 16-byte chunk and its
+// scales in one row, and how far (bytes; elements) the row of its next chunk is.
 struct Source {
-  const uint8_t *k, *v;
-  const uint16_t *ks, *vs;
-  int kst, vst, ksst, vsst;
+  const uint8_t *p;
+  const uint16_t *s;
+  int pst, sst;
 };
 
 template <int D, int G>
-__device__ __noinline__ Source source_of(const TreeParams &T, bool draft, int b, int h, int row, int c) {
-  constexpr int RSTEP = 256 / (D / 32);
+__device__ __noinline__ Source source_of(const TreeParams &T, bool draft, bool v, int b, int h, int row,
+                                         int c) {
+  constexpr int RSTEP = 128 / (D / 32);
   const RowSource &S = draft ? T.draft : T.cache;
+  const int64_t *ps = v ? S.vps : S.kps, *ss = v ? S.vss : S.kss;
   Source o;
-  o.k = S.kp + b * S.kps[0] + h * S.kps[1] + row * S.kps[2] + 16 * c;
-  o.v = S.vp + b * S.vps[0] + h * S.vps[1] + row * S.vps[2] + 16 * c;
-  o.ks = static_cast<const uint16_t *>(S.ks) + b * S.kss[0] + h * S.kss[1] + row * S.kss[2] + c * 32 / G;
-  o.vs = static_cast<const uint16_t *>(S.vs) + b * S.vss[0] + h * S.vss[1] + row * S.vss[2] + c * 32 / G;
-  o.kst = static_cast<int>(S.kps[2]) * RSTEP;
-  o.vst = static_cast<int>(S.vps[2]) * RSTEP;
-  o.ksst = static_cast<int>(S.kss[2]) * RSTEP;
-  o.vsst = static_cast<int>(S.vss[2]) * RSTEP;
+  o.p = (v ? S.vp : S.kp) + b * ps[0] + h * ps[1] + row * ps[2] + 16 * c;
+  o.s = static_cast<const uint16_t *>(v ? S.vs : S.ks) + b * ss[0] + h * ss[1] + row * ss[2] + c * 32 / G;
+  o.pst = static_cast<int>(ps[2]) * RSTEP;
+  o.sst = static_cast<int>(ss[2]) * RSTEP;
   return o;
 }
 
+// Four warps dequantize K, four V, each at its own pace: scores are asked for a
+// tile ahead of the products with V, so that V must not hold up K.
 template <int D, int G>
 __device__ __forceinline__ void dequant_role(const TcParams &P, Walk walk, const Waiter &W,
-                                             uint32_t smem, int tid) {
+                                             uint32_t smem, bool is_v, int tid) {
   constexpr int CPR = D / 32;                // 16-byte chunks per row
-  constexpr int RSTEP = 256 / CPR;           // rows between a thread's chunks
-  constexpr int NCH = KT / RSTEP;            // chunks per thread, tensor and tile
+  constexpr int RSTEP = 128 / CPR;           // rows between a thread's chunks
+  constexpr int NCH = KT / RSTEP;            // chunks per thread and tile
   constexpr int NS = G < 32 ? 2 : 1;         // scales per chunk
   using SM = Smem<D>;
   struct Regs {
-    uint4 k[NCH], v[NCH];
-    uint16_t ks[NCH][NS], vs[NCH][NS];
+    uint4 w[NCH];
+    uint16_t s[NCH][NS];
     bool draft;
   };
   const TreeParams &T = P.t;
@@ -206,7 +206,6 @@ __device__ __forceinline__ void dequant_role(const TcParams &P, Walk walk, const
   int i = 0, nctx = 0, len = 0, rem = 0;
   bool draft = false;
   Source src{};
-
   auto point = [&](bool fresh) {
     if (fresh) {
       len = static_cast<int>(context_len(T, s.b, nullptr));
@@ -216,23 +215,19 @@ __device__ __forceinline__ void dequant_role(const TcParams &P, Walk walk, const
     draft = tile >= nctx;
     const int t0 = (draft ? tile - nctx : tile) * KT + r0;
     rem = (draft ? T.ndraft : len) - t0;
-    src = source_of<D, G>(T, draft, s.b, s.kvh, t0, c);
+    src = source_of<D, G>(T, draft, is_v, s.b, s.kvh, t0, c);
   };
   auto load = [&](Regs &r) {  // and step to the tile after it
     r.draft = draft;
 #pragma unroll
     for (int k = 0; k < NCH; ++k) {
-      r.k[k] = r.v[k] = make_uint4(0, 0, 0, 0);
+      r.w[k] = make_uint4(0, 0, 0, 0);
 #pragma unroll
-      for (int e = 0; e < NS; ++e) r.ks[k][e] = r.vs[k][e] = 0;
+      for (int e = 0; e < NS; ++e) r.s[k][e] = 0;
       if (RSTEP * k < rem) {
-        r.k[k] = __ldg(reinterpret_cast<const uint4 *>(src.k + static_cast<int64_t>(k) * src.kst));
-        r.v[k] = __ldg(reinterpret_cast<const uint4 *>(src.v + static_cast<int64_t>(k) * src.vst));
+        r.w[k] = __ldg(reinterpret_cast<const uint4 *>(src.p + static_cast<int64_t>(k) * src.pst));
 #pragma unroll
-        for (int e = 0; e < NS; ++e) {
-          r.ks[k][e] = __ldg(src.ks + static_cast<int64_t>(k) * src.ksst + e);
-          r.vs[k][e] = __ldg(src.vs + static_cast<int64_t>(k) * src.vsst + e);
-        }
+        for (int e = 0; e < NS; ++e) r.s[k][e] = __ldg(src.s + static_cast<int64_t>(k) * src.sst + e);
       }
     }
     bool fresh = false;
@@ -241,36 +236,44 @@ __device__ __forceinline__ void dequant_role(const TcParams &P, Walk walk, const
       have = fresh = walk.next(P, s);
     }
     if (!fresh && !draft && s.tile + i < nctx) {
-      src.k += static_cast<int64_t>(NCH) * src.kst;
-      src.v += static_cast<int64_t>(NCH) * src.vst;
-      src.ks += static_cast<int64_t>(NCH) * src.ksst;
-      src.vs += static_cast<int64_t>(NCH) * src.vsst;
+      src.p += static_cast<int64_t>(NCH) * src.pst;
+      src.s += static_cast<int64_t>(NCH) * src.sst;
       rem -= KT;
     } else if (have) {
       point(fresh);
     }
   };
   bool big = false;
-  auto store = [&](uint32_t tile, const uint4 (&w)[NCH], const uint16_t (&sc)[NCH][NS], bool drafted,
-                   uint32_t bad) {
+  uint32_t n = 0;  // tiles so far
+  auto turn_over = [&](Regs &r) {  // a loaded tile to shared memory
+    const uint32_t st = n & 1u, use = n >> 1;
+    // marks of drafted keys: K's of the last four tiles, V's of the last two
+    // (when a stage is free again, the marks of the tile that far back have been read)
+    const uint32_t bad = smem + SM::BAD + 16 * (is_v ? 4 + st : n & 3u);
+    const uint32_t tile = smem + (is_v ? SM::V : SM::K) + st * SM::TILE;
+    W.wait((is_v ? VEMPTY : KEMPTY) + st, use + 1u);  // passes at once for the first use of a stage
+    if (r.draft) {
+      if (tid < 4) asm volatile("st.shared.u32 [%0], %1;" ::"r"(bad + 4 * tid), "r"(0u) : "memory");
+      asm volatile("bar.sync %0, 128;" ::"r"(is_v ? 3 : 2) : "memory");
+    }
 #pragma unroll
     for (int k = 0; k < NCH; ++k) {
       const int row = r0 + RSTEP * k;
       uint32_t sp[NS];
 #pragma unroll
       for (int e = 0; e < NS; ++e) {
-        sp[e] = tc::scale_pair(sc[k][e]);
-        const float f = __uint_as_float(static_cast<uint32_t>(sc[k][e]) << 16);
+        sp[e] = tc::scale_pair(r.s[k][e]);
+        const float f = __uint_as_float(static_cast<uint32_t>(r.s[k][e]) << 16);
         if (!(fabsf(f) <= tc::kMaxScale)) {
           big = true;
-          if (drafted) {  // seen by some rows only: out of the product, those rows are marked
+          if (r.draft) {  // seen by some rows only: out of the product, those rows are marked
             sp[e] = 0;
             asm volatile("red.shared.or.b32 [%0], %1;" ::"r"(bad + 4 * (row >> 5)), "r"(1u << (row & 31))
                          : "memory");
           }
         }
       }
-      const uint32_t ws[4] = {w[k].x, w[k].y, w[k].z, w[k].w};
+      const uint32_t ws[4] = {r.w[k].x, r.w[k].y, r.w[k].z, r.w[k].w};
 #pragma unroll
       for (int j0 = 0; j0 < 4; ++j0) {
         // half of the chunks go in another order: a quarter-warp's stores then
@@ -283,30 +286,9 @@ __device__ __forceinline__ void dequant_role(const TcParams &P, Walk walk, const
         tc::sts128(tile + tc::tile_off(row, 4 * c + (turn ? j0 ^ 2 : j0)), v[0], v[1], v[2], v[3]);
       }
     }
-  };
-
-  uint32_t n = 0;  // tiles so far
-  auto turn_over = [&](Regs &r) {  // a loaded tile to shared memory
-    const uint32_t st = n & 1u, use = n >> 1, bad = smem + SM::BAD + 16 * st;
-    if (r.draft) {  // the marks of the stage's last tile have been read: clear them
-      W.wait(VEMPTY + st, use + 1u);
-      if (tid < 4) asm volatile("st.shared.u32 [%0], %1;" ::"r"(bad + 4 * tid), "r"(0u) : "memory");
-      asm volatile("bar.sync 2, 256;" ::: "memory");
-    }
-#pragma unroll 1
-    for (int t = 0; t < 2; ++t) {  // K, then V, by the same code
-      W.wait((t ? VEMPTY : KEMPTY) + st, use + 1u);  // passes at once for the first use of a stage
-      store(smem + (t ? SM::V : SM::K) + st * SM::TILE, r.k, r.ks, r.draft, bad);
-      tc::fence_smem();
-      __syncwarp();
-      if ((tid & 31) == 0) mbar_arrive(W.at((t ? VFULL : KFULL) + st));
-#pragma unroll
-      for (int k = 0; k < NCH; ++k) {
-        r.k[k] = r.v[k];
-#pragma unroll
-        for (int e = 0; e < NS; ++e) r.ks[k][e] = r.vs[k][e];
-      }
-    }
+    tc::fence_smem();
+    __syncwarp();
+    if ((tid & 31) == 0) mbar_arrive(W.at((is_v ? VFULL : KFULL) + st));
     ++n;
   };
   // two tiles in flight: each is loaded while the one before it is stored
@@ -681,8 +663,9 @@ __device__ __forceinline__ void softmax_role(const TcParams &P, Walk walk, const
         l += whole ? tile_weights<false>(tS, c0, me, bits) : tile_weights<true>(tS, c0, me, bits);
         if (draft) {
           const uint32_t n = base + j;
-          W.wait(VFULL + (n & 1u), n >> 1);  // both tensors' marks
-          const uint4 bad = lds128(smem + SM::BAD + 16 * (n & 1u));
+          W.wait(VFULL + (n & 1u), n >> 1);  // V's marks; K's came with the scores
+          const uint4 bk = lds128(smem + SM::BAD + 16 * (n & 3u)), bv = lds128(smem + SM::BAD + 16 * (4 + (n & 1u)));
+          const uint4 bad = make_uint4(bk.x | bv.x, bk.y | bv.y, bk.z | bv.z, bk.w | bv.w);
           broken |= ((bad.x & bits.x) | (bad.y & bits.y) | (bad.z & bits.z) | (bad.w & bits.w)) != 0u;
         }
         tc::wait_st();
@@ -814,7 +797,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_tc(const __grid_constant__ Tc
   if (warp == 9) {
     if (lane < NBARS) mbar_init(W.at(lane), bar_count(lane));
     fence_mbar_init();
-    if (lane < 8) reinterpret_cast<uint32_t *>(smem_raw + SM::BAD)[lane] = 0u;
+    if (lane < 24) reinterpret_cast<uint32_t *>(smem_raw + SM::BAD)[lane] = 0u;
     if (lane == 0) *reinterpret_cast<volatile uint32_t *>(smem_raw + SM::MISC + 4) = 0u;
   }
   if (warp == 16) tc::alloc(smem + SM::MISC, 512);
@@ -873,7 +856,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_tc(const __grid_constant__ Tc
     softmax_role<D>(P, walk, W, smem, tmem, tid);
   } else if (warp < 16) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
-    dequant_role<D, G>(P, walk, W, smem, tid - 256);
+    dequant_role<D, G>(P, walk, W, smem, warp >= 12, tid & 127);
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
     if (warp == 16) mma_role<D>(P, walk, W, smem, tmem);
