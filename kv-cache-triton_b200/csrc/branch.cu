@@ -329,6 +329,7 @@ bool tree_tc_takes(const TreeParams &P);  // branch_tc.cu
 int64_t tree_tc_workspace(const TreeParams &P);
 int tree_tc_run(TreeParams &P, void *workspace, int64_t bytes, cudaStream_t st);
 int branch_tc_take_device_error(int *v);
+int trim_tc_take_device_error(int *v);  // trim_tc.cu
 
 int64_t tree_workspace(const TreeParams &P) {
   return tree_tc_takes(P) ? tree_tc_workspace(P) : gen_workspace(P, gen_plan(P));
@@ -407,6 +408,9 @@ int branch_take_device_error(int *v) {
   rc = cuda_status(cudaMemcpyToSymbol(g_branch_error, &zero, sizeof(int)));
   if (rc) return rc;
   rc = branch_tc_take_device_error(&t);
+  *v |= t;
+  t = 0;
+  if (!rc) rc = trim_tc_take_device_error(&t);
   *v |= t;
   return rc;
 }

@@ -129,4 +129,19 @@ __device__ __forceinline__ void warp_dequant_tile(const TreeParams &P, bool is_v
 // them, so that 32 rows read in step fall into different banks
 __host__ __device__ constexpr int row_ld(int d) { return 4 * (((d + 7) / 8 * 2) | 1); }
 
+// Scores of the cached tokens: the attention in `t` (its rows' maxima and
+// sums in t.stats), the running scores in and out.
+struct ScoreParams {
+  TreeParams t;
+  const float *in;
+  float *out;
+  int64_t is[3], os[3];  // batch, head, token strides of the scores
+  float decay;
+  int64_t keys;          // tokens in the cache: context plus drafted rows
+};
+
+int score_run(const ScoreParams &P, cudaStream_t st);      // trim.cu: any layout
+bool score_tc_takes(const ScoreParams &P);                 // trim_tc.cu
+int score_tc_run(const ScoreParams &P, cudaStream_t st);
+
 }  // namespace kv4

@@ -8,7 +8,8 @@
 // The weights are known only when a row's maximum and sum are, so the keys are
 // read twice: the attention leaves (maximum, 1 / sum) of each row, and
 // score_generic forms the weights again, a key per lane, summed over the rows
-// in a fixed order (no atomics: two calls give the same bits).
+// in a fixed order (no atomics: two calls give the same bits).  bf16 queries
+// over bf16 scales take trim_tc.cu's kernel where the layout allows.
 //
 // Eviction cuts each (sequence, KV head) to `keep` tokens: the first `sinks`,
 // the last `recent` and, of the rest, those with the highest score (equal
@@ -21,15 +22,6 @@
 
 namespace kv4 {
 namespace {
-
-struct ScoreParams {
-  TreeParams t;
-  const float *in;
-  float *out;
-  int64_t is[3], os[3];  // batch, head, token strides of the scores
-  float decay;
-  int64_t keys;          // tokens in the cache: context plus drafted rows
-};
 
 constexpr int SROWS = 8;  // query rows a warp holds at a time
 
@@ -89,6 +81,8 @@ __global__ void score_generic(const ScoreParams P, int warps, int ld, int64_t ti
   }
 }
 
+}  // namespace
+
 int score_run(const ScoreParams &P, cudaStream_t st) {
   const TreeParams &T = P.t;
   const int ld = row_ld(T.d);
@@ -107,6 +101,8 @@ int score_run(const ScoreParams &P, cudaStream_t st) {
                                                                                     tiles, tasks);
   return cuda_status(cudaGetLastError());
 }
+
+namespace {
 
 // rows [from, to) of the token dimension
 kv4_tensor token_range(const kv4_tensor *t, int64_t from, int64_t to) {
@@ -340,7 +336,7 @@ extern "C" int kv4_scored_attention(const kv4_tensor *q, const kv4_tensor *k_pac
   rc = tree_run(P.t, static_cast<char *>(workspace) + sb,
                 static_cast<int64_t>(workspace_bytes) - sb, st);
   if (rc) return rc;
-  return score_run(P, st);
+  return score_tc_takes(P) ? score_tc_run(P, st) : score_run(P, st);
 }
 
 extern "C" int kv4_evict(const kv4_tensor *k_packed, const kv4_tensor *k_scales,
