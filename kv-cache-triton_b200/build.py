@@ -3,7 +3,8 @@
     python kv-cache-triton_b200/build.py [--jobs N] [--force]
 
 Each ``csrc/*.cu`` is compiled to an object under ``_build/`` and linked into
-``kvint4/libkvint4.so`` next to the Python loader.  The CUDA runtime is linked
+``kvint4/libkvint4.so`` next to the Python loader; ``csrc/binding.cpp`` becomes
+``kvint4/_binding.so``, the torch-facing entry of the newer operators.  The CUDA runtime is linked
 statically; the driver API entry point used for TMA descriptors is fetched at
 run time, so the library loads on a machine without a GPU.
 """
@@ -62,6 +63,33 @@ def compile_one(src: str, force: bool) -> tuple[str, str]:
     return obj, r.stderr
 
 
+def build_binding(force: bool = False) -> str:
+    """The Python extension: host code over torch's C++ headers and the library."""
+    import sysconfig
+
+    import torch
+    src, out = os.path.join(CSRC, "binding.cpp"), os.path.join(HERE, "kvint4", "_binding.so")
+    deps = [src, os.path.join(INCLUDE, "kvint4.h")]
+    if not force and os.path.exists(out) and all(
+            os.path.getmtime(d) <= os.path.getmtime(out) for d in deps):
+        return out
+    troot = os.path.dirname(torch.__file__)
+    inc = [os.path.join(troot, "include"), os.path.join(troot, "include/torch/csrc/api/include"),
+           sysconfig.get_paths()["include"], os.path.join(os.path.dirname(os.path.dirname(nvcc())), "include"),
+           INCLUDE]
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-shared", "-fPIC",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
+           *[x for d in inc for x in ("-isystem" if d != INCLUDE else "-I", d)], src,
+           "-o", out + ".tmp", "-L", os.path.join(troot, "lib"), "-ltorch_python", "-ltorch_cpu",
+           "-lc10", "-lc10_cuda", f"-Wl,-rpath,{os.path.join(troot, 'lib')}",
+           "-L", os.path.join(HERE, "kvint4"), "-l:libkvint4.so", "-Wl,-rpath,$ORIGIN"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"binding build failed:\n{r.stdout}\n{r.stderr}")
+    os.replace(out + ".tmp", out)
+    return out
+
+
 def build(force: bool = False, jobs: int | None = None, verbose: bool = False) -> str:
     os.makedirs(BUILD, exist_ok=True)
     srcs = sources()
@@ -81,6 +109,7 @@ def build(force: bool = False, jobs: int | None = None, verbose: bool = False) -
         if r.returncode != 0:
             raise RuntimeError(f"link failed:\n{r.stdout}\n{r.stderr}")
         os.replace(OUT + ".tmp", OUT)
+    build_binding(force)
     return OUT
 
 

@@ -3,18 +3,18 @@
 //
 // The mathematics is branch.cu's.  All rows (node, q head of the group) that
 // read one KV head form the M dimension, 128 at a time, so a tile of 128 keys
-// is dequantized once for up to 256 rows.  One CTA per SM, 20 warps:
+// is dequantized once for up to 256 rows.  One CTA per SM, 28 warps:
 //
 //   warps 0-7    softmax: two streams of 128 threads, a thread per row.  A
 //                stream reads its scores from tensor memory, keeps the running
 //                maximum and sum, writes the weights back as f16 over the
 //                scores, and rescales its output accumulator when the maximum
 //                moved by more than 2^8 (seldom).
-//   warps 8-15   dequantization, four warps each for K and V: chunks of 16 bytes
+//   warps 8-23   dequantization, eight warps each for K and V: chunks of 16 bytes
 //                (32 codes), loaded two tiles ahead into registers, to f16 tiles
 //                in the swizzled layout of the matrix descriptors, double-buffered.
-//   warp 16      an elected lane issues S = Q K^T and O += P V for both streams.
-//   warps 17-19  turn the mask bytes of drafted tiles into 128 bits per row.
+//   warp 24      an elected lane issues S = Q K^T and O += P V for both streams.
+//   warps 25-27  turn the mask bytes of drafted tiles into 128 bits per row.
 //
 // With more than 128 rows the streams are two row tiles that share every
 // dequantized key tile; with fewer they are the even and odd key tiles of one
@@ -44,7 +44,8 @@ __device__ int g_branch_error_tc = 0;
 namespace {
 
 constexpr int KT = 128;      // keys per tile
-constexpr int THREADS = 640;  // five warpgroups of 96 registers a thread, shared out below
+constexpr int THREADS = 896;  // seven warpgroups of 72 registers a thread, shared out below
+constexpr int DQ = 256;       // threads that dequantize K, and V
 constexpr float kWeightShift = 7.0f;  // weights are written times 2^7: f16 then resolves 2^-31 of the largest
 constexpr uint32_t kWaitPolls = 1u << 11;  // of at most 1 ms each
 
@@ -124,7 +125,7 @@ struct Smem {
 enum Bar { KFULL = 0, VFULL = 2, KEMPTY = 4, VEMPTY = 6, SFULL = 8, PREADY = 10, OREADY = 12,
            MFULL = 14, MEMPTY = 16, QREADY = 18, NBARS = 19 };
 __device__ __forceinline__ int bar_count(int i) {
-  if (i < KEMPTY) return 4;           // dequantizing warps of K, of V
+  if (i < KEMPTY) return 8;           // dequantizing warps of K, of V
   if (i < PREADY) return 1;           // commits
   if (i < OREADY) return 4;           // a stream's warps
   if (i < MFULL) return 1;
@@ -154,13 +155,12 @@ struct Waiter {
 __device__ __forceinline__ void bar_softmax() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
 
 // ---------------------------------------------------------------------------
-// Four warps dequantize K, four V, each at its own pace: scores are asked for a
+// Eight warps dequantize K, eight V, each at their own pace: scores are asked for a
 // tile ahead of the products with V, so that V must not hold up K.
 template <int D, int G>
 __device__ __forceinline__ void dequant_role(const TcParams &P, Walk walk, const Waiter &W,
                                              uint32_t smem, bool is_v, int tid) {
-  constexpr int CPR = D / 32;                // 16-byte chunks per row
-  constexpr int RSTEP = 128 / CPR;           // rows between a thread's chunks
+  constexpr int RSTEP = DQ / Chunk<D>::CPR;  // rows between a thread's chunks
   constexpr int NCH = KT / RSTEP;            // chunks per thread and tile
   constexpr int NS = G < 32 ? 2 : 1;         // scales per chunk
   using SM = Smem<D>;
@@ -170,7 +170,8 @@ __device__ __forceinline__ void dequant_role(const TcParams &P, Walk walk, const
     bool draft;
   };
   const TreeParams &T = P.t;
-  const int r0 = tid / CPR, c = tid % CPR;
+  const Chunk<D> own(tid);
+  const int r0 = own.row, c = own.c;
 
   // the tile to load next: its segment, and this thread's first row in it
   Segment s;
@@ -187,7 +188,7 @@ __device__ __forceinline__ void dequant_role(const TcParams &P, Walk walk, const
     draft = tile >= nctx;
     const int t0 = (draft ? tile - nctx : tile) * KT + r0;
     rem = (draft ? T.ndraft : len) - t0;
-    src = source_of<D, G, 128>(T, draft, is_v, s.b, s.kvh, t0, c);
+    src = source_of<D, G, DQ>(T, draft, is_v, s.b, s.kvh, t0, c);
   };
   auto load = [&](Regs &r) {  // and step to the tile after it
     r.draft = draft;
@@ -226,7 +227,7 @@ __device__ __forceinline__ void dequant_role(const TcParams &P, Walk walk, const
     W.wait((is_v ? VEMPTY : KEMPTY) + st, use + 1u);  // passes at once for the first use of a stage
     if (r.draft) {
       if (tid < 4) asm volatile("st.shared.u32 [%0], %1;" ::"r"(bad + 4 * tid), "r"(0u) : "memory");
-      asm volatile("bar.sync %0, 128;" ::"r"(is_v ? 3 : 2) : "memory");
+      asm volatile("bar.sync %0, 256;" ::"r"(is_v ? 3 : 2) : "memory");
     }
 #pragma unroll
     for (int k = 0; k < NCH; ++k) {
@@ -393,47 +394,48 @@ __device__ __forceinline__ float seen(uint32_t s, int e, uint32_t bits) {
   return !MASKED || ((bits >> e) & 1u) ? f : -INFINITY;
 }
 
-// largest visible score of 32 columns
+__device__ __forceinline__ uint32_t word_of(const uint4 &v, int i) {
+  return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w;
+}
+
+// largest visible score of 16 columns
 template <bool MASKED>
-__device__ __forceinline__ void max32(const uint32_t (&s)[32], uint32_t bits, float &m0, float &m1) {
+__device__ __forceinline__ void max16(const uint32_t (&s)[16], uint32_t bits, float &m0, float &m1) {
 #pragma unroll
-  for (int e = 0; e < 32; e += 4) {
+  for (int e = 0; e < 16; e += 4) {
     m0 = max3(m0, seen<MASKED>(s[e], e, bits), seen<MASKED>(s[e + 1], e + 1, bits));
     m1 = max3(m1, seen<MASKED>(s[e + 2], e + 2, bits), seen<MASKED>(s[e + 3], e + 3, bits));
   }
 }
 
-__device__ __forceinline__ uint32_t word_of(const uint4 &v, int i) {
-  return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w;
-}
-
-// Both passes take 32 columns at a time, the next ones on their way from
-// tensor memory, in rolled loops: the kernel's roles run side by side, and the
-// code of all of them has to stay in the instruction cache.
+// Both passes take columns [32 cs, 32 ce) 16 at a time, the next ones on their
+// way from tensor memory, in rolled loops: the kernel's roles run side by side,
+// and the code of all of them has to stay in the instruction cache.
 template <bool MASKED>
-__device__ __forceinline__ float tile_max(uint32_t tS, const uint4 &bits) {
+__device__ __forceinline__ float tile_max(uint32_t tS, const uint4 &bits, int cs, int ce) {
   float m0 = -INFINITY, m1 = -INFINITY;
-  uint32_t a[32], b[32];
-  tc::ld32(tS, a);
+  uint32_t a[16], b[16];
+  tc::ld16(tS + 32 * cs, a);
 #pragma unroll 1
-  for (int c = 0; c < 4; c += 2) {
-    tc::wait_ld(a);
-    tc::ld32(tS + 32 * (c + 1), b);
-    max32<MASKED>(a, MASKED ? word_of(bits, c) : 0u, m0, m1);
-    tc::wait_ld(b);
-    if (c == 0) tc::ld32(tS + 64, a);
-    max32<MASKED>(b, MASKED ? word_of(bits, c + 1) : 0u, m0, m1);
+  for (int c = cs; c < ce; ++c) {
+    const uint32_t bw = MASKED ? word_of(bits, c) : 0u;
+    tc::wait_ld16(a);
+    tc::ld16(tS + 32 * c + 16, b);
+    max16<MASKED>(a, bw, m0, m1);
+    tc::wait_ld16(b);
+    if (c + 1 < ce) tc::ld16(tS + 32 * c + 32, a);
+    max16<MASKED>(b, bw >> 16, m0, m1);
   }
   return fmaxf(m0, m1);
 }
 
-// weights 2^(s c0 - m) of 32 scores as f16, added to the sums
+// weights 2^(s c0 - m) of 16 scores as f16, added to the sums
 template <bool MASKED>
-__device__ __forceinline__ void weights32(const uint32_t (&s)[32], uint32_t bits, uint64_t cc,
+__device__ __forceinline__ void weights16(const uint32_t (&s)[16], uint32_t bits, uint64_t cc,
                                           uint64_t mm, uint64_t &l0, uint64_t &l1, uint32_t to) {
-  uint32_t pk[16];
+  uint32_t pk[8];
 #pragma unroll
-  for (int e = 0; e < 32; e += 2) {
+  for (int e = 0; e < 16; e += 2) {
     float x0, x1;
     unpair(fma2(pair(seen<MASKED>(s[e], e, bits), seen<MASKED>(s[e + 1], e + 1, bits)), cc, mm), x0, x1);
     x0 = fast_exp2(x0);
@@ -442,25 +444,27 @@ __device__ __forceinline__ void weights32(const uint32_t (&s)[32], uint32_t bits
     else l0 = add2(l0, pair(x0, x1));
     pk[e >> 1] = pack_f16x2(x0, x1);
   }
-  tc::st16(to, pk);
+  tc::st8(to, pk);
 }
 
-// ... of a tile, written over its scores; returns their sum
+// ... of a tile's columns, written over its scores; returns their sum
 template <bool MASKED>
-__device__ __forceinline__ float tile_weights(uint32_t tS, float c0, float m, const uint4 &bits) {
+__device__ __forceinline__ float tile_weights(uint32_t tS, float c0, float m, const uint4 &bits,
+                                              int cs, int ce) {
   const uint64_t cc = pair(c0, c0), mm = pair(-m, -m);
   uint64_t l0 = 0, l1 = 0;
-  uint32_t a[32], b[32];
-  tc::ld32(tS, a);
+  uint32_t a[16], b[16];
+  tc::ld16(tS + 32 * cs, a);
 #pragma unroll 1
-  for (int c = 0; c < 4; c += 2) {
-    tc::wait_ld(a);
-    tc::ld32(tS + 32 * (c + 1), b);
-    // over columns that have been read: 16 c + 15 < 32 (c + 1)
-    weights32<MASKED>(a, MASKED ? word_of(bits, c) : 0u, cc, mm, l0, l1, tS + 16 * c);
-    tc::wait_ld(b);
-    if (c == 0) tc::ld32(tS + 64, a);
-    weights32<MASKED>(b, MASKED ? word_of(bits, c + 1) : 0u, cc, mm, l0, l1, tS + 16 * c + 16);
+  for (int c = cs; c < ce; ++c) {
+    const uint32_t bw = MASKED ? word_of(bits, c) : 0u;
+    tc::wait_ld16(a);
+    tc::ld16(tS + 32 * c + 16, b);
+    // over columns that have been read: 16 c + 7 < 32 c + 16
+    weights16<MASKED>(a, bw, cc, mm, l0, l1, tS + 16 * c);
+    tc::wait_ld16(b);
+    if (c + 1 < ce) tc::ld16(tS + 32 * c + 32, a);
+    weights16<MASKED>(b, bw >> 16, cc, mm, l0, l1, tS + 16 * c + 8);
   }
   float s0, s1;
   unpair(add2(l0, l1), s0, s1);
@@ -480,14 +484,15 @@ __device__ __forceinline__ void softmax_role(const TcParams &P, Walk walk, const
   while (walk.next(P, s)) {
     const bool two = s.nrows > 128;
     const int nt = s.ntiles, steps = two ? nt : (nt + 1 - x) / 2;
-    const int row = s.row0 + (two ? 128 * x : 0) + r;
+    // Up to 64 (32) rows lie in the tile twice (four times): each copy takes a
+    // half (a quarter) of every key tile's columns, with a maximum, a sum and an
+    // output of its own, so that all warps have work.
+    const int copies = two || s.nrows > 64 ? 1 : s.nrows > 32 ? 2 : 4, RR = 128 / copies;
+    const int copy = r / RR, cs = copy * 4 / copies, ce = cs + 4 / copies;
+    const int row = s.row0 + (two ? 128 * x + r : r & (RR - 1));
     const bool ok = row < P.rows, idle = __all_sync(0xffffffffu, !ok);
     const int node = row / T.R, head = s.kvh * T.R + row - node * T.R;
 
-    // This row of q as f16, times the power of two that brings its largest
-    // element to [2^13, 2^14): copied as it is to its place in shared memory
-    // (D / 8 lanes a row), then converted there by the row's thread.  The second
-    // stream of a single row tile only needs the factor.
     const float c0 = load_query_row<D>(T, P.rows, s.b, s.kvh, row, smem + SM::Q + x * SM::TILE, r,
                                        two || x == 0);
     tc::fence_smem();
@@ -505,7 +510,7 @@ __device__ __forceinline__ void softmax_role(const TcParams &P, Walk walk, const
       bool whole = false;
       if (draft && T.mask) {
         W.wait(MFULL + x, nm++);
-        bits = lds128(smem + SM::MASK + 16 * tid);
+        bits = lds128(smem + SM::MASK + 16 * (128 * x + (r & (RR - 1))));
         __syncwarp();
         if (lane == 0) mbar_arrive(W.at(MEMPTY + x));
       } else {  // the first `lim` keys of the tile
@@ -527,7 +532,7 @@ __device__ __forceinline__ void softmax_role(const TcParams &P, Walk walk, const
       W.wait(SFULL + x, ns);
       tc::fence_after();
       if (!idle) {  // rows past the last: their weights may be anything
-        const float mx = (whole ? tile_max<false>(tS, bits) : tile_max<true>(tS, bits)) * c0;
+        const float mx = (whole ? tile_max<false>(tS, bits, cs, ce) : tile_max<true>(tS, bits, cs, ce)) * c0;
         // the maximum moves only when a score passes it by more than 8, so that
         // weights stay below 2^8 (2^15 as written): seldom after a row's first tile
         const bool up = mx > m + 8.0f;
@@ -550,7 +555,13 @@ __device__ __forceinline__ void softmax_role(const TcParams &P, Walk walk, const
           }
         }
         const float me = m == -INFINITY ? 0.0f : m - kWeightShift;
-        l += whole ? tile_weights<false>(tS, c0, me, bits) : tile_weights<true>(tS, c0, me, bits);
+        l += whole ? tile_weights<false>(tS, c0, me, bits, cs, ce)
+                   : tile_weights<true>(tS, c0, me, bits, cs, ce);
+        if (copies > 1) {  // the other copies' columns weigh nothing here
+#pragma unroll 1
+          for (int c = 0; c < 8; ++c)
+            if (c < 2 * cs || c >= 2 * ce) tc::zero8(tS + 8 * c);
+        }
         if (draft) {
           const uint32_t n = base + j;
           W.wait(VFULL + (n & 1u), n >> 1);  // V's marks; K's came with the scores
@@ -574,96 +585,107 @@ __device__ __forceinline__ void softmax_role(const TcParams &P, Walk walk, const
       W.wait(OREADY + x, ns - 1);
       tc::fence_after();
     }
-    float2 *ml = reinterpret_cast<float2 *>(__cvta_shared_to_generic(smem + SM::ML));
-    float *xch = reinterpret_cast<float *>(__cvta_shared_to_generic(smem + SM::Q));
-    float mine = 1.0f, other = 0.0f;  // factors of this stream's and the other's output
-    const bool joined = !two && nt > 1;
-    if (!two) {
-      // each stream hands half of its columns to the other: xch [column][row]
-      ml[tid] = make_float2(m, l);
-      tc::fence_before();
-      bar_softmax();  // both streams' products are complete: Q may be overwritten
-      tc::fence_after();
-      const float2 a = ml[r], b = ml[128 + r];
-      const float M = fmaxf(a.x, b.x), Me = M == -INFINITY ? 0.0f : M;
-      const float f0 = exp2f(a.x - Me), f1 = exp2f(b.x - Me);
-      mine = x ? f1 : f0;
-      other = x ? f0 : f1;
-      m = M;
-      l = a.y * f0 + b.y * f1;
-      if (joined && !idle) {
-#pragma unroll
-        for (int c = 0; c < D / 64; ++c) {
-          uint32_t o[32];
-          tc::ld32(tO + 32 * c + (x ? 0 : D / 2), o);
-          tc::wait_ld(o);
-#pragma unroll
-          for (int e = 0; e < 32; ++e)
-            xch[(x * (D / 2) + 32 * c + e) * 128 + r] = __uint_as_float(o[e]);
-        }
-      }
-      bar_softmax();
+    const int64_t unit = static_cast<int64_t>(s.b) * T.Hkv + s.kvh;
+    const int64_t slot = 2 * static_cast<int64_t>(blockIdx.x) + (s.first ? 0 : 1);
+    if (tid == 0) {
+      int2 *at = P.shares + unit * P.blocks + (s.row0 >> 8);
+      if (s.tile == 0) at->x = s.whole ? -1 : static_cast<int>(slot);
+      if (s.last) at->y = static_cast<int>(blockIdx.x);
     }
-    if (!idle) {
-      const float inv = l > 0.0f ? 1.0f / l : (l == l ? 0.0f : l);
-      const int64_t unit = static_cast<int64_t>(s.b) * T.Hkv + s.kvh;
-      const int64_t slot = 2 * static_cast<int64_t>(blockIdx.x) + (s.first ? 0 : 1);
-      if (tid == 0) {
-        int2 *at = P.shares + unit * P.blocks + (s.row0 >> 8);
-        if (s.tile == 0) at->x = s.whole ? -1 : static_cast<int>(slot);
-        if (s.last) at->y = static_cast<int>(blockIdx.x);
-      }
-      // columns this thread writes: all of its row, or (two streams on one row) its half
-      const int cb = two ? 0 : x * (D / 2), ce = two ? D : cb + D / 2;
-      // a single tile is stream 0's alone, in its accumulator
-      const uint32_t tR = !two && !joined ? tmem + 256 + lanes : tO;
-      if (!joined) mine = 1.0f;
+    __nv_bfloat16 *out = static_cast<__nv_bfloat16 *>(T.out) + s.b * T.os[0] + head * T.os[1] +
+                         node * T.os[2];
+    float *part = T.ws_o + slot * D * WS_ROWS + row - s.row0;
+    float inv;
+    if (two) {
+      inv = l > 0.0f ? 1.0f / l : (l == l ? 0.0f : l);
 #pragma unroll 1
-      for (int col = cb; col < ce; col += 32) {
+      for (int col = 0; col < D && !idle; col += 32) {
         uint32_t o[32];
         float v[32];
-        tc::ld32(tR + col, o);
+        tc::ld32(tO + col, o);
         tc::wait_ld(o);
-#pragma unroll
-        for (int e = 0; e < 32; ++e) v[e] = __uint_as_float(o[e]) * mine;
-        if (joined) {
-#pragma unroll
-          for (int e = 0; e < 32; ++e)
-            v[e] = fmaf(xch[((1 - x) * (D / 2) + col - cb + e) * 128 + r], other, v[e]);
-        }
-        if (!ok) continue;
         // accumulator columns 8a.. hold dims 8a + (0,4,1,5,2,6,3,7)
+#pragma unroll
+        for (int e = 0; e < 32; ++e) v[(e & ~7) + ((e & 1) ? 4 : 0) + ((e & 7) >> 1)] = __uint_as_float(o[e]);
+        if (!ok) continue;
         if (s.whole) {
-          __nv_bfloat16 *g = static_cast<__nv_bfloat16 *>(T.out) + s.b * T.os[0] + head * T.os[1] +
-                             node * T.os[2] + col;
 #pragma unroll
           for (int a = 0; a < 4; ++a) {
             const float *p = v + 8 * a;
-            uint4 w;
-            w.x = pack_bf16x2(p[0] * inv, p[2] * inv);
-            w.y = pack_bf16x2(p[4] * inv, p[6] * inv);
-            w.z = pack_bf16x2(p[1] * inv, p[3] * inv);
-            w.w = pack_bf16x2(p[5] * inv, p[7] * inv);
-            reinterpret_cast<uint4 *>(g)[a] = w;
+            reinterpret_cast<uint4 *>(out + col)[a] =
+                make_uint4(pack_bf16x2(p[0] * inv, p[1] * inv), pack_bf16x2(p[2] * inv, p[3] * inv),
+                           pack_bf16x2(p[4] * inv, p[5] * inv), pack_bf16x2(p[6] * inv, p[7] * inv));
           }
         } else {
-          float *g = T.ws_o + (slot * D + col) * WS_ROWS + row - s.row0;
 #pragma unroll
-          for (int e = 0; e < 32; ++e) {
-            const int dim = (e & ~7) + ((e & 1) ? 4 : 0) + ((e & 7) >> 1);
-            g[dim * WS_ROWS] = v[e];
-          }
+          for (int e = 0; e < 32; ++e) part[(col + e) * WS_ROWS] = v[e];
         }
       }
-      if (ok && (two || x == 0)) {
-        if (!s.whole) {
-          T.ws_ml[slot * WS_ROWS + row - s.row0] = make_float2(m, l);
-        } else {
-          if (T.stats) T.stats[unit * P.rows + row] = make_float2(m, inv);
-          if (T.lse)
-            T.lse[s.b * T.ls[0] + head * T.ls[1] + node * T.ls[2]] =
-                l == 0.0f ? -INFINITY : (m + log2f(l)) * kBrLn2;
+    } else {
+      // A row's pieces (two streams, `copies` each) meet in shared memory, 32
+      // columns at a time: [piece][dim][row].  Thread t then holds row t mod RR
+      // of RR / 8 dims.
+      float2 *ml = reinterpret_cast<float2 *>(__cvta_shared_to_generic(smem + SM::ML));
+      float *xch = reinterpret_cast<float *>(__cvta_shared_to_generic(smem + SM::Q));
+      ml[tid] = make_float2(m, l);
+      tc::fence_before();
+      bar_softmax();  // all products are complete: Q may be overwritten
+      tc::fence_after();
+      float M = -INFINITY, total = 0.0f;
+#pragma unroll 1
+      for (int k = r & (RR - 1); k < 256; k += RR) M = fmaxf(M, ml[k].x);
+      const float Me = M == -INFINITY ? 0.0f : M;
+#pragma unroll 1
+      for (int k = r & (RR - 1); k < 256; k += RR) total = fmaf(ml[k].y, exp2f(ml[k].x - Me), total);
+      const float f = steps > 0 ? exp2f(m - Me) : 0.0f;
+      m = M;
+      l = total;
+      inv = l > 0.0f ? 1.0f / l : (l == l ? 0.0f : l);
+      float *mine = xch + (tid / RR) * 32 * RR + (r & (RR - 1));
+      const int nd = RR / 8, d0 = tid / RR * nd;
+#pragma unroll 1
+      for (int col = 0; col < D; col += 32) {
+        if (steps > 0) {
+          uint32_t o[32];
+          tc::ld32(tO + col, o);
+          tc::wait_ld(o);
+#pragma unroll
+          for (int e = 0; e < 32; ++e)
+            mine[((e & ~7) + ((e & 1) ? 4 : 0) + ((e & 7) >> 1)) * RR] = __uint_as_float(o[e]) * f;
+        } else {  // a single tile is stream 0's alone
+#pragma unroll 1
+          for (int e = 0; e < 32; ++e) mine[e * RR] = 0.0f;
         }
+        bar_softmax();
+#pragma unroll 1
+        for (int d = 0; d < nd; d += 4) {
+          float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+          const float *p = xch + (d0 + d) * RR + (r & (RR - 1));
+#pragma unroll 2
+          for (int k = 0; k < 2 * copies; ++k, p += 32 * RR) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] += p[e * RR];
+          }
+          if (!ok) continue;
+          if (s.whole) {
+            *reinterpret_cast<uint2 *>(out + col + d0 + d) =
+                make_uint2(pack_bf16x2(v[0] * inv, v[1] * inv), pack_bf16x2(v[2] * inv, v[3] * inv));
+          } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) part[(col + d0 + d + e) * WS_ROWS] = v[e];
+          }
+        }
+        bar_softmax();
+      }
+    }
+    if (ok && (two || tid < RR)) {
+      if (!s.whole) {
+        T.ws_ml[slot * WS_ROWS + row - s.row0] = make_float2(m, l);
+      } else {
+        if (T.stats) T.stats[unit * P.rows + row] = make_float2(m, inv);
+        if (T.lse)
+          T.lse[s.b * T.ls[0] + head * T.ls[1] + node * T.ls[2]] =
+              l == 0.0f ? -INFINITY : (m + log2f(l)) * kBrLn2;
       }
     }
     tc::fence_before();
@@ -690,7 +712,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_tc(const __grid_constant__ Tc
     if (lane < 24) reinterpret_cast<uint32_t *>(smem_raw + SM::BAD)[lane] = 0u;
     if (lane == 0) *reinterpret_cast<volatile uint32_t *>(smem_raw + SM::MISC + 4) = 0u;
   }
-  if (warp == 16) tc::alloc(smem + SM::MISC, 512);
+  if (warp == 24) tc::alloc(smem + SM::MISC, 512);
   if (warp == 8) {
     // This CTA's share: all tiles of all units lie end to end, W / n of them for
     // each CTA and one more for the first W % n.  Sequences 32 at a time, by
@@ -740,23 +762,23 @@ __global__ void __launch_bounds__(THREADS, 1) tree_tc(const __grid_constant__ Tc
   const uint32_t tmem =
       __shfl_sync(0xffffffffu, *reinterpret_cast<volatile uint32_t *>(smem_raw + SM::MISC), 0);
   const Walk walk{static_cast<uint32_t>(start[0]), start[1], start[2], start[3], start[4], true};
-  // 128 * (2 * 128 + 2 * 88 + 48) = 640 * 96 registers
+  // 128 * (2 * 120 + 4 * 56 + 40) = 896 * 72 registers
   if (warp < 8) {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 128;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 120;");
     softmax_role<D>(P, walk, W, smem, tmem, tid);
-  } else if (warp < 16) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
-    dequant_role<D, G>(P, walk, W, smem, warp >= 12, tid & 127);
+  } else if (warp < 24) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    dequant_role<D, G>(P, walk, W, smem, warp >= 16, tid & 255);
   } else {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
-    if (warp == 16) mma_role<D>(P, walk, W, smem, tmem);
-    else mask_role<D>(P, walk, W, smem, warp - 17, lane);
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+    if (warp == 24) mma_role<D>(P, walk, W, smem, tmem);
+    else mask_role<D>(P, walk, W, smem, warp - 25, lane);
   }
   __syncwarp();
   tc::fence_before();
   __syncthreads();
   tc::fence_after();
-  if (warp == 16) tc::dealloc(tmem, 512);
+  if (warp == 24) tc::dealloc(tmem, 512);
 }
 
 // Joins the partial rows of units that fell into several CTAs; units without

@@ -54,22 +54,37 @@ __device__ __noinline__ Source source_of(const TreeParams &T, bool draft, bool v
   return o;
 }
 
-// Chunk c (32 codes) of row `row` of a K or V tile, dequantized.
+// Which 16-byte chunk (32 codes) of which row a thread takes: eight neighbouring
+// lanes hold two chunks of four rows that share a 64-element panel, so that
+// their 16-byte stores fall into eight different columns of the swizzle.
+template <int D>
+struct Chunk {
+  static constexpr int CPR = D / 32;  // chunks per row
+  int row, c;
+  __device__ __forceinline__ explicit Chunk(int tid) {
+    const int lane = tid & 31;
+    if (D == 128) {
+      c = (lane & 1) | ((lane >> 2) & 2);
+      row = (tid >> 5) * 8 + ((lane >> 1) & 3) + ((lane >> 2) & 4);
+    } else {
+      c = lane & 1;
+      row = tid >> 1;
+    }
+  }
+};
+
+// Chunk c of row `row` of a K or V tile, dequantized.
 template <int D, int NS>
 __device__ __forceinline__ void store_chunk(uint32_t tile, int row, int c, const uint4 &w,
                                             const uint32_t (&scale)[NS]) {
   const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+  const uint32_t at = tile + (c >> 1) * tc::PANEL + row * 128;
+  const uint32_t col = ((c & 1) * 4) ^ (row & 7);  // 16-byte column of the chunk's first word
 #pragma unroll
-  for (int j0 = 0; j0 < 4; ++j0) {
-    // half of the chunks go in another order: a quarter-warp's stores then
-    // fall into eight different 16-byte columns
-    const bool turn = D == 128 && c >= 2;
-    const uint32_t word = turn ? ws[j0 ^ 2] : ws[j0];
-    const uint32_t sj =
-        NS == 2 ? (turn ? scale[(j0 >> 1) ^ (NS - 1)] : scale[(j0 >> 1) & (NS - 1)]) : scale[0];
+  for (int j = 0; j < 4; ++j) {
     uint32_t v[4];
-    tc::dequant_word(word, sj, v);
-    tc::sts128(tile + tc::tile_off(row, 4 * c + (turn ? j0 ^ 2 : j0)), v[0], v[1], v[2], v[3]);
+    tc::dequant_word(ws[j], scale[NS == 2 ? j >> 1 : 0], v);
+    tc::sts128(at + ((col ^ j) << 4), v[0], v[1], v[2], v[3]);
   }
 }
 

@@ -87,14 +87,15 @@ struct Waiter {
 template <int D, int G>
 __device__ __forceinline__ void dequant_role(const STcParams &P, Walk walk, const Waiter &W,
                                              uint32_t smem, int tid) {
-  constexpr int CPR = D / 32, RSTEP = 256 / CPR, NCH = KT / RSTEP, NS = G < 32 ? 2 : 1;
+  constexpr int RSTEP = 256 / Chunk<D>::CPR, NCH = KT / RSTEP, NS = G < 32 ? 2 : 1;
   using SM = Smem<D>;
   const TreeParams &T = P.s.t;
   struct Regs {
     uint4 w[NCH];
     uint16_t s[NCH][NS];
   };
-  const int r0 = tid / CPR, c = tid % CPR;
+  const Chunk<D> own(tid);
+  const int r0 = own.row, c = own.c;
   Part p;
   bool have = walk.next(P, p);
   int i = 0, pass = 0, rem = 0;

@@ -13,6 +13,7 @@ import torch
 
 from kernels.llama3._checks import check_out, check_query, check_rows, need_cuda
 from kvint4 import ops
+from kvint4._lib import binding, result
 
 
 def attention_forward_quant_gqa_scored(
@@ -39,6 +40,11 @@ def attention_forward_quant_gqa_scored(
     strides) and is updated in place when ``mass_out`` is not given.
     ``is_causal``: query ``i`` sees tokens ``t <= S - sq + i``.
     """
+    got = binding().scored(q, k_packed, k_scales, v_packed, v_scales, mass, n_q_heads, n_kv_heads,
+                           group_size, is_causal, decay, mass_out, out)
+    if got is not None:
+        return result("kv4_scored_attention", got)
+    # something about the arguments is not plainly right: say what
     cache = (k_packed, k_scales, v_packed, v_scales)
     check_rows("cache", *cache)
     check_query(q, k_packed, k_scales, n_q_heads, n_kv_heads, group_size)
@@ -78,6 +84,10 @@ def evict_by_mass(
     tokens, ``index`` int32 ``[B, n_kv_heads, keep]``; the first five are
     written into ``out`` when given (views of capacity buffers, for instance).
     """
+    got = binding().evict(k_packed, k_scales, v_packed, v_scales, mass, keep, recent, sinks, out)
+    if got is not None:
+        return result("kv4_evict", got)
+    # something about the arguments is not plainly right: say what
     cache = (k_packed, k_scales, v_packed, v_scales)
     check_rows("cache", *cache)
     b, h, s = k_packed.shape[:3]

@@ -19,6 +19,7 @@ import torch
 
 from kernels.llama3._checks import check_int32, check_out, check_query, check_rows, need_cuda
 from kvint4 import ops
+from kvint4._lib import binding, result
 
 
 def tree_attention_quant_gqa(
@@ -51,6 +52,12 @@ def tree_attention_quant_gqa(
     ``ops.device_error()`` (bit 16).  ``lse`` (f32 ``[B, n_q_heads, N]``)
     receives the log-sum-exp of each row's scores.
     """
+    got = binding().tree(q, k_packed, k_scales, v_packed, v_scales, draft_k_packed, draft_k_scales,
+                         draft_v_packed, draft_v_scales, tree_mask, n_q_heads, n_kv_heads,
+                         group_size, context_lens, out, lse)
+    if got is not None:
+        return result("kv4_tree_attention", got)
+    # something about the arguments is not plainly right: say what
     cache = (k_packed, k_scales, v_packed, v_scales)
     draft = (draft_k_packed, draft_k_scales, draft_v_packed, draft_v_scales)
     check_rows("cache", *cache)
@@ -102,6 +109,11 @@ def commit_draft_rows(
     nothing.  A sequence whose rows do not fit is left as it was and reported
     by ``ops.device_error()`` (bit 16).
     """
+    got = binding().commit(k_packed, k_scales, v_packed, v_scales, draft_k_packed, draft_k_scales,
+                           draft_v_packed, draft_v_scales, path, accepted, context_lens, lens_out)
+    if got is not None:
+        return result("kv4_commit_rows", got)
+    # something about the arguments is not plainly right: say what
     cache = (k_packed, k_scales, v_packed, v_scales)
     draft = (draft_k_packed, draft_k_scales, draft_v_packed, draft_v_scales)
     check_rows("cache", *cache)

@@ -129,6 +129,28 @@ def lib() -> ctypes.CDLL:
     return L
 
 
+_binding = None
+
+
+def binding():
+    """The compiled Python entry of the newer operators (``csrc/binding.cpp``)."""
+    global _binding
+    if _binding is None:
+        lib()
+        import torch  # noqa: F401  (its libraries first)
+
+        from . import _binding as b
+        _binding = b
+    return _binding
+
+
+def result(fn: str, got):
+    """What a binding function returned, or the library's refusal as ``Kv4Error``."""
+    if type(got) is int:
+        check(fn, got)
+    return got
+
+
 def check(fn: str, status: int) -> None:
     if status == KV4_OK:
         return
