@@ -360,7 +360,7 @@ struct CommitParams {
   uint8_t *dst[4];
   const uint8_t *src[4];
   int64_t ds[4][3], ss[4][3];  // batch, head, token strides (bytes)
-  int bytes[4];                // of a row
+  int bytes[4], vec[4];        // of a row; of one copy
   const int32_t *path, *accepted, *lens;
   int32_t *lens_out;
   int64_t path_stride;
@@ -368,33 +368,63 @@ struct CommitParams {
   int B, Hkv, nodes, width;
 };
 
-// A block per (sequence, KV head) moves its rows; the block of head 0 writes
-// the new length.  Rows are at most some tens of KB per block: the launch is
-// what such a call costs.
-__global__ void __launch_bounds__(128) commit_rows(const CommitParams P) {
-  const int b = blockIdx.x / P.Hkv, h = blockIdx.x - b * P.Hkv;
-  const int64_t len = P.lens[b], n = P.accepted[b];
-  if (len < 0 || n < 0 || n > P.width || len + n > P.cap) {  // left as it was, and reported
-    if (h == 0 && threadIdx.x == 0) {
-      atomicOr(&g_branch_error, DEV_ERR_BAD_LENGTH);
-      P.lens_out[b] = static_cast<int32_t>(len);
+constexpr int CTHREADS = 64;  // per tensor
+constexpr int CPATH = 256;    // path entries held at a time
+
+template <typename V>
+__device__ __forceinline__ void move_rows(uint8_t *dst, const uint8_t *src, int64_t ds, int64_t ss,
+                                          int bytes, const int32_t *path, int n, int nodes, int t) {
+  const int per = bytes / static_cast<int>(sizeof(V));
+  for (int e0 = t; e0 < n * per; e0 += 4 * CTHREADS) {
+    V v[4];
+    bool in[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {  // four in flight
+      const int e = e0 + u * CTHREADS, j = e / per, node = e < n * per ? path[j] : -1;
+      in[u] = node >= 0 && node < nodes;
+      if (in[u]) v[u] = __ldg(reinterpret_cast<const V *>(src + node * ss) + (e - j * per));
     }
-    return;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int e = e0 + u * CTHREADS, j = e / per;
+      if (in[u]) reinterpret_cast<V *>(dst + j * ds)[e - j * per] = v[u];
+    }
   }
-  if (h == 0 && threadIdx.x == 0) P.lens_out[b] = static_cast<int32_t>(len + n);
-  for (int k = 0; k < 4; ++k) {
-    uint8_t *dst = P.dst[k] + b * P.ds[k][0] + h * P.ds[k][1] + len * P.ds[k][2];
-    const uint8_t *src = P.src[k] + b * P.ss[k][0] + h * P.ss[k][1];
-    const int nb = P.bytes[k];
-    for (int64_t e = threadIdx.x; e < n * nb; e += blockDim.x) {
-      const int j = static_cast<int>(e / nb), c = static_cast<int>(e - static_cast<int64_t>(j) * nb);
-      const int node = P.path[b * P.path_stride + j];
-      if (node < 0 || node >= P.nodes) {
-        atomicOr(&g_branch_error, DEV_ERR_BAD_LENGTH);
-        continue;
-      }
-      dst[j * P.ds[k][2] + c] = src[node * P.ss[k][2] + c];
+}
+
+// A block per (sequence, KV head), 64 threads for each of the four tensors; the
+// block of head 0 writes the new length.  Such a call moves little: what it
+// costs is two rounds of memory latency (lengths and path, then the rows).
+__global__ void __launch_bounds__(4 * CTHREADS) commit_rows(const __grid_constant__ CommitParams P) {
+  __shared__ int32_t path[CPATH];
+  const int b = blockIdx.x / P.Hkv, h = blockIdx.x - b * P.Hkv;
+  const int k = threadIdx.x / CTHREADS, t = threadIdx.x - k * CTHREADS;
+  for (int j0 = 0; j0 == 0 || j0 < P.width; j0 += CPATH) {
+    const int j = j0 + static_cast<int>(threadIdx.x);
+    if (j < P.width) path[threadIdx.x] = P.path[b * P.path_stride + j];
+    const int64_t len = P.lens[b], n = P.accepted[b];
+    const bool fits = len >= 0 && n >= 0 && n <= P.width && len + n <= P.cap;
+    __syncthreads();
+    if (j0 == 0 && h == 0 && threadIdx.x == 0) {
+      // a sequence that does not fit is left as it was, and reported
+      if (!fits) atomicOr(&g_branch_error, DEV_ERR_BAD_LENGTH);
+      P.lens_out[b] = static_cast<int32_t>(fits ? len + n : len);
     }
+    if (!fits) return;
+    const int m = min(CPATH, static_cast<int>(n) - j0);
+    if (static_cast<int>(threadIdx.x) < m &&
+        (path[threadIdx.x] < 0 || path[threadIdx.x] >= P.nodes))
+      atomicOr(&g_branch_error, DEV_ERR_BAD_LENGTH);
+    uint8_t *dst = P.dst[k] + b * P.ds[k][0] + h * P.ds[k][1] + (len + j0) * P.ds[k][2];
+    const uint8_t *src = P.src[k] + b * P.ss[k][0] + h * P.ss[k][1];
+    switch (P.vec[k]) {
+      case 16: move_rows<uint4>(dst, src, P.ds[k][2], P.ss[k][2], P.bytes[k], path, m, P.nodes, t); break;
+      case 8: move_rows<uint2>(dst, src, P.ds[k][2], P.ss[k][2], P.bytes[k], path, m, P.nodes, t); break;
+      case 4: move_rows<uint32_t>(dst, src, P.ds[k][2], P.ss[k][2], P.bytes[k], path, m, P.nodes, t); break;
+      case 2: move_rows<uint16_t>(dst, src, P.ds[k][2], P.ss[k][2], P.bytes[k], path, m, P.nodes, t); break;
+      default: move_rows<uint8_t>(dst, src, P.ds[k][2], P.ss[k][2], P.bytes[k], path, m, P.nodes, t); break;
+    }
+    __syncthreads();
   }
 }
 
@@ -508,6 +538,7 @@ extern "C" int kv4_commit_rows(const kv4_tensor *k_packed, const kv4_tensor *k_s
       P.ds[k][i] = c->stride[i] * e;
       P.ss[k][i] = s->stride[i] * e;
     }
+    P.vec[k] = copy_width(P.dst[k], P.src[k], P.bytes[k], P.ds[k], P.ss[k]);
   }
   if (!path || !accepted || !context_lens || !lens_out || path_width < 0) return KV4_ERR_INVALID;
   const int64_t B = dst[0]->shape[0], Hkv = dst[0]->shape[1], n = src[0]->shape[2];
@@ -524,6 +555,6 @@ extern "C" int kv4_commit_rows(const kv4_tensor *k_packed, const kv4_tensor *k_s
   P.Hkv = static_cast<int>(Hkv);
   P.nodes = static_cast<int>(n);
   P.width = static_cast<int>(path_width);
-  commit_rows<<<static_cast<unsigned>(B * Hkv), 128, 0, static_cast<cudaStream_t>(stream)>>>(P);
+  commit_rows<<<static_cast<unsigned>(B * Hkv), 4 * CTHREADS, 0, static_cast<cudaStream_t>(stream)>>>(P);
   return cuda_status(cudaGetLastError());
 }

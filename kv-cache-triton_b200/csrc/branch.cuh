@@ -66,6 +66,18 @@ int tree_fill(TreeParams &P, const kv4_tensor *q, const kv4_tensor *const cache[
 int64_t tree_workspace(const TreeParams &P);
 int tree_run(TreeParams &P, void *workspace, int64_t bytes, cudaStream_t st);
 
+// Bytes of the widest copy that rows of `bytes` bytes allow, given the
+// addresses and strides (batch, head, token) of both sides.
+inline int copy_width(const void *dst, const void *src, int bytes, const int64_t (&ds)[3],
+                      const int64_t (&ss)[3]) {
+  uint64_t a = reinterpret_cast<uintptr_t>(dst) | reinterpret_cast<uintptr_t>(src) |
+               static_cast<uint64_t>(bytes);
+  for (int i = 0; i < 3; ++i) a |= static_cast<uint64_t>(ds[i] | ss[i]);
+  int v = 16;
+  while (a & (v - 1)) v >>= 1;
+  return v;
+}
+
 // one score row set of 8 elements: codes of columns [8c, 8c+8) of a packed row
 // as floats times their scale; columns at or past d are 0
 __device__ __forceinline__ void dequant8(const uint8_t *row, int64_t cs, const void *srow,

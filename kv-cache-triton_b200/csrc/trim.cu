@@ -15,7 +15,8 @@
 // the last `recent` and, of the rest, those with the highest score (equal
 // scores: the earlier token; NaN below everything).  evict_select finds the
 // threshold by radix select and writes the kept indices in token order;
-// evict_gather moves the rows.
+// evict_gather moves the rows.  The scores are read once and the kept rows
+// once, which is what eviction cannot do without; memory bounds it.
 #include <algorithm>
 
 #include "branch.cuh"
@@ -152,6 +153,7 @@ struct EvictParams {
   int32_t *index;  // [B, Hkv, keep]
   int64_t S;
   int Hkv, keep, recent, sinks;
+  bool vec;        // rows that 16-byte loads can read
 };
 
 // order-preserving 32-bit key of a score: NaN lowest, -0 as +0
@@ -161,22 +163,160 @@ __device__ __forceinline__ uint32_t score_key(float x) {
   return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
 
-constexpr int SEL = 1024;
+constexpr int SEL = 1024;   // threads per block
+constexpr int BINS = 2048;  // of one radix pass: 11, 11 and 10 bits
 
-// A block per (sequence, KV head): four passes of eight bits find the
-// threshold key, a fifth writes the kept indices by block-wide prefix sums.
-__global__ void __launch_bounds__(SEL) evict_select(const EvictParams P) {
+// exclusive prefix over the block of a pair of counts (a in the low half);
+// `total` is the whole block's
+__device__ __forceinline__ uint64_t block_prefix(uint64_t v, uint64_t *warps, uint64_t &total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  uint64_t inc = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const uint64_t y = __shfl_up_sync(0xffffffffu, inc, o);
+    if (lane >= o) inc += y;
+  }
+  __syncthreads();
+  if (lane == 31) warps[warp] = inc;
+  __syncthreads();
+  uint64_t w = warps[lane], p = w;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const uint64_t y = __shfl_up_sync(0xffffffffu, p, o);
+    if (lane >= o) p += y;
+  }
+  total = __shfl_sync(0xffffffffu, p, 31);
+  return __shfl_sync(0xffffffffu, p - w, warp) + inc - v;
+}
+
+// A cluster of `ranks` blocks per (sequence, KV head); each block takes `per`
+// tokens in a row, each thread K of them, held as keys in registers.  Three
+// passes find the threshold key (histograms in shared memory, added up over the
+// cluster through distributed shared memory), then prefix sums give every kept
+// token its place.  Scores are read once.
+template <int K>
+__global__ void __launch_bounds__(SEL) evict_select(const __grid_constant__ EvictParams P, int ranks) {
+  __shared__ uint32_t hist[2][BINS];  // by turns: a block may still read the other
+  __shared__ uint64_t warps[32], s_count;
+  __shared__ uint32_t s_bin, s_above;
+  const int tid = threadIdx.x;
+  const uint32_t rank = cluster_ctarank();
+  const int unit = blockIdx.x / ranks, b = unit / P.Hkv, h = unit - b * P.Hkv;
+  const float *mass = P.mass + b * P.ms[0] + h * P.ms[1];
+  const int lo = P.sinks, hi = static_cast<int>(P.S) - P.recent;
+  const int t0 = (static_cast<int>(rank) * SEL + tid) * K;
+  uint32_t left = static_cast<uint32_t>(P.keep - P.sinks - P.recent);  // to be taken by score
+  uint32_t key[K];
+  bool mid[K];  // takes part in the ranking
+  if (P.vec && t0 + K <= P.S) {
+#pragma unroll
+    for (int k = 0; k < K; k += 4) {
+      const float4 v = *reinterpret_cast<const float4 *>(mass + t0 + k);
+      key[k] = score_key(v.x);
+      key[k + 1] = score_key(v.y);
+      key[k + 2] = score_key(v.z);
+      key[k + 3] = score_key(v.w);
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < K; ++k) key[k] = t0 + k < P.S ? score_key(mass[(t0 + k) * P.ms[2]]) : 0u;
+  }
+#pragma unroll
+  for (int k = 0; k < K; ++k) mid[k] = t0 + k >= lo && t0 + k < hi;
+
+  uint32_t prefix = 0, known = 0;
+  const bool ranked = left > 0;
+  if (ranked) {
+#pragma unroll 1
+    for (int pass = 0; pass < 3; ++pass) {
+      const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
+      const uint32_t mask = pass == 2 ? 1023u : 2047u;
+      uint32_t *bins = hist[pass & 1];
+      bins[tid] = 0u;
+      bins[tid + SEL] = 0u;
+      __syncthreads();
+#pragma unroll
+      for (int k = 0; k < K; ++k)
+        if (mid[k] && (key[k] & known) == prefix) atomicAdd(&bins[(key[k] >> shift) & mask], 1u);
+      __syncthreads();
+      // bins from the highest down: thread t holds two of them
+      const int hb = BINS - 1 - 2 * tid;
+      uint32_t c0 = bins[hb], c1 = bins[hb - 1];
+      if (ranks > 1) {
+        cluster_sync();
+        const uint32_t at = smem_u32(bins + hb - 1);
+#pragma unroll 1
+        for (uint32_t r = 0; r < static_cast<uint32_t>(ranks); ++r) {
+          if (r == rank) continue;
+          const uint32_t a = dsmem_addr(at, r);
+          c1 += static_cast<uint32_t>(ld_dsmem_s32(a));
+          c0 += static_cast<uint32_t>(ld_dsmem_s32(a + 4));
+        }
+      }
+      uint64_t total;
+      const uint32_t above = static_cast<uint32_t>(block_prefix(c0 + c1, warps, total));
+      if (above < left && left <= above + c0) {
+        s_bin = hb;
+        s_above = above;
+      } else if (above + c0 < left && left <= above + c0 + c1) {
+        s_bin = hb - 1;
+        s_above = above + c0;
+      }
+      __syncthreads();
+      prefix |= s_bin << shift;
+      left -= s_above;
+      known |= mask << shift;
+    }
+  }
+  // now `left` of the keys equal to `prefix` are kept, the first ones
+  uint32_t gt = 0, eq = 0;
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    const bool forced = t0 + k < P.S && !mid[k];
+    if (forced || (ranked && mid[k] && key[k] > prefix)) gt |= 1u << k;
+    else if (ranked && mid[k] && key[k] == prefix) eq |= 1u << k;
+  }
+  uint64_t total;
+  uint64_t at = block_prefix(__popc(gt) | static_cast<uint64_t>(__popc(eq)) << 32, warps, total);
+  if (ranks > 1) {
+    if (tid == 0) s_count = total;
+    cluster_sync();
+    uint32_t g = 0, e = 0;
+#pragma unroll 1
+    for (uint32_t r = 0; r < rank; ++r) {
+      const uint32_t a = dsmem_addr(smem_u32(&s_count), r);
+      g += static_cast<uint32_t>(ld_dsmem_s32(a));
+      e += static_cast<uint32_t>(ld_dsmem_s32(a + 4));
+    }
+    at += g | static_cast<uint64_t>(e) << 32;
+    cluster_sync();  // nobody's shared memory goes while it is read
+  }
+  int32_t *out = P.index + static_cast<int64_t>(unit) * P.keep;
+  uint32_t g = static_cast<uint32_t>(at), e = static_cast<uint32_t>(at >> 32);
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    if ((gt >> k & 1u) || ((eq >> k & 1u) && e < left)) out[g + min(e, left)] = t0 + k;
+    g += gt >> k & 1u;
+    e += eq >> k & 1u;
+  }
+}
+
+// The same for rows longer than a cluster holds: a block per row reads the
+// scores once for each of four eight-bit passes and once more to place them.
+__global__ void __launch_bounds__(SEL) evict_select_long(const __grid_constant__ EvictParams P) {
   __shared__ int hist[256];
   __shared__ uint32_t s_prefix;
   __shared__ int s_left;
-  __shared__ int w_gt[32], w_eq[32];
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  __shared__ uint64_t warps[32];
+  const int tid = threadIdx.x;
   const int64_t b = blockIdx.x / P.Hkv, h = blockIdx.x - b * P.Hkv;
   const float *mass = P.mass + b * P.ms[0] + h * P.ms[1];
   const int64_t lo = P.sinks, hi = P.S - P.recent;
   int left = P.keep - P.sinks - P.recent;  // still to be taken among equals
+  const bool ranked = left > 0;
   uint32_t prefix = 0, known = 0;
-  if (left > 0) {
+  if (ranked) {
+#pragma unroll 1
     for (int shift = 24; shift >= 0; shift -= 8) {
       if (tid < 256) hist[tid] = 0;
       __syncthreads();
@@ -197,41 +337,56 @@ __global__ void __launch_bounds__(SEL) evict_select(const EvictParams P) {
       known |= 255u << shift;
     }
   }
-  const bool none = P.keep - P.sinks - P.recent <= 0;
   int32_t *out = P.index + static_cast<int64_t>(blockIdx.x) * P.keep;
-  int gt_base = 0, eq_base = 0;  // kept for sure, and equal to the threshold, so far
+  uint64_t base = 0;  // kept for sure (low half) and equal to the threshold, so far
   for (int64_t c = 0; c < P.S; c += SEL) {
     const int64_t t = c + tid;
     bool gt = false, eq = false;
     if (t < P.S) {
       if (t < lo || t >= hi) gt = true;
-      else if (!none) {
+      else if (ranked) {
         const uint32_t k = score_key(mass[t * P.ms[2]]);
         gt = k > prefix;
         eq = k == prefix;
       }
     }
-    const uint32_t mg = __ballot_sync(0xffffffffu, gt), me = __ballot_sync(0xffffffffu, eq);
-    __syncthreads();
-    if (lane == 0) {
-      w_gt[warp] = __popc(mg);
-      w_eq[warp] = __popc(me);
-    }
-    __syncthreads();
-    int g = gt_base, e = eq_base;
-    for (int w = 0; w < SEL / 32; ++w) {
-      if (w < warp) {
-        g += w_gt[w];
-        e += w_eq[w];
-      }
-      gt_base += w_gt[w];
-      eq_base += w_eq[w];
-    }
-    const uint32_t before = (1u << lane) - 1u;
-    g += __popc(mg & before);
-    e += __popc(me & before);
+    uint64_t total;
+    const uint64_t at =
+        base + block_prefix((gt ? 1u : 0u) | static_cast<uint64_t>(eq ? 1u : 0u) << 32, warps, total);
+    const int g = static_cast<int>(at & 0xffffffffu), e = static_cast<int>(at >> 32);
     if (gt || (eq && e < left)) out[g + min(e, left)] = static_cast<int32_t>(t);
+    base += total;
   }
+}
+
+template <int K>
+int launch_select(const EvictParams &E, int64_t units, int ranks, cudaStream_t st) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(units * ranks));
+  cfg.blockDim = dim3(SEL);
+  cfg.stream = st;
+  cudaLaunchAttribute at{};
+  at.id = cudaLaunchAttributeClusterDimension;
+  at.val.clusterDim.x = static_cast<unsigned>(ranks);
+  at.val.clusterDim.y = at.val.clusterDim.z = 1;
+  cfg.attrs = &at;
+  cfg.numAttrs = 1;
+  return cuda_status(cudaLaunchKernelEx(&cfg, evict_select<K>, E, ranks));
+}
+
+// Blocks of 1024 threads, up to 16 tokens a thread and 8 blocks a row.  Few
+// rows: more blocks each, while 4 tokens a thread and two blocks per SM remain.
+int run_select(const EvictParams &E, int64_t units, cudaStream_t st) {
+  int ranks = 1;
+  while (ranks < 8 && E.S > static_cast<int64_t>(ranks) * SEL * 16) ranks *= 2;
+  while (ranks < 8 && E.S > static_cast<int64_t>(ranks) * SEL * 4 && units * ranks * 2 <= 2 * 148)
+    ranks *= 2;
+  const int64_t per = (E.S + static_cast<int64_t>(ranks) * SEL - 1) / (static_cast<int64_t>(ranks) * SEL);
+  if (per <= 4) return launch_select<4>(E, units, ranks, st);
+  if (per <= 8) return launch_select<8>(E, units, ranks, st);
+  if (per <= 16) return launch_select<16>(E, units, ranks, st);
+  evict_select_long<<<static_cast<unsigned>(units), SEL, 0, st>>>(E);
+  return cuda_status(cudaGetLastError());
 }
 
 struct GatherParams {
@@ -258,10 +413,12 @@ __device__ __forceinline__ void gather_rows(const GatherParams &P, int k, int64_
   }
 }
 
-__global__ void __launch_bounds__(256) evict_gather(const GatherParams P) {
+// Any row sizes and alignments.
+__global__ void __launch_bounds__(256) evict_gather(const __grid_constant__ GatherParams P) {
   __shared__ int32_t idx[GROWS];
   const int64_t unit = blockIdx.x / P.tiles, b = unit / P.Hkv, h = unit - b * P.Hkv;
   const int j0 = static_cast<int>(blockIdx.x - unit * P.tiles) * GROWS, n = min(GROWS, P.keep - j0);
+  griddep_wait();  // the indices come from the kernel before
   if (static_cast<int>(threadIdx.x) < n) idx[threadIdx.x] = P.index[unit * P.keep + j0 + threadIdx.x];
   __syncthreads();
 #pragma unroll
@@ -276,14 +433,70 @@ __global__ void __launch_bounds__(256) evict_gather(const GatherParams P) {
   }
 }
 
-// the widest copy that the rows of both sides allow
-int copy_width(const GatherParams &P, int k) {
-  uint64_t a = reinterpret_cast<uintptr_t>(P.src[k]) | reinterpret_cast<uintptr_t>(P.dst[k]) |
-               static_cast<uint64_t>(P.bytes[k]);
-  for (int i = 0; i < 3; ++i) a |= static_cast<uint64_t>(P.ss[k][i] | P.ds[k][i]);
-  int v = 16;
-  while (a & (v - 1)) v >>= 1;
-  return v;
+// Packed rows of CH 16-byte chunks and scale rows of one V each (the usual
+// caches): every thread has all of its loads in flight before its first store.
+template <int CH, typename V>
+__global__ void __launch_bounds__(256) evict_gather_fast(const __grid_constant__ GatherParams P) {
+  constexpr int ROWS = 256 / CH;  // per block
+  const int64_t unit = blockIdx.x / P.tiles, b = unit / P.Hkv, h = unit - b * P.Hkv;
+  const int j0 = static_cast<int>(blockIdx.x - unit * P.tiles) * ROWS;
+  const int t = threadIdx.x, j = j0 + t / CH, c = t % CH;
+  const bool in = j < P.keep;
+  griddep_wait();
+  const int64_t at = in ? P.index[unit * P.keep + j] : 0;
+  uint4 w[2];
+  V s{};
+  uint32_t m = 0;
+  const uint8_t *src[5];
+#pragma unroll
+  for (int k = 0; k < 5; ++k) src[k] = P.src[k] + b * P.ss[k][0] + h * P.ss[k][1] + at * P.ss[k][2];
+  if (in) {
+    w[0] = __ldg(reinterpret_cast<const uint4 *>(src[0]) + c);
+    w[1] = __ldg(reinterpret_cast<const uint4 *>(src[2]) + c);
+    if (c < 2) s = __ldg(reinterpret_cast<const V *>(c ? src[3] : src[1]));
+    if (c == CH - 1) m = __ldg(reinterpret_cast<const uint32_t *>(src[4]));
+  }
+  uint8_t *dst[5];
+#pragma unroll
+  for (int k = 0; k < 5; ++k) dst[k] = P.dst[k] + b * P.ds[k][0] + h * P.ds[k][1] + j * P.ds[k][2];
+  if (in) {
+    reinterpret_cast<uint4 *>(dst[0])[c] = w[0];
+    reinterpret_cast<uint4 *>(dst[2])[c] = w[1];
+    if (c < 2) *reinterpret_cast<V *>(c ? dst[3] : dst[1]) = s;
+    if (c == CH - 1) *reinterpret_cast<uint32_t *>(dst[4]) = m;
+  }
+}
+
+template <class F>
+int launch_gather(F kernel, GatherParams &G, int rows, int64_t units, cudaStream_t st) {
+  const int64_t tiles = (G.keep + rows - 1) / rows;
+  if (units * tiles > 0x7fffffff) return KV4_ERR_UNSUPPORTED;
+  G.tiles = static_cast<int>(tiles);
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(units * tiles));
+  cfg.blockDim = dim3(256);
+  cfg.stream = st;
+  cudaLaunchAttribute at{};
+  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &at;
+  cfg.numAttrs = 1;
+  return cuda_status(cudaLaunchKernelEx(&cfg, kernel, G));
+}
+
+int run_gather(GatherParams &G, int64_t units, cudaStream_t st) {
+  const bool packed = G.vec[0] == 16 && G.vec[2] == 16 && G.bytes[0] == G.bytes[2];
+  const bool scales = G.bytes[1] == G.bytes[3] && G.vec[1] == G.bytes[1] && G.vec[3] == G.bytes[3];
+  if (packed && scales) {
+    if (G.bytes[0] == 64 && G.bytes[1] == 16) return launch_gather(evict_gather_fast<4, uint4>, G, 64, units, st);
+    if (G.bytes[0] == 64 && G.bytes[1] == 8) return launch_gather(evict_gather_fast<4, uint2>, G, 64, units, st);
+    if (G.bytes[0] == 64 && G.bytes[1] == 4) return launch_gather(evict_gather_fast<4, uint32_t>, G, 64, units, st);
+    if (G.bytes[0] == 64 && G.bytes[1] == 2) return launch_gather(evict_gather_fast<4, uint16_t>, G, 64, units, st);
+    if (G.bytes[0] == 32 && G.bytes[1] == 8) return launch_gather(evict_gather_fast<2, uint2>, G, 128, units, st);
+    if (G.bytes[0] == 32 && G.bytes[1] == 4) return launch_gather(evict_gather_fast<2, uint32_t>, G, 128, units, st);
+    if (G.bytes[0] == 32 && G.bytes[1] == 2) return launch_gather(evict_gather_fast<2, uint16_t>, G, 128, units, st);
+  }
+  return launch_gather(evict_gather, G, GROWS, units, st);
 }
 
 bool is_float(int dt) { return dt == KV4_F32 || dt == KV4_F16 || dt == KV4_BF16; }
@@ -372,15 +585,14 @@ extern "C" int kv4_evict(const kv4_tensor *k_packed, const kv4_tensor *k_scales,
       G.ss[k][i] = s->stride[at + i] * e;
       G.ds[k][i] = o->stride[at + i] * e;
     }
-    G.vec[k] = copy_width(G, k);
+    G.vec[k] = copy_width(G.dst[k], G.src[k], G.bytes[k], G.ds[k], G.ss[k]);
   }
   if (recent < 0 || sinks < 0 || keep < 0 || recent + sinks > keep || keep > S)
     return KV4_ERR_INVALID;
   if (S >= (int64_t(1) << 30)) return KV4_ERR_UNSUPPORTED;
   if (B == 0 || Hkv == 0 || keep == 0) return KV4_OK;
   if (!index) return KV4_ERR_INVALID;
-  const int64_t tiles = (keep + GROWS - 1) / GROWS;
-  if (B * Hkv * tiles > 0x7fffffff) return KV4_ERR_UNSUPPORTED;
+  if (B * Hkv > (int64_t(1) << 24)) return KV4_ERR_UNSUPPORTED;
   EvictParams E{};
   E.mass = static_cast<const float *>(score->data);
   for (int i = 0; i < 3; ++i) E.ms[i] = score->stride[i + 1];
@@ -391,13 +603,12 @@ extern "C" int kv4_evict(const kv4_tensor *k_packed, const kv4_tensor *k_scales,
   E.recent = static_cast<int>(recent);
   E.sinks = static_cast<int>(sinks);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  evict_select<<<static_cast<unsigned>(B * Hkv), SEL, 0, st>>>(E);
-  int rc = cuda_status(cudaGetLastError());
+  E.vec = (reinterpret_cast<uintptr_t>(E.mass) & 15u) == 0 && E.ms[2] == 1 && E.ms[0] % 4 == 0 &&
+          E.ms[1] % 4 == 0;
+  const int rc = run_select(E, B * Hkv, st);
   if (rc) return rc;
   G.index = index;
   G.Hkv = static_cast<int>(Hkv);
   G.keep = static_cast<int>(keep);
-  G.tiles = static_cast<int>(tiles);
-  evict_gather<<<static_cast<unsigned>(B * Hkv * tiles), 256, 0, st>>>(G);
-  return cuda_status(cudaGetLastError());
+  return run_gather(G, B * Hkv, st);
 }
