@@ -168,31 +168,33 @@ __global__ void tree_generic(const TreeParams P, const GenPlan L) {
 // One warp joins the partial rows of `parts` key ranges: ws_o [parts][rows][d]
 // unnormalised, ws_ml [parts][rows] (base-2 maximum, sum).
 template <int DC>
-__global__ void tree_merge(const TreeParams P, const GenPlan L) {
+__global__ void tree_merge(const __grid_constant__ TreeParams P, const GenPlan L) {
   const int lane = threadIdx.x & 31;
   const int64_t n = L.units * L.rows;
   const int64_t at = static_cast<int64_t>(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5);
+  griddep_wait();
   if (at >= n) return;
-  float m = -INFINITY;
-  for (int p = lane; p < L.parts; p += 32) m = fmaxf(m, P.ws_ml[p * n + at].x);
-  m = warp_max<1>(m);
-  const float base = m == -INFINITY ? 0.0f : m;
-  float l = 0.0f, acc[DC];
+  float m = -INFINITY, l = 0.0f, acc[DC];
 #pragma unroll
   for (int k = 0; k < DC; ++k) acc[k] = 0.0f;
 #pragma unroll 4
   for (int p = 0; p < L.parts; ++p) {
     const float2 ml = P.ws_ml[p * n + at];
-    const float f = exp2f(ml.x - base);
-    l = fmaf(f, ml.y, l);
+    float v[DC];
 #pragma unroll
     for (int k = 0; k < DC; ++k)
-      if (lane + 32 * k < P.d) acc[k] = fmaf(f, P.ws_o[(p * n + at) * P.d + lane + 32 * k], acc[k]);
+      v[k] = lane + 32 * k < P.d ? P.ws_o[(p * n + at) * P.d + lane + 32 * k] : 0.0f;
+    const float to = fmaxf(m, ml.x), base = to == -INFINITY ? 0.0f : to;
+    const float f = exp2f(m - base), g = exp2f(ml.x - base);
+    m = to;
+    l = fmaf(l, f, g * ml.y);
+#pragma unroll
+    for (int k = 0; k < DC; ++k) acc[k] = fmaf(acc[k], f, g * v[k]);
   }
   const int64_t unit = at / L.rows, b = unit / P.Hkv;
   const int row = static_cast<int>(at - unit * L.rows), i = row / P.R;
   const int h = static_cast<int>(unit - b * P.Hkv) * P.R + row - i * P.R;
-  const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+  const float inv = l > 0.0f ? 1.0f / l : (l == l ? 0.0f : l);
 #pragma unroll
   for (int k = 0; k < DC; ++k)
     if (lane + 32 * k < P.d)
@@ -203,7 +205,7 @@ __global__ void tree_merge(const TreeParams P, const GenPlan L) {
     if (P.stats) P.stats[at] = make_float2(m, inv);
     if (P.lse)
       P.lse[b * P.ls[0] + h * P.ls[1] + i * P.ls[2]] =
-          l > 0.0f ? (m + log2f(l)) * kBrLn2 : -INFINITY;
+          l == 0.0f ? -INFINITY : (m + log2f(l)) * kBrLn2;
   }
 }
 
@@ -232,6 +234,20 @@ int64_t gen_workspace(const TreeParams &P, const GenPlan &L) {
   return L.parts * L.units * L.rows * (static_cast<int64_t>(P.d) * 4 + 8);
 }
 
+template <int DC>
+int launch_merge(const TreeParams &P, const GenPlan &L, cudaStream_t st) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>((L.units * L.rows + 3) / 4));
+  cfg.blockDim = dim3(128);
+  cfg.stream = st;
+  cudaLaunchAttribute at{};
+  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &at;
+  cfg.numAttrs = 1;
+  return cuda_status(cudaLaunchKernelEx(&cfg, tree_merge<DC>, P, L));
+}
+
 template <int DC, int RW>
 int launch_gen(const TreeParams &P, const GenPlan &L, cudaStream_t st) {
   const int64_t blocks = (L.tasks + L.warps - 1) / L.warps;
@@ -242,11 +258,9 @@ int launch_gen(const TreeParams &P, const GenPlan &L, cudaStream_t st) {
     if (rc) return rc;
   }
   tree_generic<DC, RW><<<static_cast<unsigned>(blocks), 32 * L.warps, L.smem, st>>>(P, L);
-  int rc = cuda_status(cudaGetLastError());
+  const int rc = cuda_status(cudaGetLastError());
   if (rc || L.parts == 1) return rc;
-  const int64_t n = L.units * L.rows;
-  tree_merge<DC><<<static_cast<unsigned>((n + 3) / 4), 128, 0, st>>>(P, L);
-  return cuda_status(cudaGetLastError());
+  return launch_merge<DC>(P, L, st);
 }
 
 template <int DC>
@@ -325,25 +339,45 @@ int tree_fill(TreeParams &P, const kv4_tensor *q, const kv4_tensor *const cache[
   return KV4_OK;
 }
 
-bool tree_tc_takes(const TreeParams &P);  // branch_tc.cu
-int64_t tree_tc_workspace(const TreeParams &P);
+int tree_mma_parts(const TreeParams &P);  // branch_mma.cu
+int tree_mma_run(const TreeParams &P, cudaStream_t st);
+int branch_mma_take_device_error(int *v);
+int64_t tree_tc_workspace(const TreeParams &P);  // branch_tc.cu
 int tree_tc_run(TreeParams &P, void *workspace, int64_t bytes, cudaStream_t st);
 int branch_tc_take_device_error(int *v);
 int trim_tc_take_device_error(int *v);  // trim_tc.cu
 
+namespace {
+// what tree_merge has to know of a run of branch_mma.cu's kernel
+GenPlan mma_merge_plan(const TreeParams &P) {
+  GenPlan L{};
+  L.units = P.B * P.Hkv;
+  L.rows = P.R * P.nodes;
+  L.parts = tree_mma_parts(P);
+  return L;
+}
+}  // namespace
+
 int64_t tree_workspace(const TreeParams &P) {
+  if (tree_mma_takes(P)) return gen_workspace(P, mma_merge_plan(P));
   return tree_tc_takes(P) ? tree_tc_workspace(P) : gen_workspace(P, gen_plan(P));
 }
 
 int tree_run(TreeParams &P, void *workspace, int64_t bytes, cudaStream_t st) {
   if (P.B == 0 || P.nodes == 0) return KV4_OK;
-  if (tree_tc_takes(P)) return tree_tc_run(P, workspace, bytes, st);
-  const GenPlan L = gen_plan(P);
+  const bool mma = tree_mma_takes(P);
+  if (!mma && tree_tc_takes(P)) return tree_tc_run(P, workspace, bytes, st);
+  const GenPlan L = mma ? mma_merge_plan(P) : gen_plan(P);
   if (gen_workspace(P, L) > 0) {
     if (!workspace || bytes < gen_workspace(P, L)) return KV4_ERR_WORKSPACE;
     const int64_t n = L.parts * L.units * L.rows;
     P.ws_ml = static_cast<float2 *>(workspace);
     P.ws_o = static_cast<float *>(workspace) + 2 * n;
+  }
+  if (mma) {
+    const int rc = tree_mma_run(P, st);
+    if (rc || L.parts == 1) return rc;
+    return P.d == 64 ? launch_merge<2>(P, L, st) : launch_merge<4>(P, L, st);
   }
   if (P.d <= 64) return launch_gen_rw<2>(P, L, st);
   if (P.d <= 128) return launch_gen_rw<4>(P, L, st);
@@ -441,6 +475,9 @@ int branch_take_device_error(int *v) {
   *v |= t;
   t = 0;
   if (!rc) rc = trim_tc_take_device_error(&t);
+  *v |= t;
+  t = 0;
+  if (!rc) rc = branch_mma_take_device_error(&t);
   *v |= t;
   return rc;
 }

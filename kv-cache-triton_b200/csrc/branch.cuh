@@ -153,7 +153,9 @@ struct ScoreParams {
 };
 
 int score_run(const ScoreParams &P, cudaStream_t st);      // trim.cu: any layout
-bool score_tc_takes(const ScoreParams &P);                 // trim_tc.cu
-int score_tc_run(const ScoreParams &P, cudaStream_t st);
+bool tree_tc_takes(const TreeParams &P);                   // branch_tc.cu
+int score_tc_run(const ScoreParams &P, cudaStream_t st);   // trim_tc.cu
+bool tree_mma_takes(const TreeParams &P);                  // branch_mma.cu
+int score_mma_run(const ScoreParams &P, cudaStream_t st);
 
 }  // namespace kv4

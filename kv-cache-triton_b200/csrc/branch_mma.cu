@@ -1,0 +1,672 @@
+// Tree attention and the scores of cached tokens for few rows, and for half
+// precision: one warp, 16 rows and 16 keys at a time, all in registers.
+//
+// Single-token decoding and small trees have R to 16 rows per KV head; a
+// 128-row tensor-memory tile is mostly padding there and its operands have to
+// pass through shared memory.  Here (mma.m16n8k16, f16 operands, fp32 sums)
+//
+//   S = Q K^T   rows are M, keys N: a thread's packed words are its B operand
+//               as they are loaded: four codes' worth of shifts, the code bias
+//               taken off, no scale.  Scales multiply the fp32 sums of their
+//               group of columns, so scores are exact to fp32 rounding for any
+//               scale type.
+//   O += P V    the weights are the A operand in the registers where the scores
+//               were; V's B operand pairs the same column of two keys, so two
+//               keys' words are interleaved before they are taken apart, and
+//               values are codes times scale in f16 (exact for bf16 scales).
+//
+// Which columns a thread takes is free, as long as Q (or the output) follows:
+// thread t of four takes words t, 4 + t, ... of a row of K, thread g of eight
+// the g-th eighth of a row of V.
+//
+// A block of warps takes a range of one unit's keys, 16 keys per warp in turn;
+// its warps meet in shared memory, ranges of one unit in the workspace
+// (tree_merge of branch.cu).  The next step's loads are in flight during a step.
+// Bound: memory for one row tile; instructions (about 350 per warp and 16 keys
+// of 128 columns) are close behind.
+#include <algorithm>
+
+#include "branch.cuh"
+#include "tc_rows.cuh"
+
+namespace kv4 {
+
+// device error word of this file (folded into kv4_device_error)
+__device__ int g_branch_error_mma = 0;
+
+namespace {
+
+struct MmaPlan {
+  int64_t units;
+  int rows, row_tiles, parts;
+};
+
+constexpr int NW = 4;      // warps per block
+constexpr int BLOCKS = 3;  // per SM: 168 registers a thread
+constexpr float kShift = 7.0f;  // weights are written times 2^7 (see branch_tc.cu)
+
+template <typename ST>
+__device__ __forceinline__ float scale_of(uint16_t v);
+template <>
+__device__ __forceinline__ float scale_of<__nv_bfloat16>(uint16_t v) {
+  return __uint_as_float(static_cast<uint32_t>(v) << 16);
+}
+template <>
+__device__ __forceinline__ float scale_of<__half>(uint16_t v) {
+  return __half2float(__ushort_as_half(v));
+}
+// as f16 (bf16 scales past its range become infinite and are reported)
+template <typename ST>
+__device__ __forceinline__ uint32_t half_scale(uint16_t v) {
+  if (sizeof(ST) == 2 && DT<ST>::code == KV4_F16) return v;
+  return __half_as_ushort(__float2half_rn(scale_of<ST>(v)));
+}
+
+// A warp's 16 keys: K words [key tile of 8][32-column block], V words and the
+// scales of this thread's four keys 2t, 2t + 1, 2t + 8, 2t + 9
+template <int D, int G, bool WITH_V>
+struct Keys {
+  static constexpr int NB = D / 32, NG = D / G, VW = D / 64;
+  uint32_t k[2][NB];
+  uint32_t v[WITH_V ? 4 : 1][VW];
+  uint16_t ks[4][NG], vs[WITH_V ? 4 : 1];
+};
+
+template <int N>
+__device__ __forceinline__ void load_scales(uint16_t (&s)[N], const uint16_t *p) {
+  if (N == 4) {
+    const uint2 w = __ldg(reinterpret_cast<const uint2 *>(p));
+    s[0] = w.x & 0xffffu;
+    s[1 % N] = w.x >> 16;
+    s[2 % N] = w.y & 0xffffu;
+    s[3 % N] = w.y >> 16;
+  } else if (N == 2) {
+    const uint32_t w = __ldg(reinterpret_cast<const uint32_t *>(p));
+    s[0] = w & 0xffffu;
+    s[1 % N] = w >> 16;
+  } else {
+    s[0] = __ldg(p);
+  }
+}
+
+// Keys [k0, k0 + 16) of one source, of which those below `end` exist.
+template <int D, int G, bool WITH_V>
+__device__ __forceinline__ void load_keys(Keys<D, G, WITH_V> &x, const RowSource &S, int64_t b,
+                                          int h, int64_t k0, int64_t end, int lane) {
+  using K = Keys<D, G, WITH_V>;
+  const int g = lane >> 2, t = lane & 3;
+#pragma unroll
+  for (int n = 0; n < 2; ++n) {
+    const int64_t key = k0 + 8 * n + g;
+    const uint32_t *p =
+        reinterpret_cast<const uint32_t *>(S.kp + b * S.kps[0] + h * S.kps[1] + key * S.kps[2]) + t;
+#pragma unroll
+    for (int i = 0; i < K::NB; ++i) x.k[n][i] = key < end ? __ldg(p + 4 * i) : 0u;
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int64_t key = k0 + 2 * t + (j & 1) + 8 * (j >> 1);
+    const bool in = key < end;
+#pragma unroll
+    for (int i = 0; i < K::NG; ++i) x.ks[j][i] = 0;
+    if (in)
+      load_scales<K::NG>(x.ks[j], static_cast<const uint16_t *>(S.ks) + b * S.kss[0] +
+                                      h * S.kss[1] + key * S.kss[2]);
+    if (WITH_V) {
+#pragma unroll
+      for (int i = 0; i < K::VW; ++i) x.v[j][i] = 0u;
+      x.vs[j] = 0;
+      if (in) {
+        const uint8_t *p = S.vp + b * S.vps[0] + h * S.vps[1] + key * S.vps[2] + g * (D / 16);
+        if (K::VW == 2) {
+          const uint2 w = __ldg(reinterpret_cast<const uint2 *>(p));
+          x.v[j][0] = w.x;
+          x.v[j][K::VW - 1] = w.y;
+        } else {
+          x.v[j][0] = __ldg(reinterpret_cast<const uint32_t *>(p));
+        }
+        x.vs[j] = __ldg(static_cast<const uint16_t *>(S.vs) + b * S.vss[0] + h * S.vss[1] +
+                        key * S.vss[2] + g * (D / 8) / G);
+      }
+    }
+  }
+}
+
+// A operand of 16 (or 8) rows of q, in the column order of the K words, and the
+// factor of rows g and g + 8 from sums to base-2 exponents.  bf16 rows are
+// scaled by a power of two so that their largest element lies in
+// [2^13, 2^14): exact, as are f16 rows as they are.
+template <int D, bool HALF>
+struct Query {
+  uint32_t a[D / 16][HALF ? 2 : 4];
+  float c[HALF ? 1 : 2];
+};
+template <int D, bool HALF>
+__device__ __forceinline__ void load_query(Query<D, HALF> &Q, const TreeParams &T, int64_t b, int kvh,
+                                           int row0, int rows, int lane) {
+  const int g = lane >> 2, t = lane & 3;
+#pragma unroll
+  for (int r = 0; r < (HALF ? 1 : 2); ++r) {
+    const int row = row0 + g + 8 * r, node = row / T.R, head = kvh * T.R + row - node * T.R;
+    const uint16_t *q = static_cast<const uint16_t *>(T.q) + b * T.qs[0] + head * T.qs[1] + node * T.qs[2] + 8 * t;
+    uint4 w[D / 32];
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i)
+      w[i] = row < rows ? __ldg(reinterpret_cast<const uint4 *>(q + 32 * i)) : make_uint4(0, 0, 0, 0);
+    Q.c[r] = T.scale_log2;
+    float up = 1.0f;
+    const bool bf = T.q_dtype == KV4_BF16;
+    if (bf) {
+      uint32_t top = 0;
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i) {
+        const uint32_t u[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) top = max(top, max(u[e] & 0x7FFFu, (u[e] >> 16) & 0x7FFFu));
+      }
+      top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      int ex = 13 - (static_cast<int>(top >> 7) - 127);
+      ex = top == 0 ? 0 : min(max(ex, -126), 126);
+      up = __uint_as_float(static_cast<uint32_t>(ex + 127) << 23);
+      Q.c[r] *= __uint_as_float(static_cast<uint32_t>(127 - ex) << 23);
+    }
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) {
+      const uint32_t u[4] = {w[i].x, w[i].y, w[i].z, w[i].w};  // columns 8t .. 8t + 7 of the block
+      uint32_t p[4];                                          // pairs (0,4) (1,5) (2,6) (3,7)
+      if (bf) {
+        p[0] = pack_f16x2(bf16lo_to_f32(u[0]) * up, bf16lo_to_f32(u[2]) * up);
+        p[1] = pack_f16x2(bf16hi_to_f32(u[0]) * up, bf16hi_to_f32(u[2]) * up);
+        p[2] = pack_f16x2(bf16lo_to_f32(u[1]) * up, bf16lo_to_f32(u[3]) * up);
+        p[3] = pack_f16x2(bf16hi_to_f32(u[1]) * up, bf16hi_to_f32(u[3]) * up);
+      } else {
+        p[0] = prmt(u[0], u[2], 0x5410);
+        p[1] = prmt(u[0], u[2], 0x7632);
+        p[2] = prmt(u[1], u[3], 0x5410);
+        p[3] = prmt(u[1], u[3], 0x7632);
+      }
+      // k-step 2i: pairs 0 and 1; k-step 2i + 1: pairs 2 and 3
+      if (HALF) {
+        Q.a[2 * i][0] = p[0];
+        Q.a[2 * i][1] = p[1];
+        Q.a[2 * i + 1][0] = p[2];
+        Q.a[2 * i + 1][1] = p[3];
+      } else {
+        Q.a[2 * i][r] = p[0];
+        Q.a[2 * i][(HALF ? 0 : 2) + r] = p[1];
+        Q.a[2 * i + 1][r] = p[2];
+        Q.a[2 * i + 1][(HALF ? 0 : 2) + r] = p[3];
+      }
+    }
+  }
+}
+
+// f16 pairs (code - 8) of a word's nibbles e and e + 4
+__device__ __forceinline__ uint32_t code_pair(uint32_t w, int e) {
+  return tc::hsub2(tc::nib_pair(w >> (4 * e)), 0x64086408u);
+}
+
+// Sums of rows g (s[0], s[1]) and g + 8 (s[2], s[3]) with keys 2t, 2t + 1 of
+// key tile n, scaled group by group.
+template <int D, int G, typename ST, bool HALF, bool WITH_V>
+__device__ __forceinline__ void scores(float (&s)[4], const Query<D, HALF> &Q,
+                                       const Keys<D, G, WITH_V> &x, int n) {
+  s[0] = s[1] = s[2] = s[3] = 0.0f;
+#pragma unroll
+  for (int gr = 0; gr < D / G; ++gr) {
+    float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int i = 0; i < G / 32; ++i) {
+      const int blk = gr * (G / 32) + i;
+      const uint32_t w = x.k[n][blk];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const uint32_t *a = Q.a[2 * blk + j];
+        mma_f16_16816(c, a[0], HALF ? 0u : a[HALF ? 0 : 1], a[HALF ? 1 : 2], HALF ? 0u : a[HALF ? 0 : 3],
+                      code_pair(w, 2 * j), code_pair(w, 2 * j + 1));
+      }
+    }
+    const float k0 = scale_of<ST>(x.ks[2 * n][gr]), k1 = scale_of<ST>(x.ks[2 * n + 1][gr]);
+    s[0] = fmaf(c[0], k0, s[0]);
+    s[1] = fmaf(c[1], k1, s[1]);
+    if (!HALF) {
+      s[2] = fmaf(c[2], k0, s[2]);
+      s[3] = fmaf(c[3], k1, s[3]);
+    }
+  }
+}
+
+// which of a thread's four keys row `node` sees, as bits j (order of Keys)
+__device__ __forceinline__ uint32_t seen_keys(const TreeParams &T, int64_t b, bool draft, int node,
+                                              bool row_ok, int64_t k0, int64_t end, int t) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int64_t key = k0 + 2 * t + (j & 1) + 8 * (j >> 1);
+    bool on = row_ok && key < end;
+    if (on && draft) on = draft_visible(T, b, node, static_cast<int>(key));
+    m |= on ? 1u << j : 0u;
+  }
+  return m;
+}
+
+template <int D, int G, typename ST, bool HALF>
+__global__ void __launch_bounds__(NW * 32, BLOCKS)
+    tree_mma(const __grid_constant__ TreeParams T, const MmaPlan L) {
+  constexpr int NR = HALF ? 8 : 16, RT = HALF ? 1 : 2, DG = D / 8, LD = D + 4;
+  extern __shared__ __align__(16) float msm[];  // [NW][NR][LD] outputs, [NW][NR] float2 (m, l)
+  float2 *sml = reinterpret_cast<float2 *>(msm + NW * NR * LD);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+  const int part = static_cast<int>(blockIdx.x % L.parts);
+  const int64_t ur = blockIdx.x / L.parts;
+  const int rt = static_cast<int>(ur % L.row_tiles), row0 = rt * NR;
+  const int64_t unit = ur / L.row_tiles, b = unit / T.Hkv;
+  const int kvh = static_cast<int>(unit - b * T.Hkv);
+  const int64_t len = context_len(T, b, part == 0 && rt == 0 && kvh == 0 && threadIdx.x == 0 ? &g_branch_error_mma : nullptr);
+  const int nctx = static_cast<int>((len + 15) >> 4), steps = nctx + ((T.ndraft + 15) >> 4);
+  const int per = (steps + L.parts - 1) / L.parts;
+  const int s0 = part * per, s1 = min(steps, s0 + per);
+
+  Keys<D, G, true> cur;
+  auto fetch = [&](int s) {
+    if (s < nctx) load_keys(cur, T.cache, b, kvh, static_cast<int64_t>(s) * 16, len, lane);
+    else load_keys(cur, T.draft, b, kvh, static_cast<int64_t>(s - nctx) * 16, T.ndraft, lane);
+  };
+  int s = s0 + warp;
+  if (s < s1) fetch(s);
+  Query<D, HALF> Q;
+  load_query(Q, T, b, kvh, row0, L.rows, lane);
+  int node[RT];
+  bool ok[RT];
+  float m[RT], l[RT];
+  bool broken[RT];
+  float o[DG][HALF ? 2 : 4];
+#pragma unroll
+  for (int r = 0; r < RT; ++r) {
+    const int row = row0 + g + 8 * r;
+    ok[r] = row < L.rows;
+    node[r] = row / T.R;
+    m[r] = -INFINITY;
+    l[r] = 0.0f;
+    broken[r] = false;
+  }
+#pragma unroll
+  for (int j = 0; j < DG; ++j)
+#pragma unroll
+    for (int e = 0; e < (HALF ? 2 : 4); ++e) o[j][e] = 0.0f;
+  bool big = false;
+
+#pragma unroll 1
+  for (; s < s1; s += NW) {
+    const bool draft = s >= nctx;
+    const int64_t k0 = static_cast<int64_t>(draft ? s - nctx : s) * 16, end = draft ? T.ndraft : len;
+    float x[2][4];
+    scores<D, G, ST, HALF>(x[0], Q, cur, 0);
+    scores<D, G, ST, HALF>(x[1], Q, cur, 1);
+    // V of this step out of the way of the next step's loads
+    uint32_t vw[4][Keys<D, G, true>::VW];
+    uint16_t vs[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+#pragma unroll
+      for (int i = 0; i < Keys<D, G, true>::VW; ++i) vw[j][i] = cur.v[j][i];
+      vs[j] = cur.vs[j];
+    }
+    if (s + NW < s1) fetch(s + NW);
+
+    // scores -> weights, in place
+#pragma unroll
+    for (int r = 0; r < RT; ++r) {
+      float y[4] = {x[0][2 * r], x[0][2 * r + 1], x[1][2 * r], x[1][2 * r + 1]};
+      if (draft || k0 + 16 > end) {
+        const uint32_t on = seen_keys(T, b, draft, node[r], ok[r], k0, end, t);
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (!(on >> j & 1u)) y[j] = -INFINITY;
+        if (draft) {  // a visible key without a usable V scale: the row has no value
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const bool bad = !(fabsf(scale_of<ST>(vs[j])) <= tc::kMaxScale);
+            const uint32_t any = __ballot_sync(0xffffffffu, bad) & (0x11111111u << t);
+            if (any && (on >> j & 1u)) broken[r] = true;
+          }
+        }
+      }
+      float mx = fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3])) * Q.c[r];
+      // the maximum moves only when a score passes it by more than 8: seldom
+      if (__any_sync(0xffffffffu, mx > m[r] + 8.0f)) {
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+        const float to = mx > m[r] + 8.0f ? mx : m[r];
+        const float alpha = to == m[r] ? 1.0f : m[r] == -INFINITY ? 0.0f : fast_exp2(m[r] - to);
+        m[r] = to;
+        l[r] *= alpha;
+#pragma unroll
+        for (int j = 0; j < DG; ++j) {
+          o[j][2 * r] *= alpha;
+          o[j][2 * r + 1] *= alpha;
+        }
+      }
+      const float base = m[r] == -INFINITY ? 0.0f : m[r] - kShift;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) y[j] = fast_exp2(fmaf(y[j], Q.c[r], -base));
+      l[r] += (y[0] + y[1]) + (y[2] + y[3]);
+      x[0][2 * r] = y[0];
+      x[0][2 * r + 1] = y[1];
+      x[1][2 * r] = y[2];
+      x[1][2 * r + 1] = y[3];
+    }
+    const uint32_t a0 = pack_f16x2(x[0][0], x[0][1]), a2 = pack_f16x2(x[1][0], x[1][1]);
+    const uint32_t a1 = HALF ? 0u : pack_f16x2(x[0][2], x[0][3]);
+    const uint32_t a3 = HALF ? 0u : pack_f16x2(x[1][2], x[1][3]);
+
+    // O += P V: column j of this thread's eighth, keys in pairs
+    uint32_t sp[2];
+#pragma unroll
+    for (int p = 0; p < 2; ++p) {
+      uint32_t lo = half_scale<ST>(vs[2 * p]), hi = half_scale<ST>(vs[2 * p + 1]);
+      const bool b0 = !(fabsf(scale_of<ST>(vs[2 * p])) <= tc::kMaxScale);
+      const bool b1 = !(fabsf(scale_of<ST>(vs[2 * p + 1])) <= tc::kMaxScale);
+      big |= b0 || b1;
+      if (draft) {  // rows that see such a key are marked above
+        if (b0) lo = 0;
+        if (b1) hi = 0;
+      }
+      sp[p] = lo | hi << 16;
+    }
+#pragma unroll
+    for (int i = 0; i < Keys<D, G, true>::VW; ++i) {
+      uint32_t y[2][2];  // [key pair][half word]: the pair's words side by side
+#pragma unroll
+      for (int p = 0; p < 2; ++p) {
+        y[p][0] = prmt(vw[2 * p][i], vw[2 * p + 1][i], 0x5410);
+        y[p][1] = prmt(vw[2 * p][i], vw[2 * p + 1][i], 0x7632);
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const uint32_t b0 = tc::hmul2(code_pair(y[0][e >> 2], e & 3), sp[0]);
+        const uint32_t b1 = tc::hmul2(code_pair(y[1][e >> 2], e & 3), sp[1]);
+        float *c = o[8 * i + e];
+        if (HALF) {
+          float d[4];
+          mma_f16_16816_c(d, a0, 0u, a2, 0u, b0, b1, c[0], c[1], 0.0f, 0.0f);
+          c[0] = d[0];
+          c[1] = d[1];
+        } else {
+          mma_f16_16816(*reinterpret_cast<float(*)[4]>(c), a0, a1, a2, a3, b0, b1);
+        }
+      }
+    }
+  }
+  if (big) atomicOr(&g_branch_error_mma, DEV_ERR_F16_RANGE);
+
+  // ---- the block's warps meet ----
+#pragma unroll
+  for (int r = 0; r < RT; ++r) {
+    l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
+    l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
+    const uint32_t bad = __ballot_sync(0xffffffffu, broken[r]);
+    if (bad & (0xFu << (4 * g))) l[r] = __uint_as_float(0x7fc00000u);
+    const int at = warp * NR + g + 8 * r;
+    if (t == 0) sml[at] = make_float2(m[r] - kShift, l[r]);
+    // columns 2t and 2t + 1 of output tile j are dims 2t * DG + j and (2t + 1) * DG + j
+#pragma unroll
+    for (int j = 0; j < DG; ++j) {
+      msm[at * LD + 2 * t * DG + j] = o[j][2 * r];
+      msm[at * LD + (2 * t + 1) * DG + j] = o[j][2 * r + 1];
+    }
+  }
+  __syncthreads();
+  const int nr = min(NR, L.rows - row0);
+  for (int idx = threadIdx.x; idx < nr * (D / 2); idx += NW * 32) {
+    const int r = idx / (D / 2), c = (idx - r * (D / 2)) * 2, row = row0 + r;
+    float M = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) M = fmaxf(M, sml[w * NR + r].x);
+    const float base = M == -INFINITY ? 0.0f : M;
+    float sum = 0.0f, v0 = 0.0f, v1 = 0.0f;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) {
+      const float2 ml = sml[w * NR + r];
+      const float f = exp2f(ml.x - base);
+      sum = fmaf(ml.y, f, sum);
+      const float2 v = *reinterpret_cast<const float2 *>(msm + (w * NR + r) * LD + c);
+      v0 = fmaf(v.x, f, v0);
+      v1 = fmaf(v.y, f, v1);
+    }
+    const int64_t at = unit * L.rows + row;
+    if (L.parts > 1) {
+      const int64_t slot = static_cast<int64_t>(part) * L.units * L.rows + at;
+      *reinterpret_cast<float2 *>(T.ws_o + slot * D + c) = make_float2(v0, v1);
+      if (c == 0) T.ws_ml[slot] = make_float2(M, sum);
+      continue;
+    }
+    const int nd = row / T.R, head = kvh * T.R + row - nd * T.R;
+    const float inv = sum > 0.0f ? 1.0f / sum : (sum == sum ? 0.0f : sum);
+    const int64_t off = b * T.os[0] + head * T.os[1] + nd * T.os[2] + c;
+    *reinterpret_cast<uint32_t *>(static_cast<uint16_t *>(T.out) + off) =
+        T.q_dtype == KV4_BF16 ? pack_bf16x2(v0 * inv, v1 * inv) : pack_f16x2(v0 * inv, v1 * inv);
+    if (c == 0) {
+      if (T.stats) T.stats[at] = make_float2(M, inv);
+      if (T.lse)
+        T.lse[b * T.ls[0] + head * T.ls[1] + nd * T.ls[2]] =
+            sum == 0.0f ? -INFINITY : (M + log2f(sum)) * kBrLn2;
+    }
+  }
+}
+
+// Scores of the cached tokens: weights formed again from K, the rows' maxima and
+// sums, summed over the rows of each key (rows are lanes: three shuffles).
+template <int D, int G, typename ST, bool HALF>
+__global__ void __launch_bounds__(NW * 32, HALF ? 4 : BLOCKS)
+    score_mma(const __grid_constant__ ScoreParams P, int rows, int64_t steps_per_unit, int64_t total) {
+  constexpr int RT = HALF ? 1 : 2, NR = HALF ? 8 : 16;
+  const TreeParams &T = P.t;
+  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int64_t warps = static_cast<int64_t>(gridDim.x) * NW;
+  const int64_t w = static_cast<int64_t>(blockIdx.x) * NW + (threadIdx.x >> 5);
+  // warps take runs of one unit's 16-key steps
+  const int64_t each = total / warps, rest = total - each * warps;
+  int64_t at = w * each + min(w, rest);
+  const int64_t stop = at + each + (w < rest ? 1 : 0);
+  const int64_t nctx = (T.S + 15) >> 4;
+  griddep_wait();  // the rows' maxima and sums come from the kernel before
+#pragma unroll 1
+  while (at < stop) {
+    const int64_t unit = at / steps_per_unit, b = unit / T.Hkv;
+    const int kvh = static_cast<int>(unit - b * T.Hkv);
+    const int64_t first = at - unit * steps_per_unit, last = min(steps_per_unit, first + stop - at);
+    at += last - first;
+    const float *in = P.in + b * P.is[0] + kvh * P.is[1];
+    float *out = P.out + b * P.os[0] + kvh * P.os[1];
+#pragma unroll 1
+    for (int row0 = 0; row0 < rows; row0 += NR) {
+      Query<D, HALF> Q;
+      load_query(Q, T, b, kvh, row0, rows, lane);
+      float sm[RT], sl[RT];  // maximum and 1 / sum of rows g, g + 8
+      int node[RT];
+#pragma unroll
+      for (int r = 0; r < RT; ++r) {
+        const int row = row0 + g + 8 * r;
+        const float2 st = row < rows ? T.stats[unit * rows + row] : make_float2(0.0f, 0.0f);
+        sm[r] = st.x;
+        sl[r] = st.y;  // 0: a row that saw nothing, or none at all
+        node[r] = row / T.R;
+      }
+      Keys<D, G, false> cur;
+      auto fetch = [&](int64_t s) {
+        if (s < nctx) load_keys(cur, T.cache, b, kvh, s * 16, T.S, lane);
+        else load_keys(cur, T.draft, b, kvh, (s - nctx) * 16, T.ndraft, lane);
+      };
+      fetch(first);
+#pragma unroll 1
+      for (int64_t s = first; s < last; ++s) {
+        const bool draft = s >= nctx;
+        const int64_t k0 = (draft ? s - nctx : s) * 16, end = draft ? T.ndraft : T.S;
+        // lanes 0-15 end up with a key each
+        const int64_t mine = k0 + lane, tok = draft ? T.S + mine : mine;
+        float old = 0.0f;
+        if (lane < 16 && mine < end) old = row0 == 0 ? in[tok * P.is[2]] * P.decay : out[tok * P.os[2]];
+        float x[2][4];
+        scores<D, G, ST, HALF>(x[0], Q, cur, 0);
+        scores<D, G, ST, HALF>(x[1], Q, cur, 1);
+        if (s + 1 < last) fetch(s + 1);
+        float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int r = 0; r < RT; ++r) {
+          const float y[4] = {x[0][2 * r], x[0][2 * r + 1], x[1][2 * r], x[1][2 * r + 1]};
+          const uint32_t on = draft ? seen_keys(T, b, true, node[r], true, k0, end, t) : 0xFu;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float v = fast_exp2(fmaf(y[j], Q.c[r], -sm[r])) * sl[r];
+            if ((on >> j & 1u) && sl[r] != 0.0f) sum[j] += v;
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+#pragma unroll
+          for (int d = 4; d < 32; d <<= 1) sum[j] += __shfl_xor_sync(0xffffffffu, sum[j], d);
+        }
+        // key 8n + 2t + i of this step is sum[2n + i] of lanes with that t
+        const int src = (lane & 7) >> 1;
+        float v[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = __shfl_sync(0xffffffffu, sum[j], src);
+        const float add = lane < 8 ? (lane & 1 ? v[1] : v[0]) : (lane & 1 ? v[3] : v[2]);
+        if (lane < 16 && mine < end) out[tok * P.os[2]] = old + add;
+      }
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// host side
+// ---------------------------------------------------------------------------
+bool half_rows(int rows) { return rows <= 8; }
+
+MmaPlan mma_plan(const TreeParams &T) {
+  MmaPlan L{};
+  L.rows = T.R * T.nodes;
+  const int nr = half_rows(L.rows) ? 8 : 16;
+  L.row_tiles = (L.rows + nr - 1) / nr;
+  L.units = T.B * T.Hkv;
+  // one wave of blocks, each warp at least two steps of 16 keys
+  const int64_t steps = (T.S + 15) / 16 + (T.ndraft + 15) / 16, have = L.units * L.row_tiles;
+  const int64_t room = static_cast<int64_t>(sm_count()) * BLOCKS;
+  const int64_t most = std::max<int64_t>(1, steps / (2 * NW));
+  L.parts = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({room / have, most, 64})));
+  return L;
+}
+
+template <int D, int G, typename ST, bool HALF>
+int launch_tree(const TreeParams &T, const MmaPlan &L, cudaStream_t st) {
+  constexpr int NR = HALF ? 8 : 16;
+  constexpr int smem = NW * NR * ((D + 4) * 4 + 8);
+  static bool configured[64] = {};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) dev = 0;
+  if (!configured[dev]) {
+    const int rc = cuda_status(cudaFuncSetAttribute(
+        tree_mma<D, G, ST, HALF>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    if (rc) return rc;
+    configured[dev] = true;
+  }
+  const int64_t blocks = L.units * L.row_tiles * L.parts;
+  if (blocks > 0x7fffffff) return KV4_ERR_UNSUPPORTED;
+  tree_mma<D, G, ST, HALF><<<static_cast<unsigned>(blocks), NW * 32, smem, st>>>(T, L);
+  return cuda_status(cudaGetLastError());
+}
+
+template <int D, int G, typename ST, bool HALF>
+int launch_score(const ScoreParams &P, int rows, cudaStream_t st) {
+  const int64_t steps = (P.t.S + 15) / 16 + (P.t.ndraft + 15) / 16, total = P.t.B * P.t.Hkv * steps;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(
+      std::min<int64_t>(static_cast<int64_t>(sm_count()) * (HALF ? 4 : BLOCKS), (total + NW - 1) / NW)));
+  cfg.blockDim = dim3(NW * 32);
+  cfg.stream = st;
+  cudaLaunchAttribute at{};
+  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &at;
+  cfg.numAttrs = 1;
+  return cuda_status(cudaLaunchKernelEx(&cfg, score_mma<D, G, ST, HALF>, P, rows, steps, total));
+}
+
+// f(integral D, integral G, ST{}, bool HALF)
+template <class F>
+int by_shape(const TreeParams &T, F f) {
+  auto type = [&](auto d, auto g) {
+    auto half = [&](auto st) {
+      if (half_rows(T.R * T.nodes)) return f(d, g, st, std::true_type{});
+      return f(d, g, st, std::false_type{});
+    };
+    return T.s_dtype == KV4_BF16 ? half(__nv_bfloat16{}) : half(__half{});
+  };
+  if (T.d == 64) {
+    if (T.G == 32) return type(std::integral_constant<int, 64>{}, std::integral_constant<int, 32>{});
+    return type(std::integral_constant<int, 64>{}, std::integral_constant<int, 64>{});
+  }
+  if (T.G == 32) return type(std::integral_constant<int, 128>{}, std::integral_constant<int, 32>{});
+  if (T.G == 64) return type(std::integral_constant<int, 128>{}, std::integral_constant<int, 64>{});
+  return type(std::integral_constant<int, 128>{}, std::integral_constant<int, 128>{});
+}
+
+bool scales_ok(const RowSource &S, int64_t B, int Hkv, int64_t T, int bytes) {
+  if (T == 0) return true;
+  const int e = bytes / 2;  // elements of a row: a power of two
+  if ((reinterpret_cast<uintptr_t>(S.ks) & (bytes - 1))) return false;
+  if (S.kss[3] != 1 || S.vss[3] != 1 || S.kss[2] % e || (Hkv > 1 && S.kss[1] % e) ||
+      (B > 1 && S.kss[0] % e))
+    return false;
+  return (reinterpret_cast<uintptr_t>(S.vs) & 1u) == 0;
+}
+
+}  // namespace
+
+// Whether the kernels of this file take the call: 16-bit queries and scales, the
+// sizes they are built for, rows that aligned loads can read; and either so few
+// rows that branch_tc.cu's tiles would be mostly padding, or half precision
+// somewhere, which that file leaves alone (a product of a code and an f16 scale
+// does not fit an f16).
+bool tree_mma_takes(const TreeParams &T) {
+  if ((T.q_dtype != KV4_BF16 && T.q_dtype != KV4_F16) || (T.s_dtype != KV4_BF16 && T.s_dtype != KV4_F16))
+    return false;
+  if (T.d != 64 && T.d != 128) return false;
+  if ((T.G != 32 && T.G != 64 && T.G != 128) || T.G > T.d) return false;
+  if (!rows_ok(T.cache, T.B, T.Hkv, T.S) || !rows_ok(T.draft, T.B, T.Hkv, T.ndraft)) return false;
+  const int bytes = 2 * T.d / T.G;
+  if (!scales_ok(T.cache, T.B, T.Hkv, T.S, bytes) || !scales_ok(T.draft, T.B, T.Hkv, T.ndraft, bytes))
+    return false;
+  if (!al16(T.q) || !al16(T.out) || T.qs[3] != 1 || T.os[3] != 1) return false;
+  const int64_t n[3] = {T.B, static_cast<int64_t>(T.Hkv) * T.R, T.nodes};
+  for (int i = 0; i < 3; ++i)
+    if (n[i] > 1 && (T.qs[i] % 8 || T.os[i] % 8)) return false;
+  return T.R * T.nodes <= 16 || !tree_tc_takes(T);
+}
+
+int tree_mma_parts(const TreeParams &T) { return mma_plan(T).parts; }
+
+int tree_mma_run(const TreeParams &T, cudaStream_t st) {
+  const MmaPlan L = mma_plan(T);
+  return by_shape(T, [&](auto d, auto g, auto s, auto half) {
+    return launch_tree<decltype(d)::value, decltype(g)::value, decltype(s), decltype(half)::value>(T, L, st);
+  });
+}
+
+int score_mma_run(const ScoreParams &P, cudaStream_t st) {
+  return by_shape(P.t, [&](auto d, auto g, auto s, auto half) {
+    return launch_score<decltype(d)::value, decltype(g)::value, decltype(s), decltype(half)::value>(
+        P, P.t.R * P.t.nodes, st);
+  });
+}
+
+int branch_mma_take_device_error(int *v) {
+  int zero = 0;
+  int rc = cuda_status(cudaMemcpyFromSymbol(v, g_branch_error_mma, sizeof(int)));
+  if (rc) return rc;
+  return cuda_status(cudaMemcpyToSymbol(g_branch_error_mma, &zero, sizeof(int)));
+}
+
+}  // namespace kv4

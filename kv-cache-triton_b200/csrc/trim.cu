@@ -8,8 +8,8 @@
 // The weights are known only when a row's maximum and sum are, so the keys are
 // read twice: the attention leaves (maximum, 1 / sum) of each row, and
 // score_generic forms the weights again, a key per lane, summed over the rows
-// in a fixed order (no atomics: two calls give the same bits).  bf16 queries
-// over bf16 scales take trim_tc.cu's kernel where the layout allows.
+// in a fixed order (no atomics: two calls give the same bits).  16-bit types
+// take the kernels of branch_mma.cu and trim_tc.cu where the layout allows.
 //
 // Eviction cuts each (sequence, KV head) to `keep` tokens: the first `sinks`,
 // the last `recent` and, of the rest, those with the highest score (equal
@@ -375,11 +375,12 @@ int launch_select(const EvictParams &E, int64_t units, int ranks, cudaStream_t s
 }
 
 // Blocks of 1024 threads, up to 16 tokens a thread and 8 blocks a row.  Few
-// rows: more blocks each, while 4 tokens a thread and two blocks per SM remain.
+// rows: more blocks each, while 4 tokens a thread and an SM for each block remain
+// (128 rows of 16K: one block a row takes 14.7 us, two 21.3, four 46).
 int run_select(const EvictParams &E, int64_t units, cudaStream_t st) {
   int ranks = 1;
   while (ranks < 8 && E.S > static_cast<int64_t>(ranks) * SEL * 16) ranks *= 2;
-  while (ranks < 8 && E.S > static_cast<int64_t>(ranks) * SEL * 4 && units * ranks * 2 <= 2 * 148)
+  while (ranks < 8 && E.S > static_cast<int64_t>(ranks) * SEL * 4 && units * ranks * 2 <= 148)
     ranks *= 2;
   const int64_t per = (E.S + static_cast<int64_t>(ranks) * SEL - 1) / (static_cast<int64_t>(ranks) * SEL);
   if (per <= 4) return launch_select<4>(E, units, ranks, st);
@@ -549,7 +550,11 @@ extern "C" int kv4_scored_attention(const kv4_tensor *q, const kv4_tensor *k_pac
   rc = tree_run(P.t, static_cast<char *>(workspace) + sb,
                 static_cast<int64_t>(workspace_bytes) - sb, st);
   if (rc) return rc;
-  return score_tc_takes(P) ? score_tc_run(P, st) : score_run(P, st);
+  if (P.keys > 0 && P.t.B > 0 && P.t.nodes > 0) {
+    if (tree_mma_takes(P.t)) return score_mma_run(P, st);
+    if (tree_tc_takes(P.t)) return score_tc_run(P, st);
+  }
+  return score_run(P, st);
 }
 
 extern "C" int kv4_evict(const kv4_tensor *k_packed, const kv4_tensor *k_scales,

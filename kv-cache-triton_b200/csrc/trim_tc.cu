@@ -359,14 +359,8 @@ int launch_score(const STcParams &P, cudaStream_t st) {
 
 }  // namespace
 
-bool tree_tc_takes(const TreeParams &T);
-
-// The same calls that tree_tc takes (its statistics are in terms of this
-// file's operands as well), with at least one row.
-bool score_tc_takes(const ScoreParams &P) {
-  return tree_tc_takes(P.t) && P.t.B > 0 && P.t.nodes > 0 && P.keys > 0;
-}
-
+// For the calls that tree_tc takes, with at least one row and one key (the rows'
+// statistics are in terms of the same operands).
 int score_tc_run(const ScoreParams &S, cudaStream_t st) {
   STcParams P = score_plan(S);
   const int64_t total = S.t.B * S.t.Hkv * P.tiles;
