@@ -45,89 +45,80 @@ constexpr int NW = 4;      // warps per block
 constexpr int BLOCKS = 3;  // per SM: 168 registers a thread
 constexpr float kShift = 7.0f;  // weights are written times 2^7 (see branch_tc.cu)
 
+// scale i of a packed row of 16-bit scales
 template <typename ST>
-__device__ __forceinline__ float scale_of(uint16_t v);
-template <>
-__device__ __forceinline__ float scale_of<__nv_bfloat16>(uint16_t v) {
-  return __uint_as_float(static_cast<uint32_t>(v) << 16);
-}
-template <>
-__device__ __forceinline__ float scale_of<__half>(uint16_t v) {
-  return __half2float(__ushort_as_half(v));
-}
-// as f16 (bf16 scales past its range become infinite and are reported)
-template <typename ST>
-__device__ __forceinline__ uint32_t half_scale(uint16_t v) {
-  if (sizeof(ST) == 2 && DT<ST>::code == KV4_F16) return v;
-  return __half_as_ushort(__float2half_rn(scale_of<ST>(v)));
+__device__ __forceinline__ float scale_at(const uint32_t *w, int i) {
+  if (DT<ST>::code == KV4_BF16) return i & 1 ? bf16hi_to_f32(w[i >> 1]) : bf16lo_to_f32(w[i >> 1]);
+  return i & 1 ? f16hi_to_f32(w[i >> 1]) : f16lo_to_f32(w[i >> 1]);
 }
 
 // A warp's 16 keys: K words [key tile of 8][32-column block], V words and the
-// scales of this thread's four keys 2t, 2t + 1, 2t + 8, 2t + 9
+// scales (K's of all groups, V's of the thread's columns) of this thread's four
+// keys 2t, 2t + 1, 2t + 8, 2t + 9
 template <int D, int G, bool WITH_V>
 struct Keys {
-  static constexpr int NB = D / 32, NG = D / G, VW = D / 64;
+  static constexpr int NB = D / 32, NG = D / G, VW = D / 64, SW = (NG + 1) / 2;
   uint32_t k[2][NB];
   uint32_t v[WITH_V ? 4 : 1][VW];
-  uint16_t ks[4][NG], vs[WITH_V ? 4 : 1];
+  uint32_t ks[4][SW], vs[WITH_V ? 4 : 1];
 };
 
-template <int N>
-__device__ __forceinline__ void load_scales(uint16_t (&s)[N], const uint16_t *p) {
-  if (N == 4) {
-    const uint2 w = __ldg(reinterpret_cast<const uint2 *>(p));
-    s[0] = w.x & 0xffffu;
-    s[1 % N] = w.x >> 16;
-    s[2 % N] = w.y & 0xffffu;
-    s[3 % N] = w.y >> 16;
-  } else if (N == 2) {
-    const uint32_t w = __ldg(reinterpret_cast<const uint32_t *>(p));
-    s[0] = w & 0xffffu;
-    s[1 % N] = w >> 16;
-  } else {
-    s[0] = __ldg(p);
-  }
+// Where a lane's first words of key 0 lie; rows follow one another without gaps
+// (D / 2 bytes of codes, D / G scales), so that everything else is a constant
+// offset from there.
+struct Place {
+  const uint8_t *k, *v;
+  const uint16_t *ks, *vs;
+};
+template <int D, int G>
+__device__ __forceinline__ Place place_of(const RowSource &S, int64_t b, int h, int lane) {
+  const int g = lane >> 2, t = lane & 3;
+  Place p;
+  p.k = S.kp + b * S.kps[0] + h * S.kps[1] + g * (D / 2) + 4 * t;
+  p.v = S.vp + b * S.vps[0] + h * S.vps[1] + 2 * t * (D / 2) + g * (D / 16);
+  p.ks = static_cast<const uint16_t *>(S.ks) + b * S.kss[0] + h * S.kss[1] + 2 * t * (D / G);
+  p.vs = static_cast<const uint16_t *>(S.vs) + b * S.vss[0] + h * S.vss[1] + 2 * t * (D / G) + g * (D / 8) / G;
+  return p;
 }
 
-// Keys [k0, k0 + 16) of one source, of which those below `end` exist.
-template <int D, int G, bool WITH_V>
-__device__ __forceinline__ void load_keys(Keys<D, G, WITH_V> &x, const RowSource &S, int64_t b,
-                                          int h, int64_t k0, int64_t end, int lane) {
+// Keys [k0, k0 + 16) of one source.  TAIL: only those below `end` (at least one)
+// exist; in the place of the others the last one is read (they are masked).
+template <int D, int G, bool WITH_V, bool TAIL>
+__device__ __forceinline__ void load_keys(Keys<D, G, WITH_V> &x, const Place &P, int64_t k0, int64_t end,
+                                          int lane) {
   using K = Keys<D, G, WITH_V>;
   const int g = lane >> 2, t = lane & 3;
+  const int left = TAIL ? static_cast<int>(end - k0) - 1 : 15;  // last key that exists
 #pragma unroll
   for (int n = 0; n < 2; ++n) {
-    const int64_t key = k0 + 8 * n + g;
-    const uint32_t *p =
-        reinterpret_cast<const uint32_t *>(S.kp + b * S.kps[0] + h * S.kps[1] + key * S.kps[2]) + t;
+    const int to = TAIL ? min(8 * n + g, left) - g : 8 * n;
+    const uint32_t *p = reinterpret_cast<const uint32_t *>(P.k + (k0 + to) * (D / 2));
 #pragma unroll
-    for (int i = 0; i < K::NB; ++i) x.k[n][i] = key < end ? __ldg(p + 4 * i) : 0u;
+    for (int i = 0; i < K::NB; ++i) x.k[n][i] = __ldg(p + 4 * i);
   }
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    const int64_t key = k0 + 2 * t + (j & 1) + 8 * (j >> 1);
-    const bool in = key < end;
-#pragma unroll
-    for (int i = 0; i < K::NG; ++i) x.ks[j][i] = 0;
-    if (in)
-      load_scales<K::NG>(x.ks[j], static_cast<const uint16_t *>(S.ks) + b * S.kss[0] +
-                                      h * S.kss[1] + key * S.kss[2]);
+    const int at = (j & 1) + 8 * (j >> 1), to = TAIL ? min(2 * t + at, left) - 2 * t : at;
+    const uint16_t *p = P.ks + (k0 + to) * K::NG;
+    if (K::NG == 4) {
+      const uint2 w = __ldg(reinterpret_cast<const uint2 *>(p));
+      x.ks[j][0] = w.x;
+      x.ks[j][K::SW - 1] = w.y;
+    } else if (K::NG == 2) {
+      x.ks[j][0] = __ldg(reinterpret_cast<const uint32_t *>(p));
+    } else {
+      x.ks[j][0] = __ldg(p);
+    }
     if (WITH_V) {
-#pragma unroll
-      for (int i = 0; i < K::VW; ++i) x.v[j][i] = 0u;
-      x.vs[j] = 0;
-      if (in) {
-        const uint8_t *p = S.vp + b * S.vps[0] + h * S.vps[1] + key * S.vps[2] + g * (D / 16);
-        if (K::VW == 2) {
-          const uint2 w = __ldg(reinterpret_cast<const uint2 *>(p));
-          x.v[j][0] = w.x;
-          x.v[j][K::VW - 1] = w.y;
-        } else {
-          x.v[j][0] = __ldg(reinterpret_cast<const uint32_t *>(p));
-        }
-        x.vs[j] = __ldg(static_cast<const uint16_t *>(S.vs) + b * S.vss[0] + h * S.vss[1] +
-                        key * S.vss[2] + g * (D / 8) / G);
+      const uint8_t *q = P.v + (k0 + to) * (D / 2);
+      if (K::VW == 2) {
+        const uint2 w = __ldg(reinterpret_cast<const uint2 *>(q));
+        x.v[j][0] = w.x;
+        x.v[j][K::VW - 1] = w.y;
+      } else {
+        x.v[j][0] = __ldg(reinterpret_cast<const uint32_t *>(q));
       }
+      x.vs[j] = __ldg(P.vs + (k0 + to) * K::NG);
     }
   }
 }
@@ -186,6 +177,9 @@ __device__ __forceinline__ void load_query(Query<D, HALF> &Q, const TreeParams &
         p[2] = prmt(u[1], u[3], 0x5410);
         p[3] = prmt(u[1], u[3], 0x7632);
       }
+      // pairs 1 and 3 meet codes times 16 (see code_pair)
+      p[1] = tc::hmul2(p[1], 0x2C002C00u);
+      p[3] = tc::hmul2(p[3], 0x2C002C00u);
       // k-step 2i: pairs 0 and 1; k-step 2i + 1: pairs 2 and 3
       if (HALF) {
         Q.a[2 * i][0] = p[0];
@@ -202,8 +196,16 @@ __device__ __forceinline__ void load_query(Query<D, HALF> &Q, const TreeParams &
   }
 }
 
-// f16 pairs (code - 8) of a word's nibbles e and e + 4
+// f16 pairs of a word's nibbles e and e + 4: code - 8 for even e, 16 times that
+// for odd e, whose bits then need no shift of their own (both exact)
 __device__ __forceinline__ uint32_t code_pair(uint32_t w, int e) {
+  const uint32_t x = e < 2 ? w : w >> 8;
+  if (!(e & 1)) return tc::hsub2(tc::nib_pair(x), 0x64086408u);
+  uint32_t r;
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(x), "r"(0x00F000F0u), "r"(0x64006400u));
+  return tc::hsub2(r, 0x64806480u);
+}
+__device__ __forceinline__ uint32_t code_pair1(uint32_t w, int e) {  // code - 8 for every e
   return tc::hsub2(tc::nib_pair(w >> (4 * e)), 0x64086408u);
 }
 
@@ -227,7 +229,7 @@ __device__ __forceinline__ void scores(float (&s)[4], const Query<D, HALF> &Q,
                       code_pair(w, 2 * j), code_pair(w, 2 * j + 1));
       }
     }
-    const float k0 = scale_of<ST>(x.ks[2 * n][gr]), k1 = scale_of<ST>(x.ks[2 * n + 1][gr]);
+    const float k0 = scale_at<ST>(x.ks[2 * n], gr), k1 = scale_at<ST>(x.ks[2 * n + 1], gr);
     s[0] = fmaf(c[0], k0, s[0]);
     s[1] = fmaf(c[1], k1, s[1]);
     if (!HALF) {
@@ -269,9 +271,16 @@ __global__ void __launch_bounds__(NW * 32, BLOCKS)
   const int s0 = part * per, s1 = min(steps, s0 + per);
 
   Keys<D, G, true> cur;
+  const Place ctx = place_of<D, G>(T.cache, b, kvh, lane), dft = place_of<D, G>(T.draft, b, kvh, lane);
+  const int whole = static_cast<int>(len >> 4);  // steps of 16 context keys
   auto fetch = [&](int s) {
-    if (s < nctx) load_keys(cur, T.cache, b, kvh, static_cast<int64_t>(s) * 16, len, lane);
-    else load_keys(cur, T.draft, b, kvh, static_cast<int64_t>(s - nctx) * 16, T.ndraft, lane);
+    if (s < whole) {
+      load_keys<D, G, true, false>(cur, ctx, static_cast<int64_t>(s) * 16, 0, lane);
+    } else {
+      const bool d = s >= nctx;
+      load_keys<D, G, true, true>(cur, d ? dft : ctx, static_cast<int64_t>(d ? s - nctx : s) * 16,
+                                  d ? T.ndraft : len, lane);
+    }
   };
   int s = s0 + warp;
   if (s < s1) fetch(s);
@@ -306,7 +315,7 @@ __global__ void __launch_bounds__(NW * 32, BLOCKS)
     scores<D, G, ST, HALF>(x[1], Q, cur, 1);
     // V of this step out of the way of the next step's loads
     uint32_t vw[4][Keys<D, G, true>::VW];
-    uint16_t vs[4];
+    uint32_t vs[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
 #pragma unroll
@@ -327,7 +336,7 @@ __global__ void __launch_bounds__(NW * 32, BLOCKS)
         if (draft) {  // a visible key without a usable V scale: the row has no value
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            const bool bad = !(fabsf(scale_of<ST>(vs[j])) <= tc::kMaxScale);
+            const bool bad = !(fabsf(scale_at<ST>(&vs[j], 0)) <= tc::kMaxScale);
             const uint32_t any = __ballot_sync(0xffffffffu, bad) & (0x11111111u << t);
             if (any && (on >> j & 1u)) broken[r] = true;
           }
@@ -365,15 +374,13 @@ __global__ void __launch_bounds__(NW * 32, BLOCKS)
     uint32_t sp[2];
 #pragma unroll
     for (int p = 0; p < 2; ++p) {
-      uint32_t lo = half_scale<ST>(vs[2 * p]), hi = half_scale<ST>(vs[2 * p + 1]);
-      const bool b0 = !(fabsf(scale_of<ST>(vs[2 * p])) <= tc::kMaxScale);
-      const bool b1 = !(fabsf(scale_of<ST>(vs[2 * p + 1])) <= tc::kMaxScale);
-      big |= b0 || b1;
-      if (draft) {  // rows that see such a key are marked above
-        if (b0) lo = 0;
-        if (b1) hi = 0;
+      const float f0 = scale_at<ST>(&vs[2 * p], 0), f1 = scale_at<ST>(&vs[2 * p + 1], 0);
+      sp[p] = DT<ST>::code == KV4_F16 ? prmt(vs[2 * p], vs[2 * p + 1], 0x5410) : pack_f16x2(f0, f1);
+      const bool b0 = !(fabsf(f0) <= tc::kMaxScale), b1 = !(fabsf(f1) <= tc::kMaxScale);
+      if (b0 || b1) {
+        big = true;
+        if (draft) sp[p] &= (b0 ? 0u : 0xffffu) | (b1 ? 0u : 0xffff0000u);  // rows that see it: above
       }
-      sp[p] = lo | hi << 16;
     }
 #pragma unroll
     for (int i = 0; i < Keys<D, G, true>::VW; ++i) {
@@ -385,8 +392,8 @@ __global__ void __launch_bounds__(NW * 32, BLOCKS)
       }
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const uint32_t b0 = tc::hmul2(code_pair(y[0][e >> 2], e & 3), sp[0]);
-        const uint32_t b1 = tc::hmul2(code_pair(y[1][e >> 2], e & 3), sp[1]);
+        const uint32_t b0 = tc::hmul2(code_pair1(y[0][e >> 2], e & 3), sp[0]);
+        const uint32_t b1 = tc::hmul2(code_pair1(y[1][e >> 2], e & 3), sp[1]);
         float *c = o[8 * i + e];
         if (HALF) {
           float d[4];
@@ -460,26 +467,27 @@ __global__ void __launch_bounds__(NW * 32, BLOCKS)
 // sums, summed over the rows of each key (rows are lanes: three shuffles).
 template <int D, int G, typename ST, bool HALF>
 __global__ void __launch_bounds__(NW * 32, HALF ? 4 : BLOCKS)
-    score_mma(const __grid_constant__ ScoreParams P, int rows, int64_t steps_per_unit, int64_t total) {
+    score_mma(const __grid_constant__ ScoreParams P, int rows, uint32_t steps_per_unit, uint32_t total) {
   constexpr int RT = HALF ? 1 : 2, NR = HALF ? 8 : 16;
   const TreeParams &T = P.t;
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int64_t warps = static_cast<int64_t>(gridDim.x) * NW;
-  const int64_t w = static_cast<int64_t>(blockIdx.x) * NW + (threadIdx.x >> 5);
+  const uint32_t warps = gridDim.x * NW, w = blockIdx.x * NW + (threadIdx.x >> 5);
   // warps take runs of one unit's 16-key steps
-  const int64_t each = total / warps, rest = total - each * warps;
-  int64_t at = w * each + min(w, rest);
-  const int64_t stop = at + each + (w < rest ? 1 : 0);
-  const int64_t nctx = (T.S + 15) >> 4;
+  const uint32_t each = total / warps, rest = total - each * warps;
+  uint32_t at = w * each + min(w, rest);
+  const uint32_t stop = at + each + (w < rest ? 1u : 0u);
+  const int nctx = static_cast<int>((T.S + 15) >> 4), whole = static_cast<int>(T.S >> 4);
   griddep_wait();  // the rows' maxima and sums come from the kernel before
 #pragma unroll 1
   while (at < stop) {
-    const int64_t unit = at / steps_per_unit, b = unit / T.Hkv;
+    const uint32_t unit = at / steps_per_unit, b = unit / T.Hkv;
     const int kvh = static_cast<int>(unit - b * T.Hkv);
-    const int64_t first = at - unit * steps_per_unit, last = min(steps_per_unit, first + stop - at);
+    const int first = static_cast<int>(at - unit * steps_per_unit);
+    const int last = static_cast<int>(min(steps_per_unit, first + stop - at));
     at += last - first;
     const float *in = P.in + b * P.is[0] + kvh * P.is[1];
     float *out = P.out + b * P.os[0] + kvh * P.os[1];
+    const Place ctx = place_of<D, G>(T.cache, b, kvh, lane), dft = place_of<D, G>(T.draft, b, kvh, lane);
 #pragma unroll 1
     for (int row0 = 0; row0 < rows; row0 += NR) {
       Query<D, HALF> Q;
@@ -489,21 +497,26 @@ __global__ void __launch_bounds__(NW * 32, HALF ? 4 : BLOCKS)
 #pragma unroll
       for (int r = 0; r < RT; ++r) {
         const int row = row0 + g + 8 * r;
-        const float2 st = row < rows ? T.stats[unit * rows + row] : make_float2(0.0f, 0.0f);
+        const float2 st = row < rows ? T.stats[static_cast<int64_t>(unit) * rows + row] : make_float2(0.0f, 0.0f);
         sm[r] = st.x;
         sl[r] = st.y;  // 0: a row that saw nothing, or none at all
         node[r] = row / T.R;
       }
       Keys<D, G, false> cur;
-      auto fetch = [&](int64_t s) {
-        if (s < nctx) load_keys(cur, T.cache, b, kvh, s * 16, T.S, lane);
-        else load_keys(cur, T.draft, b, kvh, (s - nctx) * 16, T.ndraft, lane);
+      auto fetch = [&](int s) {
+        if (s < whole) {
+          load_keys<D, G, false, false>(cur, ctx, static_cast<int64_t>(s) * 16, 0, lane);
+        } else {
+          const bool d = s >= nctx;
+          load_keys<D, G, false, true>(cur, d ? dft : ctx, static_cast<int64_t>(d ? s - nctx : s) * 16,
+                                       d ? T.ndraft : T.S, lane);
+        }
       };
       fetch(first);
 #pragma unroll 1
-      for (int64_t s = first; s < last; ++s) {
+      for (int s = first; s < last; ++s) {
         const bool draft = s >= nctx;
-        const int64_t k0 = (draft ? s - nctx : s) * 16, end = draft ? T.ndraft : T.S;
+        const int64_t k0 = static_cast<int64_t>(draft ? s - nctx : s) * 16, end = draft ? T.ndraft : T.S;
         // lanes 0-15 end up with a key each
         const int64_t mine = k0 + lane, tok = draft ? T.S + mine : mine;
         float old = 0.0f;
@@ -581,6 +594,7 @@ int launch_tree(const TreeParams &T, const MmaPlan &L, cudaStream_t st) {
 template <int D, int G, typename ST, bool HALF>
 int launch_score(const ScoreParams &P, int rows, cudaStream_t st) {
   const int64_t steps = (P.t.S + 15) / 16 + (P.t.ndraft + 15) / 16, total = P.t.B * P.t.Hkv * steps;
+  if (total >= (int64_t(1) << 31)) return KV4_ERR_UNSUPPORTED;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(static_cast<unsigned>(
       std::min<int64_t>(static_cast<int64_t>(sm_count()) * (HALF ? 4 : BLOCKS), (total + NW - 1) / NW)));
@@ -591,7 +605,8 @@ int launch_score(const ScoreParams &P, int rows, cudaStream_t st) {
   at.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &at;
   cfg.numAttrs = 1;
-  return cuda_status(cudaLaunchKernelEx(&cfg, score_mma<D, G, ST, HALF>, P, rows, steps, total));
+  return cuda_status(cudaLaunchKernelEx(&cfg, score_mma<D, G, ST, HALF>, P, rows, static_cast<uint32_t>(steps),
+                                        static_cast<uint32_t>(total)));
 }
 
 // f(integral D, integral G, ST{}, bool HALF)
@@ -613,11 +628,13 @@ int by_shape(const TreeParams &T, F f) {
   return type(std::integral_constant<int, 128>{}, std::integral_constant<int, 128>{});
 }
 
-bool scales_ok(const RowSource &S, int64_t B, int Hkv, int64_t T, int bytes) {
+// rows of `pw` code bytes and `bytes` scale bytes without gaps between tokens
+bool close_rows(const RowSource &S, int64_t B, int Hkv, int64_t T, int pw, int bytes) {
   if (T == 0) return true;
-  const int e = bytes / 2;  // elements of a row: a power of two
+  const int e = bytes / 2;  // scales of a row: a power of two
+  if (T > 1 && (S.kps[2] != pw || S.vps[2] != pw || S.kss[2] != e || S.vss[2] != e)) return false;
   if ((reinterpret_cast<uintptr_t>(S.ks) & (bytes - 1))) return false;
-  if (S.kss[3] != 1 || S.vss[3] != 1 || S.kss[2] % e || (Hkv > 1 && S.kss[1] % e) ||
+  if (S.kss[3] != 1 || S.vss[3] != 1 || (Hkv > 1 && S.kss[1] % e) ||
       (B > 1 && S.kss[0] % e))
     return false;
   return (reinterpret_cast<uintptr_t>(S.vs) & 1u) == 0;
@@ -626,7 +643,7 @@ bool scales_ok(const RowSource &S, int64_t B, int Hkv, int64_t T, int bytes) {
 }  // namespace
 
 // Whether the kernels of this file take the call: 16-bit queries and scales, the
-// sizes they are built for, rows that aligned loads can read; and either so few
+// sizes they are built for, rows without gaps that aligned loads can read; and either so few
 // rows that branch_tc.cu's tiles would be mostly padding, or half precision
 // somewhere, which that file leaves alone (a product of a code and an f16 scale
 // does not fit an f16).
@@ -637,7 +654,8 @@ bool tree_mma_takes(const TreeParams &T) {
   if ((T.G != 32 && T.G != 64 && T.G != 128) || T.G > T.d) return false;
   if (!rows_ok(T.cache, T.B, T.Hkv, T.S) || !rows_ok(T.draft, T.B, T.Hkv, T.ndraft)) return false;
   const int bytes = 2 * T.d / T.G;
-  if (!scales_ok(T.cache, T.B, T.Hkv, T.S, bytes) || !scales_ok(T.draft, T.B, T.Hkv, T.ndraft, bytes))
+  if (!close_rows(T.cache, T.B, T.Hkv, T.S, T.d / 2, bytes) ||
+      !close_rows(T.draft, T.B, T.Hkv, T.ndraft, T.d / 2, bytes))
     return false;
   if (!al16(T.q) || !al16(T.out) || T.qs[3] != 1 || T.os[3] != 1) return false;
   const int64_t n[3] = {T.B, static_cast<int64_t>(T.Hkv) * T.R, T.nodes};
