@@ -21,7 +21,8 @@
 //
 // A block of warps takes a range of one unit's keys, 16 keys per warp in turn;
 // its warps meet in shared memory, ranges of one unit in the workspace
-// (tree_merge of branch.cu).  The next step's loads are in flight during a step.
+// (tree_merge of branch.cu).  Every warp has a ring of steps of its own, filled
+// by asynchronous copies three ahead; nothing waits for another warp on the way.
 // Bound: memory for one row tile; instructions (about 350 per warp and 16 keys
 // of 128 columns) are close behind.
 #include <algorithm>
@@ -42,7 +43,8 @@ struct MmaPlan {
 };
 
 constexpr int NW = 4;      // warps per block
-constexpr int BLOCKS = 3;  // per SM: 168 registers a thread
+// blocks per SM: 168 registers a thread, 128 where eight rows of 64 columns fit
+constexpr int blocks_of(int d, bool half) { return half && d == 64 ? 4 : 3; }
 constexpr float kShift = 7.0f;  // weights are written times 2^7 (see branch_tc.cu)
 
 // scale i of a packed row of 16-bit scales
@@ -52,74 +54,78 @@ __device__ __forceinline__ float scale_at(const uint32_t *w, int i) {
   return i & 1 ? f16hi_to_f32(w[i >> 1]) : f16lo_to_f32(w[i >> 1]);
 }
 
-// A warp's 16 keys: K words [key tile of 8][32-column block], V words and the
-// scales (K's of all groups, V's of the thread's columns) of this thread's four
-// keys 2t, 2t + 1, 2t + 8, 2t + 9
+// A warp's ring of steps in shared memory.  One step is 16 keys: rows of K (and
+// V) codes, padded so that the reads below meet no bank twice, then their
+// scales.  Copied asynchronously, 16 bytes of codes and 4 of scales at a time;
+// what lies past the last key becomes zeros.
 template <int D, int G, bool WITH_V>
-struct Keys {
-  static constexpr int NB = D / 32, NG = D / G, VW = D / 64, SW = (NG + 1) / 2;
-  uint32_t k[2][NB];
-  uint32_t v[WITH_V ? 4 : 1][VW];
-  uint32_t ks[4][SW], vs[WITH_V ? 4 : 1];
+struct Ring {
+  static constexpr int NG = D / G, SB = 2 * NG;           // scales of a key: number, bytes
+  static constexpr int ROW = D == 128 ? 80 : 48;          // bytes from key to key
+  static constexpr int K = 0, V = 16 * ROW, KS = WITH_V ? 32 * ROW : 16 * ROW, VS = KS + 16 * SB;
+  static constexpr int STEP = (WITH_V ? VS + 16 * SB : VS) + 15 & ~15;
+  static constexpr int DEPTH = WITH_V ? 4 : 6;
+  static constexpr int BYTES = DEPTH * STEP;
 };
 
-// Where a lane's first words of key 0 lie; rows follow one another without gaps
-// (D / 2 bytes of codes, D / G scales), so that everything else is a constant
-// offset from there.
-struct Place {
-  const uint8_t *k, *v;
-  const uint16_t *ks, *vs;
+template <int N>
+__device__ __forceinline__ void cp_async(uint32_t dst, const void *src, uint32_t n) {
+  if (N == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+  else asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// One (sequence, KV head) plane of a source
+struct Plane {
+  const uint8_t *k, *v, *ks, *vs;
 };
-template <int D, int G>
-__device__ __forceinline__ Place place_of(const RowSource &S, int64_t b, int h, int lane) {
-  const int g = lane >> 2, t = lane & 3;
-  Place p;
-  p.k = S.kp + b * S.kps[0] + h * S.kps[1] + g * (D / 2) + 4 * t;
-  p.v = S.vp + b * S.vps[0] + h * S.vps[1] + 2 * t * (D / 2) + g * (D / 16);
-  p.ks = static_cast<const uint16_t *>(S.ks) + b * S.kss[0] + h * S.kss[1] + 2 * t * (D / G);
-  p.vs = static_cast<const uint16_t *>(S.vs) + b * S.vss[0] + h * S.vss[1] + 2 * t * (D / G) + g * (D / 8) / G;
+__device__ __forceinline__ Plane plane_of(const RowSource &S, int64_t b, int h) {
+  Plane p;
+  p.k = S.kp + b * S.kps[0] + h * S.kps[1];
+  p.v = S.vp + b * S.vps[0] + h * S.vps[1];
+  p.ks = static_cast<const uint8_t *>(S.ks) + 2 * (b * S.kss[0] + h * S.kss[1]);
+  p.vs = static_cast<const uint8_t *>(S.vs) + 2 * (b * S.vss[0] + h * S.vss[1]);
   return p;
 }
 
-// Keys [k0, k0 + 16) of one source.  TAIL: only those below `end` (at least one)
-// exist; in the place of the others the last one is read (they are masked).
-template <int D, int G, bool WITH_V, bool TAIL>
-__device__ __forceinline__ void load_keys(Keys<D, G, WITH_V> &x, const Place &P, int64_t k0, int64_t end,
-                                          int lane) {
-  using K = Keys<D, G, WITH_V>;
-  const int g = lane >> 2, t = lane & 3;
-  const int left = TAIL ? static_cast<int>(end - k0) - 1 : 15;  // last key that exists
+// Start the copy of keys [k0, k0 + 16) to `to`; those from `left` on do not exist.
+template <int D, int G, bool WITH_V>
+__device__ __forceinline__ void fetch_step(const Plane &P, int64_t k0, int left, uint32_t to, int lane) {
+  using R = Ring<D, G, WITH_V>;
+  constexpr int CPR = D / 32;  // 16-byte chunks per row
+  const uint8_t *k = P.k + k0 * (D / 2), *v = P.v + k0 * (D / 2);
 #pragma unroll
-  for (int n = 0; n < 2; ++n) {
-    const int to = TAIL ? min(8 * n + g, left) - g : 8 * n;
-    const uint32_t *p = reinterpret_cast<const uint32_t *>(P.k + (k0 + to) * (D / 2));
-#pragma unroll
-    for (int i = 0; i < K::NB; ++i) x.k[n][i] = __ldg(p + 4 * i);
+  for (int i = 0; i < CPR / 2; ++i) {
+    const int row = lane / CPR + 32 / CPR * i, c = lane % CPR;
+    const uint32_t n = row < left ? 16u : 0u;
+    const int from = n ? row * (D / 2) + 16 * c : 0;
+    cp_async<16>(to + R::K + row * R::ROW + 16 * c, k + from, n);
+    if (WITH_V) cp_async<16>(to + R::V + row * R::ROW + 16 * c, v + from, n);
   }
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const int at = (j & 1) + 8 * (j >> 1), to = TAIL ? min(2 * t + at, left) - 2 * t : at;
-    const uint16_t *p = P.ks + (k0 + to) * K::NG;
-    if (K::NG == 4) {
-      const uint2 w = __ldg(reinterpret_cast<const uint2 *>(p));
-      x.ks[j][0] = w.x;
-      x.ks[j][K::SW - 1] = w.y;
-    } else if (K::NG == 2) {
-      x.ks[j][0] = __ldg(reinterpret_cast<const uint32_t *>(p));
-    } else {
-      x.ks[j][0] = __ldg(p);
-    }
-    if (WITH_V) {
-      const uint8_t *q = P.v + (k0 + to) * (D / 2);
-      if (K::VW == 2) {
-        const uint2 w = __ldg(reinterpret_cast<const uint2 *>(q));
-        x.v[j][0] = w.x;
-        x.v[j][K::VW - 1] = w.y;
-      } else {
-        x.v[j][0] = __ldg(reinterpret_cast<const uint32_t *>(q));
-      }
-      x.vs[j] = __ldg(P.vs + (k0 + to) * K::NG);
-    }
+  if (lane < 4 * R::SB) {  // 16 SB bytes of scales, four a lane
+    const int have = left * R::SB - 4 * lane;
+    const uint32_t n = have >= 4 ? 4u : have > 0 ? static_cast<uint32_t>(have) : 0u;
+    const int from = n ? 4 * lane : 0;
+    cp_async<4>(to + R::KS + 4 * lane, P.ks + k0 * R::SB + from, n);
+    if (WITH_V) cp_async<4>(to + R::VS + 4 * lane, P.vs + k0 * R::SB + from, n);
+  }
+}
+
+// scales of one key from shared memory
+template <int NG>
+__device__ __forceinline__ void lds_scales(uint32_t (&w)[(NG + 1) / 2], uint32_t at) {
+  if (NG == 4) {
+    const uint2 v = lds64(at);
+    w[0] = v.x;
+    w[(NG + 1) / 2 - 1] = v.y;
+  } else if (NG == 2) {
+    w[0] = lds32(at);
+  } else {
+    w[0] = lds16(at);
   }
 }
 
@@ -210,31 +216,36 @@ __device__ __forceinline__ uint32_t code_pair1(uint32_t w, int e) {  // code - 8
 }
 
 // Sums of rows g (s[0], s[1]) and g + 8 (s[2], s[3]) with keys 2t, 2t + 1 of
-// key tile n, scaled group by group.
+// key tile n of the step at `at`, scaled group by group.
 template <int D, int G, typename ST, bool HALF, bool WITH_V>
-__device__ __forceinline__ void scores(float (&s)[4], const Query<D, HALF> &Q,
-                                       const Keys<D, G, WITH_V> &x, int n) {
+__device__ __forceinline__ void scores(float (&s)[4], const Query<D, HALF> &Q, uint32_t at, int n, int lane) {
+  using R = Ring<D, G, WITH_V>;
+  const int g = lane >> 2, t = lane & 3;
+  uint32_t w[D / 32], k0[(R::NG + 1) / 2], k1[(R::NG + 1) / 2];
+#pragma unroll
+  for (int i = 0; i < D / 32; ++i) w[i] = lds32(at + R::K + (8 * n + g) * R::ROW + 16 * i + 4 * t);
+  lds_scales<R::NG>(k0, at + R::KS + (8 * n + 2 * t) * R::SB);
+  lds_scales<R::NG>(k1, at + R::KS + (8 * n + 2 * t + 1) * R::SB);
   s[0] = s[1] = s[2] = s[3] = 0.0f;
 #pragma unroll
-  for (int gr = 0; gr < D / G; ++gr) {
+  for (int gr = 0; gr < R::NG; ++gr) {
     float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (int i = 0; i < G / 32; ++i) {
       const int blk = gr * (G / 32) + i;
-      const uint32_t w = x.k[n][blk];
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         const uint32_t *a = Q.a[2 * blk + j];
         mma_f16_16816(c, a[0], HALF ? 0u : a[HALF ? 0 : 1], a[HALF ? 1 : 2], HALF ? 0u : a[HALF ? 0 : 3],
-                      code_pair(w, 2 * j), code_pair(w, 2 * j + 1));
+                      code_pair(w[blk], 2 * j), code_pair(w[blk], 2 * j + 1));
       }
     }
-    const float k0 = scale_at<ST>(x.ks[2 * n], gr), k1 = scale_at<ST>(x.ks[2 * n + 1], gr);
-    s[0] = fmaf(c[0], k0, s[0]);
-    s[1] = fmaf(c[1], k1, s[1]);
+    const float f0 = scale_at<ST>(k0, gr), f1 = scale_at<ST>(k1, gr);
+    s[0] = fmaf(c[0], f0, s[0]);
+    s[1] = fmaf(c[1], f1, s[1]);
     if (!HALF) {
-      s[2] = fmaf(c[2], k0, s[2]);
-      s[3] = fmaf(c[3], k1, s[3]);
+      s[2] = fmaf(c[2], f0, s[2]);
+      s[3] = fmaf(c[3], f1, s[3]);
     }
   }
 }
@@ -254,10 +265,10 @@ __device__ __forceinline__ uint32_t seen_keys(const TreeParams &T, int64_t b, bo
 }
 
 template <int D, int G, typename ST, bool HALF>
-__global__ void __launch_bounds__(NW * 32, BLOCKS)
+__global__ void __launch_bounds__(NW * 32, blocks_of(D, HALF))
     tree_mma(const __grid_constant__ TreeParams T, const MmaPlan L) {
   constexpr int NR = HALF ? 8 : 16, RT = HALF ? 1 : 2, DG = D / 8, LD = D + 4;
-  extern __shared__ __align__(16) float msm[];  // [NW][NR][LD] outputs, [NW][NR] float2 (m, l)
+  extern __shared__ __align__(16) float msm[];  // rings, later [NW][NR][LD] outputs, [NW][NR] float2 (m, l)
   float2 *sml = reinterpret_cast<float2 *>(msm + NW * NR * LD);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
   const int part = static_cast<int>(blockIdx.x % L.parts);
@@ -270,20 +281,26 @@ __global__ void __launch_bounds__(NW * 32, BLOCKS)
   const int per = (steps + L.parts - 1) / L.parts;
   const int s0 = part * per, s1 = min(steps, s0 + per);
 
-  Keys<D, G, true> cur;
-  const Place ctx = place_of<D, G>(T.cache, b, kvh, lane), dft = place_of<D, G>(T.draft, b, kvh, lane);
-  const int whole = static_cast<int>(len >> 4);  // steps of 16 context keys
-  auto fetch = [&](int s) {
-    if (s < whole) {
-      load_keys<D, G, true, false>(cur, ctx, static_cast<int64_t>(s) * 16, 0, lane);
-    } else {
-      const bool d = s >= nctx;
-      load_keys<D, G, true, true>(cur, d ? dft : ctx, static_cast<int64_t>(d ? s - nctx : s) * 16,
-                                  d ? T.ndraft : len, lane);
+  using R = Ring<D, G, true>;
+  const uint32_t ring = smem_u32(msm) + warp * R::BYTES;
+  const Plane ctx = plane_of(T.cache, b, kvh);
+  auto fetch = [&](int s, uint32_t slot) {
+    if (s < nctx) {
+      fetch_step<D, G, true>(ctx, static_cast<int64_t>(s) * 16, static_cast<int>(min(len - static_cast<int64_t>(s) * 16, int64_t(16))),
+                             ring + slot * R::STEP, lane);
+    } else if (s < s1) {
+      const Plane dft = plane_of(T.draft, b, kvh);
+      fetch_step<D, G, true>(dft, static_cast<int64_t>(s - nctx) * 16, min(T.ndraft - (s - nctx) * 16, 16),
+                             ring + slot * R::STEP, lane);
     }
+    cp_async_commit();
   };
+  // steps s0 + warp, + NW, ...: DEPTH - 1 of them on their way
   int s = s0 + warp;
-  if (s < s1) fetch(s);
+#pragma unroll 1
+  for (int i = 0; i < R::DEPTH - 1; ++i)
+    if (s + i * NW < s1) fetch(s + i * NW, i);
+    else cp_async_commit();
   Query<D, HALF> Q;
   load_query(Q, T, b, kvh, row0, L.rows, lane);
   int node[RT];
@@ -306,23 +323,27 @@ __global__ void __launch_bounds__(NW * 32, BLOCKS)
     for (int e = 0; e < (HALF ? 2 : 4); ++e) o[j][e] = 0.0f;
   bool big = false;
 
+  uint32_t slot = 0;
 #pragma unroll 1
   for (; s < s1; s += NW) {
     const bool draft = s >= nctx;
     const int64_t k0 = static_cast<int64_t>(draft ? s - nctx : s) * 16, end = draft ? T.ndraft : len;
-    float x[2][4];
-    scores<D, G, ST, HALF>(x[0], Q, cur, 0);
-    scores<D, G, ST, HALF>(x[1], Q, cur, 1);
-    // V of this step out of the way of the next step's loads
-    uint32_t vw[4][Keys<D, G, true>::VW];
-    uint32_t vs[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-#pragma unroll
-      for (int i = 0; i < Keys<D, G, true>::VW; ++i) vw[j][i] = cur.v[j][i];
-      vs[j] = cur.vs[j];
+    cp_async_wait<R::DEPTH - 2>();
+    __syncwarp();  // this step is there for all lanes, and all are done with the one before
+    {
+      const int ahead = s + (R::DEPTH - 1) * NW;
+      if (ahead < s1) fetch(ahead, slot == 0 ? R::DEPTH - 1 : slot - 1);
+      else cp_async_commit();
     }
-    if (s + NW < s1) fetch(s + NW);
+    const uint32_t at = ring + slot * R::STEP;
+    slot = slot + 1 == R::DEPTH ? 0 : slot + 1;
+    float x[2][4];
+    scores<D, G, ST, HALF, true>(x[0], Q, at, 0, lane);
+    scores<D, G, ST, HALF, true>(x[1], Q, at, 1, lane);
+    uint32_t vs[4];  // V's scales of this thread's columns, keys 2t, 2t + 1, 2t + 8, 2t + 9
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      vs[j] = lds16(at + R::VS + (2 * t + (j & 1) + 8 * (j >> 1)) * R::SB + 2 * (g * DG / G));
 
     // scores -> weights, in place
 #pragma unroll
@@ -382,8 +403,20 @@ __global__ void __launch_bounds__(NW * 32, BLOCKS)
         if (draft) sp[p] &= (b0 ? 0u : 0xffffu) | (b1 ? 0u : 0xffff0000u);  // rows that see it: above
       }
     }
+    uint32_t vw[4][D / 64];
 #pragma unroll
-    for (int i = 0; i < Keys<D, G, true>::VW; ++i) {
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t p = at + R::V + (2 * t + (j & 1) + 8 * (j >> 1)) * R::ROW + g * (D / 16);
+      if (D == 128) {
+        const uint2 w = lds64(p);
+        vw[j][0] = w.x;
+        vw[j][D / 64 - 1] = w.y;
+      } else {
+        vw[j][0] = lds32(p);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < D / 64; ++i) {
       uint32_t y[2][2];  // [key pair][half word]: the pair's words side by side
 #pragma unroll
       for (int p = 0; p < 2; ++p) {
@@ -408,7 +441,9 @@ __global__ void __launch_bounds__(NW * 32, BLOCKS)
   }
   if (big) atomicOr(&g_branch_error_mma, DEV_ERR_F16_RANGE);
 
-  // ---- the block's warps meet ----
+  // ---- the block's warps meet, where the rings were ----
+  cp_async_wait<0>();
+  __syncthreads();
 #pragma unroll
   for (int r = 0; r < RT; ++r) {
     l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
@@ -466,7 +501,7 @@ __global__ void __launch_bounds__(NW * 32, BLOCKS)
 // Scores of the cached tokens: weights formed again from K, the rows' maxima and
 // sums, summed over the rows of each key (rows are lanes: three shuffles).
 template <int D, int G, typename ST, bool HALF>
-__global__ void __launch_bounds__(NW * 32, HALF ? 4 : BLOCKS)
+__global__ void __launch_bounds__(NW * 32, HALF ? 4 : 3)
     score_mma(const __grid_constant__ ScoreParams P, int rows, uint32_t steps_per_unit, uint32_t total) {
   constexpr int RT = HALF ? 1 : 2, NR = HALF ? 8 : 16;
   const TreeParams &T = P.t;
@@ -476,7 +511,10 @@ __global__ void __launch_bounds__(NW * 32, HALF ? 4 : BLOCKS)
   const uint32_t each = total / warps, rest = total - each * warps;
   uint32_t at = w * each + min(w, rest);
   const uint32_t stop = at + each + (w < rest ? 1u : 0u);
-  const int nctx = static_cast<int>((T.S + 15) >> 4), whole = static_cast<int>(T.S >> 4);
+  const int nctx = static_cast<int>((T.S + 15) >> 4);
+  using R = Ring<D, G, false>;
+  __shared__ __align__(16) uint8_t rings[NW * R::BYTES];
+  const uint32_t ring = smem_u32(rings) + (threadIdx.x >> 5) * R::BYTES;
   griddep_wait();  // the rows' maxima and sums come from the kernel before
 #pragma unroll 1
   while (at < stop) {
@@ -487,7 +525,6 @@ __global__ void __launch_bounds__(NW * 32, HALF ? 4 : BLOCKS)
     at += last - first;
     const float *in = P.in + b * P.is[0] + kvh * P.is[1];
     float *out = P.out + b * P.os[0] + kvh * P.os[1];
-    const Place ctx = place_of<D, G>(T.cache, b, kvh, lane), dft = place_of<D, G>(T.draft, b, kvh, lane);
 #pragma unroll 1
     for (int row0 = 0; row0 < rows; row0 += NR) {
       Query<D, HALF> Q;
@@ -502,17 +539,18 @@ __global__ void __launch_bounds__(NW * 32, HALF ? 4 : BLOCKS)
         sl[r] = st.y;  // 0: a row that saw nothing, or none at all
         node[r] = row / T.R;
       }
-      Keys<D, G, false> cur;
-      auto fetch = [&](int s) {
-        if (s < whole) {
-          load_keys<D, G, false, false>(cur, ctx, static_cast<int64_t>(s) * 16, 0, lane);
-        } else {
-          const bool d = s >= nctx;
-          load_keys<D, G, false, true>(cur, d ? dft : ctx, static_cast<int64_t>(d ? s - nctx : s) * 16,
-                                       d ? T.ndraft : T.S, lane);
-        }
+      auto fetch = [&](int s, uint32_t slot) {
+        const bool d = s >= nctx;
+        const Plane p = plane_of(d ? T.draft : T.cache, b, kvh);
+        const int64_t k0 = static_cast<int64_t>(d ? s - nctx : s) * 16, end = d ? T.ndraft : T.S;
+        fetch_step<D, G, false>(p, k0, static_cast<int>(min(end - k0, int64_t(16))), ring + slot * R::STEP, lane);
+        cp_async_commit();
       };
-      fetch(first);
+#pragma unroll 1
+      for (int i = 0; i < R::DEPTH - 1; ++i)
+        if (first + i < last) fetch(first + i, i);
+        else cp_async_commit();
+      uint32_t slot = 0;
 #pragma unroll 1
       for (int s = first; s < last; ++s) {
         const bool draft = s >= nctx;
@@ -521,10 +559,15 @@ __global__ void __launch_bounds__(NW * 32, HALF ? 4 : BLOCKS)
         const int64_t mine = k0 + lane, tok = draft ? T.S + mine : mine;
         float old = 0.0f;
         if (lane < 16 && mine < end) old = row0 == 0 ? in[tok * P.is[2]] * P.decay : out[tok * P.os[2]];
+        cp_async_wait<R::DEPTH - 2>();
+        __syncwarp();  // this step is there for all lanes, and all are done with the one before
+        if (s + R::DEPTH - 1 < last) fetch(s + R::DEPTH - 1, slot == 0 ? R::DEPTH - 1 : slot - 1);
+        else cp_async_commit();
+        const uint32_t step = ring + slot * R::STEP;
+        slot = slot + 1 == R::DEPTH ? 0 : slot + 1;
         float x[2][4];
-        scores<D, G, ST, HALF>(x[0], Q, cur, 0);
-        scores<D, G, ST, HALF>(x[1], Q, cur, 1);
-        if (s + 1 < last) fetch(s + 1);
+        scores<D, G, ST, HALF, false>(x[0], Q, step, 0, lane);
+        scores<D, G, ST, HALF, false>(x[1], Q, step, 1, lane);
         float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int r = 0; r < RT; ++r) {
@@ -549,6 +592,8 @@ __global__ void __launch_bounds__(NW * 32, HALF ? 4 : BLOCKS)
         const float add = lane < 8 ? (lane & 1 ? v[1] : v[0]) : (lane & 1 ? v[3] : v[2]);
         if (lane < 16 && mine < end) out[tok * P.os[2]] = old + add;
       }
+      cp_async_wait<0>();
+      __syncwarp();  // the ring is free for the next pass
     }
   }
 }
@@ -566,7 +611,7 @@ MmaPlan mma_plan(const TreeParams &T) {
   L.units = T.B * T.Hkv;
   // one wave of blocks, each warp at least two steps of 16 keys
   const int64_t steps = (T.S + 15) / 16 + (T.ndraft + 15) / 16, have = L.units * L.row_tiles;
-  const int64_t room = static_cast<int64_t>(sm_count()) * BLOCKS;
+  const int64_t room = static_cast<int64_t>(sm_count()) * blocks_of(T.d, half_rows(L.rows));
   const int64_t most = std::max<int64_t>(1, steps / (2 * NW));
   L.parts = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({room / have, most, 64})));
   return L;
@@ -575,7 +620,8 @@ MmaPlan mma_plan(const TreeParams &T) {
 template <int D, int G, typename ST, bool HALF>
 int launch_tree(const TreeParams &T, const MmaPlan &L, cudaStream_t st) {
   constexpr int NR = HALF ? 8 : 16;
-  constexpr int smem = NW * NR * ((D + 4) * 4 + 8);
+  constexpr int meet = NW * NR * ((D + 4) * 4 + 8), rings = NW * Ring<D, G, true>::BYTES;
+  constexpr int smem = meet > rings ? meet : rings;
   static bool configured[64] = {};
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) dev = 0;
@@ -597,7 +643,7 @@ int launch_score(const ScoreParams &P, int rows, cudaStream_t st) {
   if (total >= (int64_t(1) << 31)) return KV4_ERR_UNSUPPORTED;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(static_cast<unsigned>(
-      std::min<int64_t>(static_cast<int64_t>(sm_count()) * (HALF ? 4 : BLOCKS), (total + NW - 1) / NW)));
+      std::min<int64_t>(static_cast<int64_t>(sm_count()) * (HALF ? 4 : 3), (total + NW - 1) / NW)));
   cfg.blockDim = dim3(NW * 32);
   cfg.stream = st;
   cudaLaunchAttribute at{};
@@ -631,13 +677,13 @@ int by_shape(const TreeParams &T, F f) {
 // rows of `pw` code bytes and `bytes` scale bytes without gaps between tokens
 bool close_rows(const RowSource &S, int64_t B, int Hkv, int64_t T, int pw, int bytes) {
   if (T == 0) return true;
-  const int e = bytes / 2;  // scales of a row: a power of two
+  const int e = bytes / 2;  // scales of a row
   if (T > 1 && (S.kps[2] != pw || S.vps[2] != pw || S.kss[2] != e || S.vss[2] != e)) return false;
-  if ((reinterpret_cast<uintptr_t>(S.ks) & (bytes - 1))) return false;
-  if (S.kss[3] != 1 || S.vss[3] != 1 || (Hkv > 1 && S.kss[1] % e) ||
-      (B > 1 && S.kss[0] % e))
-    return false;
-  return (reinterpret_cast<uintptr_t>(S.vs) & 1u) == 0;
+  // scales are copied four bytes at a time
+  if ((reinterpret_cast<uintptr_t>(S.ks) | reinterpret_cast<uintptr_t>(S.vs)) & 3u) return false;
+  for (const int64_t *st : {S.kss, S.vss})
+    if (st[3] != 1 || (Hkv > 1 && st[1] % 2) || (B > 1 && st[0] % 2)) return false;
+  return true;
 }
 
 }  // namespace
