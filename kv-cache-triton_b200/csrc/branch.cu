@@ -43,7 +43,7 @@ struct GenPlan {
 };
 
 template <int DC, int RW>
-__global__ void tree_generic(const TreeParams P, const GenPlan L) {
+__global__ void __launch_bounds__(128, 1) tree_generic(const TreeParams P, const GenPlan L) {
   extern __shared__ __align__(16) float gsm[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t task = static_cast<int64_t>(blockIdx.x) * L.warps + warp;
@@ -168,7 +168,7 @@ __global__ void tree_generic(const TreeParams P, const GenPlan L) {
 // One warp joins the partial rows of `parts` key ranges: ws_o [parts][rows][d]
 // unnormalised, ws_ml [parts][rows] (base-2 maximum, sum).
 template <int DC>
-__global__ void tree_merge(const __grid_constant__ TreeParams P, const GenPlan L) {
+__global__ void __launch_bounds__(128, 4) tree_merge(const __grid_constant__ TreeParams P, const GenPlan L) {
   const int lane = threadIdx.x & 31;
   const int64_t n = L.units * L.rows;
   const int64_t at = static_cast<int64_t>(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5);
@@ -429,7 +429,7 @@ __device__ __forceinline__ void move_rows(uint8_t *dst, const uint8_t *src, int6
 // A block per (sequence, KV head), 64 threads for each of the four tensors; the
 // block of head 0 writes the new length.  Such a call moves little: what it
 // costs is two rounds of memory latency (lengths and path, then the rows).
-__global__ void __launch_bounds__(4 * CTHREADS) commit_rows(const __grid_constant__ CommitParams P) {
+__global__ void __launch_bounds__(4 * CTHREADS, 2) commit_rows(const __grid_constant__ CommitParams P) {
   __shared__ int32_t path[CPATH];
   const int b = blockIdx.x / P.Hkv, h = blockIdx.x - b * P.Hkv;
   const int k = threadIdx.x / CTHREADS, t = threadIdx.x - k * CTHREADS;

@@ -688,9 +688,21 @@ bool close_rows(const RowSource &S, int64_t B, int Hkv, int64_t T, int pw, int b
 
 }  // namespace
 
+// Whether warps in registers beat tensor-memory tiles (branch_tc.cu, trim_tc.cu).
+// They take 1.3 us per SM for every 16 rows of a 128-key tile, whatever the
+// total; the tiles 2.7 us for up to 128 rows, and about 20 us to get going.
+// Measured (us, warps / tiles; 8 KV heads of 128 columns): 32 rows x 4K keys
+// 20 / 40, batch 8 of them 41 / 59; 64 rows x 4K, batch 1 20 / 43, batch 4
+// 40 / 43, batch 8 76 / 61; 128 rows x 1K 15 / 22; 64 rows x 32K 66 / 65.
+bool few_rows(const TreeParams &T) {
+  const int64_t row_tiles = (static_cast<int64_t>(T.R) * T.nodes + 15) / 16;
+  const int64_t tiles = T.B * T.Hkv * ((T.S + T.ndraft + 127) / 128);
+  return row_tiles <= 2 || tiles * (row_tiles - 2) <= 14 * static_cast<int64_t>(sm_count());
+}
+
 // Whether the kernels of this file take the call: 16-bit queries and scales, the
-// sizes they are built for, rows without gaps that aligned loads can read; and either so few
-// rows that branch_tc.cu's tiles would be mostly padding, or half precision
+// sizes they are built for, rows without gaps that aligned loads can read; and either
+// little to do, or half precision
 // somewhere, which that file leaves alone (a product of a code and an f16 scale
 // does not fit an f16).
 bool tree_mma_takes(const TreeParams &T) {
@@ -707,7 +719,7 @@ bool tree_mma_takes(const TreeParams &T) {
   const int64_t n[3] = {T.B, static_cast<int64_t>(T.Hkv) * T.R, T.nodes};
   for (int i = 0; i < 3; ++i)
     if (n[i] > 1 && (T.qs[i] % 8 || T.os[i] % 8)) return false;
-  return T.R * T.nodes <= 16 || !tree_tc_takes(T);
+  return !tree_tc_takes(T) || few_rows(T);
 }
 
 int tree_mma_parts(const TreeParams &T) { return mma_plan(T).parts; }

@@ -783,9 +783,10 @@ __global__ void __launch_bounds__(THREADS, 1) tree_tc(const __grid_constant__ Tc
 
 // Joins the partial rows of units that fell into several CTAs; units without
 // any key get zeros.  A block takes 32 rows, a lane a row, a warp D / 8 columns.
-// Kept short: a call of few tiles spends as long fetching this code as running it.
+// Four shares are in flight at a time (one block per SM as the launch bound: at
+// the compiler's own choice of 40 registers the loads come one after another).
 template <int D>
-__global__ void __launch_bounds__(256) tree_tc_merge(const __grid_constant__ TcParams P) {
+__global__ void __launch_bounds__(256, 1) tree_tc_merge(const __grid_constant__ TcParams P) {
   constexpr int C = D / 8;
   const TreeParams &T = P.t;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -799,22 +800,31 @@ __global__ void __launch_bounds__(256) tree_tc_merge(const __grid_constant__ TcP
     const int2 share = P.shares[unit * static_cast<int64_t>(P.blocks) + (blockIdx.x >> 3)];
     if (share.x < 0) return;  // written by its CTA
     // the unit is the first segment of every CTA after the one it began in
-    int64_t slot = share.x;
+    constexpr int U = 4;  // shares in flight
 #pragma unroll 1
-    for (int c = share.x >> 1; c <= share.y; ++c) {
-      // rows past the last read what nobody wrote and are dropped
-      const float2 ml = T.ws_ml[slot * WS_ROWS + (row & 255)];
-      const float *o = T.ws_o + (slot * D + warp * C) * WS_ROWS + (row & 255);
-      float v[C];
+    for (int c = share.x >> 1; c <= share.y; c += U) {
+      float2 ml[U];
+      float v[U][C];
 #pragma unroll
-      for (int k = 0; k < C; ++k) v[k] = o[k * WS_ROWS];
-      const float to = fmaxf(m, ml.x), base = to == -INFINITY ? 0.0f : to;
-      const float f = exp2f(m - base), g = exp2f(ml.x - base);
-      m = to;
-      l = fmaf(l, f, g * ml.y);
+      for (int u = 0; u < U; ++u) {
+        const int at = min(c + u, share.y);  // rows past the last read what nobody wrote and are dropped
+        const int64_t slot = at == share.x >> 1 ? share.x : 2 * static_cast<int64_t>(at);
+        ml[u] = T.ws_ml[slot * WS_ROWS + (row & 255)];
+        const float *o = T.ws_o + (slot * D + warp * C) * WS_ROWS + (row & 255);
 #pragma unroll
-      for (int k = 0; k < C; ++k) acc[k] = fmaf(acc[k], f, g * v[k]);
-      slot = 2 * static_cast<int64_t>(c + 1);
+        for (int k = 0; k < C; ++k) v[u][k] = o[k * WS_ROWS];
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        // (past the last one: read again, and weighed with nothing)
+        const float mu = c + u > share.y ? -INFINITY : ml[u].x;
+        const float to = fmaxf(m, mu), base = to == -INFINITY ? 0.0f : to;
+        const float f = exp2f(m - base), g = exp2f(mu - base);
+        m = to;
+        l = fmaf(l, f, g * ml[u].y);
+#pragma unroll
+        for (int k = 0; k < C; ++k) acc[k] = fmaf(acc[k], f, g * v[u][k]);
+      }
     }
   }
   if (row >= P.rows) return;

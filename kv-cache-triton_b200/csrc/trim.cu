@@ -27,7 +27,7 @@ namespace {
 constexpr int SROWS = 8;  // query rows a warp holds at a time
 
 // A warp per 32 keys of one (sequence, KV head).
-__global__ void score_generic(const ScoreParams P, int warps, int ld, int64_t tiles, int64_t tasks) {
+__global__ void __launch_bounds__(128, 2) score_generic(const ScoreParams P, int warps, int ld, int64_t tiles, int64_t tasks) {
   extern __shared__ __align__(16) float ssm[];
   const TreeParams &T = P.t;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -195,7 +195,7 @@ __device__ __forceinline__ uint64_t block_prefix(uint64_t v, uint64_t *warps, ui
 // cluster through distributed shared memory), then prefix sums give every kept
 // token its place.  Scores are read once.
 template <int K>
-__global__ void __launch_bounds__(SEL) evict_select(const __grid_constant__ EvictParams P, int ranks) {
+__global__ void __launch_bounds__(SEL, 1) evict_select(const __grid_constant__ EvictParams P, int ranks) {
   __shared__ uint32_t hist[2][BINS];  // by turns: a block may still read the other
   __shared__ uint64_t warps[32], s_count;
   __shared__ uint32_t s_bin, s_above;
@@ -437,7 +437,7 @@ __global__ void __launch_bounds__(256) evict_gather(const __grid_constant__ Gath
 // Packed rows of CH 16-byte chunks and scale rows of one V each (the usual
 // caches): every thread has all of its loads in flight before its first store.
 template <int CH, typename V>
-__global__ void __launch_bounds__(256) evict_gather_fast(const __grid_constant__ GatherParams P) {
+__global__ void __launch_bounds__(256, 4) evict_gather_fast(const __grid_constant__ GatherParams P) {
   constexpr int ROWS = 256 / CH;  // per block
   const int64_t unit = blockIdx.x / P.tiles, b = unit / P.Hkv, h = unit - b * P.Hkv;
   const int j0 = static_cast<int>(blockIdx.x - unit * P.tiles) * ROWS;
