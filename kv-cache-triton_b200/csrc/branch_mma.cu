@@ -701,10 +701,9 @@ bool few_rows(const TreeParams &T) {
 }
 
 // Whether the kernels of this file take the call: 16-bit queries and scales, the
-// sizes they are built for, rows without gaps that aligned loads can read; and either
-// little to do, or half precision
-// somewhere, which that file leaves alone (a product of a code and an f16 scale
-// does not fit an f16).
+// sizes they are built for, rows without gaps that aligned loads can read; and
+// either little to do, or half precision somewhere, which branch_tc.cu leaves
+// alone (a product of a code and an f16 scale does not fit an f16).
 bool tree_mma_takes(const TreeParams &T) {
   if ((T.q_dtype != KV4_BF16 && T.q_dtype != KV4_F16) || (T.s_dtype != KV4_BF16 && T.s_dtype != KV4_F16))
     return false;

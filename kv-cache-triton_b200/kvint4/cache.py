@@ -43,6 +43,9 @@ class LayerStore:
     # step (kv4_append_attention): the next fused step may then start early
     # (kv4_attn_opts.early_start), since no other kernel wrote the rows it reads
     early_ok: bool = False
+    # [B, n_kv, capacity] f32: attention weight each token received so far
+    # (``track_mass`` stores only)
+    mass_buf: torch.Tensor | None = None
 
     @property
     def capacity(self) -> int:
@@ -71,7 +74,8 @@ class Int4KVStore:
 
     def __init__(self, group_size: int = 32, *, capacity: int | None = None,
                  scale_dtype: torch.dtype | None = None, tie_mode: int = _lib.TIE_HALF_AWAY,
-                 growth: float = 1.5):
+                 growth: float = 1.5, track_mass: bool = False, mass_decay: float = 1.0,
+                 mass_window: int = 32):
         if group_size <= 0:
             raise ValueError("group_size must be > 0")
         self.group_size = int(group_size)
@@ -79,6 +83,13 @@ class Int4KVStore:
         self.scale_dtype = scale_dtype
         self.tie_mode = int(tie_mode)
         self.growth = float(growth)
+        # score the cached tokens by the attention weight they receive: from every
+        # one-token step, and from the last ``mass_window`` queries of a prompt
+        self.track_mass = bool(track_mass)
+        self.mass_decay = float(mass_decay)
+        self.mass_window = int(mass_window)
+        if self.track_mass and self.mass_window <= 0:
+            raise ValueError("mass_window must be > 0")
         self._layers: dict[int, LayerStore] = {}
 
     # -- storage ---------------------------------------------------------
@@ -94,6 +105,7 @@ class Int4KVStore:
             v_packed_buf=torch.empty(b, h, cap, pw, dtype=torch.uint8, device=dev),
             v_scales_buf=torch.empty(b, h, cap, ng, dtype=sdt, device=dev),
             seq_len=0,
+            mass_buf=torch.zeros(b, h, cap, device=dev) if self.track_mass else None,
         )
 
     def append(self, key_states: torch.Tensor, value_states: torch.Tensor, layer_idx: int) -> None:
@@ -104,6 +116,8 @@ class Int4KVStore:
         ops.append_kv(key_states, value_states, layer.k_packed_buf, layer.k_scales_buf,
                       layer.v_packed_buf, layer.v_scales_buf, layer.seq_len, self.group_size,
                       self.tie_mode)
+        if layer.mass_buf is not None:
+            layer.mass_buf[:, :, layer.seq_len:layer.seq_len + s].zero_()
         layer.seq_len += s
         layer.early_ok = False
 
@@ -114,6 +128,9 @@ class Int4KVStore:
         cache, written to ``out`` (any strides, [B, Hq, sq, d]).  A one-token
         decode step is a single launch: the attention kernel quantizes the new
         row itself (``kv4_append_attention``)."""
+        if self.track_mass:
+            self.append(key_states, value_states, layer_idx)
+            return self.attend_scored(query, layer_idx, out, is_causal=is_causal)
         layer = self._reserve(key_states, value_states, layer_idx)
         s = key_states.shape[2]
         if s != 1:
@@ -129,6 +146,57 @@ class Int4KVStore:
         layer.seq_len = n
         layer.early_ok = True
         return out
+
+    # -- scores of the cached tokens ----------------------------------------
+    def attend_scored(self, query: torch.Tensor, layer_idx: int, out: torch.Tensor, *,
+                      is_causal: bool = False) -> torch.Tensor:
+        """Attention of ``query`` over the layer's cache into ``out`` that adds the
+        weight each cached token received to the layer's scores."""
+        layer = self.layer(layer_idx)
+        if layer.mass_buf is None:
+            raise ValueError("the store does not track scores (track_mass=True)")
+        ops.scored_attention_into(query, layer.views(), self.mass(layer_idx), self.mass(layer_idx),
+                                  out, self.group_size, is_causal, self.mass_decay)
+        return out
+
+    def score_window(self, query: torch.Tensor, layer_idx: int) -> None:
+        """Score the layer's tokens by the last ``mass_window`` queries of
+        ``query`` [B, Hq, s, d], which belong to the cache's last s tokens."""
+        q = query[:, :, -self.mass_window:]
+        self.attend_scored(q, layer_idx, torch.empty(q.shape, dtype=q.dtype, device=q.device),
+                           is_causal=True)
+
+    def mass(self, layer_idx: int) -> torch.Tensor:
+        """Scores [B, n_kv, seq_len] of a layer's tokens (a view)."""
+        layer = self.layer(layer_idx)
+        if layer.mass_buf is None:
+            raise ValueError("the store does not track scores (track_mass=True)")
+        return layer.mass_buf[:, :, :layer.seq_len]
+
+    def evict(self, keep: int, *, recent: int = 0, sinks: int = 0) -> dict[int, torch.Tensor]:
+        """Cut every layer that holds more than ``keep`` tokens to the first
+        ``sinks``, the last ``recent`` and the highest scored of the rest, per KV
+        head, in token order; returns the kept token numbers
+        ``{layer: int32 [B, n_kv, keep]}`` of the layers that were cut."""
+        if not 0 <= recent + sinks <= keep or recent < 0 or sinks < 0:
+            raise ValueError("keep must be at least recent + sinks, all >= 0")
+        kept = {}
+        for layer_idx, old in self._layers.items():
+            if old.seq_len <= keep:
+                continue
+            mass = self.mass(layer_idx)
+            b, h, cap, _ = old.k_packed_buf.shape
+            new_cap = min(cap, _round_up(max(int(keep * self.growth), self.capacity_hint,
+                                             CAPACITY_ALIGN), CAPACITY_ALIGN))
+            bufs = [torch.empty(b, h, new_cap, t.shape[-1], dtype=t.dtype, device=t.device)
+                    for t in (old.k_packed_buf, old.k_scales_buf, old.v_packed_buf, old.v_scales_buf)]
+            new = LayerStore(*bufs, seq_len=keep, mass_buf=torch.zeros(b, h, new_cap, device=mass.device))
+            index = torch.empty(b, h, keep, dtype=torch.int32, device=mass.device)
+            ops.evict_into(mass, old.views(), new.views(), new.mass_buf[:, :, :keep], index,
+                           recent, sinks)
+            self._layers[layer_idx] = new
+            kept[layer_idx] = index
+        return kept
 
     def _reserve(self, key_states: torch.Tensor, value_states: torch.Tensor,
                  layer_idx: int) -> LayerStore:
@@ -161,6 +229,8 @@ class Int4KVStore:
                         (grown.k_packed_buf, grown.k_scales_buf, grown.v_packed_buf,
                          grown.v_scales_buf)):
                     dst[:, :, :n].copy_(src[:, :, :n])
+                if grown.mass_buf is not None:
+                    grown.mass_buf[:, :, :n].copy_(layer.mass_buf[:, :, :n])
                 grown.seq_len = n
                 layer = grown
                 self._layers[layer_idx] = layer
@@ -179,6 +249,8 @@ class Int4KVStore:
             idx = beam_idx.to(st.k_packed_buf.device)
             for name in ("k_packed_buf", "k_scales_buf", "v_packed_buf", "v_scales_buf"):
                 setattr(st, name, getattr(st, name).index_select(0, idx).contiguous())
+            if st.mass_buf is not None:
+                st.mass_buf = st.mass_buf.index_select(0, idx).contiguous()
             st.early_ok = False
 
     def layer(self, layer_idx: int) -> LayerStore:

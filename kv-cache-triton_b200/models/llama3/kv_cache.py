@@ -24,11 +24,22 @@ class QuantizedKVCache:
     """Per-layer INT4-packed KV cache. Compatible with HF Llama attention."""
 
     def __init__(self, group_size: int = 32, *, capacity: int | None = None,
-                 tie_mode: int = TIE_HALF_AWAY):
+                 tie_mode: int = TIE_HALF_AWAY, track_mass: bool = False, mass_decay: float = 1.0,
+                 mass_window: int = 32):
+        """``track_mass``: score the cached tokens by the attention weight they
+        receive (see ``evict``), from one-token steps and from the last
+        ``mass_window`` queries of a prompt; older weight fades by
+        ``mass_decay`` per call."""
         if group_size <= 0:
             raise ValueError("group_size must be > 0")
         self.group_size = int(group_size)
-        self._store = Int4KVStore(self.group_size, capacity=capacity, tie_mode=tie_mode)
+        self._store = Int4KVStore(self.group_size, capacity=capacity, tie_mode=tie_mode,
+                                  track_mass=track_mass, mass_decay=mass_decay,
+                                  mass_window=mass_window)
+
+    @property
+    def track_mass(self) -> bool:
+        return self._store.track_mass
 
     @property
     def _layers(self):
@@ -96,6 +107,22 @@ class QuantizedKVCache:
         return self._store.append_attend(query, key_states, value_states, layer_idx, out,
                                          n_q_heads=n_q_heads, n_kv_heads=n_kv_heads,
                                          is_causal=is_causal)
+
+    def mass(self, layer_idx: int) -> torch.Tensor:
+        """Scores ``[B, n_kv, S]`` of a layer's tokens (``track_mass`` caches)."""
+        return self._store.mass(layer_idx)
+
+    def score_window(self, query: torch.Tensor, layer_idx: int) -> None:
+        """Score the layer's tokens by the last queries of a prompt."""
+        self._store.score_window(query, layer_idx)
+
+    def evict(self, keep: int, *, recent: int = 0, sinks: int = 0) -> dict[int, torch.Tensor]:
+        """Cut every layer to ``keep`` tokens per KV head: the first ``sinks``, the
+        last ``recent`` and the highest scored of the rest; returns the kept token
+        numbers per layer.  ``get_seq_length`` is then the number of tokens held,
+        no longer the number seen: pass ``position_ids`` to the model yourself
+        (keys keep the rotary positions they were cached with)."""
+        return self._store.evict(int(keep), recent=int(recent), sinks=int(sinks))
 
     def update(
         self,

@@ -15,7 +15,10 @@ runs; everything else is Hugging Face's ``LlamaAttention``:
   against a thin cache view that quantizes the new K/V into the INT4 cache
   and hands HF the cache dequantized in the query's dtype (the reference's
   fallback, :90-99);
-* without a ``QuantizedKVCache``, HF's forward runs unchanged.
+* with a ``TreeKVCache`` (a step of speculative decoding: the tokens are the
+  nodes of a drafted tree), K/V go to the draft buffer and the nodes attend to
+  each sequence's context and to their ancestors; HF's mask is not used;
+* without either cache, HF's forward runs unchanged.
 """
 
 from __future__ import annotations
@@ -27,6 +30,7 @@ from transformers.models.llama.modeling_llama import LlamaAttention, apply_rotar
 
 from kernels.llama3.attention_quant import attention_forward_quant_gqa
 from models.llama3.kv_cache import QuantizedKVCache
+from models.llama3.tree_cache import TreeKVCache
 
 
 class _DequantizedCacheView:
@@ -49,11 +53,12 @@ class LlamaAttentionQuantized(LlamaAttention):
 
     def forward(self, hidden_states: torch.Tensor, position_embeddings=None,
                 attention_mask: torch.Tensor | None = None, past_key_values=None, **kwargs):
-        cache = past_key_values if isinstance(past_key_values, QuantizedKVCache) else None
+        cache = past_key_values if isinstance(past_key_values, (QuantizedKVCache, TreeKVCache)) else None
         if cache is None:
             return super().forward(hidden_states, position_embeddings, attention_mask,
                                    past_key_values, **kwargs)
-        if not (hidden_states.is_cuda and attention_mask is None):
+        tree = isinstance(cache, TreeKVCache)
+        if not tree and not (hidden_states.is_cuda and attention_mask is None):
             return super().forward(hidden_states, position_embeddings, attention_mask,
                                    _DequantizedCacheView(cache), **kwargs)
 
@@ -67,7 +72,9 @@ class LlamaAttentionQuantized(LlamaAttention):
         n_q, n_kv = self.config.num_attention_heads, self.config.num_key_value_heads
         s = q.shape[-2]
         out = torch.empty(*lead, n_q, self.head_dim, dtype=q.dtype, device=q.device)
-        if s == 1:
+        if tree:
+            cache.attend(self.layer_idx, q, k, v, out.transpose(1, 2))
+        elif s == 1:
             cache.append_attend(q, k, v, self.layer_idx, out.transpose(1, 2), n_q_heads=n_q,
                                 n_kv_heads=n_kv)
         else:
@@ -75,6 +82,8 @@ class LlamaAttentionQuantized(LlamaAttention):
             attention_forward_quant_gqa(q, *cache.get_quantized(self.layer_idx), n_q_heads=n_q,
                                         n_kv_heads=n_kv, group_size=self.quant_group_size,
                                         is_causal=True, out=out.transpose(1, 2))
+            if cache.track_mass:
+                cache.score_window(q, self.layer_idx)
         return self.o_proj(out.flatten(-2)), None
 
 

@@ -153,3 +153,40 @@ def test_reference_eviction_by_brute_force():
     assert br.evict_index(mass, 4, 0, 0).tolist() == [[[0, 2, 4, 5]]]
     nan = float("nan")
     assert br.evict_index(torch.tensor([[[nan, 1.0, nan, 1.0]]]), 3, 0, 0).tolist() == [[[0, 1, 3]]]
+
+
+def test_tree_helpers():
+    from models.llama3.tree_cache import accept_greedy, tree_depth, tree_mask
+    parents = torch.tensor([-1, 0, 0, 1, 3, 2, -1])
+    m = tree_mask(parents)
+    assert [sorted(torch.nonzero(r).flatten().tolist()) for r in m] == [
+        [0], [0, 1], [0, 2], [0, 1, 3], [0, 1, 3, 4], [0, 2, 5], [6]]
+    assert tree_depth(parents).tolist() == [0, 1, 1, 2, 3, 2, 0]
+    assert torch.equal(tree_mask(torch.stack((parents, parents)))[1], m)
+    # tokens: node 0 = 9; children 4, 5; grandchild of 5 is 7
+    nodes = torch.tensor([[9, 4, 5, 1, 2, 7, 9], [9, 4, 5, 1, 2, 7, 9]])
+    logits = torch.zeros(2, 7, 12)
+    logits[0, 0, 5] = logits[0, 2, 7] = logits[0, 5, 11] = 1.0  # 0 -> 5 -> 7 -> 11
+    logits[1, 0, 3] = 1.0                                       # nothing fits
+    path, accepted, token = accept_greedy(nodes, parents, logits)
+    assert accepted.tolist() == [3, 1] and token.tolist() == [11, 3]
+    assert path[0, :3].tolist() == [0, 2, 5] and path.dtype == torch.int32
+
+
+def test_tree_cache_refusals():
+    from models.llama3.kv_cache import QuantizedKVCache
+    from models.llama3.tree_cache import TreeKVCache
+    with pytest.raises(ValueError):
+        TreeKVCache(0, 1, 1, 64, capacity=8, max_nodes=4)
+    with pytest.raises(ValueError, match="empty"):
+        TreeKVCache.from_cache(QuantizedKVCache(), extra=4, max_nodes=4)
+    c = TreeKVCache(1, 1, 2, 64, capacity=8, max_nodes=4, device="cpu")
+    with pytest.raises(ValueError, match="begin"):
+        c.attend(0, torch.zeros(1, 4, 2, 64), torch.zeros(1, 2, 2, 64), torch.zeros(1, 2, 2, 64))
+    with pytest.raises(ValueError, match="nodes"):
+        c.begin(torch.ones(5, 5, dtype=torch.bool))
+    with pytest.raises(ValueError, match="bool"):
+        c.begin(torch.ones(2, 2))
+    assert c.get_mask_sizes(torch.arange(3)) == (3, 0) and len(c) == 1
+    with pytest.raises(ValueError):
+        QuantizedKVCache(track_mass=True, mass_window=0)
