@@ -9,9 +9,11 @@
 // threads.  More rows are taken 128 at a time, each pass over the CTA's keys
 // adding to what the last one wrote (same CTA, same order every time).
 //
-// Twelve warps and one that issues, two CTAs per SM: warps 0-3 sum the weights,
-// 4-11 dequantize key tiles (loaded two tiles ahead into registers) into two
-// buffers.  All (unit, tile) pairs are cut evenly over the CTAs.
+// Twelve warps and one that issues, two CTAs per SM: warps 0-3 and 4-7 sum the
+// weights of every other tile (one such group alone took 4500 cycles a tile,
+// twice what the rest needs), 8-11 dequantize key tiles (loaded two tiles ahead
+// into registers) into two buffers.  All (unit, tile) pairs are cut evenly over
+// the CTAs.
 #include <algorithm>
 
 #include "tc_rows.cuh"
@@ -26,6 +28,7 @@ namespace {
 constexpr int KT = 128;       // keys per tile
 constexpr int RT = 128;       // rows per pass
 constexpr int THREADS = 416;
+constexpr int DQ = 128;       // threads that dequantize
 constexpr uint32_t kWaitPolls = 1u << 11;  // of at most 1 ms each
 
 struct STcParams {
@@ -58,7 +61,7 @@ template <int D>
 struct Smem {
   static constexpr int TILE = KT * D * 2;
   static constexpr int Q = 0, K = TILE, END = 3 * TILE;
-  static constexpr int INFO = END;            // float4 [128]: c, -m, 1 / l of a row
+  static constexpr int INFO = END;            // per two rows: float4 (c, c, -m, -m) [64], float2 (1 / l) [64]
   static constexpr int BARS = INFO + 2048;
   static constexpr int MISC = BARS + 128;     // TMEM address, abort flag
   static constexpr int BYTES = MISC + 16;
@@ -87,7 +90,7 @@ struct Waiter {
 template <int D, int G>
 __device__ __forceinline__ void dequant_role(const STcParams &P, Walk walk, const Waiter &W,
                                              uint32_t smem, int tid) {
-  constexpr int RSTEP = 256 / Chunk<D>::CPR, NCH = KT / RSTEP, NS = G < 32 ? 2 : 1;
+  constexpr int RSTEP = DQ / Chunk<D>::CPR, NCH = KT / RSTEP, NS = G < 32 ? 2 : 1;
   using SM = Smem<D>;
   const TreeParams &T = P.s.t;
   struct Regs {
@@ -105,7 +108,7 @@ __device__ __forceinline__ void dequant_role(const STcParams &P, Walk walk, cons
     const bool draft = tile >= P.nctx;
     const int t0 = (draft ? tile - P.nctx : tile) * KT + r0;
     rem = static_cast<int>(draft ? T.ndraft : T.S) - t0;
-    src = source_of<D, G, 256>(T, draft, false, p.b, p.kvh, t0, c);
+    src = source_of<D, G, DQ>(T, draft, false, p.b, p.kvh, t0, c);
   };
   auto load = [&](Regs &r) {  // and step to the tile after it
 #pragma unroll
@@ -208,17 +211,27 @@ __device__ __forceinline__ void mma_role(const STcParams &P, Walk walk, const Wa
   }
 }
 
-// Weights of 32 rows for this thread's key, in row order.  FROM: rows below
-// `from` do not see the key.
+// Weights of 32 rows for this thread's key, in row order: even and odd rows
+// apart.  FROM: rows below `from` do not see the key.
 template <bool FROM>
-__device__ __forceinline__ void add32(const uint32_t (&s)[32], uint32_t info, int from, float &t0,
-                                      float &t1) {
+__device__ __forceinline__ void add32(const uint32_t (&s)[32], uint32_t info, uint32_t inv, int from,
+                                      uint64_t &sum) {
 #pragma unroll
-  for (int e = 0; e < 32; ++e) {
-    const uint4 v = lds128(info + 16 * e);  // c, -m, 1 / l
-    const float w = fast_exp2(fmaf(__uint_as_float(s[e]), __uint_as_float(v.x), __uint_as_float(v.y)));
-    float &t = (e & 1) ? t1 : t0;
-    if (!FROM || e >= from) t = fmaf(w, __uint_as_float(v.z), t);
+  for (int e = 0; e < 32; e += 2) {
+    const uint4 v = lds128(info + 8 * e);  // c, c, -m, -m
+    const uint2 li = lds64(inv + 4 * e);
+    float x0, x1;
+    unpair(fma2(pair(__uint_as_float(s[e]), __uint_as_float(s[e + 1])),
+                pair(__uint_as_float(v.x), __uint_as_float(v.y)),
+                pair(__uint_as_float(v.z), __uint_as_float(v.w))),
+           x0, x1);
+    x0 = fast_exp2(x0);
+    x1 = fast_exp2(x1);
+    if (FROM) {
+      if (e < from) x0 = 0.0f;
+      if (e + 1 < from) x1 = 0.0f;
+    }
+    sum = fma2(pair(x0, x1), pair(__uint_as_float(li.x), __uint_as_float(li.y)), sum);
   }
 }
 
@@ -227,8 +240,9 @@ __device__ __forceinline__ void sum_role(const STcParams &P, Walk walk, const Wa
                                          uint32_t smem, uint32_t tmem, int tid) {
   using SM = Smem<D>;
   const TreeParams &T = P.s.t;
-  const int lane = tid & 31;
-  const uint32_t tS = tmem + (static_cast<uint32_t>(tid >> 5) << 21);
+  const int lane = tid & 31, r = tid & 127;
+  const uint32_t group = tid >> 7;  // takes the tiles of its parity, in its own buffer
+  const uint32_t tS = tmem + 128 * group + (static_cast<uint32_t>((tid >> 5) & 3) << 21);
   Part p;
   uint32_t n = 0;
   while (walk.next(P, p)) {
@@ -237,52 +251,65 @@ __device__ __forceinline__ void sum_role(const STcParams &P, Walk walk, const Wa
     float *out = P.s.out + p.b * P.s.os[0] + p.kvh * P.s.os[1];
 #pragma unroll 1
     for (int pass = 0; pass < P.passes; ++pass) {
-      const int row = pass * RT + tid, cols = pass_cols(P, pass);
-      // all products with the last queries are complete: this thread has read
-      // their scores
-      asm volatile("bar.sync 1, 128;" ::: "memory");
-      const float c0 = load_query_row<D>(T, P.rows, p.b, p.kvh, row, smem + SM::Q, tid, true);
-      float4 f = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-      if (row < P.rows) {
-        const float2 st = T.stats[static_cast<int64_t>(unit) * P.rows + row];
-        // a row that saw nothing weighs nothing: 2^0 * 0
-        if (st.y != 0.0f) f = make_float4(c0, -st.x, st.y, 0.0f);
+      const int cols = pass_cols(P, pass);
+      // all products with the last queries are complete: their scores have been
+      // read, and what the last pass added can be read
+      asm volatile("bar.sync 1, 256;" ::: "memory");
+      if (group == 0) {
+        const int row = pass * RT + r;
+        const float c0 = load_query_row<D>(T, P.rows, p.b, p.kvh, row, smem + SM::Q, r, true);
+        float c = 0.0f, nm = 0.0f, li = 0.0f;
+        if (row < P.rows) {
+          const float2 st = T.stats[static_cast<int64_t>(unit) * P.rows + row];
+          // a row that saw nothing weighs nothing: 2^0 * 0
+          if (st.y != 0.0f) {
+            c = c0;
+            nm = -st.x;
+            li = st.y;
+          }
+        }
+        float *info = reinterpret_cast<float *>(__cvta_shared_to_generic(smem + SM::INFO));
+        info[(r >> 1) * 4 + (r & 1)] = c;
+        info[(r >> 1) * 4 + 2 + (r & 1)] = nm;
+        info[256 + r] = li;
+        tc::fence_smem();
+        tc::fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(W.at(QREADY));
       }
-      tc::sts128(smem + SM::INFO + 16 * tid, __float_as_uint(f.x), __float_as_uint(f.y),
-                 __float_as_uint(f.z), 0u);
-      tc::fence_smem();
-      tc::fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(W.at(QREADY));
-      asm volatile("bar.sync 1, 128;" ::: "memory");  // everyone's rows are in INFO
+      asm volatile("bar.sync 1, 256;" ::: "memory");  // everyone's rows are in INFO
 #pragma unroll 1
       for (int i = 0; i < p.ntiles; ++i, ++n) {
+        if ((n & 1u) != group) continue;
         const int tile = p.tile + i;
         const bool draft = tile >= P.nctx;
-        const int key = (draft ? tile - P.nctx : tile) * KT + tid;  // within its source
+        const int key = (draft ? tile - P.nctx : tile) * KT + r;  // within its source
         const bool ok = key < (draft ? T.ndraft : static_cast<int>(T.S));
         const int64_t t = draft ? T.S + key : key;
-        float old = 0.0f;
-        if (ok) old = pass == 0 ? in[t * P.s.is[2]] * P.s.decay : out[t * P.s.os[2]];
-        const uint32_t st = n & 1u;
-        W.wait(SFULL + st, n >> 1);
+        const float *from_where = pass == 0 ? in + t * P.s.is[2] : out + t * P.s.os[2];
+        float old = 0.0f;  // not used before the sums are there
+        if (ok) old = *from_where;
+        W.wait(SFULL + group, n >> 1);
         tc::fence_after();
         // query i sees drafted key j iff j <= i + shift
         const int from = draft && T.causal ? max(0, key - T.shift) * T.R - pass * RT : 0;
         const bool some = __any_sync(0xffffffffu, from > 0);
-        float t0 = 0.0f, t1 = 0.0f;
+        uint64_t sum = 0;
 #pragma unroll 1
         for (int c = 0; c < cols; c += 32) {
           uint32_t s[32];
-          tc::ld32(tS + 128 * st + c, s);
+          tc::ld32(tS + c, s);
           tc::wait_ld(s);
-          if (some) add32<true>(s, smem + SM::INFO + 16 * c, from - c, t0, t1);
-          else add32<false>(s, smem + SM::INFO + 16 * c, 0, t0, t1);
+          const uint32_t info = smem + SM::INFO + 8 * c;
+          if (some) add32<true>(s, info, info + 1024 - 4 * c, from - c, sum);
+          else add32<false>(s, info, info + 1024 - 4 * c, 0, sum);
         }
         tc::fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(W.at(SEMPTY + st));
-        if (ok) out[t * P.s.os[2]] = old + (t0 + t1);
+        if (lane == 0) mbar_arrive(W.at(SEMPTY + group));
+        float t0, t1;
+        unpair(sum, t0, t1);
+        if (ok) out[t * P.s.os[2]] = fmaf(old, pass == 0 ? P.s.decay : 1.0f, t0 + t1);
       }
     }
   }
@@ -299,8 +326,8 @@ __global__ void __launch_bounds__(THREADS, 2) score_tc(const __grid_constant__ S
     if (tid == 0) atomicOr(&g_trim_error_tc, DEV_ERR_MBAR_TIMEOUT);
     return;
   }
-  if (warp == 4) {
-    if (lane < NBARS) mbar_init(W.at(lane), lane < KEMPTY ? 8 : lane < SEMPTY ? 1 : 4);
+  if (warp == 8) {
+    if (lane < NBARS) mbar_init(W.at(lane), lane >= KEMPTY && lane < SEMPTY ? 1 : 4);
     fence_mbar_init();
     if (lane == 0) *reinterpret_cast<volatile uint32_t *>(smem_raw + SM::MISC + 4) = 0u;
   }
@@ -313,8 +340,8 @@ __global__ void __launch_bounds__(THREADS, 2) score_tc(const __grid_constant__ S
   const uint32_t each = P.total / gridDim.x, rest = P.total - each * gridDim.x;
   const Walk walk{blockIdx.x * each + min(blockIdx.x, rest), each + (blockIdx.x < rest ? 1u : 0u)};
   griddep_wait();  // the rows' maxima and sums come from the kernel before
-  if (warp < 4) sum_role<D>(P, walk, W, smem, tmem, tid);
-  else if (warp < 12) dequant_role<D, G>(P, walk, W, smem, tid - 128);
+  if (warp < 8) sum_role<D>(P, walk, W, smem, tmem, tid);
+  else if (warp < 12) dequant_role<D, G>(P, walk, W, smem, tid - 256);
   else mma_role<D>(P, walk, W, smem, tmem);
   __syncwarp();
   tc::fence_before();
