@@ -3,18 +3,18 @@
 //
 // The mathematics is branch.cu's.  All rows (node, q head of the group) that
 // read one KV head form the M dimension, 128 at a time, so a tile of 128 keys
-// is dequantized once for up to 256 rows.  One CTA per SM, 28 warps:
+// is dequantized once for up to 256 rows.  One CTA per SM, 20 warps:
 //
 //   warps 0-7    softmax: two streams of 128 threads, a thread per row.  A
 //                stream reads its scores from tensor memory, keeps the running
 //                maximum and sum, writes the weights back as f16 over the
 //                scores, and rescales its output accumulator when the maximum
 //                moved by more than 2^8 (seldom).
-//   warps 8-23   dequantization, eight warps each for K and V: chunks of 16 bytes
+//   warps 8-15   dequantization, four warps each for K and V: chunks of 16 bytes
 //                (32 codes), loaded two tiles ahead into registers, to f16 tiles
 //                in the swizzled layout of the matrix descriptors, double-buffered.
-//   warp 24      an elected lane issues S = Q K^T and O += P V for both streams.
-//   warps 25-27  turn the mask bytes of drafted tiles into 128 bits per row.
+//   warp 16      an elected lane issues S = Q K^T and O += P V for both streams.
+//   warps 17-19  turn the mask bytes of drafted tiles into 128 bits per row.
 //
 // With more than 128 rows the streams are two row tiles that share every
 // dequantized key tile; with fewer they are the even and odd key tiles of one
@@ -44,8 +44,8 @@ __device__ int g_branch_error_tc = 0;
 namespace {
 
 constexpr int KT = 128;      // keys per tile
-constexpr int THREADS = 896;  // seven warpgroups of 72 registers a thread, shared out below
-constexpr int DQ = 256;       // threads that dequantize K, and V
+constexpr int THREADS = 640;  // five warpgroups of 96 registers a thread, shared out below
+constexpr int DQ = 128;       // threads that dequantize K, and V
 constexpr float kWeightShift = 7.0f;  // weights are written times 2^7: f16 then resolves 2^-31 of the largest
 constexpr uint32_t kWaitPolls = 1u << 11;  // of at most 1 ms each
 
@@ -125,7 +125,7 @@ struct Smem {
 enum Bar { KFULL = 0, VFULL = 2, KEMPTY = 4, VEMPTY = 6, SFULL = 8, PREADY = 10, OREADY = 12,
            MFULL = 14, MEMPTY = 16, QREADY = 18, NBARS = 19 };
 __device__ __forceinline__ int bar_count(int i) {
-  if (i < KEMPTY) return 8;           // dequantizing warps of K, of V
+  if (i < KEMPTY) return 4;           // dequantizing warps of K, of V
   if (i < PREADY) return 1;           // commits
   if (i < OREADY) return 4;           // a stream's warps
   if (i < MFULL) return 1;
@@ -155,7 +155,7 @@ struct Waiter {
 __device__ __forceinline__ void bar_softmax() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
 
 // ---------------------------------------------------------------------------
-// Eight warps dequantize K, eight V, each at their own pace: scores are asked for a
+// Four warps dequantize K, four V, each at their own pace: scores are asked for a
 // tile ahead of the products with V, so that V must not hold up K.
 template <int D, int G>
 __device__ __forceinline__ void dequant_role(const TcParams &P, Walk walk, const Waiter &W,
@@ -227,7 +227,7 @@ __device__ __forceinline__ void dequant_role(const TcParams &P, Walk walk, const
     W.wait((is_v ? VEMPTY : KEMPTY) + st, use + 1u);  // passes at once for the first use of a stage
     if (r.draft) {
       if (tid < 4) asm volatile("st.shared.u32 [%0], %1;" ::"r"(bad + 4 * tid), "r"(0u) : "memory");
-      asm volatile("bar.sync %0, 256;" ::"r"(is_v ? 3 : 2) : "memory");
+      asm volatile("bar.sync %0, 128;" ::"r"(is_v ? 3 : 2) : "memory");
     }
 #pragma unroll
     for (int k = 0; k < NCH; ++k) {
@@ -712,7 +712,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_tc(const __grid_constant__ Tc
     if (lane < 24) reinterpret_cast<uint32_t *>(smem_raw + SM::BAD)[lane] = 0u;
     if (lane == 0) *reinterpret_cast<volatile uint32_t *>(smem_raw + SM::MISC + 4) = 0u;
   }
-  if (warp == 24) tc::alloc(smem + SM::MISC, 512);
+  if (warp == 16) tc::alloc(smem + SM::MISC, 512);
   if (warp == 8) {
     // This CTA's share: all tiles of all units lie end to end, W / n of them for
     // each CTA and one more for the first W % n.  Sequences 32 at a time, by
@@ -762,23 +762,25 @@ __global__ void __launch_bounds__(THREADS, 1) tree_tc(const __grid_constant__ Tc
   const uint32_t tmem =
       __shfl_sync(0xffffffffu, *reinterpret_cast<volatile uint32_t *>(smem_raw + SM::MISC), 0);
   const Walk walk{static_cast<uint32_t>(start[0]), start[1], start[2], start[3], start[4], true};
-  // 128 * (2 * 120 + 4 * 56 + 40) = 896 * 72 registers
+  // 128 * (2 * 104 + 2 * 96 + 80) = 640 * 96 registers: no role spills.  Sixteen
+  // dequantizing warps (896 threads of 72 registers) spill: 160 us instead of 148
+  // at 64 nodes x 16K x 64 heads, batch 4.
   if (warp < 8) {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 120;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 104;");
     softmax_role<D>(P, walk, W, smem, tmem, tid);
-  } else if (warp < 24) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
-    dequant_role<D, G>(P, walk, W, smem, warp >= 16, tid & 255);
+  } else if (warp < 16) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
+    dequant_role<D, G>(P, walk, W, smem, warp >= 12, tid & 127);
   } else {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
-    if (warp == 24) mma_role<D>(P, walk, W, smem, tmem);
-    else mask_role<D>(P, walk, W, smem, warp - 25, lane);
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+    if (warp == 16) mma_role<D>(P, walk, W, smem, tmem);
+    else mask_role<D>(P, walk, W, smem, warp - 17, lane);
   }
   __syncwarp();
   tc::fence_before();
   __syncthreads();
   tc::fence_after();
-  if (warp == 24) tc::dealloc(tmem, 512);
+  if (warp == 16) tc::dealloc(tmem, 512);
 }
 
 // Joins the partial rows of units that fell into several CTAs; units without
