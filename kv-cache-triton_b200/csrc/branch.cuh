@@ -34,6 +34,7 @@ struct TreeParams {
   const int32_t *lens;  // context rows of each sequence, or null: all of them
   int64_t B;
   int Hkv, R, nodes, ndraft, d, G, causal, shift;
+  int words;           // rows can be read in 4-byte words of eight codes of one group
   int64_t S;           // context rows in the cache views
   float scale_log2;    // sm_scale * log2(e)
   float2 *stats;       // per (unit, row): base-2 maximum and 1 / sum; or null
@@ -78,63 +79,132 @@ inline int copy_width(const void *dst, const void *src, int bytes, const int64_t
   return v;
 }
 
-// one score row set of 8 elements: codes of columns [8c, 8c+8) of a packed row
-// as floats times their scale; columns at or past d are 0
-__device__ __forceinline__ void dequant8(const uint8_t *row, int64_t cs, const void *srow,
-                                         int64_t scs, int sdt, int G, int pb, int d, int c,
-                                         float (&v)[8]) {
-  const int e0 = 8 * c;
-  if ((G & 7) == 0 && cs == 1 && e0 + 8 <= d &&
-      ((reinterpret_cast<uintptr_t>(row) + (e0 >> 1)) & 3) == 0) {
-    const uint32_t w = __ldg(reinterpret_cast<const uint32_t *>(row + (e0 >> 1)));
-    const float s = load_as_f32(srow, sdt, (e0 / G) * scs);
+// 8 elements of a packed row as floats times their scale, element by element:
+// columns [8c, 8c + 8), those at or past d are 0
+template <typename ST>
+__device__ __forceinline__ void dequant8(const uint8_t *row, int64_t cs, const ST *srow, int64_t scs,
+                                         int G, int pb, int d, int c, float (&v)[8]) {
 #pragma unroll
-    for (int k = 0; k < 8; ++k) v[k] = static_cast<float>(static_cast<int>((w >> (4 * k)) & 15u) - 8) * s;
-  } else {
-#pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      const int e = e0 + k;
-      v[k] = 0.0f;
-      if (e < d) {
-        const int g = e / G, nib = g * 2 * pb + (e - g * G);
-        const uint32_t byte = row[(nib >> 1) * cs];
-        const int code = (nib & 1) ? byte >> 4 : byte & 15;
-        v[k] = static_cast<float>(code - 8) * load_as_f32(srow, sdt, g * scs);
-      }
+  for (int k = 0; k < 8; ++k) {
+    const int e = 8 * c + k;
+    v[k] = 0.0f;
+    if (e < d) {
+      const int g = e / G, nib = g * 2 * pb + (e - g * G);
+      const uint32_t byte = row[(nib >> 1) * cs];
+      const int code = (nib & 1) ? byte >> 4 : byte & 15;
+      v[k] = static_cast<float>(code - 8) * to_f32(srow[g * scs]);
     }
   }
 }
 
 // 32 rows (keys t0 .. t0+31 of `len` context rows then draft rows) of K or V
 // as floats in shared memory, ld floats apart, by one warp; rows at or past
-// `end` are 0.  d is padded with zeros to a multiple of 8.
-__device__ __forceinline__ void warp_dequant_tile(const TreeParams &P, bool is_v, int64_t b, int h,
+// `end` are 0.  d is padded with zeros to a multiple of 8.  Where rows allow it
+// a lane takes eight columns per word, four words in flight.
+template <typename ST>
+__device__ __forceinline__ void warp_dequant_rows(const TreeParams &P, bool is_v, int64_t b, int h,
                                                   int64_t len, int64_t t0, int64_t end, float *dst,
                                                   int ld, int lane) {
   const int d8 = (P.d + 7) >> 3, pb = (P.G + 1) >> 1;
+  auto row_of = [&](int64_t t, const uint8_t *&p, const ST *&s, int64_t &cs, int64_t &scs) {
+    const bool ctx = t < len;
+    const RowSource &S = ctx ? P.cache : P.draft;
+    const int64_t row = ctx ? t : t - len;
+    const int64_t *ps = is_v ? S.vps : S.kps, *ss = is_v ? S.vss : S.kss;
+    p = (is_v ? S.vp : S.kp) + b * ps[0] + h * ps[1] + row * ps[2];
+    s = static_cast<const ST *>(is_v ? S.vs : S.ks) + b * ss[0] + h * ss[1] + row * ss[2];
+    cs = ps[3];
+    scs = ss[3];
+  };
+  if (P.words) {
+    const int lg = __ffs(P.G) - 1;  // groups of a power of two, at least 8
+#pragma unroll 1
+    for (int i0 = lane; i0 < 32 * d8; i0 += 4 * 32) {
+      uint32_t w[4];
+      ST s[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int idx = i0 + 32 * u, r = idx / d8, c = idx - r * d8;
+        w[u] = 0x88888888u;
+        s[u] = from_f32<ST>(0.0f);
+        if (idx < 32 * d8 && t0 + r < end) {
+          const uint8_t *p;
+          const ST *q;
+          int64_t cs, scs;
+          row_of(t0 + r, p, q, cs, scs);
+          w[u] = __ldg(reinterpret_cast<const uint32_t *>(p) + c);
+          s[u] = q[((8 * c) >> lg) * scs];
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int idx = i0 + 32 * u, r = idx / d8, c = idx - r * d8;
+        if (idx >= 32 * d8) break;
+        const float f = to_f32(s[u]);
+        float v[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] = static_cast<float>(static_cast<int>((w[u] >> (4 * k)) & 15u) - 8) * f;
+        float4 *o = reinterpret_cast<float4 *>(dst + r * ld + 8 * c);
+        o[0] = make_float4(v[0], v[1], v[2], v[3]);
+        o[1] = make_float4(v[4], v[5], v[6], v[7]);
+      }
+    }
+    return;
+  }
+#pragma unroll 1
   for (int idx = lane; idx < 32 * d8; idx += 32) {
     const int r = idx / d8, c = idx - r * d8;
-    const int64_t t = t0 + r;
-    float v[8];
-    if (t < end) {
-      const bool ctx = t < len;
-      const RowSource &S = ctx ? P.cache : P.draft;
-      const int64_t row = ctx ? t : t - len;
-      const uint8_t *p = is_v ? S.vp : S.kp;
-      const int64_t *ps = is_v ? S.vps : S.kps, *ss = is_v ? S.vss : S.kss;
-      const int64_t so = b * ss[0] + h * ss[1] + row * ss[2];
-      const char *sp = static_cast<const char *>(is_v ? S.vs : S.ks) +
-                       so * (P.s_dtype == KV4_F32 ? 4 : 2);
-      dequant8(p + b * ps[0] + h * ps[1] + row * ps[2], ps[3], sp, ss[3], P.s_dtype, P.G, pb, P.d,
-               c, v);
-    } else {
-#pragma unroll
-      for (int k = 0; k < 8; ++k) v[k] = 0.0f;
+    float v[8] = {};
+    if (t0 + r < end) {
+      const uint8_t *p;
+      const ST *q;
+      int64_t cs, scs;
+      row_of(t0 + r, p, q, cs, scs);
+      dequant8<ST>(p, cs, q, scs, P.G, pb, P.d, c, v);
     }
     float4 *o = reinterpret_cast<float4 *>(dst + r * ld + 8 * c);
     o[0] = make_float4(v[0], v[1], v[2], v[3]);
     o[1] = make_float4(v[4], v[5], v[6], v[7]);
   }
+}
+__device__ __forceinline__ void warp_dequant_tile(const TreeParams &P, bool is_v, int64_t b, int h,
+                                                  int64_t len, int64_t t0, int64_t end, float *dst,
+                                                  int ld, int lane) {
+  if (P.s_dtype == KV4_F32) warp_dequant_rows<float>(P, is_v, b, h, len, t0, end, dst, ld, lane);
+  else if (P.s_dtype == KV4_F16) warp_dequant_rows<__half>(P, is_v, b, h, len, t0, end, dst, ld, lane);
+  else warp_dequant_rows<__nv_bfloat16>(P, is_v, b, h, len, t0, end, dst, ld, lane);
+}
+
+// Rows [row0, row0 + n) of a KV head's queries (row = node * R + head of the
+// group) as floats in shared memory, ld apart, by one warp; rows at or past
+// `rows` and columns past d are 0.
+template <typename QT>
+__device__ __forceinline__ void warp_query_rows(const TreeParams &P, int64_t b, int kvh, int row0, int n,
+                                                int rows, float *dst, int ld, int lane) {
+  const int w = (P.d + 7) & ~7;
+#pragma unroll 1
+  for (int i0 = lane; i0 < n * w; i0 += 8 * 32) {
+    QT v[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      const int idx = i0 + 32 * u, r = idx / w, c = idx - r * w, row = row0 + r;
+      const int i = row / P.R, h = kvh * P.R + row - i * P.R;
+      v[u] = from_f32<QT>(0.0f);
+      if (idx < n * w && row < rows && c < P.d)
+        v[u] = static_cast<const QT *>(P.q)[b * P.qs[0] + h * P.qs[1] + i * P.qs[2] + c * P.qs[3]];
+    }
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      const int idx = i0 + 32 * u, r = idx / w;
+      if (idx < n * w) dst[r * ld + idx - r * w] = to_f32(v[u]);
+    }
+  }
+}
+__device__ __forceinline__ void warp_query(const TreeParams &P, int64_t b, int kvh, int row0, int n,
+                                           int rows, float *dst, int ld, int lane) {
+  if (P.q_dtype == KV4_F32) warp_query_rows<float>(P, b, kvh, row0, n, rows, dst, ld, lane);
+  else if (P.q_dtype == KV4_F16) warp_query_rows<__half>(P, b, kvh, row0, n, rows, dst, ld, lane);
+  else warp_query_rows<__nv_bfloat16>(P, b, kvh, row0, n, rows, dst, ld, lane);
 }
 
 // shared-memory row length of a d-wide row: float4 steps, an odd number of

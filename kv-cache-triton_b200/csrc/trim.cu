@@ -43,13 +43,7 @@ __global__ void __launch_bounds__(128, 2) score_generic(const ScoreParams P, int
   for (int r0 = 0; r0 < rows; r0 += SROWS) {
     __syncwarp();
     const int nr = min(SROWS, rows - r0);
-    for (int r = 0; r < nr; ++r) {
-      const int row = r0 + r, i = row / T.R, h = kvh * T.R + row - i * T.R;
-      for (int c = lane; c < 8 * d8; c += 32)
-        sQ[r * ld + c] = c < T.d ? load_as_f32(T.q, T.q_dtype,
-                                               b * T.qs[0] + h * T.qs[1] + i * T.qs[2] + c * T.qs[3])
-                                 : 0.0f;
-    }
+    warp_query(T, b, kvh, r0, nr, rows, sQ, ld, lane);
     __syncwarp();
     float s[SROWS];
 #pragma unroll
