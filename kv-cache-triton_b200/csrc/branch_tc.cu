@@ -762,9 +762,10 @@ __global__ void __launch_bounds__(THREADS, 1) tree_tc(const __grid_constant__ Tc
   const uint32_t tmem =
       __shfl_sync(0xffffffffu, *reinterpret_cast<volatile uint32_t *>(smem_raw + SM::MISC), 0);
   const Walk walk{static_cast<uint32_t>(start[0]), start[1], start[2], start[3], start[4], true};
-  // 128 * (2 * 104 + 2 * 96 + 80) = 640 * 96 registers: no role spills.  Sixteen
-  // dequantizing warps (896 threads of 72 registers) spill: 160 us instead of 148
-  // at 64 nodes x 16K x 64 heads, batch 4.
+  // 128 * (2 * 104 + 2 * 96 + 80) = 640 * 96 registers: nothing spills but
+  // groups of 16 of 128 columns, a little.  Sixteen dequantizing warps (896
+  // threads of 72 registers) all spill: 160 us instead of 148 at 64 nodes x 16K x
+  // 64 heads, batch 4.
   if (warp < 8) {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 104;");
     softmax_role<D>(P, walk, W, smem, tmem, tid);
