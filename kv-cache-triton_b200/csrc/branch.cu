@@ -20,7 +20,7 @@
 // take branch_tc.cu's kernel where the layout allows.
 #include <algorithm>
 
-#include "branch.cuh"
+#include "merge.cuh"
 
 namespace kv4 {
 
@@ -35,12 +35,6 @@ __device__ __forceinline__ float warp_max(float v) {
   for (int o = 16; o; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
   return v;
 }
-
-struct GenPlan {
-  int64_t units, tasks;  // units = B * Hkv; tasks = units * row_tiles * parts
-  int rows, row_tiles, parts, warps, ld;
-  size_t smem;
-};
 
 template <int DC, int RW>
 __global__ void __launch_bounds__(128, 1) tree_generic(const TreeParams P, const GenPlan L) {
@@ -96,6 +90,10 @@ __global__ void __launch_bounds__(128, 1) tree_generic(const TreeParams P, const
       bool see = t < k1 && row < L.rows;
       if (see && t >= len) see = draft_visible(P, b, row / P.R, static_cast<int>(t - len));
       const float x = see ? s[r] * P.scale_log2 : -INFINITY;
+      if (P.kept && t < k1 && row < L.rows) {
+        const int64_t slot = t < len ? t : ((len + 15) & ~int64_t(15)) + t - len;
+        P.kept[kept_at(unit, kept_blocks(P), slot, row, L.rows)] = see ? s[r] : -INFINITY;
+      }
       const float mn = fmaxf(m[r], warp_max<RW>(x));
       const float base = mn == -INFINITY ? 0.0f : mn;
       const float a = exp2f(m[r] - base), p = exp2f(x - base);
@@ -133,6 +131,7 @@ __global__ void __launch_bounds__(128, 1) tree_generic(const TreeParams P, const
     const int row = r0 + r;
     if (row >= L.rows) continue;
     const int64_t at = unit * L.rows + row;
+    if (P.kept && part == 0 && lane == 0) P.kept_c[at] = P.scale_log2;
     if (L.parts == 1) {
       const int i = row / P.R, h = kvh * P.R + row - i * P.R;
       const float inv = l[r] > 0.0f ? 1.0f / l[r] : 0.0f;
@@ -158,48 +157,11 @@ __global__ void __launch_bounds__(128, 1) tree_generic(const TreeParams P, const
   }
 }
 
-// One warp joins the partial rows of `parts` key ranges: ws_o [parts][rows][d]
-// unnormalised, ws_ml [parts][rows] (base-2 maximum, sum).
 template <int DC>
 __global__ void __launch_bounds__(128, 4) tree_merge(const __grid_constant__ TreeParams P, const GenPlan L) {
-  const int lane = threadIdx.x & 31;
-  const int64_t n = L.units * L.rows;
   const int64_t at = static_cast<int64_t>(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5);
   griddep_wait();
-  if (at >= n) return;
-  float m = -INFINITY, l = 0.0f, acc[DC];
-#pragma unroll
-  for (int k = 0; k < DC; ++k) acc[k] = 0.0f;
-#pragma unroll 4
-  for (int p = 0; p < L.parts; ++p) {
-    const float2 ml = P.ws_ml[p * n + at];
-    float v[DC];
-#pragma unroll
-    for (int k = 0; k < DC; ++k)
-      v[k] = lane + 32 * k < P.d ? P.ws_o[(p * n + at) * P.d + lane + 32 * k] : 0.0f;
-    const float to = fmaxf(m, ml.x), base = to == -INFINITY ? 0.0f : to;
-    const float f = exp2f(m - base), g = exp2f(ml.x - base);
-    m = to;
-    l = fmaf(l, f, g * ml.y);
-#pragma unroll
-    for (int k = 0; k < DC; ++k) acc[k] = fmaf(acc[k], f, g * v[k]);
-  }
-  const int64_t unit = at / L.rows, b = unit / P.Hkv;
-  const int row = static_cast<int>(at - unit * L.rows), i = row / P.R;
-  const int h = static_cast<int>(unit - b * P.Hkv) * P.R + row - i * P.R;
-  const float inv = l > 0.0f ? 1.0f / l : (l == l ? 0.0f : l);
-#pragma unroll
-  for (int k = 0; k < DC; ++k)
-    if (lane + 32 * k < P.d)
-      store_from_f32(P.out, P.q_dtype,
-                     b * P.os[0] + h * P.os[1] + i * P.os[2] + (lane + 32 * k) * P.os[3],
-                     acc[k] * inv);
-  if (lane == 0) {
-    if (P.stats) P.stats[at] = make_float2(m, inv);
-    if (P.lse)
-      P.lse[b * P.ls[0] + h * P.ls[1] + i * P.ls[2]] =
-          l == 0.0f ? -INFINITY : (m + log2f(l)) * kBrLn2;
-  }
+  if (at < L.units * L.rows) merge_row<DC>(P, L, at, threadIdx.x & 31);
 }
 
 constexpr int kSms = 148;
@@ -252,7 +214,7 @@ int launch_gen(const TreeParams &P, const GenPlan &L, cudaStream_t st) {
   }
   tree_generic<DC, RW><<<static_cast<unsigned>(blocks), 32 * L.warps, L.smem, st>>>(P, L);
   const int rc = cuda_status(cudaGetLastError());
-  if (rc || L.parts == 1) return rc;
+  if (rc || L.parts == 1 || P.kept) return rc;  // score_kept joins the parts itself
   return launch_merge<DC>(P, L, st);
 }
 
@@ -358,16 +320,23 @@ GenPlan mma_merge_plan(const TreeParams &P) {
 }
 }  // namespace
 
+GenPlan tree_plan(const TreeParams &P) { return tree_mma_takes(P) ? mma_merge_plan(P) : gen_plan(P); }
+
+// The largest that any output can ask for: where q allows the other kernels, an
+// output with other strides or at another address may still leave the call to
+// tree_generic.
 int64_t tree_workspace(const TreeParams &P) {
-  if (tree_mma_takes(P)) return gen_workspace(P, mma_merge_plan(P));
-  return tree_tc_takes(P) ? tree_tc_workspace(P) : gen_workspace(P, gen_plan(P));
+  int64_t most = gen_workspace(P, gen_plan(P));
+  if (tree_mma_takes(P)) most = std::max(most, gen_workspace(P, mma_merge_plan(P)));
+  else if (tree_tc_takes(P)) most = std::max(most, tree_tc_workspace(P));
+  return most;
 }
 
 int tree_run(TreeParams &P, void *workspace, int64_t bytes, cudaStream_t st) {
   if (P.B == 0 || P.nodes == 0) return KV4_OK;
   const bool mma = tree_mma_takes(P);
   if (!mma && tree_tc_takes(P)) return tree_tc_run(P, workspace, bytes, st);
-  const GenPlan L = mma ? mma_merge_plan(P) : gen_plan(P);
+  const GenPlan L = tree_plan(P);
   if (gen_workspace(P, L) > 0) {
     if (!workspace || bytes < gen_workspace(P, L)) return KV4_ERR_WORKSPACE;
     const int64_t n = L.parts * L.units * L.rows;
@@ -376,7 +345,7 @@ int tree_run(TreeParams &P, void *workspace, int64_t bytes, cudaStream_t st) {
   }
   if (mma) {
     const int rc = tree_mma_run(P, st);
-    if (rc || L.parts == 1) return rc;
+    if (rc || L.parts == 1 || P.kept) return rc;
     return P.d == 64 ? launch_merge<2>(P, L, st) : launch_merge<4>(P, L, st);
   }
   if (P.d <= 64) return launch_gen_rw<2>(P, L, st);

@@ -40,7 +40,18 @@ struct TreeParams {
   float2 *stats;       // per (unit, row): base-2 maximum and 1 / sum; or null
   float *ws_o;         // split partials, see the kernels
   float2 *ws_ml;
+  float *kept;         // raw scores of every row, see kept_at; or null
+  float *kept_c;       // per (unit, row): factor from those to base-2 exponents
 };
+
+// Kept scores lie in blocks of 16 keys, [unit][block][row][16]; context rows
+// fill whole blocks, drafted rows begin a new one.
+__host__ __device__ __forceinline__ int64_t kept_blocks(const TreeParams &P) {
+  return ((P.S + 15) >> 4) + ((P.ndraft + 15) >> 4);
+}
+__device__ __forceinline__ int64_t kept_at(int64_t unit, int64_t blocks, int64_t slot, int row, int rows) {
+  return ((unit * blocks + (slot >> 4)) * rows + row) * 16 + (slot & 15);
+}
 
 // context rows of sequence b; an entry outside [0, S] is reported and read as 0
 __device__ __forceinline__ int64_t context_len(const TreeParams &P, int64_t b, int *err) {
@@ -222,7 +233,6 @@ struct ScoreParams {
   int64_t keys;          // tokens in the cache: context plus drafted rows
 };
 
-int score_run(const ScoreParams &P, cudaStream_t st);      // trim.cu: any layout
 bool tree_tc_takes(const TreeParams &P);                   // branch_tc.cu
 int score_tc_run(const ScoreParams &P, cudaStream_t st);   // trim_tc.cu
 bool tree_mma_takes(const TreeParams &P);                  // branch_mma.cu

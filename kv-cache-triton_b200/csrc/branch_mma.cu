@@ -43,8 +43,6 @@ struct MmaPlan {
 };
 
 constexpr int NW = 4;      // warps per block
-// blocks per SM: 168 registers a thread, 128 where eight rows of 64 columns fit
-constexpr int blocks_of(int d, bool half) { return half && d == 64 ? 4 : 3; }
 constexpr float kShift = 7.0f;  // weights are written times 2^7 (see branch_tc.cu)
 
 // scale i of a packed row of 16-bit scales
@@ -217,8 +215,8 @@ __device__ __forceinline__ uint32_t code_pair1(uint32_t w, int e) {  // code - 8
 
 // Sums of rows g (s[0], s[1]) and g + 8 (s[2], s[3]) with keys 2t, 2t + 1 of
 // key tile n of the step at `at`, scaled group by group.
-template <int D, int G, typename ST, bool HALF, bool WITH_V>
-__device__ __forceinline__ void scores(float (&s)[4], const Query<D, HALF> &Q, uint32_t at, int n, int lane) {
+template <int D, int G, typename ST, bool WITH_V>
+__device__ __forceinline__ void scores(float (&s)[4], const Query<D, false> &Q, uint32_t at, int n, int lane) {
   using R = Ring<D, G, WITH_V>;
   const int g = lane >> 2, t = lane & 3;
   uint32_t w[D / 32], k0[(R::NG + 1) / 2], k1[(R::NG + 1) / 2];
@@ -236,17 +234,14 @@ __device__ __forceinline__ void scores(float (&s)[4], const Query<D, HALF> &Q, u
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         const uint32_t *a = Q.a[2 * blk + j];
-        mma_f16_16816(c, a[0], HALF ? 0u : a[HALF ? 0 : 1], a[HALF ? 1 : 2], HALF ? 0u : a[HALF ? 0 : 3],
-                      code_pair(w[blk], 2 * j), code_pair(w[blk], 2 * j + 1));
+        mma_f16_16816(c, a[0], a[1], a[2], a[3], code_pair(w[blk], 2 * j), code_pair(w[blk], 2 * j + 1));
       }
     }
     const float f0 = scale_at<ST>(k0, gr), f1 = scale_at<ST>(k1, gr);
     s[0] = fmaf(c[0], f0, s[0]);
     s[1] = fmaf(c[1], f1, s[1]);
-    if (!HALF) {
-      s[2] = fmaf(c[2], f0, s[2]);
-      s[3] = fmaf(c[3], f1, s[3]);
-    }
+    s[2] = fmaf(c[2], f0, s[2]);
+    s[3] = fmaf(c[3], f1, s[3]);
   }
 }
 
@@ -264,202 +259,12 @@ __device__ __forceinline__ uint32_t seen_keys(const TreeParams &T, int64_t b, bo
   return m;
 }
 
-template <int D, int G, typename ST, bool HALF>
-__global__ void __launch_bounds__(NW * 32, blocks_of(D, HALF))
-    tree_mma(const __grid_constant__ TreeParams T, const MmaPlan L) {
-  constexpr int NR = HALF ? 8 : 16, RT = HALF ? 1 : 2, DG = D / 8, LD = D + 4;
-  extern __shared__ __align__(16) float msm[];  // rings, later [NW][NR][LD] outputs, [NW][NR] float2 (m, l)
-  float2 *sml = reinterpret_cast<float2 *>(msm + NW * NR * LD);
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
-  const int part = static_cast<int>(blockIdx.x % L.parts);
-  const int64_t ur = blockIdx.x / L.parts;
-  const int rt = static_cast<int>(ur % L.row_tiles), row0 = rt * NR;
-  const int64_t unit = ur / L.row_tiles, b = unit / T.Hkv;
-  const int kvh = static_cast<int>(unit - b * T.Hkv);
-  const int64_t len = context_len(T, b, part == 0 && rt == 0 && kvh == 0 && threadIdx.x == 0 ? &g_branch_error_mma : nullptr);
-  const int nctx = static_cast<int>((len + 15) >> 4), steps = nctx + ((T.ndraft + 15) >> 4);
-  const int per = (steps + L.parts - 1) / L.parts;
-  const int s0 = part * per, s1 = min(steps, s0 + per);
-
-  using R = Ring<D, G, true>;
-  const uint32_t ring = smem_u32(msm) + warp * R::BYTES;
-  const Plane ctx = plane_of(T.cache, b, kvh);
-  auto fetch = [&](int s, uint32_t slot) {
-    if (s < nctx) {
-      fetch_step<D, G, true>(ctx, static_cast<int64_t>(s) * 16, static_cast<int>(min(len - static_cast<int64_t>(s) * 16, int64_t(16))),
-                             ring + slot * R::STEP, lane);
-    } else if (s < s1) {
-      const Plane dft = plane_of(T.draft, b, kvh);
-      fetch_step<D, G, true>(dft, static_cast<int64_t>(s - nctx) * 16, min(T.ndraft - (s - nctx) * 16, 16),
-                             ring + slot * R::STEP, lane);
-    }
-    cp_async_commit();
-  };
-  // steps s0 + warp, + NW, ...: DEPTH - 1 of them on their way
-  int s = s0 + warp;
-#pragma unroll 1
-  for (int i = 0; i < R::DEPTH - 1; ++i)
-    if (s + i * NW < s1) fetch(s + i * NW, i);
-    else cp_async_commit();
-  Query<D, HALF> Q;
-  load_query(Q, T, b, kvh, row0, L.rows, lane);
-  int node[RT];
-  bool ok[RT];
-  float m[RT], l[RT];
-  bool broken[RT];
-  float o[DG][HALF ? 2 : 4];
-#pragma unroll
-  for (int r = 0; r < RT; ++r) {
-    const int row = row0 + g + 8 * r;
-    ok[r] = row < L.rows;
-    node[r] = row / T.R;
-    m[r] = -INFINITY;
-    l[r] = 0.0f;
-    broken[r] = false;
-  }
-#pragma unroll
-  for (int j = 0; j < DG; ++j)
-#pragma unroll
-    for (int e = 0; e < (HALF ? 2 : 4); ++e) o[j][e] = 0.0f;
-  bool big = false;
-
-  uint32_t slot = 0;
-#pragma unroll 1
-  for (; s < s1; s += NW) {
-    const bool draft = s >= nctx;
-    const int64_t k0 = static_cast<int64_t>(draft ? s - nctx : s) * 16, end = draft ? T.ndraft : len;
-    cp_async_wait<R::DEPTH - 2>();
-    __syncwarp();  // this step is there for all lanes, and all are done with the one before
-    {
-      const int ahead = s + (R::DEPTH - 1) * NW;
-      if (ahead < s1) fetch(ahead, slot == 0 ? R::DEPTH - 1 : slot - 1);
-      else cp_async_commit();
-    }
-    const uint32_t at = ring + slot * R::STEP;
-    slot = slot + 1 == R::DEPTH ? 0 : slot + 1;
-    float x[2][4];
-    scores<D, G, ST, HALF, true>(x[0], Q, at, 0, lane);
-    scores<D, G, ST, HALF, true>(x[1], Q, at, 1, lane);
-    uint32_t vs[4];  // V's scales of this thread's columns, keys 2t, 2t + 1, 2t + 8, 2t + 9
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      vs[j] = lds16(at + R::VS + (2 * t + (j & 1) + 8 * (j >> 1)) * R::SB + 2 * (g * DG / G));
-
-    // scores -> weights, in place
-#pragma unroll
-    for (int r = 0; r < RT; ++r) {
-      float y[4] = {x[0][2 * r], x[0][2 * r + 1], x[1][2 * r], x[1][2 * r + 1]};
-      if (draft || k0 + 16 > end) {
-        const uint32_t on = seen_keys(T, b, draft, node[r], ok[r], k0, end, t);
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (!(on >> j & 1u)) y[j] = -INFINITY;
-        if (draft) {  // a visible key without a usable V scale: the row has no value
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const bool bad = !(fabsf(scale_at<ST>(&vs[j], 0)) <= tc::kMaxScale);
-            const uint32_t any = __ballot_sync(0xffffffffu, bad) & (0x11111111u << t);
-            if (any && (on >> j & 1u)) broken[r] = true;
-          }
-        }
-      }
-      float mx = fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3])) * Q.c[r];
-      // the maximum moves only when a score passes it by more than 8: seldom
-      if (__any_sync(0xffffffffu, mx > m[r] + 8.0f)) {
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-        const float to = mx > m[r] + 8.0f ? mx : m[r];
-        const float alpha = to == m[r] ? 1.0f : m[r] == -INFINITY ? 0.0f : fast_exp2(m[r] - to);
-        m[r] = to;
-        l[r] *= alpha;
-#pragma unroll
-        for (int j = 0; j < DG; ++j) {
-          o[j][2 * r] *= alpha;
-          o[j][2 * r + 1] *= alpha;
-        }
-      }
-      const float base = m[r] == -INFINITY ? 0.0f : m[r] - kShift;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) y[j] = fast_exp2(fmaf(y[j], Q.c[r], -base));
-      l[r] += (y[0] + y[1]) + (y[2] + y[3]);
-      x[0][2 * r] = y[0];
-      x[0][2 * r + 1] = y[1];
-      x[1][2 * r] = y[2];
-      x[1][2 * r + 1] = y[3];
-    }
-    const uint32_t a0 = pack_f16x2(x[0][0], x[0][1]), a2 = pack_f16x2(x[1][0], x[1][1]);
-    const uint32_t a1 = HALF ? 0u : pack_f16x2(x[0][2], x[0][3]);
-    const uint32_t a3 = HALF ? 0u : pack_f16x2(x[1][2], x[1][3]);
-
-    // O += P V: column j of this thread's eighth, keys in pairs
-    uint32_t sp[2];
-#pragma unroll
-    for (int p = 0; p < 2; ++p) {
-      const float f0 = scale_at<ST>(&vs[2 * p], 0), f1 = scale_at<ST>(&vs[2 * p + 1], 0);
-      sp[p] = DT<ST>::code == KV4_F16 ? prmt(vs[2 * p], vs[2 * p + 1], 0x5410) : pack_f16x2(f0, f1);
-      const bool b0 = !(fabsf(f0) <= tc::kMaxScale), b1 = !(fabsf(f1) <= tc::kMaxScale);
-      if (b0 || b1) {
-        big = true;
-        if (draft) sp[p] &= (b0 ? 0u : 0xffffu) | (b1 ? 0u : 0xffff0000u);  // rows that see it: above
-      }
-    }
-    uint32_t vw[4][D / 64];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const uint32_t p = at + R::V + (2 * t + (j & 1) + 8 * (j >> 1)) * R::ROW + g * (D / 16);
-      if (D == 128) {
-        const uint2 w = lds64(p);
-        vw[j][0] = w.x;
-        vw[j][D / 64 - 1] = w.y;
-      } else {
-        vw[j][0] = lds32(p);
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < D / 64; ++i) {
-      uint32_t y[2][2];  // [key pair][half word]: the pair's words side by side
-#pragma unroll
-      for (int p = 0; p < 2; ++p) {
-        y[p][0] = prmt(vw[2 * p][i], vw[2 * p + 1][i], 0x5410);
-        y[p][1] = prmt(vw[2 * p][i], vw[2 * p + 1][i], 0x7632);
-      }
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const uint32_t b0 = tc::hmul2(code_pair1(y[0][e >> 2], e & 3), sp[0]);
-        const uint32_t b1 = tc::hmul2(code_pair1(y[1][e >> 2], e & 3), sp[1]);
-        float *c = o[8 * i + e];
-        if (HALF) {
-          float d[4];
-          mma_f16_16816_c(d, a0, 0u, a2, 0u, b0, b1, c[0], c[1], 0.0f, 0.0f);
-          c[0] = d[0];
-          c[1] = d[1];
-        } else {
-          mma_f16_16816(*reinterpret_cast<float(*)[4]>(c), a0, a1, a2, a3, b0, b1);
-        }
-      }
-    }
-  }
-  if (big) atomicOr(&g_branch_error_mma, DEV_ERR_F16_RANGE);
-
-  // ---- the block's warps meet, where the rings were ----
-  cp_async_wait<0>();
-  __syncthreads();
-#pragma unroll
-  for (int r = 0; r < RT; ++r) {
-    l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
-    l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
-    const uint32_t bad = __ballot_sync(0xffffffffu, broken[r]);
-    if (bad & (0xFu << (4 * g))) l[r] = __uint_as_float(0x7fc00000u);
-    const int at = warp * NR + g + 8 * r;
-    if (t == 0) sml[at] = make_float2(m[r] - kShift, l[r]);
-    // columns 2t and 2t + 1 of output tile j are dims 2t * DG + j and (2t + 1) * DG + j
-#pragma unroll
-    for (int j = 0; j < DG; ++j) {
-      msm[at * LD + 2 * t * DG + j] = o[j][2 * r];
-      msm[at * LD + (2 * t + 1) * DG + j] = o[j][2 * r + 1];
-    }
-  }
-  __syncthreads();
+// The block's warps' outputs [NW][NR][D + 4] and (maximum, sum) [NW][NR] become
+// the call's output, or the block's partial rows.
+template <int D, int NR>
+__device__ __forceinline__ void meet(const TreeParams &T, const MmaPlan &L, const float *msm, const float2 *sml,
+                                     int64_t unit, int64_t b, int kvh, int part, int row0) {
+  constexpr int LD = D + 4;
   const int nr = min(NR, L.rows - row0);
   for (int idx = threadIdx.x; idx < nr * (D / 2); idx += NW * 32) {
     const int r = idx / (D / 2), c = (idx - r * (D / 2)) * 2, row = row0 + r;
@@ -498,12 +303,434 @@ __global__ void __launch_bounds__(NW * 32, blocks_of(D, HALF))
   }
 }
 
+template <int D, int G, typename ST>
+__global__ void __launch_bounds__(NW * 32, 3)
+    tree_mma(const __grid_constant__ TreeParams T, const MmaPlan L) {
+  constexpr int NR = 16, RT = 2, DG = D / 8, LD = D + 4;
+  extern __shared__ __align__(16) float msm[];  // rings, later [NW][NR][LD] outputs, [NW][NR] float2 (m, l)
+  float2 *sml = reinterpret_cast<float2 *>(msm + NW * NR * LD);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+  const int part = static_cast<int>(blockIdx.x % L.parts);
+  const int64_t ur = blockIdx.x / L.parts;
+  const int rt = static_cast<int>(ur % L.row_tiles), row0 = rt * NR;
+  const int64_t unit = ur / L.row_tiles, b = unit / T.Hkv;
+  const int kvh = static_cast<int>(unit - b * T.Hkv);
+  const int64_t len = context_len(T, b, part == 0 && rt == 0 && kvh == 0 && threadIdx.x == 0 ? &g_branch_error_mma : nullptr);
+  const int nctx = static_cast<int>((len + 15) >> 4), steps = nctx + ((T.ndraft + 15) >> 4);
+  const int per = (steps + L.parts - 1) / L.parts;
+  const int s0 = part * per, s1 = min(steps, s0 + per);
+
+  using R = Ring<D, G, true>;
+  const uint32_t ring = smem_u32(msm) + warp * R::BYTES;
+  const Plane ctx = plane_of(T.cache, b, kvh);
+  auto fetch = [&](int s, uint32_t slot) {
+    if (s < nctx) {
+      fetch_step<D, G, true>(ctx, static_cast<int64_t>(s) * 16, static_cast<int>(min(len - static_cast<int64_t>(s) * 16, int64_t(16))),
+                             ring + slot * R::STEP, lane);
+    } else if (s < s1) {
+      const Plane dft = plane_of(T.draft, b, kvh);
+      fetch_step<D, G, true>(dft, static_cast<int64_t>(s - nctx) * 16, min(T.ndraft - (s - nctx) * 16, 16),
+                             ring + slot * R::STEP, lane);
+    }
+    cp_async_commit();
+  };
+  // steps s0 + warp, + NW, ...: DEPTH - 1 of them on their way
+  int s = s0 + warp;
+#pragma unroll 1
+  for (int i = 0; i < R::DEPTH - 1; ++i)
+    if (s + i * NW < s1) fetch(s + i * NW, i);
+    else cp_async_commit();
+  Query<D, false> Q;
+  load_query(Q, T, b, kvh, row0, L.rows, lane);
+  int node[RT];
+  bool ok[RT];
+  float m[RT], l[RT];
+  bool broken[RT];
+  float o[DG][4];
+#pragma unroll
+  for (int r = 0; r < RT; ++r) {
+    const int row = row0 + g + 8 * r;
+    ok[r] = row < L.rows;
+    node[r] = row / T.R;
+    m[r] = -INFINITY;
+    l[r] = 0.0f;
+    broken[r] = false;
+  }
+#pragma unroll
+  for (int j = 0; j < DG; ++j)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[j][e] = 0.0f;
+  bool big = false;
+  // kept scores of rows g and g + 8 (one row tile holds them all)
+  float *const kept = T.kept ? T.kept + kept_at(unit, steps, 2 * t, g, L.rows) : nullptr;
+  if (T.kept && part == 0 && warp == 0 && t == 0) {
+#pragma unroll
+    for (int r = 0; r < RT; ++r)
+      if (ok[r]) T.kept_c[unit * L.rows + g + 8 * r] = Q.c[r];
+  }
+
+  uint32_t slot = 0;
+#pragma unroll 1
+  for (; s < s1; s += NW) {
+    const bool draft = s >= nctx;
+    const int64_t k0 = static_cast<int64_t>(draft ? s - nctx : s) * 16, end = draft ? T.ndraft : len;
+    cp_async_wait<R::DEPTH - 2>();
+    __syncwarp();  // this step is there for all lanes, and all are done with the one before
+    {
+      const int ahead = s + (R::DEPTH - 1) * NW;
+      if (ahead < s1) fetch(ahead, slot == 0 ? R::DEPTH - 1 : slot - 1);
+      else cp_async_commit();
+    }
+    const uint32_t at = ring + slot * R::STEP;
+    slot = slot + 1 == R::DEPTH ? 0 : slot + 1;
+    float x[2][4];
+    scores<D, G, ST, true>(x[0], Q, at, 0, lane);
+    scores<D, G, ST, true>(x[1], Q, at, 1, lane);
+    uint32_t vs[4];  // V's scales of this thread's columns, keys 2t, 2t + 1, 2t + 8, 2t + 9
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      vs[j] = lds16(at + R::VS + (2 * t + (j & 1) + 8 * (j >> 1)) * R::SB + 2 * (g * DG / G));
+
+    // scores -> weights, in place
+#pragma unroll
+    for (int r = 0; r < RT; ++r) {
+      float y[4] = {x[0][2 * r], x[0][2 * r + 1], x[1][2 * r], x[1][2 * r + 1]};
+      if (draft || k0 + 16 > end) {
+        const uint32_t on = seen_keys(T, b, draft, node[r], ok[r], k0, end, t);
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (!(on >> j & 1u)) y[j] = -INFINITY;
+        if (draft) {  // a visible key without a usable V scale: the row has no value
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const bool bad = !(fabsf(scale_at<ST>(&vs[j], 0)) <= tc::kMaxScale);
+            const uint32_t any = __ballot_sync(0xffffffffu, bad) & (0x11111111u << t);
+            if (any && (on >> j & 1u)) broken[r] = true;
+          }
+        }
+      }
+      if (kept && ok[r]) {
+        float *p = kept + (static_cast<int64_t>(s) * L.rows + 8 * r) * 16;
+        *reinterpret_cast<float2 *>(p) = make_float2(y[0], y[1]);
+        *reinterpret_cast<float2 *>(p + 8) = make_float2(y[2], y[3]);
+      }
+      float mx = fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3])) * Q.c[r];
+      // the maximum moves only when a score passes it by more than 8: seldom
+      if (__any_sync(0xffffffffu, mx > m[r] + 8.0f)) {
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+        const float to = mx > m[r] + 8.0f ? mx : m[r];
+        const float alpha = to == m[r] ? 1.0f : m[r] == -INFINITY ? 0.0f : fast_exp2(m[r] - to);
+        m[r] = to;
+        l[r] *= alpha;
+#pragma unroll
+        for (int j = 0; j < DG; ++j) {
+          o[j][2 * r] *= alpha;
+          o[j][2 * r + 1] *= alpha;
+        }
+      }
+      const float base = m[r] == -INFINITY ? 0.0f : m[r] - kShift;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) y[j] = fast_exp2(fmaf(y[j], Q.c[r], -base));
+      l[r] += (y[0] + y[1]) + (y[2] + y[3]);
+      x[0][2 * r] = y[0];
+      x[0][2 * r + 1] = y[1];
+      x[1][2 * r] = y[2];
+      x[1][2 * r + 1] = y[3];
+    }
+    const uint32_t a0 = pack_f16x2(x[0][0], x[0][1]), a2 = pack_f16x2(x[1][0], x[1][1]);
+    const uint32_t a1 = pack_f16x2(x[0][2], x[0][3]);
+    const uint32_t a3 = pack_f16x2(x[1][2], x[1][3]);
+
+    // O += P V: column j of this thread's eighth, keys in pairs
+    uint32_t sp[2];
+#pragma unroll
+    for (int p = 0; p < 2; ++p) {
+      const float f0 = scale_at<ST>(&vs[2 * p], 0), f1 = scale_at<ST>(&vs[2 * p + 1], 0);
+      sp[p] = DT<ST>::code == KV4_F16 ? prmt(vs[2 * p], vs[2 * p + 1], 0x5410) : pack_f16x2(f0, f1);
+      const bool b0 = !(fabsf(f0) <= tc::kMaxScale), b1 = !(fabsf(f1) <= tc::kMaxScale);
+      if (b0 || b1) {
+        big = true;
+        if (draft) sp[p] &= (b0 ? 0u : 0xffffu) | (b1 ? 0u : 0xffff0000u);  // rows that see it: above
+      }
+    }
+    uint32_t vw[4][D / 64];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t p = at + R::V + (2 * t + (j & 1) + 8 * (j >> 1)) * R::ROW + g * (D / 16);
+      if (D == 128) {
+        const uint2 w = lds64(p);
+        vw[j][0] = w.x;
+        vw[j][D / 64 - 1] = w.y;
+      } else {
+        vw[j][0] = lds32(p);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < D / 64; ++i) {
+      uint32_t y[2][2];  // [key pair][half word]: the pair's words side by side
+#pragma unroll
+      for (int p = 0; p < 2; ++p) {
+        y[p][0] = prmt(vw[2 * p][i], vw[2 * p + 1][i], 0x5410);
+        y[p][1] = prmt(vw[2 * p][i], vw[2 * p + 1][i], 0x7632);
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const uint32_t b0 = tc::hmul2(code_pair1(y[0][e >> 2], e & 3), sp[0]);
+        const uint32_t b1 = tc::hmul2(code_pair1(y[1][e >> 2], e & 3), sp[1]);
+        mma_f16_16816(o[8 * i + e], a0, a1, a2, a3, b0, b1);
+      }
+    }
+  }
+  if (big) atomicOr(&g_branch_error_mma, DEV_ERR_F16_RANGE);
+
+  // ---- the block's warps meet, where the rings were ----
+  cp_async_wait<0>();
+  __syncthreads();
+#pragma unroll
+  for (int r = 0; r < RT; ++r) {
+    l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
+    l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
+    const uint32_t bad = __ballot_sync(0xffffffffu, broken[r]);
+    if (bad & (0xFu << (4 * g))) l[r] = __uint_as_float(0x7fc00000u);
+    const int at = warp * NR + g + 8 * r;
+    if (t == 0) sml[at] = make_float2(m[r] - kShift, l[r]);
+    // columns 2t and 2t + 1 of output tile j are dims 2t * DG + j and (2t + 1) * DG + j
+#pragma unroll
+    for (int j = 0; j < DG; ++j) {
+      msm[at * LD + 2 * t * DG + j] = o[j][2 * r];
+      msm[at * LD + (2 * t + 1) * DG + j] = o[j][2 * r + 1];
+    }
+  }
+  __syncthreads();
+  meet<D, NR>(T, L, msm, sml, unit, b, kvh, part, row0);
+}
+
+// Up to 8 rows: keys are M (or, for V, columns), rows N, so that no half of a
+// product is padding.  Weights become the B operand of the second product by a
+// transpose within the warp.  Against rows as M: half the products, no spills.
+template <int D, int G, typename ST>
+__global__ void __launch_bounds__(NW * 32, 4) tree_mma8(const __grid_constant__ TreeParams T, const MmaPlan L) {
+  constexpr int NR = 8, DG = D / 8, LD = D + 4;
+  extern __shared__ __align__(16) float msm[];  // rings, later [NW][NR][LD] outputs, [NW][NR] float2 (m, l)
+  float2 *sml = reinterpret_cast<float2 *>(msm + NW * NR * LD);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+  const int part = static_cast<int>(blockIdx.x % L.parts);
+  const int64_t unit = blockIdx.x / L.parts, b = unit / T.Hkv;
+  const int kvh = static_cast<int>(unit - b * T.Hkv);
+  const int64_t len = context_len(T, b, part == 0 && kvh == 0 && threadIdx.x == 0 ? &g_branch_error_mma : nullptr);
+  const int nctx = static_cast<int>((len + 15) >> 4), steps = nctx + ((T.ndraft + 15) >> 4);
+  const int per = (steps + L.parts - 1) / L.parts;
+  const int s0 = part * per, s1 = min(steps, s0 + per);
+
+  using R = Ring<D, G, true>;
+  const uint32_t ring = smem_u32(msm) + warp * R::BYTES;
+  const Plane ctx = plane_of(T.cache, b, kvh);
+  auto fetch = [&](int s, uint32_t slot) {
+    if (s < nctx) {
+      fetch_step<D, G, true>(ctx, static_cast<int64_t>(s) * 16, static_cast<int>(min(len - static_cast<int64_t>(s) * 16, int64_t(16))),
+                             ring + slot * R::STEP, lane);
+    } else if (s < s1) {
+      const Plane dft = plane_of(T.draft, b, kvh);
+      fetch_step<D, G, true>(dft, static_cast<int64_t>(s - nctx) * 16, min(T.ndraft - (s - nctx) * 16, 16),
+                             ring + slot * R::STEP, lane);
+    }
+    cp_async_commit();
+  };
+  int s = s0 + warp;
+#pragma unroll 1
+  for (int i = 0; i < R::DEPTH - 1; ++i)
+    if (s + i * NW < s1) fetch(s + i * NW, i);
+    else cp_async_commit();
+  Query<D, true> Q;  // of row g
+  load_query(Q, T, b, kvh, 0, L.rows, lane);
+  if (T.kept_c && part == 0 && warp == 0 && t == 0 && g < L.rows) T.kept_c[unit * L.rows + g] = Q.c[0];
+  // this thread's scores are those of rows 2t, 2t + 1 with keys g, g + 8
+  const float c[2] = {__shfl_sync(0xffffffffu, Q.c[0], 8 * t), __shfl_sync(0xffffffffu, Q.c[0], 8 * t + 4)};
+  const bool ok[2] = {2 * t < L.rows, 2 * t + 1 < L.rows};
+  float *const kept = T.kept ? T.kept + kept_at(unit, steps, g, 2 * t, L.rows) : nullptr;
+  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+  bool broken[2] = {false, false};
+  float o[D / 16][4];  // columns 2j, 2j + 1 of eighth g, rows 2t, 2t + 1
+#pragma unroll
+  for (int j = 0; j < D / 16; ++j)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[j][e] = 0.0f;
+  bool big = false;
+
+  uint32_t slot = 0;
+#pragma unroll 1
+  for (; s < s1; s += NW) {
+    const bool draft = s >= nctx;
+    const int64_t k0 = static_cast<int64_t>(draft ? s - nctx : s) * 16, end = draft ? T.ndraft : len;
+    cp_async_wait<R::DEPTH - 2>();
+    __syncwarp();  // this step is there for all lanes, and all are done with the one before
+    {
+      const int ahead = s + (R::DEPTH - 1) * NW;
+      if (ahead < s1) fetch(ahead, slot == 0 ? R::DEPTH - 1 : slot - 1);
+      else cp_async_commit();
+    }
+    const uint32_t at = ring + slot * R::STEP;
+    slot = slot + 1 == R::DEPTH ? 0 : slot + 1;
+
+    // S = K Q^T, scaled group by group
+    float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};  // (key g, rows 2t, 2t + 1), (key g + 8, the same)
+    {
+      uint32_t w0[D / 32], w1[D / 32], f0[(R::NG + 1) / 2], f1[(R::NG + 1) / 2];
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i) {
+        w0[i] = lds32(at + R::K + g * R::ROW + 16 * i + 4 * t);
+        w1[i] = lds32(at + R::K + (g + 8) * R::ROW + 16 * i + 4 * t);
+      }
+      lds_scales<R::NG>(f0, at + R::KS + g * R::SB);
+      lds_scales<R::NG>(f1, at + R::KS + (g + 8) * R::SB);
+#pragma unroll
+      for (int gr = 0; gr < R::NG; ++gr) {
+        float y[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int i = 0; i < G / 32; ++i) {
+          const int blk = gr * (G / 32) + i;
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+            mma_f16_16816(y, code_pair(w0[blk], 2 * j), code_pair(w1[blk], 2 * j), code_pair(w0[blk], 2 * j + 1),
+                          code_pair(w1[blk], 2 * j + 1), Q.a[2 * blk + j][0], Q.a[2 * blk + j][1]);
+        }
+        const float k0f = scale_at<ST>(f0, gr), k1f = scale_at<ST>(f1, gr);
+        x[0] = fmaf(y[0], k0f, x[0]);
+        x[1] = fmaf(y[1], k0f, x[1]);
+        x[2] = fmaf(y[2], k1f, x[2]);
+        x[3] = fmaf(y[3], k1f, x[3]);
+      }
+    }
+    uint32_t vs[4];  // V's scales of eighth g, keys 2t, 2t + 1, 2t + 8, 2t + 9
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      vs[j] = lds16(at + R::VS + (2 * t + (j & 1) + 8 * (j >> 1)) * R::SB + 2 * (g * DG / G));
+
+    if (draft || k0 + 16 > end) {
+      uint32_t bad = 0;  // keys of this step without a usable V scale
+      if (draft) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (!(fabsf(scale_at<ST>(&vs[j], 0)) <= tc::kMaxScale)) bad |= 1u << (2 * t + (j & 1) + 8 * (j >> 1));
+        bad = __reduce_or_sync(0xffffffffu, bad);
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int r = e & 1, k = g + 8 * (e >> 1);
+        bool on = ok[r] && k0 + k < end;
+        if (on && draft) on = draft_visible(T, b, (2 * t + r) / T.R, static_cast<int>(k0) + k);
+        if (!on) x[e] = -INFINITY;
+        else if (bad >> k & 1u) broken[r] = true;  // the row has no value
+      }
+    }
+    if (kept) {
+      float *p = kept + static_cast<int64_t>(s) * L.rows * 16;
+      if (ok[0]) {
+        p[0] = x[0];
+        p[8] = x[2];
+      }
+      if (ok[1]) {
+        p[16] = x[1];
+        p[24] = x[3];
+      }
+    }
+    // scores -> weights, in place; the maximum moves only when a score passes it
+    // by more than 8: seldom
+    float mx[2] = {fmaxf(x[0], x[2]) * c[0], fmaxf(x[1], x[3]) * c[1]};
+    if (__any_sync(0xffffffffu, mx[0] > m[0] + 8.0f || mx[1] > m[1] + 8.0f)) {
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+#pragma unroll
+        for (int d = 4; d < 32; d <<= 1) mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], d));
+        const float to = mx[r] > m[r] + 8.0f ? mx[r] : m[r];
+        const float alpha = to == m[r] ? 1.0f : m[r] == -INFINITY ? 0.0f : fast_exp2(m[r] - to);
+        m[r] = to;
+        l[r] *= alpha;
+#pragma unroll
+        for (int j = 0; j < D / 16; ++j) {
+          o[j][r] *= alpha;
+          o[j][2 + r] *= alpha;
+        }
+      }
+    }
+    const float base[2] = {m[0] == -INFINITY ? 0.0f : m[0] - kShift, m[1] == -INFINITY ? 0.0f : m[1] - kShift};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[e] = fast_exp2(fmaf(x[e], c[e & 1], -base[e & 1]));
+    l[0] += x[0] + x[2];
+    l[1] += x[1] + x[3];
+    const uint32_t p0 = movmatrix_trans(pack_f16x2(x[0], x[1]));  // row g, keys 2t, 2t + 1
+    const uint32_t p1 = movmatrix_trans(pack_f16x2(x[2], x[3]));  // keys 2t + 8, 2t + 9
+
+    // O^T += V^T P^T: two columns of this thread's eighth, keys in pairs
+    uint32_t sp[2];
+#pragma unroll
+    for (int p = 0; p < 2; ++p) {
+      const float f0 = scale_at<ST>(&vs[2 * p], 0), f1 = scale_at<ST>(&vs[2 * p + 1], 0);
+      sp[p] = DT<ST>::code == KV4_F16 ? prmt(vs[2 * p], vs[2 * p + 1], 0x5410) : pack_f16x2(f0, f1);
+      const bool b0 = !(fabsf(f0) <= tc::kMaxScale), b1 = !(fabsf(f1) <= tc::kMaxScale);
+      if (b0 || b1) {
+        big = true;
+        if (draft) sp[p] &= (b0 ? 0u : 0xffffu) | (b1 ? 0u : 0xffff0000u);  // rows that see it: above
+      }
+    }
+    uint32_t vw[4][D / 64];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t p = at + R::V + (2 * t + (j & 1) + 8 * (j >> 1)) * R::ROW + g * (D / 16);
+      if (D == 128) {
+        const uint2 w = lds64(p);
+        vw[j][0] = w.x;
+        vw[j][D / 64 - 1] = w.y;
+      } else {
+        vw[j][0] = lds32(p);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < D / 64; ++i) {
+      uint32_t y[2][2];  // [key pair][half word]: the pair's words side by side
+#pragma unroll
+      for (int p = 0; p < 2; ++p) {
+        y[p][0] = prmt(vw[2 * p][i], vw[2 * p + 1][i], 0x5410);
+        y[p][1] = prmt(vw[2 * p][i], vw[2 * p + 1][i], 0x7632);
+      }
+#pragma unroll
+      for (int e = 0; e < 8; e += 2) {
+        uint32_t a[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          a[k] = tc::hmul2(code_pair1(y[k >> 1][e >> 2], (e & 3) + (k & 1)), sp[k >> 1]);
+        mma_f16_16816(o[4 * i + e / 2], a[0], a[1], a[2], a[3], p0, p1);
+      }
+    }
+  }
+  if (big) atomicOr(&g_branch_error_mma, DEV_ERR_F16_RANGE);
+
+  // ---- the block's warps meet, where the rings were ----
+  cp_async_wait<0>();
+  __syncthreads();
+#pragma unroll
+  for (int r = 0; r < 2; ++r) {
+#pragma unroll
+    for (int d = 4; d < 32; d <<= 1) l[r] += __shfl_xor_sync(0xffffffffu, l[r], d);
+    const uint32_t bad = __ballot_sync(0xffffffffu, broken[r]);
+    if (bad & (0x11111111u << t)) l[r] = __uint_as_float(0x7fc00000u);
+    const int row = warp * NR + 2 * t + r;
+    if (g == 0) sml[row] = make_float2(m[r] - kShift, l[r]);
+#pragma unroll
+    for (int j = 0; j < D / 16; ++j)
+      *reinterpret_cast<float2 *>(msm + row * LD + g * DG + 2 * j) = make_float2(o[j][r], o[j][2 + r]);
+  }
+  __syncthreads();
+  meet<D, NR>(T, L, msm, sml, unit, b, kvh, part, 0);
+}
+
 // Scores of the cached tokens: weights formed again from K, the rows' maxima and
 // sums, summed over the rows of each key (rows are lanes: three shuffles).
-template <int D, int G, typename ST, bool HALF>
-__global__ void __launch_bounds__(NW * 32, HALF ? 4 : 3)
+template <int D, int G, typename ST>
+__global__ void __launch_bounds__(NW * 32, 3)
     score_mma(const __grid_constant__ ScoreParams P, int rows, uint32_t steps_per_unit, uint32_t total) {
-  constexpr int RT = HALF ? 1 : 2, NR = HALF ? 8 : 16;
+  constexpr int RT = 2, NR = 16;
   const TreeParams &T = P.t;
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const uint32_t warps = gridDim.x * NW, w = blockIdx.x * NW + (threadIdx.x >> 5);
@@ -527,7 +754,7 @@ __global__ void __launch_bounds__(NW * 32, HALF ? 4 : 3)
     float *out = P.out + b * P.os[0] + kvh * P.os[1];
 #pragma unroll 1
     for (int row0 = 0; row0 < rows; row0 += NR) {
-      Query<D, HALF> Q;
+      Query<D, false> Q;
       load_query(Q, T, b, kvh, row0, rows, lane);
       float sm[RT], sl[RT];  // maximum and 1 / sum of rows g, g + 8
       int node[RT];
@@ -566,8 +793,8 @@ __global__ void __launch_bounds__(NW * 32, HALF ? 4 : 3)
         const uint32_t step = ring + slot * R::STEP;
         slot = slot + 1 == R::DEPTH ? 0 : slot + 1;
         float x[2][4];
-        scores<D, G, ST, HALF, false>(x[0], Q, step, 0, lane);
-        scores<D, G, ST, HALF, false>(x[1], Q, step, 1, lane);
+        scores<D, G, ST, false>(x[0], Q, step, 0, lane);
+        scores<D, G, ST, false>(x[1], Q, step, 1, lane);
         float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int r = 0; r < RT; ++r) {
@@ -611,7 +838,7 @@ MmaPlan mma_plan(const TreeParams &T) {
   L.units = T.B * T.Hkv;
   // one wave of blocks, each warp at least two steps of 16 keys
   const int64_t steps = (T.S + 15) / 16 + (T.ndraft + 15) / 16, have = L.units * L.row_tiles;
-  const int64_t room = static_cast<int64_t>(sm_count()) * blocks_of(T.d, half_rows(L.rows));
+  const int64_t room = static_cast<int64_t>(sm_count()) * (half_rows(L.rows) ? 4 : 3);
   const int64_t most = std::max<int64_t>(1, steps / (2 * NW));
   L.parts = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({room / have, most, 64})));
   return L;
@@ -620,30 +847,31 @@ MmaPlan mma_plan(const TreeParams &T) {
 template <int D, int G, typename ST, bool HALF>
 int launch_tree(const TreeParams &T, const MmaPlan &L, cudaStream_t st) {
   constexpr int NR = HALF ? 8 : 16;
-  constexpr int meet = NW * NR * ((D + 4) * 4 + 8), rings = NW * Ring<D, G, true>::BYTES;
-  constexpr int smem = meet > rings ? meet : rings;
+  constexpr int meeting = NW * NR * ((D + 4) * 4 + 8), rings = NW * Ring<D, G, true>::BYTES;
+  constexpr int smem = meeting > rings ? meeting : rings;
+  const auto kernel = HALF ? tree_mma8<D, G, ST> : tree_mma<D, G, ST>;
   static bool configured[64] = {};
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) dev = 0;
   if (!configured[dev]) {
-    const int rc = cuda_status(cudaFuncSetAttribute(
-        tree_mma<D, G, ST, HALF>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    const int rc = cuda_status(
+        cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
     if (rc) return rc;
     configured[dev] = true;
   }
   const int64_t blocks = L.units * L.row_tiles * L.parts;
   if (blocks > 0x7fffffff) return KV4_ERR_UNSUPPORTED;
-  tree_mma<D, G, ST, HALF><<<static_cast<unsigned>(blocks), NW * 32, smem, st>>>(T, L);
+  kernel<<<static_cast<unsigned>(blocks), NW * 32, smem, st>>>(T, L);
   return cuda_status(cudaGetLastError());
 }
 
-template <int D, int G, typename ST, bool HALF>
+template <int D, int G, typename ST>
 int launch_score(const ScoreParams &P, int rows, cudaStream_t st) {
   const int64_t steps = (P.t.S + 15) / 16 + (P.t.ndraft + 15) / 16, total = P.t.B * P.t.Hkv * steps;
   if (total >= (int64_t(1) << 31)) return KV4_ERR_UNSUPPORTED;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(static_cast<unsigned>(
-      std::min<int64_t>(static_cast<int64_t>(sm_count()) * (HALF ? 4 : 3), (total + NW - 1) / NW)));
+      std::min<int64_t>(static_cast<int64_t>(sm_count()) * 3, (total + NW - 1) / NW)));
   cfg.blockDim = dim3(NW * 32);
   cfg.stream = st;
   cudaLaunchAttribute at{};
@@ -651,19 +879,15 @@ int launch_score(const ScoreParams &P, int rows, cudaStream_t st) {
   at.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &at;
   cfg.numAttrs = 1;
-  return cuda_status(cudaLaunchKernelEx(&cfg, score_mma<D, G, ST, HALF>, P, rows, static_cast<uint32_t>(steps),
+  return cuda_status(cudaLaunchKernelEx(&cfg, score_mma<D, G, ST>, P, rows, static_cast<uint32_t>(steps),
                                         static_cast<uint32_t>(total)));
 }
 
-// f(integral D, integral G, ST{}, bool HALF)
+// f(integral D, integral G, ST{})
 template <class F>
 int by_shape(const TreeParams &T, F f) {
   auto type = [&](auto d, auto g) {
-    auto half = [&](auto st) {
-      if (half_rows(T.R * T.nodes)) return f(d, g, st, std::true_type{});
-      return f(d, g, st, std::false_type{});
-    };
-    return T.s_dtype == KV4_BF16 ? half(__nv_bfloat16{}) : half(__half{});
+    return T.s_dtype == KV4_BF16 ? f(d, g, __nv_bfloat16{}) : f(d, g, __half{});
   };
   if (T.d == 64) {
     if (T.G == 32) return type(std::integral_constant<int, 64>{}, std::integral_constant<int, 32>{});
@@ -725,15 +949,16 @@ int tree_mma_parts(const TreeParams &T) { return mma_plan(T).parts; }
 
 int tree_mma_run(const TreeParams &T, cudaStream_t st) {
   const MmaPlan L = mma_plan(T);
-  return by_shape(T, [&](auto d, auto g, auto s, auto half) {
-    return launch_tree<decltype(d)::value, decltype(g)::value, decltype(s), decltype(half)::value>(T, L, st);
+  return by_shape(T, [&](auto d, auto g, auto s) {
+    constexpr int D = decltype(d)::value, G = decltype(g)::value;
+    if (half_rows(L.rows)) return launch_tree<D, G, decltype(s), true>(T, L, st);
+    return launch_tree<D, G, decltype(s), false>(T, L, st);
   });
 }
 
 int score_mma_run(const ScoreParams &P, cudaStream_t st) {
-  return by_shape(P.t, [&](auto d, auto g, auto s, auto half) {
-    return launch_score<decltype(d)::value, decltype(g)::value, decltype(s), decltype(half)::value>(
-        P, P.t.R * P.t.nodes, st);
+  return by_shape(P.t, [&](auto d, auto g, auto s) {
+    return launch_score<decltype(d)::value, decltype(g)::value, decltype(s)>(P, P.t.R * P.t.nodes, st);
   });
 }
 

@@ -19,7 +19,7 @@
 // once, which is what eviction cannot do without; memory bounds it.
 #include <algorithm>
 
-#include "branch.cuh"
+#include "merge.cuh"
 
 namespace kv4 {
 namespace {
@@ -76,7 +76,100 @@ __global__ void __launch_bounds__(128, 2) score_generic(const ScoreParams P, int
   }
 }
 
-}  // namespace
+constexpr int KTHREADS = 256;  // of score_kept
+constexpr int KROWS = 16;      // most rows of a KV head whose scores are kept
+
+// Few rows (single tokens above all): the attention keeps its scores, 4 bytes a
+// row and key where the keys themselves are d / 2 and their scales, so nothing
+// is read or multiplied twice, and its parts are joined here too.  The first
+// `joins` blocks join the outputs, a warp per row; the others take 256 keys of a
+// (sequence, KV head) each: their warps join the rows' maxima and sums, then a
+// thread sums the weights of its key.
+template <int DC>
+__global__ void __launch_bounds__(KTHREADS, 4)
+    score_kept(const __grid_constant__ ScoreParams P, const GenPlan L, int joins, int blocks) {
+  __shared__ float sm[KROWS], sl[KROWS], sc[KROWS];
+  const TreeParams &T = P.t;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  if (static_cast<int>(blockIdx.x) < joins) {
+    const int64_t at = static_cast<int64_t>(blockIdx.x) * (KTHREADS / 32) + warp;
+    griddep_wait();
+    if (at < L.units * L.rows) merge_row<DC>(T, L, at, lane);
+    return;
+  }
+  const int at = static_cast<int>(blockIdx.x) - joins, unit = at / blocks, b = unit / T.Hkv;
+  const int kvh = unit - b * T.Hkv;
+  const int64_t slot = static_cast<int64_t>(at - unit * blocks) * KTHREADS + tid;
+  const int64_t ctx = (T.S + 15) & ~int64_t(15), t = slot < ctx ? slot : T.S + slot - ctx;
+  const bool on = slot < ctx ? slot < T.S : t < P.keys;
+  // what this reads was there before the attention began
+  const float old = on ? P.in[b * P.is[0] + kvh * P.is[1] + t * P.is[2]] * P.decay : 0.0f;
+  griddep_wait();
+  const int64_t n = L.units * L.rows, first = static_cast<int64_t>(unit) * L.rows;
+  for (int r = warp; r < L.rows; r += KTHREADS / 32) {
+    float m = -INFINITY, l = 0.0f, inv;
+    if (L.parts > 1) {
+      for (int p = lane; p < L.parts; p += 32) {
+        const float2 ml = T.ws_ml[p * n + first + r];
+        const float to = fmaxf(m, ml.x), base = to == -INFINITY ? 0.0f : to;
+        l = l * exp2f(m - base) + ml.y * exp2f(ml.x - base);
+        m = to;
+      }
+      float top = m;
+#pragma unroll
+      for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+      l *= exp2f(m - (top == -INFINITY ? 0.0f : top));
+      m = top;
+#pragma unroll
+      for (int o = 16; o; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+      inv = l > 0.0f ? 1.0f / l : (l == l ? 0.0f : l);
+    } else {
+      const float2 st = T.stats[first + r];
+      m = st.x;
+      inv = st.y;
+    }
+    if (lane == 0) {
+      sm[r] = m;
+      sl[r] = inv;  // 0: a row that saw nothing
+      sc[r] = T.kept_c[first + r];
+    }
+  }
+  __syncthreads();
+  if (!on) return;
+  const float *x = T.kept + kept_at(unit, kept_blocks(T), slot, 0, L.rows);
+  float sum = 0.0f;
+#pragma unroll 4
+  for (int r = 0; r < L.rows; ++r) {
+    const float y = x[16 * r];
+    if (sl[r] != 0.0f) sum += exp2f(fmaf(y, sc[r], -sm[r])) * sl[r];
+  }
+  P.out[b * P.os[0] + kvh * P.os[1] + t * P.os[2]] = old + sum;
+}
+
+template <int DC>
+int launch_kept(const ScoreParams &P, cudaStream_t st) {
+  const GenPlan L = tree_plan(P.t);
+  const int64_t joins = L.parts > 1 ? (L.units * L.rows + KTHREADS / 32 - 1) / (KTHREADS / 32) : 0;
+  const int64_t blocks = (16 * kept_blocks(P.t) + KTHREADS - 1) / KTHREADS, all = joins + L.units * blocks;
+  if (all > 0x7fffffff) return KV4_ERR_UNSUPPORTED;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(all));
+  cfg.blockDim = dim3(KTHREADS);
+  cfg.stream = st;
+  cudaLaunchAttribute at{};
+  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &at;
+  cfg.numAttrs = 1;
+  return cuda_status(cudaLaunchKernelEx(&cfg, score_kept<DC>, P, L, static_cast<int>(joins), static_cast<int>(blocks)));
+}
+
+int kept_run(const ScoreParams &P, cudaStream_t st) {
+  if (P.t.d <= 64) return launch_kept<2>(P, st);
+  if (P.t.d <= 128) return launch_kept<4>(P, st);
+  if (P.t.d <= 256) return launch_kept<8>(P, st);
+  return launch_kept<16>(P, st);
+}
 
 int score_run(const ScoreParams &P, cudaStream_t st) {
   const TreeParams &T = P.t;
@@ -96,8 +189,6 @@ int score_run(const ScoreParams &P, cudaStream_t st) {
                                                                                     tiles, tasks);
   return cuda_status(cudaGetLastError());
 }
-
-namespace {
 
 // rows [from, to) of the token dimension
 kv4_tensor token_range(const kv4_tensor *t, int64_t from, int64_t to) {
@@ -136,6 +227,13 @@ int scored_fill(TreeParams &P, kv4_tensor ctx[4], kv4_tensor tail[4], const kv4_
 
 int64_t stats_bytes(const TreeParams &P) {
   return (P.B * P.Hkv * P.nodes * P.R * static_cast<int64_t>(sizeof(float2)) + 255) / 256 * 256;
+}
+
+// kept scores and their factors, where few enough rows read a KV head
+int64_t kept_bytes(const TreeParams &P) {
+  const int64_t rows = static_cast<int64_t>(P.R) * P.nodes;
+  if (rows > KROWS) return 0;
+  return (P.B * P.Hkv * rows * (16 * kept_blocks(P) + 1) * 4 + 255) / 256 * 256;
 }
 
 // ---------------------------------------------------------------------------
@@ -509,7 +607,7 @@ extern "C" int64_t kv4_scored_workspace(const kv4_tensor *q, const kv4_tensor *k
   kv4_tensor ctx[4], tail[4];
   TreeParams P{};
   const int rc = scored_fill(P, ctx, tail, q, cache, q, group_size, is_causal, 0.0f);
-  return rc ? -rc : stats_bytes(P) + tree_workspace(P);
+  return rc ? -rc : stats_bytes(P) + kept_bytes(P) + tree_workspace(P);
 }
 
 extern "C" int kv4_scored_attention(const kv4_tensor *q, const kv4_tensor *k_packed,
@@ -538,16 +636,23 @@ extern "C" int kv4_scored_attention(const kv4_tensor *q, const kv4_tensor *k_pac
   }
   P.decay = decay;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const int64_t sb = stats_bytes(P.t);
-  if (sb > 0 && (!workspace || static_cast<int64_t>(workspace_bytes) < sb)) return KV4_ERR_WORKSPACE;
+  if (P.t.B == 0 || P.t.Hkv == 0) return KV4_OK;
+  // a call that leaves nothing but scores to scale
+  const bool work = P.keys > 0 && P.t.nodes > 0, mma = tree_mma_takes(P.t), tc = !mma && tree_tc_takes(P.t);
+  const bool keep = work && !tc && kept_bytes(P.t) > 0;
+  const int64_t sb = stats_bytes(P.t), kb = keep ? kept_bytes(P.t) : 0;
+  if (sb + kb > 0 && (!workspace || static_cast<int64_t>(workspace_bytes) < sb + kb)) return KV4_ERR_WORKSPACE;
   P.t.stats = static_cast<float2 *>(workspace);
-  rc = tree_run(P.t, static_cast<char *>(workspace) + sb,
-                static_cast<int64_t>(workspace_bytes) - sb, st);
-  if (rc) return rc;
-  if (P.keys > 0 && P.t.B > 0 && P.t.nodes > 0) {
-    if (tree_mma_takes(P.t)) return score_mma_run(P, st);
-    if (tree_tc_takes(P.t)) return score_tc_run(P, st);
+  if (keep) {
+    P.t.kept = reinterpret_cast<float *>(static_cast<char *>(workspace) + sb);
+    P.t.kept_c = P.t.kept + P.t.B * P.t.Hkv * P.t.R * P.t.nodes * 16 * kept_blocks(P.t);
   }
+  rc = tree_run(P.t, static_cast<char *>(workspace) + sb + kb,
+                static_cast<int64_t>(workspace_bytes) - sb - kb, st);
+  if (rc) return rc;
+  if (keep) return kept_run(P, st);
+  if (work && mma) return score_mma_run(P, st);
+  if (work && tc) return score_tc_run(P, st);
   return score_run(P, st);
 }
 

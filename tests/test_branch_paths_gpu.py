@@ -180,3 +180,47 @@ def test_scored_much_work(d, group):
 @pytest.mark.parametrize("dtype,sdtype", [(torch.float16, torch.float16), (BF16, torch.float16)])
 def test_scored_much_work_in_half_precision(dtype, sdtype):
     _scored(2, 64, 8, 32, 700, 128, 32, dtype, sdtype=sdtype, decay=0.9, seed=3)
+
+
+@pytest.mark.parametrize("dtype,group", [(BF16, 16), (BF16, 32), (torch.float16, 32), (torch.float32, 32)])
+def test_output_layout_may_differ_from_the_queries(dtype, group):
+    """An output that only element-wise stores can write takes another kernel."""
+    from kernels.llama3.evict import attention_forward_quant_gqa_scored
+    from kernels.llama3.tree_attention_quant import tree_attention_quant_gqa
+    b, hq, hkv, s, d = 2, 8, 2, 700, 128
+    for n in (1, 3, 40):
+        cache = [t.cuda() for t in br.random_rows(b, hkv, s, d, group, dtype, 1)]
+        draft = [t.cuda() for t in br.random_rows(b, hkv, n, d, group, dtype, 2)]
+        q = torch.randn(b, hq, n, d, generator=torch.Generator().manual_seed(3)).to(dtype).cuda()
+        odd = torch.full((b, hq, n, d + 1), float("nan"), dtype=dtype, device="cuda")[..., 1:]
+        mask = br.tree_mask(1, n, 4)[0].cuda()
+        mass = torch.zeros(b, hkv, s, device="cuda")
+        tree = tree_attention_quant_gqa(q, *cache, *draft, mask, n_q_heads=hq, n_kv_heads=hkv,
+                                        group_size=group, out=odd)
+        k, v = (torch.cat((br.values(*cache[i:i + 2], group, d), br.values(*draft[i:i + 2], group, d)), 2)
+                for i in (0, 2))
+        seen = torch.ones(n, s + n, dtype=torch.bool)
+        seen[:, s:] = mask.cpu()
+        for x in range(b):
+            ref, _, X, A = br.attend(q[x].cpu().double(), k[x], v[x], seen)
+            br.check_out(tree[x], ref, X, A, s + n)
+        odd = torch.full((b, hq, n, d + 1), float("nan"), dtype=dtype, device="cuda")[..., 1:]
+        out, new = attention_forward_quant_gqa_scored(q, *cache, mass, n_q_heads=hq, n_kv_heads=hkv,
+                                                      group_size=group, is_causal=True, out=odd)
+        seen = torch.ones(n, s, dtype=torch.bool).tril(s - n)
+        for x in range(b):
+            ref, p, X, A = br.attend(q[x].cpu().double(), k[x, :, :s], v[x, :, :s], seen)
+            br.check_out(out[x], ref, X, A, s)
+            add = p.reshape(hkv, -1, s)
+            rel = br.weight_bound(X, d, s).reshape(hkv, -1, 1) + br.U32 * (add.shape[1] + 8)
+            want = add.sum(1)
+            assert bool(((new[x].cpu().double() - want).abs()
+                         <= (rel * add).sum(1) + br.U32 * 2 * want + 1e-30).all())
+
+
+@pytest.mark.parametrize("dtype", [BF16, torch.float16, torch.float32])
+@pytest.mark.parametrize("hq,hkv,sq", [(8, 2, 4), (16, 1, 1), (17, 1, 1), (9, 1, 1), (8, 1, 1), (6, 2, 5)])
+def test_scored_few_rows(dtype, hq, hkv, sq):
+    for s in (17, 100, 1000, 9001):
+        _scored(2, hq, hkv, sq, s, 128, 32, dtype, causal=True, decay=0.9, seed=s)
+        _scored(2, hq, hkv, sq, s, 64, 64, dtype, causal=False, decay=0.9, seed=s)
