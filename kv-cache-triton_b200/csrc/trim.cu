@@ -84,8 +84,8 @@ constexpr int KROWS = 16;      // most rows of a KV head whose scores are kept
 // is read or multiplied twice, and its parts are joined here too.  The first
 // `joins` blocks join the outputs, a warp per row; the others take 256 keys of a
 // (sequence, KV head) each: their warps join the rows' maxima and sums, then a
-// thread sums the weights of its key.
-template <int DC>
+// thread sums the weights of its keys, PER of them.
+template <int DC, int PER>
 __global__ void __launch_bounds__(KTHREADS, 4)
     score_kept(const __grid_constant__ ScoreParams P, const GenPlan L, int joins, int blocks) {
   __shared__ float sm[KROWS], sl[KROWS], sc[KROWS];
@@ -99,11 +99,18 @@ __global__ void __launch_bounds__(KTHREADS, 4)
   }
   const int at = static_cast<int>(blockIdx.x) - joins, unit = at / blocks, b = unit / T.Hkv;
   const int kvh = unit - b * T.Hkv;
-  const int64_t slot = static_cast<int64_t>(at - unit * blocks) * KTHREADS + tid;
-  const int64_t ctx = (T.S + 15) & ~int64_t(15), t = slot < ctx ? slot : T.S + slot - ctx;
-  const bool on = slot < ctx ? slot < T.S : t < P.keys;
-  // what this reads was there before the attention began
-  const float old = on ? P.in[b * P.is[0] + kvh * P.is[1] + t * P.is[2]] * P.decay : 0.0f;
+  const int64_t slot0 = static_cast<int64_t>(at - unit * blocks) * (PER * KTHREADS) + tid;
+  const int64_t ctx = (T.S + 15) & ~int64_t(15);
+  const float *in = P.in + b * P.is[0] + kvh * P.is[1];
+  float *out = P.out + b * P.os[0] + kvh * P.os[1];
+  float sum[PER];
+  bool on[PER];
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int64_t slot = slot0 + i * KTHREADS, t = slot < ctx ? slot : T.S + slot - ctx;
+    on[i] = slot < ctx ? slot < T.S : t < P.keys;
+    sum[i] = on[i] ? in[t * P.is[2]] * P.decay : 0.0f;  // was there before the attention began
+  }
   griddep_wait();
   const int64_t n = L.units * L.rows, first = static_cast<int64_t>(unit) * L.rows;
   for (int r = warp; r < L.rows; r += KTHREADS / 32) {
@@ -135,22 +142,31 @@ __global__ void __launch_bounds__(KTHREADS, 4)
     }
   }
   __syncthreads();
-  if (!on) return;
-  const float *x = T.kept + kept_at(unit, kept_blocks(T), slot, 0, L.rows);
-  float sum = 0.0f;
+  const int64_t blks = kept_blocks(T);
+  const float *x[PER];
+#pragma unroll
+  for (int i = 0; i < PER; ++i) x[i] = T.kept + kept_at(unit, blks, on[i] ? slot0 + i * KTHREADS : 0, 0, L.rows);
 #pragma unroll 4
   for (int r = 0; r < L.rows; ++r) {
-    const float y = x[16 * r];
-    if (sl[r] != 0.0f) sum += exp2f(fmaf(y, sc[r], -sm[r])) * sl[r];
+    const float m = sm[r], inv = sl[r], c = sc[r];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const float y = x[i][16 * r];
+      if (inv != 0.0f) sum[i] += exp2f(fmaf(y, c, -m)) * inv;
+    }
   }
-  P.out[b * P.os[0] + kvh * P.os[1] + t * P.os[2]] = old + sum;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int64_t slot = slot0 + i * KTHREADS, t = slot < ctx ? slot : T.S + slot - ctx;
+    if (on[i]) out[t * P.os[2]] = sum[i];
+  }
 }
 
-template <int DC>
+template <int DC, int PER>
 int launch_kept(const ScoreParams &P, cudaStream_t st) {
   const GenPlan L = tree_plan(P.t);
   const int64_t joins = L.parts > 1 ? (L.units * L.rows + KTHREADS / 32 - 1) / (KTHREADS / 32) : 0;
-  const int64_t blocks = (16 * kept_blocks(P.t) + KTHREADS - 1) / KTHREADS, all = joins + L.units * blocks;
+  const int64_t blocks = (16 * kept_blocks(P.t) + PER * KTHREADS - 1) / (PER * KTHREADS), all = joins + L.units * blocks;
   if (all > 0x7fffffff) return KV4_ERR_UNSUPPORTED;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(static_cast<unsigned>(all));
@@ -161,14 +177,21 @@ int launch_kept(const ScoreParams &P, cudaStream_t st) {
   at.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &at;
   cfg.numAttrs = 1;
-  return cuda_status(cudaLaunchKernelEx(&cfg, score_kept<DC>, P, L, static_cast<int>(joins), static_cast<int>(blocks)));
+  return cuda_status(cudaLaunchKernelEx(&cfg, score_kept<DC, PER>, P, L, static_cast<int>(joins), static_cast<int>(blocks)));
+}
+
+// four keys a thread once that still gives every SM a block
+template <int DC>
+int launch_kept_per(const ScoreParams &P, cudaStream_t st) {
+  const bool many = P.t.B * P.t.Hkv * (16 * kept_blocks(P.t) / (4 * KTHREADS)) >= 148;
+  return many ? launch_kept<DC, 4>(P, st) : launch_kept<DC, 1>(P, st);
 }
 
 int kept_run(const ScoreParams &P, cudaStream_t st) {
-  if (P.t.d <= 64) return launch_kept<2>(P, st);
-  if (P.t.d <= 128) return launch_kept<4>(P, st);
-  if (P.t.d <= 256) return launch_kept<8>(P, st);
-  return launch_kept<16>(P, st);
+  if (P.t.d <= 64) return launch_kept_per<2>(P, st);
+  if (P.t.d <= 128) return launch_kept_per<4>(P, st);
+  if (P.t.d <= 256) return launch_kept_per<8>(P, st);
+  return launch_kept_per<16>(P, st);
 }
 
 int score_run(const ScoreParams &P, cudaStream_t st) {
