@@ -11,7 +11,7 @@
 //                scores, and rescales its output accumulator when the maximum
 //                moved by more than 2^8 (seldom).
 //   warps 8-15   dequantization, four warps each for K and V: chunks of 16 bytes
-//                (32 codes), loaded two tiles ahead into registers, to f16 tiles
+//                (32 codes), loaded a tile ahead into registers, to f16 tiles
 //                in the swizzled layout of the matrix descriptors, double-buffered.
 //   warp 16      an elected lane issues S = Q K^T and O += P V for both streams.
 //   warps 17-19  turn the mask bytes of drafted tiles into 128 bits per row.
@@ -73,6 +73,11 @@ struct Segment {
   bool first;               // the CTA's first segment
 };
 
+// rows of a 128-row tile that differ: up to 64 (32) lie in it twice (four times)
+__device__ __forceinline__ int tile_rows(const Segment &s) {
+  return s.nrows > 64 ? 128 : s.nrows > 32 ? 64 : 32;
+}
+
 // walks a CTA's segments; every role walks its own copy
 struct Walk {
   uint32_t left;            // tiles still to do
@@ -115,7 +120,8 @@ struct Smem {
   static constexpr int Q = 0, K = 2 * TILE, V = 4 * TILE, END = 6 * TILE;
   static constexpr int ML = END;            // float2 [2][128]
   static constexpr int MASK = ML + 2048;    // uint4 [2][128]: a row's visible keys of a drafted tile
-  static constexpr int BAD = MASK + 4096;   // uint32 [4 + 2][4]: drafted keys without a usable scale in K, V
+  static constexpr int QC = MASK + 4096;    // float [2][128]: a row's factor from scores to base-2 exponents
+  static constexpr int BAD = QC + 1024;   // uint32 [4 + 2][4]: drafted keys without a usable scale in K, V
   static constexpr int BARS = BAD + 96;     // mbarriers
   static constexpr int MISC = BARS + 160;   // TMEM address, abort flag, walk start
   static constexpr int BYTES = MISC + 64;
@@ -123,7 +129,7 @@ struct Smem {
 
 // barriers (pairs: by stage or by stream) and their arrival counts
 enum Bar { KFULL = 0, VFULL = 2, KEMPTY = 4, VEMPTY = 6, SFULL = 8, PREADY = 10, OREADY = 12,
-           MFULL = 14, MEMPTY = 16, QREADY = 18, NBARS = 19 };
+           MFULL = 14, MEMPTY = 16, QREADY = 18, QFREE = 19, NBARS = 20 };
 __device__ __forceinline__ int bar_count(int i) {
   if (i < KEMPTY) return 4;           // dequantizing warps of K, of V
   if (i < PREADY) return 1;           // commits
@@ -173,25 +179,21 @@ __device__ __forceinline__ void dequant_role(const TcParams &P, Walk walk, const
   const Chunk<D> own(tid);
   const int r0 = own.row, c = own.c;
 
-  // the tile to load next: its segment, and this thread's first row in it
   Segment s;
-  bool have = walk.next(P, s);
-  int i = 0, nctx = 0, len = 0, rem = 0;
-  bool draft = false;
+  int nctx = 0, len = 0, rem = 0;
   Source src{};
-  auto point = [&](bool fresh) {
-    if (fresh) {
-      len = static_cast<int>(context_len(T, s.b, nullptr));
-      nctx = (len + KT - 1) / KT;
-    }
+  auto load = [&](Regs &r, int i) {  // tile i of the segment
     const int tile = s.tile + i;
-    draft = tile >= nctx;
-    const int t0 = (draft ? tile - nctx : tile) * KT + r0;
-    rem = (draft ? T.ndraft : len) - t0;
-    src = source_of<D, G, DQ>(T, draft, is_v, s.b, s.kvh, t0, c);
-  };
-  auto load = [&](Regs &r) {  // and step to the tile after it
-    r.draft = draft;
+    r.draft = tile >= nctx;
+    if (i == 0 || tile == nctx) {
+      const int t0 = (r.draft ? tile - nctx : tile) * KT + r0;
+      rem = (r.draft ? T.ndraft : len) - t0;
+      src = source_of<D, G, DQ>(T, r.draft, is_v, s.b, s.kvh, t0, c);
+    } else {
+      src.p += static_cast<int64_t>(NCH) * src.pst;
+      src.s += static_cast<int64_t>(NCH) * src.sst;
+      rem -= KT;
+    }
 #pragma unroll
     for (int k = 0; k < NCH; ++k) {
       r.w[k] = make_uint4(0, 0, 0, 0);
@@ -202,18 +204,6 @@ __device__ __forceinline__ void dequant_role(const TcParams &P, Walk walk, const
 #pragma unroll
         for (int e = 0; e < NS; ++e) r.s[k][e] = __ldg(src.s + static_cast<int64_t>(k) * src.sst + e);
       }
-    }
-    bool fresh = false;
-    if (++i == s.ntiles) {
-      i = 0;
-      have = fresh = walk.next(P, s);
-    }
-    if (!fresh && !draft && s.tile + i < nctx) {
-      src.p += static_cast<int64_t>(NCH) * src.pst;
-      src.s += static_cast<int64_t>(NCH) * src.sst;
-      rem -= KT;
-    } else if (have) {
-      point(fresh);
     }
   };
   bool big = false;
@@ -253,19 +243,37 @@ __device__ __forceinline__ void dequant_role(const TcParams &P, Walk walk, const
     if ((tid & 31) == 0) mbar_arrive(W.at((is_v ? VFULL : KFULL) + st));
     ++n;
   };
-  // two tiles in flight: each is loaded while the one before it is stored
-  Regs a, b2;
-  bool ha = false, hb = false;
-  if (have) point(true);
+  // the next tile is on its way while one waits for its stage and is stored
+  Regs a;
+  bool narrow = false;  // the segment before had one row tile
 #pragma unroll 1
-  do {
-    if (ha) turn_over(a);
-    ha = have;
-    if (ha) load(a);
-    if (hb) turn_over(b2);
-    hb = have;
-    if (hb) load(b2);
-  } while (ha);
+  for (uint32_t seg = 0; walk.next(P, s); ++seg) {
+    len = static_cast<int>(context_len(T, s.b, nullptr));
+    nctx = (len + KT - 1) / KT;
+    load(a, 0);
+    // The segment's queries, a row tile by K's warps and one by V's: as soon as
+    // the scores of the segment before are out (and its exchange, which uses
+    // their place, is over), beside its last softmax and its epilogue.
+    if (seg > 0) {
+      W.wait(KEMPTY + ((n - 1) & 1u), (n - 1) >> 1);
+      if (narrow) W.wait(QFREE, seg - 1);
+    }
+    const bool two = s.nrows > 128;
+    narrow = !two;
+    if (two || !is_v) {
+      const int row = s.row0 + (two ? 128 * is_v + tid : tid & (tile_rows(s) - 1));
+      const float c0 = load_query_row<D>(T, P.rows, s.b, s.kvh, row, smem + SM::Q + is_v * SM::TILE, tid);
+      asm volatile("st.shared.f32 [%0], %1;" ::"r"(smem + SM::QC + 4 * (128 * is_v + tid)), "f"(c0) : "memory");
+    }
+    tc::fence_smem();
+    __syncwarp();
+    if ((tid & 31) == 0) mbar_arrive(W.at(QREADY));
+#pragma unroll 1
+    for (int i = 0; i < s.ntiles; ++i) {
+      turn_over(a);
+      if (i + 1 < s.ntiles) load(a, i + 1);
+    }
+  }
   if (big) atomicOr(&g_branch_error_tc, DEV_ERR_F16_RANGE);
 }
 
@@ -480,26 +488,23 @@ __device__ __forceinline__ void softmax_role(const TcParams &P, Walk walk, const
   const uint32_t lanes = static_cast<uint32_t>((tid >> 5) & 3) << 21;  // 32 lanes per warp
   const uint32_t tS = tmem + 128 * x + lanes, tO = tmem + 256 + 128 * x + lanes;
   Segment s;
-  uint32_t ns = 0, nm = 0, base = 0;  // steps and drafted tiles of this stream; tiles before this segment
+  // steps and drafted tiles of this stream; segments; tiles before this segment
+  uint32_t ns = 0, nm = 0, seg = 0, base = 0;
   while (walk.next(P, s)) {
     const bool two = s.nrows > 128;
     const int nt = s.ntiles, steps = two ? nt : (nt + 1 - x) / 2;
     // Up to 64 (32) rows lie in the tile twice (four times): each copy takes a
     // half (a quarter) of every key tile's columns, with a maximum, a sum and an
     // output of its own, so that all warps have work.
-    const int copies = two || s.nrows > 64 ? 1 : s.nrows > 32 ? 2 : 4, RR = 128 / copies;
+    const int RR = tile_rows(s), copies = 128 / RR;
     const int copy = r / RR, cs = copy * 4 / copies, ce = cs + 4 / copies;
     const int row = s.row0 + (two ? 128 * x + r : r & (RR - 1));
     const bool ok = row < P.rows, idle = __all_sync(0xffffffffu, !ok);
     const int node = row / T.R, head = s.kvh * T.R + row - node * T.R;
 
-    const float c0 = load_query_row<D>(T, P.rows, s.b, s.kvh, row, smem + SM::Q + x * SM::TILE, r,
-                                       two || x == 0);
-    tc::fence_smem();
-    tc::fence_before();
-    __syncwarp();
-    if (lane == 0) mbar_arrive(W.at(QREADY));
     const int len = static_cast<int>(context_len(T, s.b, nullptr)), nctx = (len + KT - 1) / KT;
+    W.wait(QREADY, seg++);
+    const float c0 = __uint_as_float(lds32(smem + SM::QC + 4 * (two ? tid : r & (RR - 1))));
 
     float m = -INFINITY, l = 0.0f;
     bool broken = false;  // saw a key without a usable scale
@@ -689,7 +694,8 @@ __device__ __forceinline__ void softmax_role(const TcParams &P, Walk walk, const
       }
     }
     tc::fence_before();
-    bar_softmax();  // nobody writes Q or the exchange area of the next segment early
+    __syncwarp();
+    if (lane == 0) mbar_arrive(W.at(QFREE));
   }
 }
 
@@ -762,15 +768,14 @@ __global__ void __launch_bounds__(THREADS, 1) tree_tc(const __grid_constant__ Tc
   const uint32_t tmem =
       __shfl_sync(0xffffffffu, *reinterpret_cast<volatile uint32_t *>(smem_raw + SM::MISC), 0);
   const Walk walk{static_cast<uint32_t>(start[0]), start[1], start[2], start[3], start[4], true};
-  // 128 * (2 * 104 + 2 * 96 + 80) = 640 * 96 registers: nothing spills but
-  // groups of 16 of 128 columns, a little.  Sixteen dequantizing warps (896
-  // threads of 72 registers) all spill: 160 us instead of 148 at 64 nodes x 16K x
-  // 64 heads, batch 4.
+  // 128 * (2 * 96 + 2 * 104 + 80) = 640 * 96 registers.  Measured at 64 nodes x 16K
+  // x 64 heads, batch 4: 146 us, 148 with 104 / 88 / 96; sixteen dequantizing or
+  // sixteen softmax warps (896 threads, two to a row there) spill: 160 and 154.
   if (warp < 8) {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 104;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
     softmax_role<D>(P, walk, W, smem, tmem, tid);
   } else if (warp < 16) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 104;");
     dequant_role<D, G>(P, walk, W, smem, warp >= 12, tid & 127);
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");

@@ -93,11 +93,10 @@ __device__ __forceinline__ void store_chunk(uint32_t tile, int row, int c, const
 // [2^13, 2^14): copied as it is to its place in shared memory (D / 8 lanes a
 // row), then converted there by its own thread.  The calling warp holds 32
 // consecutive rows, r = 0 mod 32 in lane 0; rows at or past `rows` become
-// zeros.  Returns the factor from scores to base-2 exponents.  convert = false:
-// only that (the tile's contents are then of no use).
+// zeros.  Returns the factor from scores to base-2 exponents.
 template <int D>
 __device__ __forceinline__ float load_query_row(const TreeParams &T, int rows, int b, int kvh,
-                                                int row, uint32_t tile, int r, bool convert) {
+                                                int row, uint32_t tile, int r) {
   constexpr int LPR = D / 8, RPI = 32 / LPR;  // lanes per row, rows at a time
   const int lane = threadIdx.x & 31;
   {
@@ -105,49 +104,50 @@ __device__ __forceinline__ float load_query_row(const TreeParams &T, int rows, i
     const __nv_bfloat16 *q = static_cast<const __nv_bfloat16 *>(T.q) + b * T.qs[0] +
                              static_cast<int64_t>(kvh * T.R) * T.qs[1] + 8 * k;
     const int dn = RPI / T.R, dh = RPI - dn * T.R;
-    int qn = (first + rl) / T.R, qh = first + rl - qn * T.R;  // node and head of this lane's row
-#pragma unroll 2
+    const int qn = (first + rl) / T.R;
+    int qh = first + rl - qn * T.R;  // head of this lane's row
+    const __nv_bfloat16 *p = q + qh * T.qs[1] + qn * T.qs[2];
+    const int64_t step = dh * T.qs[1] + dn * T.qs[2], wrap = T.qs[2] - T.R * T.qs[1];
+    const uint32_t to = tile + (k >> 3) * tc::PANEL + (r & ~31) * 128;
+#pragma unroll 4
     for (int g = rl; g < 32; g += RPI) {
       const bool in = first + g < rows;
-      cp_async16(tile + tc::tile_off((r & ~31) + g, k),
-                 in ? q + qh * T.qs[1] + qn * T.qs[2] : static_cast<const __nv_bfloat16 *>(T.q),
+      cp_async16(to + g * 128 + (((k & 7) ^ (g & 7)) << 4), in ? p : static_cast<const __nv_bfloat16 *>(T.q),
                  in ? 16u : 0u);
-      qn += dn;
+      p += step;
       qh += dh;
       if (qh >= T.R) {
         qh -= T.R;
-        ++qn;
+        p += wrap;
       }
     }
     cp_async_wait_all();
     __syncwarp();
   }
-  uint32_t top = 0;  // largest |q| as bits: bf16 magnitudes order like integers
+  uint32_t top2 = 0;  // largest |q| as bits: bf16 magnitudes order like integers
 #pragma unroll 4
   for (int k = 0; k < D / 8; ++k) {
     const uint4 w = lds128(tile + tc::tile_off(r, k));
-    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-    for (int e = 0; e < 4; ++e) top = max(top, max(u[e] & 0x7FFFu, (u[e] >> 16) & 0x7FFFu));
+    top2 = __vmaxu2(top2, __vmaxu2(__vmaxu2(w.x & 0x7FFF7FFFu, w.y & 0x7FFF7FFFu),
+                                   __vmaxu2(w.z & 0x7FFF7FFFu, w.w & 0x7FFF7FFFu)));
   }
+  const uint32_t top = max(top2 & 0xFFFFu, top2 >> 16);
   int ex = 13 - (static_cast<int>(top >> 7) - 127);
   ex = top == 0 ? 0 : min(max(ex, -126), 126);
-  if (convert) {
-    const float up = __uint_as_float(static_cast<uint32_t>(ex + 127) << 23);
+  const float up = __uint_as_float(static_cast<uint32_t>(ex + 127) << 23);
 #pragma unroll 4
-    for (int k = 0; k < D / 8; ++k) {
-      const uint32_t at = tile + tc::tile_off(r, k);
-      const uint4 w = lds128(at);
-      const uint32_t u[4] = {w.x, w.y, w.z, w.w};
-      float f[8];
+  for (int k = 0; k < D / 8; ++k) {
+    const uint32_t at = tile + tc::tile_off(r, k);
+    const uint4 w = lds128(at);
+    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+    float f[8];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        f[2 * e] = bf16lo_to_f32(u[e]) * up;
-        f[2 * e + 1] = bf16hi_to_f32(u[e]) * up;
-      }
-      tc::sts128(at, pack_f16x2(f[0], f[4]), pack_f16x2(f[1], f[5]), pack_f16x2(f[2], f[6]),
-                 pack_f16x2(f[3], f[7]));
+    for (int e = 0; e < 4; ++e) {
+      f[2 * e] = bf16lo_to_f32(u[e]) * up;
+      f[2 * e + 1] = bf16hi_to_f32(u[e]) * up;
     }
+    tc::sts128(at, pack_f16x2(f[0], f[4]), pack_f16x2(f[1], f[5]), pack_f16x2(f[2], f[6]),
+               pack_f16x2(f[3], f[7]));
   }
   return T.scale_log2 * __uint_as_float(static_cast<uint32_t>(127 - ex) << 23);
 }

@@ -257,7 +257,7 @@ __device__ __forceinline__ void sum_role(const STcParams &P, Walk walk, const Wa
       asm volatile("bar.sync 1, 256;" ::: "memory");
       if (group == 0) {
         const int row = pass * RT + r;
-        const float c0 = load_query_row<D>(T, P.rows, p.b, p.kvh, row, smem + SM::Q, r, true);
+        const float c0 = load_query_row<D>(T, P.rows, p.b, p.kvh, row, smem + SM::Q, r);
         float c = 0.0f, nm = 0.0f, li = 0.0f;
         if (row < P.rows) {
           const float2 st = T.stats[static_cast<int64_t>(unit) * P.rows + row];
