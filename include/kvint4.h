@@ -336,6 +336,11 @@ int kv4_prefill_attention(const kv4_tensor *q, const kv4_tensor *k_packed,
  * strides; all four scale tensors have one dtype.  `workspace` holds at least
  * kv4_tree_workspace() bytes (device, 16-byte aligned, any contents; a
  * negative result of that function is minus a status).
+ * 16-bit queries and scales take tensor-core kernels whose V operand (and, for
+ * bf16 with much work, K operand) is f16, exact while scales stay below
+ * 65504/8: a larger or non-finite scale in the context sets bit 8 of
+ * kv4_device_error (output not valid).  One in a drafted row makes the nodes
+ * that see the row NaN and no others, and sets the bit as well.
  */
 int64_t kv4_tree_workspace(const kv4_tensor *q, const kv4_tensor *k_packed,
                            const kv4_tensor *k_scales, const kv4_tensor *v_packed,
@@ -373,7 +378,8 @@ int kv4_commit_rows(const kv4_tensor *k_packed, const kv4_tensor *k_scales,
  *   score_out[b, g, t] = decay * score_in[b, g, t] + the softmax weight that
  *   token t received, summed over the queries and over the q heads of KV head g.
  * score_in, score_out: f32 [1, B, Hkv, S] (any strides; they may be the same
- * tensor).  Shapes, dtypes and workspace as for kv4_tree_attention, with
+ * tensor).  is_causal: query i sees tokens t <= S - sq + i.  Shapes, dtypes, the
+ * range of scales and workspace as for kv4_tree_attention, with
  * kv4_scored_workspace() bytes.
  */
 int64_t kv4_scored_workspace(const kv4_tensor *q, const kv4_tensor *k_packed,
@@ -403,8 +409,8 @@ int kv4_evict(const kv4_tensor *k_packed, const kv4_tensor *k_scales, const kv4_
 
 /* Read-and-clear the device error word (synchronizes the stream): bit 1 a
    bounded mbarrier wait expired, bit 2 a page id outside the pool, bit 4 a
-   peer exchange wait expired, bit 8 kv4_prefill_attention met K/V values
-   outside the f16 range, bit 16 a context length, accepted count or path node
+   peer exchange wait expired, bit 8 K/V values outside the f16 range
+   (kv4_prefill_attention, kv4_tree_attention, kv4_scored_attention), bit 16 a context length, accepted count or path node
    out of range (kv4_tree_attention, kv4_commit_rows). */
 int kv4_device_error(void *stream, int *flag_out);
 

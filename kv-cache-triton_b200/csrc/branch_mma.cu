@@ -914,14 +914,15 @@ bool close_rows(const RowSource &S, int64_t B, int Hkv, int64_t T, int pw, int b
 
 // Whether warps in registers beat tensor-memory tiles (branch_tc.cu, trim_tc.cu).
 // They take 1.3 us per SM for every 16 rows of a 128-key tile, whatever the
-// total; the tiles 2.7 us for up to 128 rows, and about 20 us to get going.
-// Measured (us, warps / tiles; 8 KV heads of 128 columns): 32 rows x 4K keys
-// 20 / 40, batch 8 of them 41 / 59; 64 rows x 4K, batch 1 20 / 43, batch 4
-// 40 / 43, batch 8 76 / 61; 128 rows x 1K 15 / 22; 64 rows x 32K 66 / 65.
+// total; the tiles 1.5 to 1.9 us for up to 128 rows, and about 18 us to begin and
+// to join.  Measured (us, warps / tiles; 8 KV heads of 128 columns): 16 rows x
+// 4K keys, batch 16 42 / 62; 32 rows x 4K, batch 1 17 / 37, batch 8 42 / 43, batch
+// 16 79 / 62; 48 rows x 4K, batch 4 33 / 37, batch 8 56 / 44; 64 rows x 4K, batch 1
+// 18 / 40, batch 4 41 / 37; 128 rows x 4K 26 / 44, x 1K, batch 4 28 / 34.
 bool few_rows(const TreeParams &T) {
   const int64_t row_tiles = (static_cast<int64_t>(T.R) * T.nodes + 15) / 16;
   const int64_t tiles = T.B * T.Hkv * ((T.S + T.ndraft + 127) / 128);
-  return row_tiles <= 2 || tiles * (row_tiles - 2) <= 14 * static_cast<int64_t>(sm_count());
+  return tiles * (2 * row_tiles - 3) <= 26 * static_cast<int64_t>(sm_count());
 }
 
 // Whether the kernels of this file take the call: 16-bit queries and scales, the
