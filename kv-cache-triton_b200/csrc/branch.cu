@@ -166,10 +166,15 @@ __global__ void __launch_bounds__(128, 4) tree_merge(const __grid_constant__ Tre
 
 constexpr int kSms = 148;
 
+// Rows a warp holds: eight share one dequantized tile, fewer where there are no
+// more (4 rows x 4000 keys x 8 heads of 128, batch 4, fp32: 63 us instead of 76;
+// four for 12 rows x 777: 26 us instead of 23).
+int rows_per_warp(int rows) { return rows <= 2 ? 2 : rows <= 4 ? 4 : 8; }
+
 GenPlan gen_plan(const TreeParams &P) {
   GenPlan L{};
   L.rows = P.R * P.nodes;
-  const int rw = L.rows <= 2 ? 2 : 8;
+  const int rw = rows_per_warp(L.rows);
   L.row_tiles = (L.rows + rw - 1) / rw;
   L.units = P.B * P.Hkv;
   L.ld = row_ld(P.d);
@@ -220,7 +225,11 @@ int launch_gen(const TreeParams &P, const GenPlan &L, cudaStream_t st) {
 
 template <int DC>
 int launch_gen_rw(const TreeParams &P, const GenPlan &L, cudaStream_t st) {
-  return L.rows <= 2 ? launch_gen<DC, 2>(P, L, st) : launch_gen<DC, 8>(P, L, st);
+  switch (rows_per_warp(L.rows)) {
+    case 2: return launch_gen<DC, 2>(P, L, st);
+    case 4: return launch_gen<DC, 4>(P, L, st);
+    default: return launch_gen<DC, 8>(P, L, st);
+  }
 }
 
 bool is_float(int dt) { return dt == KV4_F32 || dt == KV4_F16 || dt == KV4_BF16; }
