@@ -55,7 +55,7 @@ __global__ void __launch_bounds__(128, 1) tree_generic(const TreeParams P, const
   const int64_t k0 = part * per * 32, k1 = min(total, k0 + per * 32);
   const int r0 = rt * RW, d8 = (P.d + 7) >> 3;
 
-  warp_query(P, b, kvh, r0, RW, L.rows, sQ, L.ld, lane);
+  warp_query<RW>(P, b, kvh, r0, L.rows, sQ, L.ld, lane);
   float m[RW], l[RW], acc[RW][DC];
 #pragma unroll
   for (int r = 0; r < RW; ++r) {
@@ -299,12 +299,13 @@ int tree_fill(TreeParams &P, const kv4_tensor *q, const kv4_tensor *const cache[
   P.d = static_cast<int>(d);
   P.G = G;
   P.S = S;
-  P.words = G >= 8 && (G & (G - 1)) == 0 && d % 8 == 0;
+  P.words = G < 8 || (G & (G - 1)) || d % 8 ? 0 : d % 32 ? 4 : 16;
   for (const RowSource *src : {&P.cache, &P.draft}) {
     if (src == &P.draft && P.ndraft == 0) continue;
     uint64_t bits = reinterpret_cast<uintptr_t>(src->kp) | reinterpret_cast<uintptr_t>(src->vp);
     for (int i = 0; i < 3; ++i) bits |= static_cast<uint64_t>(src->kps[i] | src->vps[i]);
     if ((bits & 3u) || src->kps[3] != 1 || src->vps[3] != 1) P.words = 0;
+    if (bits & 15u) P.words = std::min(P.words, 4);
   }
   P.scale_log2 = (sm_scale > 0.0f ? sm_scale : 1.0f / sqrtf(static_cast<float>(d))) * kBrLog2e;
   return KV4_OK;

@@ -34,7 +34,7 @@ struct TreeParams {
   const int32_t *lens;  // context rows of each sequence, or null: all of them
   int64_t B;
   int Hkv, R, nodes, ndraft, d, G, causal, shift;
-  int words;           // rows can be read in 4-byte words of eight codes of one group
+  int words;           // bytes that rows of codes can be read in (16, 4: eight codes of a group a word; 0: one)
   int64_t S;           // context rows in the cache views
   float scale_log2;    // sm_scale * log2(e)
   float2 *stats;       // per (unit, row): base-2 maximum and 1 / sum; or null
@@ -109,73 +109,74 @@ __device__ __forceinline__ void dequant8(const uint8_t *row, int64_t cs, const S
 }
 
 // 32 rows (keys t0 .. t0+31 of `len` context rows then draft rows) of K or V
-// as floats in shared memory, ld floats apart, by one warp; rows at or past
-// `end` are 0.  d is padded with zeros to a multiple of 8.  Where rows allow it
-// a lane takes eight columns per word, four words in flight.
+// as floats in shared memory, ld floats apart, by one warp, a row per lane; rows
+// at or past `end` are 0.  d is padded with zeros to a multiple of 8.  Where rows
+// can be read in words, up to 16 of them (128 columns) are in flight.
 template <typename ST>
 __device__ __forceinline__ void warp_dequant_rows(const TreeParams &P, bool is_v, int64_t b, int h,
                                                   int64_t len, int64_t t0, int64_t end, float *dst,
                                                   int ld, int lane) {
   const int d8 = (P.d + 7) >> 3, pb = (P.G + 1) >> 1;
-  auto row_of = [&](int64_t t, const uint8_t *&p, const ST *&s, int64_t &cs, int64_t &scs) {
-    const bool ctx = t < len;
-    const RowSource &S = ctx ? P.cache : P.draft;
-    const int64_t row = ctx ? t : t - len;
-    const int64_t *ps = is_v ? S.vps : S.kps, *ss = is_v ? S.vss : S.kss;
-    p = (is_v ? S.vp : S.kp) + b * ps[0] + h * ps[1] + row * ps[2];
-    s = static_cast<const ST *>(is_v ? S.vs : S.ks) + b * ss[0] + h * ss[1] + row * ss[2];
-    cs = ps[3];
-    scs = ss[3];
-  };
+  const int64_t t = t0 + lane;
+  const bool in = t < end, ctx = t < len;
+  const RowSource &S = ctx ? P.cache : P.draft;
+  const int64_t row = ctx ? t : t - len;
+  const int64_t *ps = is_v ? S.vps : S.kps, *ss = is_v ? S.vss : S.kss;
+  const uint8_t *p = (is_v ? S.vp : S.kp) + b * ps[0] + h * ps[1] + row * ps[2];
+  const ST *q = static_cast<const ST *>(is_v ? S.vs : S.ks) + b * ss[0] + h * ss[1] + row * ss[2];
+  const int64_t cs = ps[3], scs = ss[3];
+  float4 *o = reinterpret_cast<float4 *>(dst + lane * ld);
   if (P.words) {
     const int lg = __ffs(P.G) - 1;  // groups of a power of two, at least 8
+    const uint32_t *pw = reinterpret_cast<const uint32_t *>(p);
 #pragma unroll 1
-    for (int i0 = lane; i0 < 32 * d8; i0 += 4 * 32) {
-      uint32_t w[4];
-      ST s[4];
+    for (int c0 = 0; c0 < d8; c0 += 16) {
+      uint32_t w[16];
+      ST s[16];
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const int idx = i0 + 32 * u, r = idx / d8, c = idx - r * d8;
-        w[u] = 0x88888888u;
-        s[u] = from_f32<ST>(0.0f);
-        if (idx < 32 * d8 && t0 + r < end) {
-          const uint8_t *p;
-          const ST *q;
-          int64_t cs, scs;
-          row_of(t0 + r, p, q, cs, scs);
-          w[u] = __ldg(reinterpret_cast<const uint32_t *>(p) + c);
-          s[u] = q[((8 * c) >> lg) * scs];
+      for (int u = 0; u < 16; u += 4) {
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if (in && c0 + u < d8) {
+          if (P.words == 16) {
+            v = __ldg(reinterpret_cast<const uint4 *>(pw + c0 + u));
+          } else {
+            v.x = __ldg(pw + c0 + u);
+            if (c0 + u + 1 < d8) v.y = __ldg(pw + c0 + u + 1);
+            if (c0 + u + 2 < d8) v.z = __ldg(pw + c0 + u + 2);
+            if (c0 + u + 3 < d8) v.w = __ldg(pw + c0 + u + 3);
+          }
+        }
+        w[u] = v.x;
+        w[u + 1] = v.y;
+        w[u + 2] = v.z;
+        w[u + 3] = v.w;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          s[u + e] = from_f32<ST>(0.0f);
+          if (e > 0 && P.G >= 32) s[u + e] = s[u];
+          else if (in && c0 + u + e < d8) s[u + e] = q[((8 * (c0 + u + e)) >> lg) * scs];
         }
       }
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const int idx = i0 + 32 * u, r = idx / d8, c = idx - r * d8;
-        if (idx >= 32 * d8) break;
+      for (int u = 0; u < 16; ++u) {
+        if (c0 + u >= d8) break;
         const float f = to_f32(s[u]);
         float v[8];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) v[k] = static_cast<float>(static_cast<int>((w[u] >> (4 * k)) & 15u) - 8) * f;
-        float4 *o = reinterpret_cast<float4 *>(dst + r * ld + 8 * c);
-        o[0] = make_float4(v[0], v[1], v[2], v[3]);
-        o[1] = make_float4(v[4], v[5], v[6], v[7]);
+        for (int k = 0; k < 8; ++k)  // 2^23 + code, then code - 8: exact
+          v[k] = (__uint_as_float(0x4B000000u | ((w[u] >> (4 * k)) & 15u)) - 8388616.0f) * f;
+        o[2 * (c0 + u)] = make_float4(v[0], v[1], v[2], v[3]);
+        o[2 * (c0 + u) + 1] = make_float4(v[4], v[5], v[6], v[7]);
       }
     }
     return;
   }
 #pragma unroll 1
-  for (int idx = lane; idx < 32 * d8; idx += 32) {
-    const int r = idx / d8, c = idx - r * d8;
+  for (int c = 0; c < d8; ++c) {
     float v[8] = {};
-    if (t0 + r < end) {
-      const uint8_t *p;
-      const ST *q;
-      int64_t cs, scs;
-      row_of(t0 + r, p, q, cs, scs);
-      dequant8<ST>(p, cs, q, scs, P.G, pb, P.d, c, v);
-    }
-    float4 *o = reinterpret_cast<float4 *>(dst + r * ld + 8 * c);
-    o[0] = make_float4(v[0], v[1], v[2], v[3]);
-    o[1] = make_float4(v[4], v[5], v[6], v[7]);
+    if (in) dequant8<ST>(p, cs, q, scs, P.G, pb, P.d, c, v);
+    o[2 * c] = make_float4(v[0], v[1], v[2], v[3]);
+    o[2 * c + 1] = make_float4(v[4], v[5], v[6], v[7]);
   }
 }
 __device__ __forceinline__ void warp_dequant_tile(const TreeParams &P, bool is_v, int64_t b, int h,
@@ -186,36 +187,34 @@ __device__ __forceinline__ void warp_dequant_tile(const TreeParams &P, bool is_v
   else warp_dequant_rows<__nv_bfloat16>(P, is_v, b, h, len, t0, end, dst, ld, lane);
 }
 
-// Rows [row0, row0 + n) of a KV head's queries (row = node * R + head of the
+// N rows from row0 on of a KV head's queries (row = node * R + head of the
 // group) as floats in shared memory, ld apart, by one warp; rows at or past
 // `rows` and columns past d are 0.
-template <typename QT>
-__device__ __forceinline__ void warp_query_rows(const TreeParams &P, int64_t b, int kvh, int row0, int n,
+template <typename QT, int N>
+__device__ __forceinline__ void warp_query_rows(const TreeParams &P, int64_t b, int kvh, int row0,
                                                 int rows, float *dst, int ld, int lane) {
   const int w = (P.d + 7) & ~7;
+  const QT *q[N];
+#pragma unroll
+  for (int r = 0; r < N; ++r) {
+    const int row = row0 + r, i = row / P.R, h = kvh * P.R + row - i * P.R;
+    q[r] = row < rows ? static_cast<const QT *>(P.q) + b * P.qs[0] + h * P.qs[1] + i * P.qs[2] : nullptr;
+  }
 #pragma unroll 1
-  for (int i0 = lane; i0 < n * w; i0 += 8 * 32) {
-    QT v[8];
+  for (int c = lane; c < w; c += 32) {
+    QT v[N];
 #pragma unroll
-    for (int u = 0; u < 8; ++u) {
-      const int idx = i0 + 32 * u, r = idx / w, c = idx - r * w, row = row0 + r;
-      const int i = row / P.R, h = kvh * P.R + row - i * P.R;
-      v[u] = from_f32<QT>(0.0f);
-      if (idx < n * w && row < rows && c < P.d)
-        v[u] = static_cast<const QT *>(P.q)[b * P.qs[0] + h * P.qs[1] + i * P.qs[2] + c * P.qs[3]];
-    }
+    for (int r = 0; r < N; ++r) v[r] = q[r] && c < P.d ? q[r][c * P.qs[3]] : from_f32<QT>(0.0f);
 #pragma unroll
-    for (int u = 0; u < 8; ++u) {
-      const int idx = i0 + 32 * u, r = idx / w;
-      if (idx < n * w) dst[r * ld + idx - r * w] = to_f32(v[u]);
-    }
+    for (int r = 0; r < N; ++r) dst[r * ld + c] = to_f32(v[r]);
   }
 }
-__device__ __forceinline__ void warp_query(const TreeParams &P, int64_t b, int kvh, int row0, int n,
-                                           int rows, float *dst, int ld, int lane) {
-  if (P.q_dtype == KV4_F32) warp_query_rows<float>(P, b, kvh, row0, n, rows, dst, ld, lane);
-  else if (P.q_dtype == KV4_F16) warp_query_rows<__half>(P, b, kvh, row0, n, rows, dst, ld, lane);
-  else warp_query_rows<__nv_bfloat16>(P, b, kvh, row0, n, rows, dst, ld, lane);
+template <int N>
+__device__ __forceinline__ void warp_query(const TreeParams &P, int64_t b, int kvh, int row0, int rows,
+                                           float *dst, int ld, int lane) {
+  if (P.q_dtype == KV4_F32) warp_query_rows<float, N>(P, b, kvh, row0, rows, dst, ld, lane);
+  else if (P.q_dtype == KV4_F16) warp_query_rows<__half, N>(P, b, kvh, row0, rows, dst, ld, lane);
+  else warp_query_rows<__nv_bfloat16, N>(P, b, kvh, row0, rows, dst, ld, lane);
 }
 
 // shared-memory row length of a d-wide row: float4 steps, an odd number of

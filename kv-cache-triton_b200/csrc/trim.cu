@@ -43,7 +43,7 @@ __global__ void __launch_bounds__(128, 2) score_generic(const ScoreParams P, int
   for (int r0 = 0; r0 < rows; r0 += SROWS) {
     __syncwarp();
     const int nr = min(SROWS, rows - r0);
-    warp_query(T, b, kvh, r0, nr, rows, sQ, ld, lane);
+    warp_query<SROWS>(T, b, kvh, r0, rows, sQ, ld, lane);
     __syncwarp();
     float s[SROWS];
 #pragma unroll
