@@ -65,13 +65,39 @@ __global__ void __launch_bounds__(128, 1) tree_generic(const TreeParams P, const
     for (int k = 0; k < DC; ++k) acc[r][k] = 0.0f;
   }
 
-  for (int64_t t0 = k0; t0 < k1; t0 += 32) {
+  // K's tile, then V's over it, by the same code: two copies of it miss the
+  // instruction cache
+  int64_t t0 = k0;
+#pragma unroll 1
+  for (bool is_v = false; t0 < k1; is_v = !is_v) {
     __syncwarp();
-    warp_dequant_tile(P, false, b, kvh, len, t0, k1, sT, L.ld, lane);
+    warp_dequant_tile(P, is_v, b, kvh, len, t0, k1, sT, L.ld, lane);
     __syncwarp();
+    if (is_v) {
+      // a drafted row may hold anything where a node does not see it: there a
+      // weight of zero leaves it out instead of multiplying it
+      const bool guard = t0 + 32 > len;
+#pragma unroll 4
+      for (int j = 0; j < 32; ++j) {
+        float v[DC], p[RW];
+#pragma unroll
+        for (int k = 0; k < DC; ++k) v[k] = lane + 32 * k < 8 * d8 ? sT[j * L.ld + lane + 32 * k] : 0.0f;
+#pragma unroll
+        for (int r = 0; r < RW; ++r) p[r] = sP[j * RW + r];
+#pragma unroll
+        for (int r = 0; r < RW; ++r) {
+          if (guard && p[r] == 0.0f) continue;
+#pragma unroll
+          for (int k = 0; k < DC; ++k) acc[r][k] = fmaf(p[r], v[k], acc[r][k]);
+        }
+      }
+      t0 += 32;
+      continue;
+    }
     float s[RW];
 #pragma unroll
     for (int r = 0; r < RW; ++r) s[r] = 0.0f;
+#pragma unroll 2
     for (int c = 0; c < 2 * d8; ++c) {
       const float4 k4 = *reinterpret_cast<const float4 *>(sT + lane * L.ld + 4 * c);
 #pragma unroll
@@ -102,26 +128,6 @@ __global__ void __launch_bounds__(128, 1) tree_generic(const TreeParams P, const
 #pragma unroll
       for (int k = 0; k < DC; ++k) acc[r][k] *= a;
       sP[lane * RW + r] = p;
-    }
-    __syncwarp();
-    warp_dequant_tile(P, true, b, kvh, len, t0, k1, sT, L.ld, lane);
-    __syncwarp();
-    // a drafted row may hold anything where a node does not see it: there a
-    // weight of zero leaves it out instead of multiplying it
-    const bool guard = t0 + 32 > len;
-#pragma unroll 4
-    for (int j = 0; j < 32; ++j) {
-      float v[DC], p[RW];
-#pragma unroll
-      for (int k = 0; k < DC; ++k) v[k] = lane + 32 * k < 8 * d8 ? sT[j * L.ld + lane + 32 * k] : 0.0f;
-#pragma unroll
-      for (int r = 0; r < RW; ++r) p[r] = sP[j * RW + r];
-#pragma unroll
-      for (int r = 0; r < RW; ++r) {
-        if (guard && p[r] == 0.0f) continue;
-#pragma unroll
-        for (int k = 0; k < DC; ++k) acc[r][k] = fmaf(p[r], v[k], acc[r][k]);
-      }
     }
   }
 #pragma unroll
@@ -181,10 +187,14 @@ GenPlan gen_plan(const TreeParams &P) {
   const size_t per_warp = sizeof(float) * (32 * L.ld + rw * L.ld + 32 * rw);
   L.warps = static_cast<int>(std::max<size_t>(1, std::min<size_t>(4, 100 * 1024 / per_warp)));
   L.smem = per_warp * L.warps;
-  // ranges of at least 32 keys, enough of them for about eight warps per SM
+  // ranges of at least 32 keys, as many as the SMs take at once (a block more on
+  // a few of them runs alone at the end: 64 rows x 2000 x 8 heads of 128, batch 2,
+  // 153 us with 320 blocks, 88 with 288)
   const int64_t tiles = (P.S + P.ndraft + 31) / 32, have = L.units * L.row_tiles;
-  const int64_t want = (8 * kSms + have - 1) / have;
-  L.parts = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({want, tiles, 256})));
+  const int64_t room = kSms * L.warps * std::min<int64_t>(3, 200 * 1024 / L.smem);
+  const int64_t want = std::max<int64_t>(1, std::min<int64_t>(room / have, 256));
+  const int64_t per = std::max<int64_t>(1, (tiles + want - 1) / want);
+  L.parts = static_cast<int>(std::max<int64_t>(1, (tiles + per - 1) / per));
   L.tasks = have * L.parts;
   return L;
 }
