@@ -224,3 +224,84 @@ def test_scored_few_rows(dtype, hq, hkv, sq):
     for s in (17, 100, 1000, 9001):
         _scored(2, hq, hkv, sq, s, 128, 32, dtype, causal=True, decay=0.9, seed=s)
         _scored(2, hq, hkv, sq, s, 64, 64, dtype, causal=False, decay=0.9, seed=s)
+
+
+@pytest.mark.parametrize("dtype", [BF16, torch.float16, torch.float32])
+@pytest.mark.parametrize("bad", [math.nan, math.inf, 3e4])
+def test_unseen_rows_do_not_matter_to_few_rows(dtype, bad):
+    """As above, for calls of at most eight rows per KV head."""
+    from kernels.llama3.tree_attention_quant import tree_attention_quant_gqa
+    from kvint4 import ops
+    b, h, n, s, d, group = 2, 2, 7, 200, 64, 32
+    cache = [t.cuda() for t in br.random_rows(b, h, s, d, group, dtype, 1)]
+    draft = [t.cuda() for t in br.random_rows(b, h, n, d, group, dtype, 2)]
+    q = torch.randn(b, h, n, d, generator=torch.Generator().manual_seed(3)).to(dtype).cuda()
+    mask = br.tree_mask(b, n, 4).cuda()
+    mask[:, :, 3] = False
+    mask[:, 3, 3] = mask[:, 5, 3] = True
+    lens = torch.tensor([s - 3, 17], dtype=torch.int32, device="cuda")
+
+    def call():
+        return tree_attention_quant_gqa(q, *cache, *draft, mask, n_q_heads=h, n_kv_heads=h,
+                                        group_size=group, context_lens=lens)
+
+    want = call()
+    for x in range(b):
+        for t in (cache[1], cache[3]):
+            t[x, :, int(lens[x]):] = bad
+    ops.device_error()
+    assert torch.equal(call(), want)
+    assert ops.device_error() == 0
+    for which in (1, 3):
+        kept = draft[which][:, :, 3].clone()
+        draft[which][:, :, 3] = bad
+        got = call()
+        draft[which][:, :, 3] = kept
+        others = [i for i in range(n) if i not in (3, 5)]
+        assert torch.equal(got[:, :, others], want[:, :, others])
+        if not math.isfinite(bad) and which == 3:
+            assert not bool(torch.isfinite(got[:, :, 3]).all(-1).any())
+    ops.device_error()
+
+
+@pytest.mark.parametrize("dtype,group", [(BF16, 32), (BF16, 16), (torch.float16, 32), (torch.float32, 32)])
+def test_offsets_past_32_bits(dtype, group):
+    """Sequences of a cache that lie more than 2**32 elements apart."""
+    from kernels.llama3.evict import attention_forward_quant_gqa_scored, evict_by_mass
+    from kernels.llama3.tree_attention_quant import commit_draft_rows, tree_attention_quant_gqa
+    b, hq, hkv, n, s, d, far = 2, 8, 2, 5, 300, 128, (1 << 32) + 4096
+    room = torch.empty(far + (1 << 20), dtype=torch.uint8, device="cuda")
+    wide = torch.empty(far + (1 << 20), dtype=dtype, device="cuda")
+    small = [t.cuda() for t in br.random_rows(b, hkv, s, d, group, dtype, 1)]
+    cache = []
+    for i, t in enumerate(small):  # K's and V's tensors side by side in the same buffer
+        src = wide if i & 1 else room
+        v = src.as_strided(t.shape, (far, s * t.shape[3], t.shape[3], 1), (i >> 1) * (1 << 19))
+        v.copy_(t)
+        cache.append(v)
+    draft = [t.cuda() for t in br.random_rows(b, hkv, n, d, group, dtype, 2)]
+    q = torch.randn(b, hq, n, d, generator=torch.Generator().manual_seed(3)).to(dtype).cuda()
+    mask = br.tree_mask(b, n, 4).cuda()
+    lens = torch.tensor([s - 9, 100], dtype=torch.int32, device="cuda")
+    heads = dict(n_q_heads=hq, n_kv_heads=hkv, group_size=group)
+
+    def calls(c):
+        mass = torch.rand(b, hkv, s, generator=torch.Generator().manual_seed(5)).cuda()
+        out = [tree_attention_quant_gqa(q, *c, *draft, mask, context_lens=lens, **heads)]
+        out += attention_forward_quant_gqa_scored(q[:, :, :1].contiguous(), *c, mass, **heads)
+        out += attention_forward_quant_gqa_scored(q, *c, mass, is_causal=True, **heads)
+        out += evict_by_mass(*c, mass, keep=100, recent=5, sinks=2)
+        path = torch.tensor([[0, 2, 4], [1, 3, 0]], dtype=torch.int32, device="cuda")
+        out.append(commit_draft_rows(*c, *draft, path, torch.tensor([3, 2], dtype=torch.int32, device="cuda"),
+                                     context_lens=lens))
+        return out + [t.clone() for t in c]
+
+    for got, want in zip(calls(cache), calls([t.clone() for t in small])):
+        assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("nodes", [3, 4, 5])
+@pytest.mark.parametrize("d,group", [(512, 32), (200, 8), (64, 16), (96, 32)])
+def test_any_shape_row_counts(nodes, d, group):
+    _run(2, 2, 2, nodes, 150, d, group, torch.float32, seed=d)
+    _scored(2, 2, 2, nodes, 150, d, group, torch.float32, causal=True, seed=d)
