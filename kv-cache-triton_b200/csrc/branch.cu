@@ -16,8 +16,13 @@
 // dequantizes K into its own shared memory (lane = key for the scores), then V
 // over it (lane = column for the output), with the running maximum and sum of
 // the softmax per row.  Warps never wait for one another; ranges of one unit
-// meet in tree_merge through the workspace.  bf16 queries over bf16 scales
-// take branch_tc.cu's kernel where the layout allows.
+// meet in tree_merge through the workspace.  16-bit types take branch_tc.cu's
+// and branch_mma.cu's kernels where the layout allows.
+// Bound by instructions: 6000 for 8 rows x 32 keys x 128 columns, a third of them
+// the products, at two warps a scheduler (shared memory holds no more tiles).
+// Measured, fp32: 64 rows x 2016 keys of 128 columns in 16 units 88 us with the join
+// (12 TFLOP/s); 12 rows x 789 keys of 64 columns in 24 units 15.6 us and 5 to join,
+// where a warp has one tile and its chain counts.
 #include <algorithm>
 
 #include "merge.cuh"
@@ -418,6 +423,7 @@ __device__ __forceinline__ void move_rows(uint8_t *dst, const uint8_t *src, int6
 // A block per (sequence, KV head), 64 threads for each of the four tensors; the
 // block of head 0 writes the new length.  Such a call moves little: what it
 // costs is two rounds of memory latency (lengths and path, then the rows).
+// Measured, 8 heads of 128 columns: 2.4 us for one sequence, 2.8 for 32.
 __global__ void __launch_bounds__(4 * CTHREADS, 2) commit_rows(const __grid_constant__ CommitParams P) {
   __shared__ int32_t path[CPATH];
   const int b = blockIdx.x / P.Hkv, h = blockIdx.x - b * P.Hkv;

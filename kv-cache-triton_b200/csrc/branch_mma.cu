@@ -1,11 +1,12 @@
 // Tree attention and the scores of cached tokens for few rows, and for half
-// precision: one warp, 16 rows and 16 keys at a time, all in registers.
+// precision: one warp, up to 16 rows and 16 keys at a time, all in registers.
 //
 // Single-token decoding and small trees have R to 16 rows per KV head; a
 // 128-row tensor-memory tile is mostly padding there and its operands have to
 // pass through shared memory.  Here (mma.m16n8k16, f16 operands, fp32 sums)
 //
-//   S = Q K^T   rows are M, keys N: a thread's packed words are its B operand
+//   S = Q K^T   rows are M, keys N (up to 8 rows: the other way round, see
+//               tree_mma8): a thread's packed words are its B operand
 //               as they are loaded: four codes' worth of shifts, the code bias
 //               taken off, no scale.  Scales multiply the fp32 sums of their
 //               group of columns, so scores are exact to fp32 rounding for any
@@ -23,8 +24,11 @@
 // its warps meet in shared memory, ranges of one unit in the workspace
 // (tree_merge of branch.cu).  Every warp has a ring of steps of its own, filled
 // by asynchronous copies three ahead; nothing waits for another warp on the way.
-// Bound: memory for one row tile; instructions (about 350 per warp and 16 keys
-// of 128 columns) are close behind.
+// Bound: instructions, about 450 per warp and 16 keys of 128 columns, a third of
+// which take codes apart; memory next.  Measured, 8 KV heads of 128 columns: single
+// tokens of 4 rows, 16 sequences x 4096, 29.5 us (84 MB: 2.8 TB/s, a step in 60 % of
+// the issue slots); 8 nodes x 512 7.3 us, of which loads that wait for one another
+// are most; 32 rows x 4096, batch 4, 23 us.
 #include <algorithm>
 
 #include "branch.cuh"
@@ -508,7 +512,8 @@ __global__ void __launch_bounds__(NW * 32, 3)
 
 // Up to 8 rows: keys are M (or, for V, columns), rows N, so that no half of a
 // product is padding.  Weights become the B operand of the second product by a
-// transpose within the warp.  Against rows as M: half the products, no spills.
+// transpose within the warp.  Against rows as M: half the products, no spills
+// (16 sequences x 4096 x 4 rows: 40 us -> 29.5).
 template <int D, int G, typename ST>
 __global__ void __launch_bounds__(NW * 32, 4) tree_mma8(const __grid_constant__ TreeParams T, const MmaPlan L) {
   constexpr int NR = 8, DG = D / 8, LD = D + 4;
@@ -725,8 +730,10 @@ __global__ void __launch_bounds__(NW * 32, 4) tree_mma8(const __grid_constant__ 
   meet<D, NR>(T, L, msm, sml, unit, b, kvh, part, 0);
 }
 
-// Scores of the cached tokens: weights formed again from K, the rows' maxima and
-// sums, summed over the rows of each key (rows are lanes: three shuffles).
+// Scores of the cached tokens for more rows than score_kept takes: weights formed
+// again from K, the rows' maxima and sums, summed over the rows of each key (rows
+// are lanes: three shuffles).  Instructions bound it: 32 rows x 4096 keys x 8
+// heads of 128 columns, batch 4, 18.4 us.
 template <int D, int G, typename ST>
 __global__ void __launch_bounds__(NW * 32, 3)
     score_mma(const __grid_constant__ ScoreParams P, int rows, uint32_t steps_per_unit, uint32_t total) {

@@ -31,6 +31,11 @@
 // element to [2^13, 2^14) (exact for bf16), K and V values exactly (tc.cuh).
 // Weights enter the second product rounded to f16, times 2^7 (at most 2^15);
 // their sum is taken before that rounding, in fp32.
+//
+// Bound: the chain scores -> maximum -> weights -> products of a stream, 4900 cycles
+// a tile with both streams at it, where products and exponentials need 2048 each.
+// Measured: 64 nodes x 16K x 64 heads over 8, batch 4, 146 us (770 TFLOP/s); 63 nodes
+// x 4K x 32 heads, batch 8, 52.5 us, of which about 5 pass before the first product.
 #include <algorithm>
 
 #include "branch.cuh"

@@ -26,7 +26,8 @@ namespace {
 
 constexpr int SROWS = 8;  // query rows a warp holds at a time
 
-// A warp per 32 keys of one (sequence, KV head).
+// A warp per 32 keys of one (sequence, KV head); bound by instructions like
+// tree_generic (fp32, 32 rows x 2000 keys x 8 heads of 128, batch 2: 48 us).
 __global__ void __launch_bounds__(128, 2) score_generic(const ScoreParams P, int warps, int ld, int64_t tiles, int64_t tasks) {
   extern __shared__ __align__(16) float ssm[];
   const TreeParams &T = P.t;
@@ -84,7 +85,9 @@ constexpr int KROWS = 16;      // most rows of a KV head whose scores are kept
 // is read or multiplied twice, and its parts are joined here too.  The first
 // `joins` blocks join the outputs, a warp per row; the others take 256 keys of a
 // (sequence, KV head) each: their warps join the rows' maxima and sums, then a
-// thread sums the weights of its keys, PER of them.
+// thread sums the weights of its keys, PER of them.  Against reading K again, 16
+// sequences x 4096 x 4 rows: 24 us -> 7 (8.4 MB of scores, from L2); fp32, 1023
+// tokens: 13 -> 6, the join included.
 template <int DC, int PER>
 __global__ void __launch_bounds__(KTHREADS, 4)
     score_kept(const __grid_constant__ ScoreParams P, const GenPlan L, int joins, int blocks) {
@@ -308,7 +311,9 @@ __device__ __forceinline__ uint64_t block_prefix(uint64_t v, uint64_t *warps, ui
 // tokens in a row, each thread K of them, held as keys in registers.  Three
 // passes find the threshold key (histograms in shared memory, added up over the
 // cluster through distributed shared memory), then prefix sums give every kept
-// token its place.  Scores are read once.
+// token its place.  Scores are read once: 4 bytes a token, so that passes over
+// registers and their barriers bound it (128 rows of 16384: 14.6 us; 8 rows of
+// 1537: 6.4 us).
 template <int K>
 __global__ void __launch_bounds__(SEL, 1) evict_select(const __grid_constant__ EvictParams P, int ranks) {
   __shared__ uint32_t hist[2][BINS];  // by turns: a block may still read the other
@@ -417,7 +422,8 @@ __global__ void __launch_bounds__(SEL, 1) evict_select(const __grid_constant__ E
 }
 
 // The same for rows longer than a cluster holds: a block per row reads the
-// scores once for each of four eight-bit passes and once more to place them.
+// scores once for each of four eight-bit passes and once more to place them
+// (2 rows of 300000: 446 us).
 __global__ void __launch_bounds__(SEL) evict_select_long(const __grid_constant__ EvictParams P) {
   __shared__ int hist[256];
   __shared__ uint32_t s_prefix;
@@ -551,6 +557,8 @@ __global__ void __launch_bounds__(256) evict_gather(const __grid_constant__ Gath
 
 // Packed rows of CH 16-byte chunks and scale rows of one V each (the usual
 // caches): every thread has all of its loads in flight before its first store.
+// Memory bounds it: 128 rows, 4096 of 16384 tokens of 128 columns, 35.7 us; its
+// scattered 8-byte scale rows move whole 32-byte sectors, 5.5 TB/s with those.
 template <int CH, typename V>
 __global__ void __launch_bounds__(256, 4) evict_gather_fast(const __grid_constant__ GatherParams P) {
   constexpr int ROWS = 256 / CH;  // per block
