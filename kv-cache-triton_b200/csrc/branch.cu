@@ -326,7 +326,8 @@ int tree_fill(TreeParams &P, const kv4_tensor *q, const kv4_tensor *const cache[
   return KV4_OK;
 }
 
-int tree_mma_parts(const TreeParams &P);  // branch_mma.cu
+int tree_mma_parts(const TreeParams &P);   // branch_mma.cu
+bool tree_mma_joins(const TreeParams &P);  // within the kernel
 int tree_mma_run(const TreeParams &P, cudaStream_t st);
 int branch_mma_take_device_error(int *v);
 int64_t tree_tc_workspace(const TreeParams &P);  // branch_tc.cu
@@ -370,7 +371,7 @@ int tree_run(TreeParams &P, void *workspace, int64_t bytes, cudaStream_t st) {
   }
   if (mma) {
     const int rc = tree_mma_run(P, st);
-    if (rc || L.parts == 1 || P.kept) return rc;
+    if (rc || L.parts == 1 || P.kept || tree_mma_joins(P)) return rc;
     return P.d == 64 ? launch_merge<2>(P, L, st) : launch_merge<4>(P, L, st);
   }
   if (P.d <= 64) return launch_gen_rw<2>(P, L, st);
