@@ -923,10 +923,12 @@ MmaPlan mma_plan(const TreeParams &T) {
   const int nr = half_rows(L.rows) ? 8 : 16;
   L.row_tiles = (L.rows + nr - 1) / nr;
   L.units = T.B * T.Hkv;
-  // one wave of blocks, each warp at least two steps of 16 keys
+  // one wave of blocks, each warp at least two steps of 16 keys; four where a
+  // cluster does not hold the parts (32 rows x 4096 of 8 heads: 15.0 us with 16
+  // parts, 16.9 with 27; 4 rows x 2048 7.4 with 8, 8.2 with 16)
   const int64_t steps = (T.S + 15) / 16 + (T.ndraft + 15) / 16, have = L.units * L.row_tiles;
   const int64_t room = static_cast<int64_t>(sm_count()) * (half_rows(L.rows) ? 4 : 3);
-  const int64_t most = std::max<int64_t>(1, steps / (2 * NW));
+  const int64_t most = std::max({int64_t(1), std::min<int64_t>(kClusterParts, steps / (2 * NW)), steps / (4 * NW)});
   L.parts = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({room / have, most, 64})));
   L.cluster = L.parts > 1 && L.parts <= kClusterParts && !T.kept;  // score_kept joins the parts itself
   return L;
