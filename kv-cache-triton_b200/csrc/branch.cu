@@ -15,13 +15,13 @@
 // in fp32 FFMA.  A warp owns RW rows and a range of keys: 32 keys at a time it
 // dequantizes K into its own shared memory (lane = key for the scores), then V
 // over it (lane = column for the output), with the running maximum and sum of
-// the softmax per row.  Warps never wait for one another; ranges of one unit
-// meet in tree_merge through the workspace.  16-bit types take branch_tc.cu's
+// the softmax per row.  A block's warps meet at the end, blocks of one unit in
+// tree_merge through the workspace.  16-bit types take branch_tc.cu's
 // and branch_mma.cu's kernels where the layout allows.
 // Bound by instructions: 6000 for 8 rows x 32 keys x 128 columns, a third of them
 // the products, at two warps a scheduler (shared memory holds no more tiles).
-// Measured, fp32: 64 rows x 2016 keys of 128 columns in 16 units 88 us with the join
-// (12 TFLOP/s); 12 rows x 789 keys of 64 columns in 24 units 15.6 us and 5 to join,
+// Measured, fp32: 64 rows x 2016 keys of 128 columns in 16 units 94 us with the join
+// (11 TFLOP/s); 12 rows x 789 keys of 64 columns in 24 units 15.6 us and 3 to join,
 // where a warp has one tile and its chain counts.
 #include <algorithm>
 
@@ -45,19 +45,18 @@ template <int DC, int RW>
 __global__ void __launch_bounds__(128, 1) tree_generic(const TreeParams P, const GenPlan L) {
   extern __shared__ __align__(16) float gsm[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t task = static_cast<int64_t>(blockIdx.x) * L.warps + warp;
-  if (task >= L.tasks) return;
-  float *sT = gsm + warp * (32 * L.ld + RW * L.ld + 32 * RW);  // K or V tile
-  float *sQ = sT + 32 * L.ld, *sP = sQ + RW * L.ld;            // rows of q; weights [key][RW]
-  const int part = static_cast<int>(task % L.parts);
-  const int64_t ur = task / L.parts;
+  const int area = 32 * L.ld + RW * L.ld + 32 * RW;  // floats of a warp
+  float *sT = gsm + warp * area;                     // K or V tile
+  float *sQ = sT + 32 * L.ld, *sP = sQ + RW * L.ld;  // rows of q; weights [key][RW]
+  const int part = static_cast<int>(blockIdx.x % L.parts);
+  const int64_t ur = blockIdx.x / L.parts;
   const int rt = static_cast<int>(ur % L.row_tiles);
   const int64_t unit = ur / L.row_tiles, b = unit / P.Hkv;
   const int kvh = static_cast<int>(unit - b * P.Hkv);
-  const int64_t len = context_len(P, b, part == 0 && rt == 0 && lane == 0 ? &g_branch_error : nullptr);
+  const int64_t len = context_len(P, b, part == 0 && rt == 0 && threadIdx.x == 0 ? &g_branch_error : nullptr);
   const int64_t total = len + P.ndraft, tiles = (total + 31) >> 5;
-  const int64_t per = (tiles + L.parts - 1) / L.parts;
-  const int64_t k0 = part * per * 32, k1 = min(total, k0 + per * 32);
+  const int64_t ranges = static_cast<int64_t>(L.parts) * L.warps, per = (tiles + ranges - 1) / ranges;
+  const int64_t k0 = (part * L.warps + warp) * per * 32, k1 = min(total, k0 + per * 32);
   const int r0 = rt * RW, d8 = (P.d + 7) >> 3;
 
   warp_query<RW>(P, b, kvh, r0, L.rows, sQ, L.ld, lane);
@@ -135,35 +134,59 @@ __global__ void __launch_bounds__(128, 1) tree_generic(const TreeParams P, const
       sP[lane * RW + r] = p;
     }
   }
+  // ---- the block's warps meet: outputs where the tiles were, (m, l) for the weights ----
+  __syncwarp();
 #pragma unroll
   for (int r = 0; r < RW; ++r) {
 #pragma unroll
     for (int o = 16; o; o >>= 1) l[r] += __shfl_xor_sync(0xffffffffu, l[r], o);
+#pragma unroll
+    for (int k = 0; k < DC; ++k)
+      if (lane + 32 * k < P.d) sT[r * L.ld + lane + 32 * k] = acc[r][k];
+    if (lane == 0) *reinterpret_cast<float2 *>(sP + 2 * r) = make_float2(m[r], l[r]);
+  }
+  __syncthreads();
+#pragma unroll 1
+  for (int r = warp; r < RW && r0 + r < L.rows; r += L.warps) {
     const int row = r0 + r;
-    if (row >= L.rows) continue;
+    const float *o = gsm + r * L.ld, *ml = gsm + 32 * L.ld + RW * L.ld + 2 * r;
+    float M = -INFINITY, sum = 0.0f, v[DC];
+#pragma unroll 1
+    for (int w = 0; w < L.warps; ++w) M = fmaxf(M, ml[w * area]);
+    const float base = M == -INFINITY ? 0.0f : M;
+#pragma unroll
+    for (int k = 0; k < DC; ++k) v[k] = 0.0f;
+#pragma unroll 1
+    for (int w = 0; w < L.warps; ++w) {
+      const float f = exp2f(ml[w * area] - base);
+      sum = fmaf(ml[w * area + 1], f, sum);
+#pragma unroll
+      for (int k = 0; k < DC; ++k)
+        if (lane + 32 * k < P.d) v[k] = fmaf(o[w * area + lane + 32 * k], f, v[k]);
+    }
     const int64_t at = unit * L.rows + row;
     if (P.kept && part == 0 && lane == 0) P.kept_c[at] = P.scale_log2;
     if (L.parts == 1) {
       const int i = row / P.R, h = kvh * P.R + row - i * P.R;
-      const float inv = l[r] > 0.0f ? 1.0f / l[r] : 0.0f;
+      const float inv = sum > 0.0f ? 1.0f / sum : (sum == sum ? 0.0f : sum);
 #pragma unroll
       for (int k = 0; k < DC; ++k)
         if (lane + 32 * k < P.d)
           store_from_f32(P.out, P.q_dtype,
                          b * P.os[0] + h * P.os[1] + i * P.os[2] + (lane + 32 * k) * P.os[3],
-                         acc[r][k] * inv);
+                         v[k] * inv);
       if (lane == 0) {
-        if (P.stats) P.stats[at] = make_float2(m[r], inv);
+        if (P.stats) P.stats[at] = make_float2(M, inv);
         if (P.lse)
           P.lse[b * P.ls[0] + h * P.ls[1] + i * P.ls[2]] =
-              l[r] > 0.0f ? (m[r] + log2f(l[r])) * kBrLn2 : -INFINITY;
+              sum == 0.0f ? -INFINITY : (M + log2f(sum)) * kBrLn2;
       }
     } else {
       const int64_t slot = static_cast<int64_t>(part) * L.units * L.rows + at;
 #pragma unroll
       for (int k = 0; k < DC; ++k)
-        if (lane + 32 * k < P.d) P.ws_o[slot * P.d + lane + 32 * k] = acc[r][k];
-      if (lane == 0) P.ws_ml[slot] = make_float2(m[r], l[r]);
+        if (lane + 32 * k < P.d) P.ws_o[slot * P.d + lane + 32 * k] = v[k];
+      if (lane == 0) P.ws_ml[slot] = make_float2(M, sum);
     }
   }
 }
@@ -178,8 +201,8 @@ __global__ void __launch_bounds__(128, 4) tree_merge(const __grid_constant__ Tre
 constexpr int kSms = 148;
 
 // Rows a warp holds: eight share one dequantized tile, fewer where there are no
-// more (4 rows x 4000 keys x 8 heads of 128, batch 4, fp32: 63 us instead of 76;
-// four for 12 rows x 777: 26 us instead of 23).
+// more (measured before the block's warps met: 4 rows x 4000 keys x 8 heads of 128,
+// batch 4, fp32, 63 us instead of 76; four for 12 rows x 777 26 instead of 23).
 int rows_per_warp(int rows) { return rows <= 2 ? 2 : rows <= 4 ? 4 : 8; }
 
 GenPlan gen_plan(const TreeParams &P) {
@@ -192,15 +215,14 @@ GenPlan gen_plan(const TreeParams &P) {
   const size_t per_warp = sizeof(float) * (32 * L.ld + rw * L.ld + 32 * rw);
   L.warps = static_cast<int>(std::max<size_t>(1, std::min<size_t>(4, 100 * 1024 / per_warp)));
   L.smem = per_warp * L.warps;
-  // ranges of at least 32 keys, as many as the SMs take at once (a block more on
-  // a few of them runs alone at the end: 64 rows x 2000 x 8 heads of 128, batch 2,
-  // 153 us with 320 blocks, 88 with 288)
+  // blocks of at least 32 keys a warp, as many as the SMs take at once (a block
+  // more on a few of them runs alone at the end: 64 rows x 2000 x 8 heads of 128,
+  // batch 2: 153 us with 320 blocks of four warps, 94 with 256)
   const int64_t tiles = (P.S + P.ndraft + 31) / 32, have = L.units * L.row_tiles;
-  const int64_t room = kSms * L.warps * std::min<int64_t>(3, 200 * 1024 / L.smem);
-  const int64_t want = std::max<int64_t>(1, std::min<int64_t>(room / have, 256));
-  const int64_t per = std::max<int64_t>(1, (tiles + want - 1) / want);
+  const int64_t room = kSms * std::min<int64_t>(3, 200 * 1024 / L.smem);
+  const int64_t want = std::max<int64_t>(1, std::min<int64_t>(room / have, 64)) * L.warps;
+  const int64_t per = std::max<int64_t>(1, (tiles + want - 1) / want) * L.warps;
   L.parts = static_cast<int>(std::max<int64_t>(1, (tiles + per - 1) / per));
-  L.tasks = have * L.parts;
   return L;
 }
 
@@ -225,7 +247,7 @@ int launch_merge(const TreeParams &P, const GenPlan &L, cudaStream_t st) {
 
 template <int DC, int RW>
 int launch_gen(const TreeParams &P, const GenPlan &L, cudaStream_t st) {
-  const int64_t blocks = (L.tasks + L.warps - 1) / L.warps;
+  const int64_t blocks = L.units * L.row_tiles * L.parts;
   if (blocks > 0x7fffffff) return KV4_ERR_UNSUPPORTED;
   if (L.smem > 48 * 1024) {
     const int rc = cuda_status(cudaFuncSetAttribute(

@@ -7,7 +7,7 @@ namespace kv4 {
 
 // how tree_generic's or tree_mma's work was cut; units = B * Hkv
 struct GenPlan {
-  int64_t units, tasks;  // tasks = units * row_tiles * parts
+  int64_t units;
   int rows, row_tiles, parts, warps, ld;
   size_t smem;
 };
