@@ -181,6 +181,12 @@ __device__ __forceinline__ uint32_t hmul2(uint32_t a, uint32_t b) {
   asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
   return r;
 }
+// what a * b loses when it is rounded to p (exact above the subnormals)
+__device__ __forceinline__ uint32_t hrest2(uint32_t a, uint32_t b, uint32_t p) {
+  uint32_t r;
+  asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(p ^ 0x80008000u));
+  return r;
+}
 // f16 pair (1024 + code) of nibbles 0 and 4 of x
 __device__ __forceinline__ uint32_t nib_pair(uint32_t x) {
   uint32_t r;
