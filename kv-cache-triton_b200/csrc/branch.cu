@@ -98,21 +98,18 @@ __global__ void __launch_bounds__(128, 1) tree_generic(const TreeParams P, const
       t0 += 32;
       continue;
     }
-    float s[RW];
+    float4 part4[RW];  // four sums per score: a quarter of the roundings in a row
 #pragma unroll
-    for (int r = 0; r < RW; ++r) s[r] = 0.0f;
+    for (int r = 0; r < RW; ++r) part4[r] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll 2
     for (int c = 0; c < 2 * d8; ++c) {
       const float4 k4 = *reinterpret_cast<const float4 *>(sT + lane * L.ld + 4 * c);
 #pragma unroll
-      for (int r = 0; r < RW; ++r) {
-        const float4 q4 = *reinterpret_cast<const float4 *>(sQ + r * L.ld + 4 * c);
-        s[r] = fmaf(q4.x, k4.x, s[r]);
-        s[r] = fmaf(q4.y, k4.y, s[r]);
-        s[r] = fmaf(q4.z, k4.z, s[r]);
-        s[r] = fmaf(q4.w, k4.w, s[r]);
-      }
+      for (int r = 0; r < RW; ++r) fma4(part4[r], *reinterpret_cast<const float4 *>(sQ + r * L.ld + 4 * c), k4);
     }
+    float s[RW];
+#pragma unroll
+    for (int r = 0; r < RW; ++r) s[r] = sum4(part4[r]);
     const int64_t t = t0 + lane;
 #pragma unroll
     for (int r = 0; r < RW; ++r) {

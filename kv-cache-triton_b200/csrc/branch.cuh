@@ -217,6 +217,16 @@ __device__ __forceinline__ void warp_query(const TreeParams &P, int64_t b, int k
   else warp_query_rows<__nv_bfloat16, N>(P, b, kvh, row0, rows, dst, ld, lane);
 }
 
+// four sums side by side: a quarter of the roundings in a row (error of an fp32 score
+// of 64 columns against 64 bits: half of one sum's)
+__device__ __forceinline__ void fma4(float4 &s, const float4 &a, const float4 &b) {
+  s.x = fmaf(a.x, b.x, s.x);
+  s.y = fmaf(a.y, b.y, s.y);
+  s.z = fmaf(a.z, b.z, s.z);
+  s.w = fmaf(a.w, b.w, s.w);
+}
+__device__ __forceinline__ float sum4(const float4 &s) { return (s.x + s.y) + (s.z + s.w); }
+
 // shared-memory row length of a d-wide row: float4 steps, an odd number of
 // them, so that 32 rows read in step fall into different banks
 __host__ __device__ constexpr int row_ld(int d) { return 4 * (((d + 7) / 8 * 2) | 1); }

@@ -21,14 +21,14 @@
 // the g-th eighth of a row of V.
 //
 // A block of warps takes a range of one unit's keys, 16 keys per warp in turn;
-// its warps meet in shared memory, ranges of one unit in the workspace
-// (tree_merge of branch.cu).  Every warp has a ring of steps of its own, filled
+// its warps meet in shared memory, up to eight ranges of one unit in a cluster,
+// more in the workspace (tree_merge of branch.cu).  Every warp has a ring of steps of its own, filled
 // by asynchronous copies three ahead; nothing waits for another warp on the way.
 // Bound: instructions, about 450 per warp and 16 keys of 128 columns, a third of
 // which take codes apart; memory next.  Measured, 8 KV heads of 128 columns: single
 // tokens of 4 rows, 16 sequences x 4096, 29.5 us (84 MB: 2.8 TB/s, a step in 60 % of
-// the issue slots); 8 nodes x 512 7.3 us, of which loads that wait for one another
-// are most; 32 rows x 4096, batch 4, 23 us.
+// the issue slots); 8 nodes x 512 8.9 us with the join, most of it loads that wait
+// for one another; 32 rows x 4096, batch 4, 23 us.
 #include <algorithm>
 
 #include "branch.cuh"

@@ -46,19 +46,15 @@ __global__ void __launch_bounds__(128, 2) score_generic(const ScoreParams P, int
     const int nr = min(SROWS, rows - r0);
     warp_query<SROWS>(T, b, kvh, r0, rows, sQ, ld, lane);
     __syncwarp();
-    float s[SROWS];
+    float4 s[SROWS];  // four sums per score, as in tree_generic
 #pragma unroll
-    for (int r = 0; r < SROWS; ++r) s[r] = 0.0f;
+    for (int r = 0; r < SROWS; ++r) s[r] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     for (int c = 0; c < 2 * d8; ++c) {
       const float4 k4 = *reinterpret_cast<const float4 *>(sK + lane * ld + 4 * c);
 #pragma unroll
       for (int r = 0; r < SROWS; ++r) {
         if (r >= nr) break;
-        const float4 q4 = *reinterpret_cast<const float4 *>(sQ + r * ld + 4 * c);
-        s[r] = fmaf(q4.x, k4.x, s[r]);
-        s[r] = fmaf(q4.y, k4.y, s[r]);
-        s[r] = fmaf(q4.z, k4.z, s[r]);
-        s[r] = fmaf(q4.w, k4.w, s[r]);
+        fma4(s[r], *reinterpret_cast<const float4 *>(sQ + r * ld + 4 * c), k4);
       }
     }
 #pragma unroll
@@ -68,7 +64,7 @@ __global__ void __launch_bounds__(128, 2) score_generic(const ScoreParams P, int
       bool see = t < P.keys;
       if (see && t >= T.S) see = draft_visible(T, b, row / T.R, static_cast<int>(t - T.S));
       const float2 st = T.stats[unit * rows + row];
-      if (see && st.y > 0.0f) total = fmaf(exp2f(s[r] * T.scale_log2 - st.x), st.y, total);
+      if (see && st.y > 0.0f) total = fmaf(exp2f(fmaf(sum4(s[r]), T.scale_log2, -st.x)), st.y, total);
     }
   }
   if (t < P.keys) {
