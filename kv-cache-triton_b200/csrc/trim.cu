@@ -83,7 +83,7 @@ constexpr int KROWS = 16;      // most rows of a KV head whose scores are kept
 // (sequence, KV head) each: their warps join the rows' maxima and sums, then a
 // thread sums the weights of its keys, PER of them.  Against reading K again, 16
 // sequences x 4096 x 4 rows: 24 us -> 7 (8.4 MB of scores, from L2); fp32, 1023
-// tokens: 13 -> 6, the join included.
+// tokens: 13 -> 3.3, the join included.
 template <int DC, int PER>
 __global__ void __launch_bounds__(KTHREADS, 4)
     score_kept(const __grid_constant__ ScoreParams P, const GenPlan L, int joins, int blocks) {
@@ -111,6 +111,19 @@ __global__ void __launch_bounds__(KTHREADS, 4)
     sum[i] = on[i] ? in[t * P.is[2]] * P.decay : 0.0f;  // was there before the attention began
   }
   griddep_wait();
+  // The first rows' scores are on their way while maxima and sums are joined: 3.7 us
+  // -> 3.2 for one query x 1023, fp32; with four keys a thread their registers
+  // cost what they gain.
+  constexpr int EARLY = PER == 1 ? 4 : 0;
+  const int64_t blks = kept_blocks(T);
+  const float *x[PER];
+  float early[EARLY + 1][PER];
+#pragma unroll
+  for (int i = 0; i < PER; ++i) x[i] = T.kept + kept_at(unit, blks, on[i] ? slot0 + i * KTHREADS : 0, 0, L.rows);
+#pragma unroll
+  for (int r = 0; r < EARLY; ++r)
+#pragma unroll
+    for (int i = 0; i < PER; ++i) early[r][i] = r < L.rows ? x[i][16 * r] : 0.0f;
   const int64_t n = L.units * L.rows, first = static_cast<int64_t>(unit) * L.rows;
   for (int r = warp; r < L.rows; r += KTHREADS / 32) {
     float m = -INFINITY, l = 0.0f, inv;
@@ -141,18 +154,21 @@ __global__ void __launch_bounds__(KTHREADS, 4)
     }
   }
   __syncthreads();
-  const int64_t blks = kept_blocks(T);
-  const float *x[PER];
-#pragma unroll
-  for (int i = 0; i < PER; ++i) x[i] = T.kept + kept_at(unit, blks, on[i] ? slot0 + i * KTHREADS : 0, 0, L.rows);
-#pragma unroll 4
-  for (int r = 0; r < L.rows; ++r) {
+  auto add = [&](int r, const float (&y)[PER]) {
     const float m = sm[r], inv = sl[r], c = sc[r];
+    if (inv == 0.0f) return;
 #pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      const float y = x[i][16 * r];
-      if (inv != 0.0f) sum[i] += exp2f(fmaf(y, c, -m)) * inv;
-    }
+    for (int i = 0; i < PER; ++i) sum[i] += exp2f(fmaf(y[i], c, -m)) * inv;
+  };
+#pragma unroll
+  for (int r = 0; r < EARLY; ++r)
+    if (r < L.rows) add(r, early[r]);
+#pragma unroll 4
+  for (int r = EARLY; r < L.rows; ++r) {
+    float y[PER];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) y[i] = x[i][16 * r];
+    add(r, y);
   }
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
