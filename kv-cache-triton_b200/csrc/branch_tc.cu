@@ -128,13 +128,13 @@ struct Smem {
   static constexpr int QC = MASK + 4096;    // float [2][128]: a row's factor from scores to base-2 exponents
   static constexpr int BAD = QC + 1024;   // uint32 [4 + 2][4]: drafted keys without a usable scale in K, V
   static constexpr int BARS = BAD + 96;     // mbarriers
-  static constexpr int MISC = BARS + 160;   // TMEM address, abort flag, walk start
+  static constexpr int MISC = BARS + 176;   // TMEM address, abort flag, walk start
   static constexpr int BYTES = MISC + 64;
 };
 
 // barriers (pairs: by stage or by stream) and their arrival counts
 enum Bar { KFULL = 0, VFULL = 2, KEMPTY = 4, VEMPTY = 6, SFULL = 8, PREADY = 10, OREADY = 12,
-           MFULL = 14, MEMPTY = 16, QREADY = 18, QFREE = 19, NBARS = 20 };
+           MFULL = 14, MEMPTY = 16, QREADY = 18, QFREE = 19, QSEEN = 20, NBARS = 21 };
 __device__ __forceinline__ int bar_count(int i) {
   if (i < KEMPTY) return 4;           // dequantizing warps of K, of V
   if (i < PREADY) return 1;           // commits
@@ -257,10 +257,15 @@ __device__ __forceinline__ void dequant_role(const TcParams &P, Walk walk, const
     nctx = (len + KT - 1) / KT;
     load(a, 0);
     // The segment's queries, a row tile by K's warps and one by V's: as soon as
-    // the scores of the segment before are out (and its exchange, which uses
-    // their place, is over), beside its last softmax and its epilogue.
+    // the scores of the segment before are out and the softmax warps have its
+    // factors, beside its last softmax and its epilogue; behind that epilogue where
+    // its exchange uses the queries' place.  QSEEN is waited for in every segment:
+    // it keeps QREADY from running ahead of a softmax warp by two phases, which a
+    // wait by parity takes for none, and says that segment seg - 2 is over, without
+    // which the wait for QFREE could pass a phase early.
     if (seg > 0) {
       W.wait(KEMPTY + ((n - 1) & 1u), (n - 1) >> 1);
+      W.wait(QSEEN, seg - 1);
       if (narrow) W.wait(QFREE, seg - 1);
     }
     const bool two = s.nrows > 128;
@@ -510,6 +515,8 @@ __device__ __forceinline__ void softmax_role(const TcParams &P, Walk walk, const
     const int len = static_cast<int>(context_len(T, s.b, nullptr)), nctx = (len + KT - 1) / KT;
     W.wait(QREADY, seg++);
     const float c0 = __uint_as_float(lds32(smem + SM::QC + 4 * (two ? tid : r & (RR - 1))));
+    __syncwarp();
+    if (lane == 0) mbar_arrive(W.at(QSEEN));
 
     float m = -INFINITY, l = 0.0f;
     bool broken = false;  // saw a key without a usable scale
