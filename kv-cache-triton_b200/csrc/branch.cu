@@ -282,7 +282,7 @@ int fill_source(RowSource &S, const kv4_tensor *const t[4], int64_t B, int64_t H
     if (x->shape[3] != t[k & 1]->shape[3]) return KV4_ERR_SHAPE;
     int64_t *st = k == 0 ? S.kps : k == 1 ? S.kss : k == 2 ? S.vps : S.vss;
     for (int i = 0; i < 4; ++i) st[i] = x->stride[i];
-    if (T > 0 && !x->data) return KV4_ERR_INVALID;
+    if (B > 0 && T > 0 && !x->data) return KV4_ERR_INVALID;
   }
   S.kp = static_cast<const uint8_t *>(t[0]->data);
   S.ks = t[1]->data;
@@ -371,6 +371,7 @@ GenPlan tree_plan(const TreeParams &P) { return tree_mma_takes(P) ? mma_merge_pl
 // output with other strides or at another address may still leave the call to
 // tree_generic.
 int64_t tree_workspace(const TreeParams &P) {
+  if (P.B == 0 || P.nodes == 0) return 0;  // nothing to cut into parts
   int64_t most = gen_workspace(P, gen_plan(P));
   if (tree_mma_takes(P)) most = std::max(most, gen_workspace(P, mma_merge_plan(P)));
   else if (tree_tc_takes(P)) most = std::max(most, tree_tc_workspace(P));
