@@ -336,9 +336,11 @@ int kv4_prefill_attention(const kv4_tensor *q, const kv4_tensor *k_packed,
  * strides; all four scale tensors have one dtype.  `workspace` holds at least
  * kv4_tree_workspace() bytes (device, 16-byte aligned, any contents; a
  * negative result of that function is minus a status).
- * 16-bit queries and scales take tensor-core kernels whose V operand (and, for
- * bf16 with much work, K operand) is f16, exact while scales stay below
- * 65504/8: a larger or non-finite scale in the context sets bit 8 of
+ * 16-bit queries and scales take tensor-core kernels whose operands are f16.  A
+ * power of two common to some rows of a KV head brings bf16 scales of up to 2^100
+ * into its range; scales down to 2^-27 of the largest of those rows keep all their
+ * bits, smaller ones are off by up to 2^-35 of it.  V scales in f16 have to stay
+ * below 65504/8.  A larger or non-finite scale in the context sets bit 8 of
  * kv4_device_error (output not valid).  One in a drafted row makes the nodes
  * that see the row NaN and no others, and sets the bit as well.
  */

@@ -51,6 +51,46 @@ constexpr int NW = 4;             // warps per block
 constexpr int kClusterParts = 8;  // most blocks that join as a cluster
 constexpr float kShift = 7.0f;  // weights are written times 2^7 (see branch_tc.cu)
 
+// The power of two 2^e in a warp's V operands and output sums (bf16 scales; see
+// tc.cuh): it moves when a step's scales are not exact at the present one.
+struct VShift {
+  int e = 0, least = tc::kMaxShift;  // least: smallest so far; sums move up by 2^48 at most, which they can
+  float up = 1.0f;                   // 2^e
+};
+__device__ __forceinline__ float max3nan(float a, float b, float c) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+// Whether the step's scales, four of them times 2^e, are not all exact in f16 (a
+// zero counts as too small: seldom, and looked at again in shift_for).
+__device__ __forceinline__ bool not_exact(const float (&f)[4]) {
+  const float top = max3nan(max3nan(fabsf(f[0]), fabsf(f[1]), fabsf(f[2])), fabsf(f[3]), 0.0f);
+  const float low = fminf(fminf(fabsf(f[0]), fabsf(f[1])), fminf(fabsf(f[2]), fabsf(f[3])));
+  return !(top < 4096.0f) || low < 0x1p-17f;
+}
+// The step's power of two; returns what the sums so far have to be multiplied with.
+// The whole warp takes part; vs: its 16-bit scales.
+__device__ __forceinline__ float shift_for(VShift &V, const uint32_t (&vs)[4]) {
+  uint32_t top = 0;
+  bool exact = true;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const uint32_t u = tc::scale_bits(vs[j]);
+    exact = exact && tc::scale_exact(u);
+    if (tc::scale_usable(u)) top = max(top, u);
+  }
+  exact = __all_sync(0xffffffffu, exact);
+  top = __reduce_max_sync(0xffffffffu, top);
+  int e = V.e;
+  if (top != 0u) e = min(exact ? 0 : tc::scale_shift(top), V.least + 48);
+  const float factor = tc::pow2(e - V.e);
+  V.e = e;
+  V.least = min(V.least, e);
+  V.up = tc::pow2(e);
+  return factor;
+}
+
 // Code times an f16 scale has up to 14 bits: what f16 cuts off goes through the
 // product on its own, so that an f16 output has no error of V's: 2.3e-4 from the
 // 64-bit result instead of 3.1e-4 at 17 nodes x 1000 (a plain fp32 form: 2.1e-4), for
@@ -63,6 +103,51 @@ template <typename ST>
 __device__ __forceinline__ float scale_at(const uint32_t *w, int i) {
   if (DT<ST>::code == KV4_BF16) return i & 1 ? bf16hi_to_f32(w[i >> 1]) : bf16lo_to_f32(w[i >> 1]);
   return i & 1 ? f16hi_to_f32(w[i >> 1]) : f16lo_to_f32(w[i >> 1]);
+}
+
+// whether a V scale can be an operand; one that cannot is reported
+template <typename ST>
+__device__ __forceinline__ bool usable(uint32_t s) {
+  if (kRest<ST>) return fabsf(scale_at<ST>(&s, 0)) <= tc::kMaxScale;
+  return tc::scale_usable(tc::scale_bits(s));
+}
+
+// V's scales of a step, keys in pairs, as f16; `rescale(f)` multiplies the sums so
+// far.  The whole warp takes part.
+template <typename ST, class F>
+__device__ __forceinline__ void v_scales(uint32_t (&sp)[2], const uint32_t (&vs)[4], VShift &V, bool draft,
+                                         bool &big, F rescale) {
+  float f[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) f[j] = scale_at<ST>(&vs[j], 0);
+  if (kRest<ST>) {
+#pragma unroll
+    for (int p = 0; p < 2; ++p) {
+      sp[p] = prmt(vs[2 * p], vs[2 * p + 1], 0x5410);
+      const bool b0 = !(fabsf(f[2 * p]) <= tc::kMaxScale), b1 = !(fabsf(f[2 * p + 1]) <= tc::kMaxScale);
+      if (b0 || b1) {
+        big = true;
+        if (draft) sp[p] &= (b0 ? 0u : 0xffffu) | (b1 ? 0u : 0xffff0000u);  // rows that see it are marked
+      }
+    }
+    return;
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j) f[j] *= V.up;
+  if (__any_sync(0xffffffffu, not_exact(f))) {
+    const float factor = shift_for(V, vs);
+    if (factor != 1.0f) rescale(factor);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      f[j] = scale_at<ST>(&vs[j], 0) * V.up;
+      if (!usable<ST>(vs[j])) {
+        big = true;
+        if (draft) f[j] = 0.0f;  // rows that see it are marked
+      }
+    }
+  }
+  sp[0] = pack_f16x2(f[0], f[1]);
+  sp[1] = pack_f16x2(f[2], f[3]);
 }
 
 // A warp's ring of steps in shared memory.  One step is 16 keys: rows of K (and
@@ -450,6 +535,7 @@ __global__ void __launch_bounds__(NW * 32, 3)
 #pragma unroll
     for (int e = 0; e < 4; ++e) o[j][e] = 0.0f;
   bool big = false;
+  VShift V;
   // kept scores of rows g and g + 8 (one row tile holds them all)
   float *const kept = T.kept ? T.kept + kept_at(unit, steps, 2 * t, g, L.rows) : nullptr;
   if (T.kept && part == 0 && warp == 0 && t == 0) {
@@ -492,7 +578,7 @@ __global__ void __launch_bounds__(NW * 32, 3)
         if (draft) {  // a visible key without a usable V scale: the row has no value
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            const bool bad = !(fabsf(scale_at<ST>(&vs[j], 0)) <= tc::kMaxScale);
+            const bool bad = !usable<ST>(vs[j]);
             const uint32_t any = __ballot_sync(0xffffffffu, bad) & (0x11111111u << t);
             if (any && (on >> j & 1u)) broken[r] = true;
           }
@@ -533,16 +619,12 @@ __global__ void __launch_bounds__(NW * 32, 3)
 
     // O += P V: column j of this thread's eighth, keys in pairs
     uint32_t sp[2];
+    v_scales<ST>(sp, vs, V, draft, big, [&](float f) {
 #pragma unroll
-    for (int p = 0; p < 2; ++p) {
-      const float f0 = scale_at<ST>(&vs[2 * p], 0), f1 = scale_at<ST>(&vs[2 * p + 1], 0);
-      sp[p] = DT<ST>::code == KV4_F16 ? prmt(vs[2 * p], vs[2 * p + 1], 0x5410) : pack_f16x2(f0, f1);
-      const bool b0 = !(fabsf(f0) <= tc::kMaxScale), b1 = !(fabsf(f1) <= tc::kMaxScale);
-      if (b0 || b1) {
-        big = true;
-        if (draft) sp[p] &= (b0 ? 0u : 0xffffu) | (b1 ? 0u : 0xffff0000u);  // rows that see it: above
-      }
-    }
+      for (int j = 0; j < DG; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[j][e] *= f;
+    });
     uint32_t vw[4][D / 64];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -576,6 +658,7 @@ __global__ void __launch_bounds__(NW * 32, 3)
   if (big) atomicOr(&g_branch_error_mma, DEV_ERR_F16_RANGE);
 
   // ---- the block's warps meet, where the rings were ----
+  const float down = tc::pow2(-V.e);
   cp_async_wait<0>();
   __syncthreads();
 #pragma unroll
@@ -589,8 +672,8 @@ __global__ void __launch_bounds__(NW * 32, 3)
     // columns 2t and 2t + 1 of output tile j are dims 2t * DG + j and (2t + 1) * DG + j
 #pragma unroll
     for (int j = 0; j < DG; ++j) {
-      msm[at * LD + 2 * t * DG + j] = o[j][2 * r];
-      msm[at * LD + (2 * t + 1) * DG + j] = o[j][2 * r + 1];
+      msm[at * LD + 2 * t * DG + j] = o[j][2 * r] * down;
+      msm[at * LD + (2 * t + 1) * DG + j] = o[j][2 * r + 1] * down;
     }
   }
   __syncthreads();
@@ -650,6 +733,7 @@ __global__ void __launch_bounds__(NW * 32, 4) tree_mma8(const __grid_constant__ 
 #pragma unroll
     for (int e = 0; e < 4; ++e) o[j][e] = 0.0f;
   bool big = false;
+  VShift V;
 
   uint32_t slot = 0;
 #pragma unroll 1
@@ -705,7 +789,7 @@ __global__ void __launch_bounds__(NW * 32, 4) tree_mma8(const __grid_constant__ 
       if (draft) {
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-          if (!(fabsf(scale_at<ST>(&vs[j], 0)) <= tc::kMaxScale)) bad |= 1u << (2 * t + (j & 1) + 8 * (j >> 1));
+          if (!usable<ST>(vs[j])) bad |= 1u << (2 * t + (j & 1) + 8 * (j >> 1));
         bad = __reduce_or_sync(0xffffffffu, bad);
       }
 #pragma unroll
@@ -757,16 +841,12 @@ __global__ void __launch_bounds__(NW * 32, 4) tree_mma8(const __grid_constant__ 
 
     // O^T += V^T P^T: two columns of this thread's eighth, keys in pairs
     uint32_t sp[2];
+    v_scales<ST>(sp, vs, V, draft, big, [&](float f) {
 #pragma unroll
-    for (int p = 0; p < 2; ++p) {
-      const float f0 = scale_at<ST>(&vs[2 * p], 0), f1 = scale_at<ST>(&vs[2 * p + 1], 0);
-      sp[p] = DT<ST>::code == KV4_F16 ? prmt(vs[2 * p], vs[2 * p + 1], 0x5410) : pack_f16x2(f0, f1);
-      const bool b0 = !(fabsf(f0) <= tc::kMaxScale), b1 = !(fabsf(f1) <= tc::kMaxScale);
-      if (b0 || b1) {
-        big = true;
-        if (draft) sp[p] &= (b0 ? 0u : 0xffffu) | (b1 ? 0u : 0xffff0000u);  // rows that see it: above
-      }
-    }
+      for (int j = 0; j < D / 16; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[j][e] *= f;
+    });
     uint32_t vw[4][D / 64];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -804,6 +884,7 @@ __global__ void __launch_bounds__(NW * 32, 4) tree_mma8(const __grid_constant__ 
   if (big) atomicOr(&g_branch_error_mma, DEV_ERR_F16_RANGE);
 
   // ---- the block's warps meet, where the rings were ----
+  const float down = tc::pow2(-V.e);
   cp_async_wait<0>();
   __syncthreads();
 #pragma unroll
@@ -816,7 +897,7 @@ __global__ void __launch_bounds__(NW * 32, 4) tree_mma8(const __grid_constant__ 
     if (g == 0) sml[row] = make_float2(m[r] - kShift, l[r]);
 #pragma unroll
     for (int j = 0; j < D / 16; ++j)
-      *reinterpret_cast<float2 *>(msm + row * LD + g * DG + 2 * j) = make_float2(o[j][r], o[j][2 + r]);
+      *reinterpret_cast<float2 *>(msm + row * LD + g * DG + 2 * j) = make_float2(o[j][r] * down, o[j][2 + r] * down);
   }
   __syncthreads();
   if (L.cluster) meet_cluster<D, NR>(T, L, msm, sml, unit, b, kvh, part, 0);

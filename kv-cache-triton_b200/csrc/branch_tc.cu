@@ -127,7 +127,9 @@ struct Smem {
   static constexpr int MASK = ML + 2048;    // uint4 [2][128]: a row's visible keys of a drafted tile
   static constexpr int QC = MASK + 4096;    // float [2][128]: a row's factor from scores to base-2 exponents
   static constexpr int BAD = QC + 1024;   // uint32 [4 + 2][4]: drafted keys without a usable scale in K, V
-  static constexpr int BARS = BAD + 96;     // mbarriers
+  static constexpr int TOPS = BAD + 96;     // uint32 [2][4]: by K's and by V's warps: each one's largest scales
+  static constexpr int POWERS = TOPS + 32;  // int16 [4][2]: powers of two of K and of V in the last four tiles
+  static constexpr int BARS = POWERS + 16;  // mbarriers
   static constexpr int MISC = BARS + 176;   // TMEM address, abort flag, walk start
   static constexpr int BYTES = MISC + 64;
 };
@@ -177,7 +179,7 @@ __device__ __forceinline__ void dequant_role(const TcParams &P, Walk walk, const
   using SM = Smem<D>;
   struct Regs {
     uint4 w[NCH];
-    uint16_t s[NCH][NS];
+    uint16_t s[NCH * NS], sv[NCH * NS];  // scales; K's warps: V's beside them
     bool draft;
   };
   const TreeParams &T = P.t;
@@ -186,7 +188,7 @@ __device__ __forceinline__ void dequant_role(const TcParams &P, Walk walk, const
 
   Segment s;
   int nctx = 0, len = 0, rem = 0;
-  Source src{};
+  Source src{}, vsrc{};
   auto load = [&](Regs &r, int i) {  // tile i of the segment
     const int tile = s.tile + i;
     r.draft = tile >= nctx;
@@ -194,24 +196,30 @@ __device__ __forceinline__ void dequant_role(const TcParams &P, Walk walk, const
       const int t0 = (r.draft ? tile - nctx : tile) * KT + r0;
       rem = (r.draft ? T.ndraft : len) - t0;
       src = source_of<D, G, DQ>(T, r.draft, is_v, s.b, s.kvh, t0, c);
+      if (!is_v) vsrc = source_of<D, G, DQ>(T, r.draft, true, s.b, s.kvh, t0, c);
     } else {
       src.p += static_cast<int64_t>(NCH) * src.pst;
       src.s += static_cast<int64_t>(NCH) * src.sst;
+      vsrc.s += static_cast<int64_t>(NCH) * vsrc.sst;
       rem -= KT;
     }
 #pragma unroll
     for (int k = 0; k < NCH; ++k) {
       r.w[k] = make_uint4(0, 0, 0, 0);
 #pragma unroll
-      for (int e = 0; e < NS; ++e) r.s[k][e] = 0;
+      for (int e = NS * k; e < NS * k + NS; ++e) r.s[e] = r.sv[e] = 0;
       if (RSTEP * k < rem) {
         r.w[k] = __ldg(reinterpret_cast<const uint4 *>(src.p + static_cast<int64_t>(k) * src.pst));
 #pragma unroll
-        for (int e = 0; e < NS; ++e) r.s[k][e] = __ldg(src.s + static_cast<int64_t>(k) * src.sst + e);
+        for (int e = 0; e < NS; ++e) {
+          r.s[NS * k + e] = __ldg(src.s + static_cast<int64_t>(k) * src.sst + e);
+          if (!is_v) r.sv[NS * k + e] = __ldg(vsrc.s + static_cast<int64_t>(k) * vsrc.sst + e);
+        }
       }
     }
   };
   bool big = false;
+  int least = 0;   // smallest power of two in V's tiles of the segment
   uint32_t n = 0;  // tiles so far
   auto turn_over = [&](Regs &r) {  // a loaded tile to shared memory
     const uint32_t st = n & 1u, use = n >> 1;
@@ -219,29 +227,56 @@ __device__ __forceinline__ void dequant_role(const TcParams &P, Walk walk, const
     // (when a stage is free again, the marks of the tile that far back have been read)
     const uint32_t bad = smem + SM::BAD + 16 * (is_v ? 4 + st : n & 3u);
     const uint32_t tile = smem + (is_v ? SM::V : SM::K) + st * SM::TILE;
+    // The tile's powers of two (see tc.cuh).  K's warps find V's as well, from the
+    // same scales by the same rule, so that the softmax warps have it with the
+    // scores and need not wait for V (2 % of a tile).
+    bool odd = tc::scales_odd(r.s);
+    if (!is_v) odd = odd || tc::scales_odd(r.sv);
     W.wait((is_v ? VEMPTY : KEMPTY) + st, use + 1u);  // passes at once for the first use of a stage
-    if (r.draft) {
-      if (tid < 4) asm volatile("st.shared.u32 [%0], %1;" ::"r"(bad + 4 * tid), "r"(0u) : "memory");
+    if (r.draft && tid < 4) asm volatile("st.shared.u32 [%0], %1;" ::"r"(bad + 4 * tid), "r"(0u) : "memory");
+    int shift = 0, vshift = 0;
+    odd = tc::barrier_any(is_v ? 3 : 2, odd);
+    if (odd) {
+      // the four warps put their largest scales together (low half: their own)
+      const uint32_t tops = smem + SM::TOPS + 16 * is_v;
+      uint32_t top = tc::scales_top(r.s);
+      if (!is_v) top |= tc::scales_top(r.sv) << 16;
+      if ((tid & 31) == 0) asm volatile("st.shared.u32 [%0], %1;" ::"r"(tops + 4 * (tid >> 5)), "r"(top) : "memory");
       asm volatile("bar.sync %0, 128;" ::"r"(is_v ? 3 : 2) : "memory");
+      const uint4 t = lds128(tops);  // (not written again before the next tile's first barrier)
+      const uint32_t m = __vmaxu2(__vmaxu2(t.x & 0x7FFF7FFFu, t.y & 0x7FFF7FFFu),
+                                  __vmaxu2(t.z & 0x7FFF7FFFu, t.w & 0x7FFF7FFFu));
+      const uint32_t not_exact = t.x | t.y | t.z | t.w;
+      if (not_exact & 0x8000u) shift = tc::scale_shift(m & 0xFFFFu);
+      if (not_exact >> 31) vshift = tc::scale_shift(m >> 16);
+    }
+    // V's sums of earlier tiles move up by 2^48 at most, which they can
+    (is_v ? shift : vshift) = min(is_v ? shift : vshift, least + 48);
+    least = min(least, is_v ? shift : vshift);
+    if (!is_v && tid == 0)
+      asm volatile("st.shared.u32 [%0], %1;" ::"r"(smem + SM::POWERS + 4 * (n & 3u)),
+                   "r"((static_cast<uint32_t>(shift) & 0xFFFFu) | static_cast<uint32_t>(vshift) << 16)
+                   : "memory");
+    if (odd || shift != 0) {
+      const float up = tc::pow2(shift);
+#pragma unroll
+      for (int k = 0; k < NCH * NS; ++k) {
+        r.s[k] = tc::scale_shifted(r.s[k], up);
+        if (r.s[k] != 0x7F80u) continue;
+        big = true;
+        if (r.draft) {  // seen by some rows only: out of the product, those rows are marked
+          const int row = r0 + RSTEP * (k / NS);
+          r.s[k] = 0;
+          asm volatile("red.shared.or.b32 [%0], %1;" ::"r"(bad + 4 * (row >> 5)), "r"(1u << (row & 31)) : "memory");
+        }
+      }
     }
 #pragma unroll
     for (int k = 0; k < NCH; ++k) {
-      const int row = r0 + RSTEP * k;
       uint32_t sp[NS];
 #pragma unroll
-      for (int e = 0; e < NS; ++e) {
-        sp[e] = tc::scale_pair(r.s[k][e]);
-        const float f = __uint_as_float(static_cast<uint32_t>(r.s[k][e]) << 16);
-        if (!(fabsf(f) <= tc::kMaxScale)) {
-          big = true;
-          if (r.draft) {  // seen by some rows only: out of the product, those rows are marked
-            sp[e] = 0;
-            asm volatile("red.shared.or.b32 [%0], %1;" ::"r"(bad + 4 * (row >> 5)), "r"(1u << (row & 31))
-                         : "memory");
-          }
-        }
-      }
-      store_chunk<D, NS>(tile, row, c, r.w[k], sp);
+      for (int e = 0; e < NS; ++e) sp[e] = tc::scale_pair(r.s[NS * k + e]);
+      store_chunk<D, NS>(tile, r0 + RSTEP * k, c, r.w[k], sp);
     }
     tc::fence_smem();
     __syncwarp();
@@ -255,6 +290,7 @@ __device__ __forceinline__ void dequant_role(const TcParams &P, Walk walk, const
   for (uint32_t seg = 0; walk.next(P, s); ++seg) {
     len = static_cast<int>(context_len(T, s.b, nullptr));
     nctx = (len + KT - 1) / KT;
+    least = tc::kMaxShift;
     load(a, 0);
     // The segment's queries, a row tile by K's warps and one by V's: as soon as
     // the scores of the segment before are out and the softmax warps have its
@@ -520,6 +556,7 @@ __device__ __forceinline__ void softmax_role(const TcParams &P, Walk walk, const
 
     float m = -INFINITY, l = 0.0f;
     bool broken = false;  // saw a key without a usable scale
+    uint32_t vpower = 0;  // power of two in this stream's output (V's half of a tile's powers)
     for (int i = 0; i < steps; ++i) {
       const int j = two ? i : 2 * i + x, tile = s.tile + j;
       const bool draft = tile >= nctx;
@@ -549,6 +586,33 @@ __device__ __forceinline__ void softmax_role(const TcParams &P, Walk walk, const
       W.wait(SFULL + x, ns);
       tc::fence_after();
       if (!idle) {  // rows past the last: their weights may be anything
+        const uint32_t n = base + j, powers = lds32(smem + SM::POWERS + 4 * (n & 3u));
+        auto scale_columns = [](uint32_t at, int from, int to, float f) {
+#pragma unroll 1
+          for (int col = from; col < to; col += 32) {
+            uint32_t o[32];
+            tc::ld32(at + col, o);
+            tc::wait_ld(o);
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+            tc::st32(at + col, o);
+          }
+        };
+        if (powers != vpower) {  // seldom
+          const int ks = static_cast<int16_t>(powers & 0xFFFFu), vs = static_cast<int16_t>(powers >> 16),
+                    was = static_cast<int16_t>(vpower >> 16);
+          if (ks != 0) {
+            scale_columns(tS, 32 * cs, 32 * ce, tc::pow2(-ks));
+            tc::wait_st();
+          }
+          if (i > 0 && vs != was) {
+            W.wait(OREADY + x, ns - 1);
+            tc::fence_after();
+            scale_columns(tO, 0, D, tc::pow2(vs - was));
+            tc::wait_st();
+          }
+          vpower = powers & 0xFFFF0000u;
+        }
         const float mx = (whole ? tile_max<false>(tS, bits, cs, ce) : tile_max<true>(tS, bits, cs, ce)) * c0;
         // the maximum moves only when a score passes it by more than 8, so that
         // weights stay below 2^8 (2^15 as written): seldom after a row's first tile
@@ -560,15 +624,7 @@ __device__ __forceinline__ void softmax_role(const TcParams &P, Walk walk, const
           if (i > 0) {
             W.wait(OREADY + x, ns - 1);
             tc::fence_after();
-#pragma unroll 1
-            for (int c = 0; c < D; c += 32) {
-              uint32_t o[32];
-              tc::ld32(tO + c, o);
-              tc::wait_ld(o);
-#pragma unroll
-              for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
-              tc::st32(tO + c, o);
-            }
+            scale_columns(tO, 0, D, alpha);
           }
         }
         const float me = m == -INFINITY ? 0.0f : m - kWeightShift;
@@ -580,7 +636,6 @@ __device__ __forceinline__ void softmax_role(const TcParams &P, Walk walk, const
             if (c < 2 * cs || c >= 2 * ce) tc::zero8(tS + 8 * c);
         }
         if (draft) {
-          const uint32_t n = base + j;
           W.wait(VFULL + (n & 1u), n >> 1);  // V's marks; K's came with the scores
           const uint4 bk = lds128(smem + SM::BAD + 16 * (n & 3u)), bv = lds128(smem + SM::BAD + 16 * (4 + (n & 1u)));
           const uint4 bad = make_uint4(bk.x | bv.x, bk.y | bv.y, bk.z | bv.z, bk.w | bv.w);
@@ -613,6 +668,7 @@ __device__ __forceinline__ void softmax_role(const TcParams &P, Walk walk, const
                          node * T.os[2];
     float *part = T.ws_o + slot * D * WS_ROWS + row - s.row0;
     float inv;
+    const float down = tc::pow2(-static_cast<int16_t>(vpower >> 16));
     if (two) {
       inv = l > 0.0f ? 1.0f / l : (l == l ? 0.0f : l);
 #pragma unroll 1
@@ -623,7 +679,7 @@ __device__ __forceinline__ void softmax_role(const TcParams &P, Walk walk, const
         tc::wait_ld(o);
         // accumulator columns 8a.. hold dims 8a + (0,4,1,5,2,6,3,7)
 #pragma unroll
-        for (int e = 0; e < 32; ++e) v[(e & ~7) + ((e & 1) ? 4 : 0) + ((e & 7) >> 1)] = __uint_as_float(o[e]);
+        for (int e = 0; e < 32; ++e) v[(e & ~7) + ((e & 1) ? 4 : 0) + ((e & 7) >> 1)] = __uint_as_float(o[e]) * down;
         if (!ok) continue;
         if (s.whole) {
 #pragma unroll
@@ -654,7 +710,7 @@ __device__ __forceinline__ void softmax_role(const TcParams &P, Walk walk, const
       const float Me = M == -INFINITY ? 0.0f : M;
 #pragma unroll 1
       for (int k = r & (RR - 1); k < 256; k += RR) total = fmaf(ml[k].y, exp2f(ml[k].x - Me), total);
-      const float f = steps > 0 ? exp2f(m - Me) : 0.0f;
+      const float f = steps > 0 ? exp2f(m - Me) * down : 0.0f;
       m = M;
       l = total;
       inv = l > 0.0f ? 1.0f / l : (l == l ? 0.0f : l);

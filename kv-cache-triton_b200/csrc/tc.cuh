@@ -196,19 +196,85 @@ __device__ __forceinline__ uint32_t nib_pair(uint32_t x) {
 
 // Eight codes of a packed word times a scale (f16, in both halves), in the dim
 // order 0,4,1,5,2,6,3,7: (1024 + code) - 1032 is exact, and so is the product
-// of a 4-bit code and a bf16 scale's 8 significant bits while it is a normal f16.
+// of a 4-bit code and a bf16 scale's 8 significant bits (in the range below).
 __device__ __forceinline__ void dequant_word(uint32_t w, uint32_t scale, uint32_t (&v)[4]) {
 #pragma unroll
   for (int e = 0; e < 4; ++e) v[e] = hmul2(hsub2(nib_pair(w >> (4 * e)), 0x64086408u), scale);
 }
 
-// a bf16 scale as f16 in both halves; values past the f16 range become infinite
+// ---- bf16 scales in f16 operands ----
+// A scale of 8 significant bits times a code is exact in f16 while the scale lies
+// in [2^-17, 2^12): f16 steps by 2^-24 at its lower end, and 8 * 2^12 is below its
+// upper.  Scales elsewhere are first multiplied by a power of two 2^e, the same
+// for all scales of a key tile (or of a warp's step), and whatever was
+// multiplied with them by 2^-e in fp32: with the largest brought to [2^10, 2^11),
+// all down to 2^-27 of it are exact.  e = 0 while all lie in that range as they are.
+constexpr uint32_t kExactLo = 110u << 7, kExactSpan = 29u << 7;  // bits of 2^-17; of 2^-17 .. 2^12
+constexpr uint32_t kUsableEnd = 227u << 7;                       // 2^100: a larger scale is reported, not used
+constexpr int kMaxShift = 96;
+
+__device__ __forceinline__ uint32_t scale_bits(uint32_t bf) { return bf & 0x7FFFu; }  // |scale|, ordered
+__device__ __forceinline__ bool scale_usable(uint32_t bits) { return bits < kUsableEnd; }
+__device__ __forceinline__ bool scale_exact(uint32_t bits) {
+  return bits == 0u || bits - kExactLo < kExactSpan;
+}
+// Whether some of N scales are not exact as they are.
+template <int N>
+__device__ __forceinline__ bool scales_odd(const uint16_t (&x)[N]) {
+  uint32_t lo = 0xFFFFFFFFu, hi = 0;
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    lo = min(lo, scale_bits(x[k]) - 1u);  // zeros last
+    hi = max(hi, scale_bits(x[k]));
+  }
+  return lo < kExactLo - 1u || hi >= kExactLo + kExactSpan;
+}
+// A warp's largest usable scale (bits), and bit 15 where some are not exact.
+template <int N>
+__device__ __forceinline__ uint32_t scales_top(const uint16_t (&x)[N]) {
+  uint32_t top = 0;
+  bool exact = true;
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    const uint32_t u = scale_bits(x[k]);
+    exact = exact && scale_exact(u);
+    if (scale_usable(u)) top = max(top, u);
+  }
+  return __reduce_max_sync(0xffffffffu, top) | (__all_sync(0xffffffffu, exact) ? 0u : 0x8000u);
+}
+// 2^e, e held within the normal numbers
+__device__ __forceinline__ float pow2(int e) {
+  return __uint_as_float(static_cast<uint32_t>(min(max(e, -126), 127) + 127) << 23);
+}
+// e for the largest usable scale (as bits)
+__device__ __forceinline__ int scale_shift(uint32_t top) {
+  return min(10 + 127 - static_cast<int>(top >> 7), kMaxShift);
+}
+// a bf16 scale times 2^e (exact); one that is not usable becomes infinite
+__device__ __forceinline__ uint16_t scale_shifted(uint16_t bf, float up) {
+  if (!scale_usable(scale_bits(bf))) return 0x7F80u;
+  return static_cast<uint16_t>(__float_as_uint(__uint_as_float(static_cast<uint32_t>(bf) << 16) * up) >> 16);
+}
+// a bf16 scale as f16 in both halves; an infinite one stays so
 __device__ __forceinline__ uint32_t scale_pair(uint16_t bf) {
   const uint32_t h = __half_as_ushort(__float2half_rn(__uint_as_float(static_cast<uint32_t>(bf) << 16)));
   return h | (h << 16);
 }
+// barrier `id` of 128 threads (whole warps); true where `p` is for any of them
+__device__ __forceinline__ bool barrier_any(int id, bool p) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.b32 p, %2, 0;\n\t"
+      "bar.red.or.pred q, %1, 128, p;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(r)
+      : "r"(id), "r"(p ? 1u : 0u)
+      : "memory");
+  return r != 0u;
+}
 
-// largest |scale| whose products with -8 .. 7 stay finite in f16
+// largest |f16 scale| whose products with -8 .. 7 stay finite in f16
 constexpr float kMaxScale = 65504.0f / 8.0f;
 
 }  // namespace tc

@@ -61,6 +61,8 @@ template <int D>
 struct Chunk {
   static constexpr int CPR = D / 32;  // chunks per row
   int row, c;
+  // of the four warps that take a tile, the one that row r is with
+  static __device__ __forceinline__ int warp_of(int r) { return (D == 128 ? r >> 3 : r >> 4) & 3; }
   __device__ __forceinline__ explicit Chunk(int tid) {
     const int lane = tid & 31;
     if (D == 128) {

@@ -64,7 +64,8 @@ struct Smem {
   static constexpr int TILE = KT * D * 2;
   static constexpr int Q = 0, K = TILE, END = 3 * TILE;
   static constexpr int INFO = END;            // per two rows: float4 (c, c, -m, -m) [64], float2 (1 / l) [64]
-  static constexpr int BARS = INFO + 2048;
+  static constexpr int KFAC = INFO + 2048;    // float [4][4]: by tile and warp, what the scores of its rows are multiplied with
+  static constexpr int BARS = KFAC + 64;
   static constexpr int MISC = BARS + 128;     // TMEM address, abort flag
   static constexpr int BYTES = MISC + 16;
 };
@@ -97,7 +98,7 @@ __device__ __forceinline__ void dequant_role(const STcParams &P, Walk walk, cons
   const TreeParams &T = P.s.t;
   struct Regs {
     uint4 w[NCH];
-    uint16_t s[NCH][NS];
+    uint16_t s[NCH * NS];
   };
   const Chunk<D> own(tid);
   const int r0 = own.row, c = own.c;
@@ -117,11 +118,11 @@ __device__ __forceinline__ void dequant_role(const STcParams &P, Walk walk, cons
     for (int k = 0; k < NCH; ++k) {
       r.w[k] = make_uint4(0, 0, 0, 0);
 #pragma unroll
-      for (int e = 0; e < NS; ++e) r.s[k][e] = 0;
+      for (int e = NS * k; e < NS * k + NS; ++e) r.s[e] = 0;
       if (RSTEP * k < rem) {
         r.w[k] = __ldg(reinterpret_cast<const uint4 *>(src.p + static_cast<int64_t>(k) * src.pst));
 #pragma unroll
-        for (int e = 0; e < NS; ++e) r.s[k][e] = __ldg(src.s + static_cast<int64_t>(k) * src.sst + e);
+        for (int e = 0; e < NS; ++e) r.s[NS * k + e] = __ldg(src.s + static_cast<int64_t>(k) * src.sst + e);
       }
     }
     if (++i < p.ntiles && p.tile + i != P.nctx) {
@@ -143,15 +144,30 @@ __device__ __forceinline__ void dequant_role(const STcParams &P, Walk walk, cons
   uint32_t n = 0;
   auto turn_over = [&](Regs &r) {
     const uint32_t st = n & 1u, use = n >> 1, tile = smem + SM::K + st * SM::TILE;
+    // the power of two of this warp's rows (see tc.cuh)
+    float down = 1.0f;
+    if (__any_sync(0xffffffffu, tc::scales_odd(r.s))) {
+      const uint32_t top = tc::scales_top(r.s);
+      if (top & 0x8000u) {
+        const int shift = tc::scale_shift(top & 0x7FFFu);
+        const float up = tc::pow2(shift);
+        down = tc::pow2(-shift);
+#pragma unroll
+        for (int k = 0; k < NCH * NS; ++k) {
+          r.s[k] = tc::scale_shifted(r.s[k], up);
+          big = big || r.s[k] == 0x7F80u;
+        }
+      }
+    }
     W.wait(KEMPTY + st, use + 1u);  // passes at once for the first use of a stage
+    if ((tid & 31) == 0)
+      asm volatile("st.shared.f32 [%0], %1;" ::"r"(smem + SM::KFAC + 16 * (n & 3u) + 4 * (tid >> 5)), "f"(down)
+                   : "memory");
 #pragma unroll
     for (int k = 0; k < NCH; ++k) {
       uint32_t sp[NS];
 #pragma unroll
-      for (int e = 0; e < NS; ++e) {
-        sp[e] = tc::scale_pair(r.s[k][e]);
-        big |= !(fabsf(__uint_as_float(static_cast<uint32_t>(r.s[k][e]) << 16)) <= tc::kMaxScale);
-      }
+      for (int e = 0; e < NS; ++e) sp[e] = tc::scale_pair(r.s[NS * k + e]);
       store_chunk<D, NS>(tile, r0 + RSTEP * k, c, r.w[k], sp);
     }
     tc::fence_smem();
@@ -296,12 +312,20 @@ __device__ __forceinline__ void sum_role(const STcParams &P, Walk walk, const Wa
         // query i sees drafted key j iff j <= i + shift
         const int from = draft && T.causal ? max(0, key - T.shift) * T.R - pass * RT : 0;
         const bool some = __any_sync(0xffffffffu, from > 0);
+        // of the warp that dequantized this key; seldom other than 1.  Its place is
+        // written again four tiles on, behind SEMPTY below
+        const float kf = __uint_as_float(lds32(smem + SM::KFAC + 16 * (n & 3u) + 4 * Chunk<D>::warp_of(r)));
+        const bool shifted = __any_sync(0xffffffffu, kf != 1.0f);
         uint64_t sum = 0;
 #pragma unroll 1
         for (int c = 0; c < cols; c += 32) {
           uint32_t s[32];
           tc::ld32(tS + c, s);
           tc::wait_ld(s);
+          if (shifted) {
+#pragma unroll
+            for (int e = 0; e < 32; ++e) s[e] = __float_as_uint(__uint_as_float(s[e]) * kf);
+          }
           const uint32_t info = smem + SM::INFO + 8 * c;
           if (some) add32<true>(s, info, info + 1024 - 4 * c, from - c, sum);
           else add32<false>(s, info, info + 1024 - 4 * c, 0, sum);
