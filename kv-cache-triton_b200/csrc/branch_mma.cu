@@ -226,9 +226,9 @@ __device__ __forceinline__ void lds_scales(uint32_t (&w)[(NG + 1) / 2], uint32_t
 }
 
 // A operand of 16 (or 8) rows of q, in the column order of the K words, and the
-// factor of rows g and g + 8 from sums to base-2 exponents.  bf16 rows are
-// scaled by a power of two so that their largest element lies in
-// [2^13, 2^14): exact, as are f16 rows as they are.
+// factor of rows g and g + 8 from sums to base-2 exponents.  Rows are scaled by a
+// power of two so that their largest element lies in [2^13, 2^14): exact down to
+// 2^-23 of it (bf16: 2^-26), and off by at most 2^-34 of it below that.
 template <int D, bool HALF>
 struct Query {
   uint32_t a[D / 16][HALF ? 2 : 4];
@@ -247,38 +247,31 @@ __device__ __forceinline__ void load_query(Query<D, HALF> &Q, const TreeParams &
     for (int i = 0; i < D / 32; ++i)
       w[i] = row < rows ? __ldg(reinterpret_cast<const uint4 *>(q + 32 * i)) : make_uint4(0, 0, 0, 0);
     Q.c[r] = T.scale_log2;
-    float up = 1.0f;
     const bool bf = T.q_dtype == KV4_BF16;
-    if (bf) {
-      uint32_t top = 0;
+    uint32_t top = 0;  // largest |q| as bits: magnitudes of either type order like integers
 #pragma unroll
-      for (int i = 0; i < D / 32; ++i) {
-        const uint32_t u[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
+    for (int i = 0; i < D / 32; ++i) {
+      const uint32_t u[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
 #pragma unroll
-        for (int e = 0; e < 4; ++e) top = max(top, max(u[e] & 0x7FFFu, (u[e] >> 16) & 0x7FFFu));
-      }
-      top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-      top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      int ex = 13 - (static_cast<int>(top >> 7) - 127);
-      ex = top == 0 ? 0 : min(max(ex, -126), 126);
-      up = __uint_as_float(static_cast<uint32_t>(ex + 127) << 23);
-      Q.c[r] *= __uint_as_float(static_cast<uint32_t>(127 - ex) << 23);
+      for (int e = 0; e < 4; ++e) top = max(top, max(u[e] & 0x7FFFu, (u[e] >> 16) & 0x7FFFu));
     }
+    top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+    int ex = 13 - (static_cast<int>(__float_as_uint(bf ? bf16lo_to_f32(top) : f16lo_to_f32(top)) >> 23) - 127);
+    ex = top == 0 ? 0 : min(max(ex, -126), 126);
+    const float up = tc::pow2(ex);
+    Q.c[r] *= tc::pow2(-ex);
 #pragma unroll
     for (int i = 0; i < D / 32; ++i) {
       const uint32_t u[4] = {w[i].x, w[i].y, w[i].z, w[i].w};  // columns 8t .. 8t + 7 of the block
-      uint32_t p[4];                                          // pairs (0,4) (1,5) (2,6) (3,7)
-      if (bf) {
-        p[0] = pack_f16x2(bf16lo_to_f32(u[0]) * up, bf16lo_to_f32(u[2]) * up);
-        p[1] = pack_f16x2(bf16hi_to_f32(u[0]) * up, bf16hi_to_f32(u[2]) * up);
-        p[2] = pack_f16x2(bf16lo_to_f32(u[1]) * up, bf16lo_to_f32(u[3]) * up);
-        p[3] = pack_f16x2(bf16hi_to_f32(u[1]) * up, bf16hi_to_f32(u[3]) * up);
-      } else {
-        p[0] = prmt(u[0], u[2], 0x5410);
-        p[1] = prmt(u[0], u[2], 0x7632);
-        p[2] = prmt(u[1], u[3], 0x5410);
-        p[3] = prmt(u[1], u[3], 0x7632);
+      float lo[4], hi[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        lo[e] = (bf ? bf16lo_to_f32(u[e]) : f16lo_to_f32(u[e])) * up;
+        hi[e] = (bf ? bf16hi_to_f32(u[e]) : f16hi_to_f32(u[e])) * up;
       }
+      uint32_t p[4] = {pack_f16x2(lo[0], lo[2]), pack_f16x2(hi[0], hi[2]),  // pairs (0,4) (1,5) (2,6) (3,7)
+                       pack_f16x2(lo[1], lo[3]), pack_f16x2(hi[1], hi[3])};
       // pairs 1 and 3 meet codes times 16 (see code_pair)
       p[1] = tc::hmul2(p[1], 0x2C002C00u);
       p[3] = tc::hmul2(p[3], 0x2C002C00u);
