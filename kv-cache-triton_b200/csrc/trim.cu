@@ -63,8 +63,8 @@ __global__ void __launch_bounds__(128, 2) score_generic(const ScoreParams P, int
       const int row = r0 + r;
       bool see = t < P.keys;
       if (see && t >= T.S) see = draft_visible(T, b, row / T.R, static_cast<int>(t - T.S));
-      const float2 st = T.stats[unit * rows + row];
-      if (see && st.y > 0.0f) total = fmaf(exp2f(fmaf(sum4(s[r]), T.scale_log2, -st.x)), st.y, total);
+      const float2 st = T.stats[unit * rows + row];  // 1 / sum 0: a row that saw nothing; NaN: a row without a value
+      if (see && st.y != 0.0f) total = fmaf(exp2f(fmaf(sum4(s[r]), T.scale_log2, -st.x)), st.y, total);
     }
   }
   if (t < P.keys) {
