@@ -449,11 +449,12 @@ __global__ void __launch_bounds__(4 * CTHREADS, 2) commit_rows(const __grid_cons
   __shared__ int32_t path[CPATH];
   const int b = blockIdx.x / P.Hkv, h = blockIdx.x - b * P.Hkv;
   const int k = threadIdx.x / CTHREADS, t = threadIdx.x - k * CTHREADS;
+  // read once: with one head lens_out may be lens, and is written below
+  const int64_t len = P.lens[b], n = P.accepted[b];
+  const bool fits = len >= 0 && n >= 0 && n <= P.width && len + n <= P.cap;
   for (int j0 = 0; j0 == 0 || j0 < P.width; j0 += CPATH) {
     const int j = j0 + static_cast<int>(threadIdx.x);
     if (j < P.width) path[threadIdx.x] = P.path[b * P.path_stride + j];
-    const int64_t len = P.lens[b], n = P.accepted[b];
-    const bool fits = len >= 0 && n >= 0 && n <= P.width && len + n <= P.cap;
     __syncthreads();
     if (j0 == 0 && h == 0 && threadIdx.x == 0) {
       // a sequence that does not fit is left as it was, and reported
