@@ -127,18 +127,22 @@ class Int4KVStore:
         """``append`` followed by attention of ``query`` over the whole layer
         cache, written to ``out`` (any strides, [B, Hq, sq, d]).  A one-token
         decode step is a single launch: the attention kernel quantizes the new
-        row itself (``kv4_append_attention``)."""
-        if self.track_mass:
+        row itself (``kv4_append_attention``).  ``track_mass`` stores score the
+        tokens by one query, or by the last ``mass_window`` of several."""
+        s = key_states.shape[2]
+        if self.track_mass and s == 1 and query.shape[2] == 1:
             self.append(key_states, value_states, layer_idx)
             return self.attend_scored(query, layer_idx, out, is_causal=is_causal)
         layer = self._reserve(key_states, value_states, layer_idx)
-        s = key_states.shape[2]
-        if s != 1:
+        if s != 1 or self.track_mass:
             self.append(key_states, value_states, layer_idx)
             kp, ks, vp, vs = self.layer(layer_idx).views()
-            return frontend.attention(query, kp, ks, vp, vs, n_q_heads=n_q_heads,
-                                      n_kv_heads=n_kv_heads, group_size=self.group_size,
-                                      is_causal=is_causal, out=out)
+            frontend.attention(query, kp, ks, vp, vs, n_q_heads=n_q_heads,
+                               n_kv_heads=n_kv_heads, group_size=self.group_size,
+                               is_causal=is_causal, out=out)
+            if self.track_mass:
+                self.score_window(query, layer_idx)
+            return out
         n = layer.seq_len + 1
         ops.append_attention_descs(query, key_states, value_states, layer.view_descs(n), out,
                                    self.group_size, is_causal, self.tie_mode,
