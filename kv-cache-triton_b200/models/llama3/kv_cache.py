@@ -29,7 +29,7 @@ class QuantizedKVCache:
         """``track_mass``: score the cached tokens by the attention weight they
         receive (see ``evict``), from one-token steps and from the last
         ``mass_window`` queries of a prompt; older weight fades by
-        ``mass_decay`` per call."""
+        ``mass_decay`` per call.  Attention under a mask scores nothing."""
         if group_size <= 0:
             raise ValueError("group_size must be > 0")
         self.group_size = int(group_size)
@@ -119,7 +119,8 @@ class QuantizedKVCache:
     def evict(self, keep: int, *, recent: int = 0, sinks: int = 0) -> dict[int, torch.Tensor]:
         """Cut every layer to ``keep`` tokens per KV head: the first ``sinks``, the
         last ``recent`` and the highest scored of the rest; returns the kept token
-        numbers per layer.  ``get_seq_length`` is then the number of tokens held,
+        numbers per layer.  Tokens without scores are not ranked: ``ValueError``
+        unless ``recent`` covers them.  ``get_seq_length`` is then the number of tokens held,
         no longer the number seen: pass ``position_ids`` to the model yourself
         (keys keep the rotary positions they were cached with)."""
         return self._store.evict(int(keep), recent=int(recent), sinks=int(sinks))

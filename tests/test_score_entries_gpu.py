@@ -37,3 +37,54 @@ def test_append_attend_scores_by_the_window(chunks, causal):
     for s in chunks:
         total = 0.75 * total + 4 * min(s, 16)
     assert bool(((fused.mass(0).sum(-1) - total).abs() < 1e-2).all())
+
+
+def test_tokens_without_scores_are_not_ranked():
+    from kvint4.cache import Int4KVStore
+    store = Int4KVStore(32, track_mass=True, mass_window=16)
+    q, k, v = _data(200, 1)
+    for layer in (0, 1):
+        store.append(k[:, :, :150], v[:, :, :150], layer)
+    store.score_window(q[:, :, :150], 0)
+    before = [t.clone() for layer in (0, 1) for t in store.layer(layer).views()]
+    with pytest.raises(ValueError, match="layer 1.*150 tokens"):
+        store.evict(60, recent=8)
+    for x, y in zip(before, [t for layer in (0, 1) for t in store.layer(layer).views()]):
+        assert torch.equal(x, y)  # layer 0 neither
+    store.score_window(q[:, :, :150], 1)
+    for layer in (0, 1):
+        store.append(k[:, :, 150:], v[:, :, 150:], layer)
+    with pytest.raises(ValueError, match="50 tokens"):
+        store.evict(60, recent=49)
+    assert store.evict(200) == {}
+    store.crop(180)
+    assert set(store.evict(60, recent=30)) == {0, 1}  # the tokens without scores are the recent ones
+    with pytest.raises(ValueError, match="30 tokens"):
+        store.append(k[:, :, :30], v[:, :, :30], 0)
+        store.evict(40, recent=20)
+    store.crop(60)
+    assert set(store.evict(40)) == {0, 1}
+
+
+def test_a_masked_prompt_is_not_cut_blindly():
+    from transformers import LlamaConfig, LlamaForCausalLM
+
+    from models.llama3.kv_cache import QuantizedKVCache
+    from models.llama3.llama3_quant import replace_llama_attention_with_quantized
+    torch.manual_seed(0)
+    with torch.device("cuda"):
+        model = LlamaForCausalLM(LlamaConfig(
+            vocab_size=97, hidden_size=256, intermediate_size=256, num_hidden_layers=2, num_attention_heads=4,
+            num_key_value_heads=2, head_dim=64, tie_word_embeddings=False)).to(torch.bfloat16).eval()
+    replace_llama_attention_with_quantized(model)
+    ids = torch.randint(0, 97, (2, 40), device="cuda")
+    keep = torch.ones_like(ids)
+    keep[1, :9] = 0  # padding
+    with torch.inference_mode():
+        cache = QuantizedKVCache(track_mass=True)
+        model(input_ids=ids, past_key_values=cache, use_cache=True, attention_mask=keep)
+        with pytest.raises(ValueError, match="no scores"):
+            cache.evict(20, recent=4)
+        cache = QuantizedKVCache(track_mass=True)
+        model(input_ids=ids, past_key_values=cache, use_cache=True)
+        assert set(cache.evict(20, recent=4)) == {0, 1}
