@@ -365,7 +365,8 @@ int kv4_tree_attention(const kv4_tensor *q, const kv4_tensor *k_packed, const kv
  * path, accepted, context_lens, lens_out: device int32; path_width bounds
  * accepted.  A sequence whose length, count or capacity does not fit is left
  * as it was (lens_out = context_lens), a node outside the draft is skipped;
- * both set bit 16 of kv4_device_error.  Unit stride in the last dimension.
+ * both set bit 16 of kv4_device_error.  Unit stride in the last dimension; cache
+ * and drafted rows do not overlap.
  */
 int kv4_commit_rows(const kv4_tensor *k_packed, const kv4_tensor *k_scales,
                     const kv4_tensor *v_packed, const kv4_tensor *v_scales,
@@ -380,7 +381,8 @@ int kv4_commit_rows(const kv4_tensor *k_packed, const kv4_tensor *k_scales,
  *   score_out[b, g, t] = decay * score_in[b, g, t] + the softmax weight that
  *   token t received, summed over the queries and over the q heads of KV head g.
  * score_in, score_out: f32 [1, B, Hkv, S] (any strides; they may be the same
- * tensor).  is_causal: query i sees tokens t <= S - sq + i.  Shapes, dtypes, the
+ * tensor, but overlap neither otherwise nor with the rest; out overlaps nothing
+ * that is read).  is_causal: query i sees tokens t <= S - sq + i.  Shapes, dtypes, the
  * range of scales and workspace as for kv4_tree_attention, with
  * kv4_scored_workspace() bytes.
  */

@@ -9,6 +9,8 @@
 // one by one and raises), or the status when the library refused.
 #include <Python.h>
 
+#include <algorithm>
+
 #include <ATen/ATen.h>
 #include <ATen/EmptyTensor.h>
 #include <c10/cuda/CUDACachingAllocator.h>
@@ -82,10 +84,82 @@ void on_device(const at::Tensor &t, const at::Tensor &like) {
   need(t.is_cuda() && t.get_device() == like.get_device());
 }
 
+// a written tensor: no expanded view
+void written(const at::Tensor &t) {
+  for (int64_t i = 0; i < t.dim(); ++i) need(t.size(i) <= 1 || t.stride(i) != 0);
+}
+
+// Whether two tensors share a byte (views of one buffer may interleave without
+// that).  Distances between two elements are sums of step * x, low <= x <= high;
+// the largest steps are tried first, as far as the smaller ones can make up for them.
+struct Overlap {
+  struct Step { int64_t by, low, high, least, most; };
+  Step s[8];
+  int n = 0, left = 4096;  // places looked at: more only for strides that nest in no way
+  int64_t a_size, b_size;
+
+  void add(const at::Tensor &t, int64_t sign) {
+    for (int64_t i = 0; i < t.dim(); ++i) {
+      const int64_t by = t.stride(i) * t.element_size(), high = t.size(i) - 1;
+      if (high == 0 || by == 0) continue;
+      int k = 0;
+      while (k < n && s[k].by != by) ++k;
+      if (k == n) s[n++] = Step{by, 0, 0, 0, 0};
+      (sign > 0 ? s[k].high : s[k].low) += sign * high;
+    }
+  }
+  bool reach(int i, int64_t at) {
+    if (--left < 0) return true;
+    if (i == n) return -a_size < at && at < b_size;
+    const Step &k = s[i];
+    const int64_t by = k.by, to = k.most - at, from = at - k.least;
+    const int64_t first = std::max(k.low, -(from >= 0 ? from / by : -((-from + by - 1) / by)));
+    const int64_t last = std::min(k.high, to >= 0 ? to / by : -((-to + by - 1) / by));
+    for (int64_t x = first; x <= last; ++x)
+      if (reach(i + 1, at + by * x)) return true;
+    return false;
+  }
+  bool operator()(const at::Tensor &a, const at::Tensor &b) {
+    const auto pa = reinterpret_cast<uintptr_t>(a.data_ptr()), pb = reinterpret_cast<uintptr_t>(b.data_ptr());
+    a_size = a.element_size();
+    b_size = b.element_size();
+    add(a, 1);
+    add(b, -1);
+    std::sort(s, s + n, [](const Step &x, const Step &y) { return x.by > y.by; });
+    int64_t least = 1 - a_size, most = b_size - 1;  // where the elements overlap
+    for (int k = n - 1; k >= 0; --k) {
+      s[k].least = least;
+      s[k].most = most;
+      least -= s[k].by * s[k].high;
+      most -= s[k].by * s[k].low;
+    }
+    return reach(0, static_cast<int64_t>(pa - pb));
+  }
+};
+// a tensor and its extent, which tells most of them apart
+struct View {
+  const at::Tensor *t = nullptr;
+  uintptr_t from = 0, to = 0;
+  View() = default;
+  View(const at::Tensor &x) : t(&x) {
+    if (x.numel() == 0) return;
+    from = reinterpret_cast<uintptr_t>(x.data_ptr());
+    int64_t last = 0;
+    const auto sizes = x.sizes(), strides = x.strides();
+    for (size_t i = 0; i < sizes.size(); ++i) last += (sizes[i] - 1) * strides[i];
+    to = from + (last + 1) * x.element_size();
+  }
+};
+bool overlap(const View &a, const View &b) {
+  return a.from < b.to && b.from < a.to && Overlap{}(*a.t, *b.t);
+}
+void apart(const View &a, const View &b) { need(!overlap(a, b)); }
+
 // four tensors of packed K/V rows, [B, Hkv, tokens, ...]
 struct Rows {
   const at::Tensor *t[4];
   kv4_tensor d[4];
+  View v[4];
   explicit Rows(PyObject *const *a, const at::Tensor *like = nullptr) {
     for (int i = 0; i < 4; ++i) {
       t[i] = &tensor(a[i]);
@@ -96,7 +170,10 @@ struct Rows {
     need(t[0]->sizes() == t[2]->sizes() && t[1]->sizes() == t[3]->sizes());
     need(t[1]->scalar_type() == t[3]->scalar_type());
     for (int i = 0; i < 3; ++i) need(t[0]->size(i) == t[1]->size(i));
-    for (int i = 0; i < 4; ++i) d[i] = desc(*t[i]);
+    for (int i = 0; i < 4; ++i) {
+      d[i] = desc(*t[i]);
+      v[i] = View(*t[i]);
+    }
   }
   bool unit_columns() const {
     for (const at::Tensor *x : t)
@@ -117,6 +194,13 @@ void check_query(const at::Tensor &q, const Rows &c, int64_t n_q, int64_t n_kv, 
 void check_int32(const at::Tensor &t, const at::Tensor &like) {
   need(t.scalar_type() == at::kInt && t.is_contiguous());
   on_device(t, like);
+}
+
+void apart(const View &a, const Rows &rows) {
+  for (const View &v : rows.v) apart(a, v);
+}
+bool same_view(const at::Tensor &a, const at::Tensor &b) {
+  return a.data_ptr() == b.data_ptr() && a.sizes() == b.sizes() && a.strides() == b.strides();
 }
 
 // a contiguous tensor on the current device (the guard's), from the caching
@@ -162,6 +246,13 @@ PyObject *tree(PyObject *const *a) {
          lse->size(1) == n_q && lse->size(2) == n);
     on_device(*lse, q);
     dl = desc(lse->unsqueeze(-1));
+    written(*lse);
+    const View v(*lse);
+    apart(v, q);
+    apart(v, mask);
+    if (lens) apart(v, *lens);
+    apart(v, cache);
+    apart(v, draft);
   }
   const c10::cuda::CUDAGuard guard(q.get_device());
   at::Tensor out;
@@ -171,6 +262,14 @@ PyObject *tree(PyObject *const *a) {
     out = tensor(a[14]);
     need(out.sizes() == q.sizes() && out.scalar_type() == q.scalar_type());
     on_device(out, q);
+    written(out);
+    const View v(out);
+    if (!same_view(out, q)) apart(v, q);
+    apart(v, mask);
+    if (lens) apart(v, *lens);
+    if (lse) apart(v, *lse);
+    apart(v, cache);
+    apart(v, draft);
   }
   if (q.numel() == 0) return THPVariable_Wrap(out);
   const kv4_tensor dq = desc(q), dm = desc(mask), dout = desc(out);
@@ -199,6 +298,12 @@ PyObject *commit(PyObject *const *a) {
   check_int32(lens, k);
   need(path.dim() == 2 && path.size(0) == b && accepted.dim() == 1 && accepted.size(0) == b &&
        lens.dim() == 1 && lens.size(0) == b);
+  const View read[3] = {path, accepted, lens};
+  for (int i = 0; i < 4; ++i) {
+    written(*cache.t[i]);
+    apart(cache.v[i], draft);
+    for (const View &v : read) apart(cache.v[i], v);
+  }
   const c10::cuda::CUDAGuard guard(k.get_device());
   at::Tensor out;
   if (a[11] == Py_None) {
@@ -206,7 +311,11 @@ PyObject *commit(PyObject *const *a) {
   } else {
     out = tensor(a[11]);
     check_int32(out, k);
-    need(out.dim() == 1 && out.size(0) == b && out.data_ptr() != lens.data_ptr());
+    need(out.dim() == 1 && out.size(0) == b);
+    const View to(out);
+    for (const View &v : read) apart(to, v);
+    apart(to, cache);
+    apart(to, draft);
   }
   const kv4_tensor *c = cache.d, *f = draft.d;
   ok(kv4_commit_rows(c, c + 1, c + 2, c + 3, f, f + 1, f + 2, f + 3, path.data_ptr<int32_t>(),
@@ -236,6 +345,11 @@ PyObject *scored(PyObject *const *a) {
   check_mass(mass);
   const at::Tensor &to = a[11] == Py_None ? mass : tensor(a[11]);
   check_mass(to);
+  written(to);
+  const View tv(to);
+  if (!same_view(to, mass)) apart(tv, mass);
+  apart(tv, q);
+  apart(tv, cache);
   const c10::cuda::CUDAGuard guard(q.get_device());
   at::Tensor out;
   if (a[12] == Py_None) {
@@ -244,6 +358,10 @@ PyObject *scored(PyObject *const *a) {
     out = tensor(a[12]);
     need(out.sizes() == q.sizes() && out.scalar_type() == q.scalar_type());
     on_device(out, q);
+    written(out);
+    const View v(out);
+    for (const at::Tensor *t : {&q, &mass, &to}) apart(v, *t);
+    apart(v, cache);
   }
   const kv4_tensor dq = desc(q), din = desc(mass), dto = desc(to), dout = desc(out);
   const kv4_tensor *c = cache.d;
@@ -284,6 +402,11 @@ PyObject *evict(PyObject *const *a) {
       if (i < 4)
         need(out[i].size(3) == like.size(3) && (like.size(3) <= 1 || out[i].stride(3) == 1));
       on_device(out[i], k);
+      written(out[i]);
+      const View v(out[i]);
+      apart(v, cache);
+      apart(v, mass);
+      for (int j = 0; j < i; ++j) apart(v, out[j]);
     }
   }
   const at::Tensor index = fresh({b, h, keep}, at::kInt);
@@ -298,6 +421,8 @@ PyObject *evict(PyObject *const *a) {
   PyTuple_SET_ITEM(r, 5, THPVariable_Wrap(index));
   return r;
 }
+
+PyObject *overlaps(PyObject *const *a) { return PyBool_FromLong(overlap(View(tensor(a[0])), View(tensor(a[1])))); }
 
 // No exception leaves a C entry: what the arguments lack is None, what the
 // library refuses is its status, anything else (out of memory, ...) a Python error.
@@ -335,6 +460,7 @@ PyMethodDef method(const char *name) {
 
 PyMethodDef methods[] = {method<tree, 16>("tree"), method<commit, 12>("commit"),
                          method<scored, 13>("scored"), method<evict, 9>("evict"),
+                         method<overlaps, 2>("overlap"),
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "_binding", nullptr, -1, methods,
                           nullptr, nullptr, nullptr, nullptr};

@@ -6,6 +6,8 @@ import math
 
 import torch
 
+from kvint4._lib import binding
+
 FLOATS = (torch.bfloat16, torch.float16, torch.float32)
 
 
@@ -64,3 +66,25 @@ def need_cuda(name: str, *ts) -> None:
         raise ValueError(f"{name} expects CUDA tensors")
     if any(t.device != ts[0].device for t in ts):
         raise ValueError(f"{name} expects all tensors on one device")
+
+
+def overlap(a, b) -> bool:
+    """Whether some element of ``a`` shares a byte with one of ``b`` (views of one
+    buffer may interleave without that)."""
+    return a.device == b.device and binding().overlap(a, b)
+
+
+def check_written(name: str, t) -> None:
+    if any(n > 1 and st == 0 for n, st in zip(t.shape, t.stride())):
+        raise ValueError(f"{name} must not be an expanded view: it is written")
+
+
+def check_apart(name: str, t, others: dict) -> None:
+    """``t`` is written while ``others`` are read or written."""
+    for other, x in others.items():
+        if x is not None and overlap(t, x):
+            raise ValueError(f"{name} must not overlap {other}")
+
+
+def same_view(a, b) -> bool:
+    return a.data_ptr() == b.data_ptr() and a.shape == b.shape and a.stride() == b.stride()

@@ -11,7 +11,8 @@ from __future__ import annotations
 
 import torch
 
-from kernels.llama3._checks import check_out, check_query, check_rows, need_cuda
+from kernels.llama3._checks import (check_apart, check_out, check_query, check_rows, check_written, need_cuda,
+                                    same_view)
 from kvint4 import ops
 from kvint4._lib import binding, result
 
@@ -37,7 +38,8 @@ def attention_forward_quant_gqa_scored(
     Returns ``(out, mass_out)`` with ``mass_out[b, g, t] = decay * mass[b, g, t]
     +`` the softmax weight of token ``t``, summed over the queries and over the
     q heads of KV head ``g``.  ``mass`` is f32 ``[B, n_kv_heads, S]`` (any
-    strides) and is updated in place when ``mass_out`` is not given.
+    strides) and is updated in place when ``mass_out`` is not given.  ``out`` and
+    another ``mass_out`` must not overlap each other nor anything that is read.
     ``is_causal``: query ``i`` sees tokens ``t <= S - sq + i``.
     """
     got = binding().scored(q, k_packed, k_scales, v_packed, v_scales, mass, n_q_heads, n_kv_heads,
@@ -49,12 +51,19 @@ def attention_forward_quant_gqa_scored(
     check_rows("cache", *cache)
     check_query(q, k_packed, k_scales, n_q_heads, n_kv_heads, group_size)
     shape = k_packed.shape[:3]
-    need_cuda("attention_forward_quant_gqa_scored", q, *cache, mass)
-    check_out("mass", mass, shape, torch.float32, q)
+    read = dict(zip(("q", "k_packed", "k_scales", "v_packed", "v_scales"), (q, *cache)))
     if mass_out is None:
         mass_out = mass
-    else:
-        check_out("mass_out", mass_out, shape, torch.float32, q)
+    elif not same_view(mass_out, mass):
+        check_apart("mass_out", mass_out, {"mass": mass})
+    check_written("mass_out", mass_out)
+    check_apart("mass_out", mass_out, read)
+    if out is not None:
+        check_written("out", out)
+        check_apart("out", out, {**read, "mass": mass, "mass_out": mass_out})
+    need_cuda("attention_forward_quant_gqa_scored", q, *cache, mass)
+    check_out("mass", mass, shape, torch.float32, q)
+    check_out("mass_out", mass_out, shape, torch.float32, q)
     if out is None:
         out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     else:
@@ -82,7 +91,8 @@ def evict_by_mass(
     scores: the earlier token; NaN below everything), in token order.  Returns
     ``(k_packed, k_scales, v_packed, v_scales, mass, index)`` of the kept
     tokens, ``index`` int32 ``[B, n_kv_heads, keep]``; the first five are
-    written into ``out`` when given (views of capacity buffers, for instance).
+    written into ``out`` when given (views of other capacity buffers, for
+    instance: rows are moved all at once, so ``out`` must not overlap the inputs).
     """
     got = binding().evict(k_packed, k_scales, v_packed, v_scales, mass, keep, recent, sinks, out)
     if got is not None:
@@ -98,6 +108,11 @@ def evict_by_mass(
         raise ValueError(f"keep must lie between recent + sinks = {recent + sinks} and the {s} cached tokens")
     if any(t.shape[-1] > 1 and t.stride(-1) != 1 for t in cache):
         raise ValueError("cache rows need a unit stride in the last dimension")
+    if out is not None and len(out) == 5:
+        read = dict(zip(("k_packed", "k_scales", "v_packed", "v_scales", "mass"), (*cache, mass)))
+        for i, o in enumerate(out):
+            check_written("out", o)
+            check_apart("out", o, {**read, **{f"out[{j}]": out[j] for j in range(i)}})
     need_cuda("evict_by_mass", *cache, mass)
     check_out("mass", mass, (b, h, s), torch.float32, k_packed)
     if out is None:

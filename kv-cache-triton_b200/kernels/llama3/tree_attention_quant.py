@@ -9,7 +9,7 @@ touches the cache:
     out = tree_attention_quant_gqa(q, *cache, *draft, mask, ...)
     lens = commit_draft_rows(*cache, *draft, path, accepted, context_lens=lens)
 
-``kvint4.tree.TreeKVCache`` keeps these buffers for all layers of a model.
+``models.llama3.tree_cache.TreeKVCache`` keeps these buffers for all layers of a model.
 The reference has no counterpart (it decodes one token at a time).
 """
 
@@ -17,7 +17,8 @@ from __future__ import annotations
 
 import torch
 
-from kernels.llama3._checks import check_int32, check_out, check_query, check_rows, need_cuda
+from kernels.llama3._checks import (check_apart, check_int32, check_out, check_query, check_rows, check_written,
+                                    need_cuda, same_view)
 from kvint4 import ops
 from kvint4._lib import binding, result
 
@@ -50,7 +51,8 @@ def tree_attention_quant_gqa(
     that sees nothing gives zeros.  ``context_lens`` is int32 ``[B]`` on the
     device; an entry outside ``[0, S]`` reads as 0 and is reported by
     ``ops.device_error()`` (bit 16).  ``lse`` (f32 ``[B, n_q_heads, N]``)
-    receives the log-sum-exp of each row's scores.
+    receives the log-sum-exp of each row's scores.  ``out`` (which may be ``q``
+    itself) and ``lse`` must not overlap each other nor anything that is read.
     """
     got = binding().tree(q, k_packed, k_scales, v_packed, v_scales, draft_k_packed, draft_k_scales,
                          draft_v_packed, draft_v_scales, tree_mask, n_q_heads, n_kv_heads,
@@ -70,6 +72,15 @@ def tree_attention_quant_gqa(
         raise ValueError("draft scales must match the cache's scales")
     if tree_mask.dtype != torch.bool or tuple(tree_mask.shape) not in ((n, n), (b, n, n)):
         raise ValueError("tree_mask must be bool [N, N] or [B, N, N]")
+    names = ("k_packed", "k_scales", "v_packed", "v_scales")
+    read = {**dict(zip(names, cache)), **dict(zip((f"draft_{x}" for x in names), draft)),
+            "tree_mask": tree_mask, "context_lens": context_lens}
+    if out is not None:
+        check_written("out", out)
+        check_apart("out", out, read if same_view(out, q) else {"q": q, **read})
+    if lse is not None:
+        check_written("lse", lse)
+        check_apart("lse", lse, {"q": q, "out": out, **read})
     need_cuda("tree_attention_quant_gqa", q, *cache, *draft, tree_mask)
     if context_lens is not None:
         check_int32("context_lens", context_lens, (b,), q)
@@ -106,7 +117,8 @@ def commit_draft_rows(
     Cache row ``context_lens[b] + j`` becomes drafted row ``path[b, j]`` for
     ``j < accepted[b]``.  ``path`` is int32 ``[B, width]``, ``accepted`` and
     ``context_lens`` int32 ``[B]``, all on the device; the host waits for
-    nothing.  A sequence whose rows do not fit is left as it was and reported
+    nothing.  Cache and drafted rows must not overlap, nor ``lens_out`` what is
+    read.  A sequence whose rows do not fit is left as it was and reported
     by ``ops.device_error()`` (bit 16).
     """
     got = binding().commit(k_packed, k_scales, v_packed, v_scales, draft_k_packed, draft_k_scales,
@@ -124,6 +136,15 @@ def commit_draft_rows(
         if (c.shape[-1] > 1 and c.stride(-1) != 1) or (f.shape[-1] > 1 and f.stride(-1) != 1):
             raise ValueError("cache and draft rows need a unit stride in the last dimension")
     b = k_packed.shape[0]
+    names = ("k_packed", "k_scales", "v_packed", "v_scales")
+    read = {**dict(zip((f"draft_{x}" for x in names), draft)), "path": path, "accepted": accepted}
+    for name, c in zip(names, cache):
+        check_written(name, c)
+        check_apart(name, c, {**read, "context_lens": context_lens})
+    if lens_out is not None:
+        if lens_out.data_ptr() == context_lens.data_ptr():
+            raise ValueError("lens_out must not be context_lens")
+        check_apart("lens_out", lens_out, {**read, **dict(zip(names, cache)), "context_lens": context_lens})
     need_cuda("commit_draft_rows", *cache, *draft, path, accepted, context_lens)
     if path.dim() != 2:
         raise ValueError("path must be [B, width]")
@@ -134,7 +155,5 @@ def commit_draft_rows(
         lens_out = torch.empty_like(context_lens)
     else:
         check_int32("lens_out", lens_out, (b,), k_packed)
-        if lens_out.data_ptr() == context_lens.data_ptr():
-            raise ValueError("lens_out must not be context_lens")
     ops.commit_rows(k_packed, cache, draft, path, accepted, context_lens, lens_out)
     return lens_out
