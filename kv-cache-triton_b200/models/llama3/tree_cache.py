@@ -108,10 +108,12 @@ class TreeKVCache:
 
     def commit(self, path: torch.Tensor, accepted: torch.Tensor) -> None:
         """Move the accepted nodes (``path`` int32 ``[B, width]``, the first
-        ``accepted[b]`` of each row) behind each sequence's context."""
-        new = None
+        ``accepted[b]`` of each row) of the step's tree behind each sequence's context."""
+        if self._mask is None:
+            raise ValueError("begin() a step first")
+        n, new = self._mask.shape[-1], None
         for cache, draft in zip(self._cache, self._draft):
-            new = commit_draft_rows(*cache, *draft, path, accepted, context_lens=self.lens)
+            new = commit_draft_rows(*cache, *[t[:, :, :n] for t in draft], path, accepted, context_lens=self.lens)
         self.lens = new
         self._mask = None
 
