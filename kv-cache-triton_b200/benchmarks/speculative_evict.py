@@ -129,6 +129,7 @@ def run(batch=4, prompt_len=4096, keep=1024, steps=64, layers=4, branch=4, depth
                 calls += 1
 
         tree_ms = timed(tree_run)
+        tree.check()
     same = (got[:, :steps + 1] == want)
     lead = same.int().cumprod(1).sum(1)
     return {

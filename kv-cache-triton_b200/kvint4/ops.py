@@ -443,5 +443,19 @@ def device_error(dev: torch.device | None = None) -> int:
     L = lib()
     flag = ctypes.c_int(0)
     dev = dev or torch.device("cuda", torch.cuda.current_device())
-    check("kv4_device_error", L.kv4_device_error(_stream(dev), ctypes.byref(flag)))
+    with torch.cuda.device(dev):  # each device has a word of its own
+        check("kv4_device_error", L.kv4_device_error(_stream(dev), ctypes.byref(flag)))
     return flag.value
+
+
+DEVICE_ERRORS = {1: "a bounded wait expired (output not valid)", 2: "a page id outside the pool",
+                 4: "a peer exchange wait expired", 8: "a scale out of the kernels' range (output not valid)",
+                 16: "a context length, accepted count or path node out of range"}
+
+
+def check_device(dev: torch.device | None = None) -> None:
+    """Wait for the device and raise if a call since the last look could not do its work."""
+    flag = device_error(dev)
+    if flag:
+        raise RuntimeError("; ".join(text for bit, text in DEVICE_ERRORS.items() if flag & bit)
+                           or f"device error {flag}")

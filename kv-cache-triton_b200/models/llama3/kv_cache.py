@@ -16,6 +16,7 @@ from __future__ import annotations
 
 import torch
 
+from kvint4 import ops
 from kvint4._lib import TIE_HALF_AWAY
 from kvint4.cache import Int4KVStore
 
@@ -124,6 +125,12 @@ class QuantizedKVCache:
         no longer the number seen: pass ``position_ids`` to the model yourself
         (keys keep the rotary positions they were cached with)."""
         return self._store.evict(int(keep), recent=int(recent), sinks=int(sinks))
+
+    def check(self) -> None:
+        """Wait for the device and raise ``RuntimeError`` if a call since the last
+        check could not do its work (on this device, whoever made it)."""
+        for layer in self._layers.values():
+            ops.check_device(layer.k_packed_buf.device)
 
     def update(
         self,

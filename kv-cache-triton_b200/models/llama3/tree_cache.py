@@ -9,7 +9,9 @@ nodes of the current tree.  One step:
     path, accepted, token = accept_greedy(nodes, parents, logits)
     cache.commit(path, accepted)          # accepted K/V move behind the context
 
-Nothing in a step waits for the device: lengths, paths and counts stay there.
+Nothing in a step waits for the device: lengths, paths and counts stay there
+(``tree_mask``, for a new shape of tree, does wait).  What a step could not do, a
+path that no longer fits the capacity for instance, ``check()`` raises.
 Rejected nodes are never in the cache.  The reference decodes one token at a
 time and has no counterpart.
 """
@@ -116,6 +118,11 @@ class TreeKVCache:
             new = commit_draft_rows(*cache, *[t[:, :, :n] for t in draft], path, accepted, context_lens=self.lens)
         self.lens = new
         self._mask = None
+
+    def check(self) -> None:
+        """Wait for the device and raise ``RuntimeError`` if a call since the last
+        check could not do its work (on this device, whoever made it)."""
+        ops.check_device(self.lens.device)
 
     # -- what Hugging Face's model asks of a cache ----------------------------
     def get_seq_length(self, layer_idx: int = 0) -> int:

@@ -47,3 +47,25 @@ def test_commit_without_a_step():
     with pytest.raises(ValueError, match="begin"):
         tree.commit(path, one)
     assert tree.lens.tolist() == [1, 1]
+
+
+def test_check_reports_a_path_that_does_not_fit():
+    from kvint4 import ops
+    from models.llama3.kv_cache import QuantizedKVCache
+    from models.llama3.tree_cache import TreeKVCache
+    ops.device_error()
+    tree = TreeKVCache(1, 2, 2, 64, capacity=64, max_nodes=8)
+    tree.lens.fill_(tree.capacity - 1)
+    _step(tree, 3, 2)
+    tree.check()
+    path = torch.tensor([[0, 1]] * 2, dtype=torch.int32, device="cuda")
+    tree.commit(path, torch.tensor([2, 1], dtype=torch.int32, device="cuda"))
+    with pytest.raises(RuntimeError, match="accepted count"):
+        tree.check()
+    tree.check()
+    assert tree.lens.tolist() == [tree.capacity - 1, tree.capacity]
+    plain = QuantizedKVCache()
+    plain.check()
+    x = torch.randn(1, 2, 5, 64, device="cuda").to(torch.bfloat16)
+    plain.append(x, x, 0)
+    plain.check()
