@@ -200,7 +200,7 @@ class Int4KVStore:
                 continue
             mass = self.mass(layer_idx)
             b, h, cap, _ = old.k_packed_buf.shape
-            new_cap = min(cap, _round_up(max(int(keep * self.growth), self.capacity_hint,
+            new_cap = min(cap, _round_up(max(keep, int(keep * self.growth), self.capacity_hint,
                                              CAPACITY_ALIGN), CAPACITY_ALIGN))
             bufs = [torch.empty(b, h, new_cap, t.shape[-1], dtype=t.dtype, device=t.device)
                     for t in (old.k_packed_buf, old.k_scales_buf, old.v_packed_buf, old.v_scales_buf)]
