@@ -293,9 +293,9 @@ class Int4KVStore:
         return total
 
     def capacity_nbytes(self) -> int:
-        """Bytes actually reserved on the device (including headroom)."""
+        """Bytes actually reserved on the device (including headroom and scores)."""
         total = 0
         for st in self._layers.values():
-            for t in (st.k_packed_buf, st.k_scales_buf, st.v_packed_buf, st.v_scales_buf):
-                total += t.element_size() * t.numel()
+            for t in (st.k_packed_buf, st.k_scales_buf, st.v_packed_buf, st.v_scales_buf, st.mass_buf):
+                total += t.element_size() * t.numel() if t is not None else 0
         return total

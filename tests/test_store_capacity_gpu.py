@@ -32,3 +32,10 @@ def test_eviction_has_room_for_what_it_keeps(growth):
     out = torch.empty_like(q[:, :, :1])
     store.append_attend(q[:, :, :1], k[:, :, :1], v[:, :, :1], 0, out, n_q_heads=4, n_kv_heads=2)
     assert store.layer(0).seq_len == 701
+
+
+def test_reserved_bytes_count_the_scores():
+    store, *_ = _store(1.5, 300, capacity=1024)
+    rows = 2 * 2 * 1024
+    assert store.capacity_nbytes() == rows * (2 * (32 + 2 * 2) + 4)
+    assert store.nbytes() == 2 * 2 * 300 * 2 * (32 + 2 * 2)  # packed rows and scales held
