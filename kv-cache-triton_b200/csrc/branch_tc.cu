@@ -235,6 +235,7 @@ __device__ __forceinline__ void dequant_role(const TcParams &P, Walk walk, const
     W.wait((is_v ? VEMPTY : KEMPTY) + st, use + 1u);  // passes at once for the first use of a stage
     if (r.draft && tid < 4) asm volatile("st.shared.u32 [%0], %1;" ::"r"(bad + 4 * tid), "r"(0u) : "memory");
     int shift = 0, vshift = 0;
+    __syncwarp();
     odd = tc::barrier_any(is_v ? 3 : 2, odd);
     if (odd) {
       // the four warps put their largest scales together (low half: their own)
