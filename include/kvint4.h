@@ -339,10 +339,10 @@ int kv4_prefill_attention(const kv4_tensor *q, const kv4_tensor *k_packed,
  * 16-bit queries and scales take tensor-core kernels whose operands are f16.  A
  * power of two common to some rows of a KV head brings bf16 scales of up to 2^100
  * into its range; scales down to 2^-27 of the largest of those rows keep all their
- * bits, smaller ones are off by up to 2^-35 of it.  V scales in f16 have to stay
- * below 65504/8.  A larger or non-finite scale in the context sets bit 8 of
- * kv4_device_error (output not valid).  One in a drafted row makes the nodes
- * that see the row NaN and no others, and sets the bit as well.
+ * bits, smaller ones are off by up to 2^-35 of it.  f16 scales are used as they
+ * are.  A larger or non-finite scale of V (of K too, where there is much work) in
+ * the context sets bit 8 of kv4_device_error (output not valid).  One in a drafted
+ * row makes the nodes that see the row NaN and no others, and sets the bit as well.
  */
 int64_t kv4_tree_workspace(const kv4_tensor *q, const kv4_tensor *k_packed,
                            const kv4_tensor *k_scales, const kv4_tensor *v_packed,

@@ -51,8 +51,8 @@ constexpr int NW = 4;             // warps per block
 constexpr int kClusterParts = 8;  // most blocks that join as a cluster
 constexpr float kShift = 7.0f;  // weights are written times 2^7 (see branch_tc.cu)
 
-// The power of two 2^e in a warp's V operands and output sums (bf16 scales; see
-// tc.cuh): it moves when a step's scales are not exact at the present one.
+// The power of two 2^e in a warp's V operands and output sums: it moves when a
+// step's scales are not exact at the present one (see tc.cuh; f16 scales: v_scales).
 struct VShift {
   int e = 0, least = tc::kMaxShift;  // least: smallest so far; sums move up by 2^48 at most, which they can
   float up = 1.0f;                   // 2^e
@@ -108,8 +108,7 @@ __device__ __forceinline__ float scale_at(const uint32_t *w, int i) {
 // whether a V scale can be an operand; one that cannot is reported
 template <typename ST>
 __device__ __forceinline__ bool usable(uint32_t s) {
-  if (kRest<ST>) return fabsf(scale_at<ST>(&s, 0)) <= tc::kMaxScale;
-  return tc::scale_usable(tc::scale_bits(s));
+  return kRest<ST> ? (s & 0x7FFFu) < 0x7C00u : tc::scale_usable(tc::scale_bits(s));
 }
 
 // V's scales of a step, keys in pairs, as f16; `rescale(f)` multiplies the sums so
@@ -117,21 +116,40 @@ __device__ __forceinline__ bool usable(uint32_t s) {
 template <typename ST, class F>
 __device__ __forceinline__ void v_scales(uint32_t (&sp)[2], const uint32_t (&vs)[4], VShift &V, bool draft,
                                          bool &big, F rescale) {
-  float f[4];
-#pragma unroll
-  for (int j = 0; j < 4; ++j) f[j] = scale_at<ST>(&vs[j], 0);
   if (kRest<ST>) {
+    // f16 scales are operands as they are; those from 2^13 on, whose products with
+    // codes f16 does not hold, times 2^-4, and then all others too
+    const uint32_t end = V.e == 0 ? 0x7000u : 0x7C00u;
+    bool over = false;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) over = over || (vs[j] & 0x7FFFu) >= end;
+    uint32_t keep[2] = {0xffffffffu, 0xffffffffu};
+    if (__any_sync(0xffffffffu, over)) {
+      bool large = false;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (usable<ST>(vs[j])) {
+          large = large || (vs[j] & 0x7FFFu) >= 0x7000u;
+        } else {
+          big = true;
+          if (draft) keep[j >> 1] &= j & 1 ? 0xffffu : 0xffff0000u;  // rows that see it are marked
+        }
+      }
+      if (V.e == 0 && __any_sync(0xffffffffu, large)) {
+        V.e = -4;
+        rescale(0.0625f);
+      }
+    }
 #pragma unroll
     for (int p = 0; p < 2; ++p) {
-      sp[p] = prmt(vs[2 * p], vs[2 * p + 1], 0x5410);
-      const bool b0 = !(fabsf(f[2 * p]) <= tc::kMaxScale), b1 = !(fabsf(f[2 * p + 1]) <= tc::kMaxScale);
-      if (b0 || b1) {
-        big = true;
-        if (draft) sp[p] &= (b0 ? 0u : 0xffffu) | (b1 ? 0u : 0xffff0000u);  // rows that see it are marked
-      }
+      sp[p] = prmt(vs[2 * p], vs[2 * p + 1], 0x5410) & keep[p];
+      if (V.e != 0) sp[p] = tc::hmul2(sp[p], 0x2C002C00u);
     }
     return;
   }
+  float f[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) f[j] = scale_at<ST>(&vs[j], 0);
 #pragma unroll
   for (int j = 0; j < 4; ++j) f[j] *= V.up;
   if (__any_sync(0xffffffffu, not_exact(f))) {

@@ -274,8 +274,5 @@ __device__ __forceinline__ bool barrier_any(int id, bool p) {
   return r != 0u;
 }
 
-// largest |f16 scale| whose products with -8 .. 7 stay finite in f16
-constexpr float kMaxScale = 65504.0f / 8.0f;
-
 }  // namespace tc
 }  // namespace kv4

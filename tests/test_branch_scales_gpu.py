@@ -196,3 +196,32 @@ def test_scored_scales(path, rows_scale):
 @pytest.mark.parametrize("pattern", ["random", "falling"])
 def test_scored_scales_apart(path, low, pattern):
     _scored(SCORED[path], q_scale=1.0, spread=(low, pattern), seed=7)
+
+
+# f16 scales from 8192 on, whose products with codes f16 does not hold: a cache of
+# f16 values holds scales of up to 65504 / 7
+@pytest.mark.parametrize("path", ["up to 8 rows", "warps", "any shape"])
+@pytest.mark.parametrize("where", ["first", "last", "draft", "all"])
+def test_large_f16_scales(path, where):
+    from kernels.llama3.tree_attention_quant import tree_attention_quant_gqa
+    from kvint4 import ops
+    b, hq, hkv, n, s, d, group = PATHS[path]
+    cache, draft = br.random_rows(b, hkv, s, d, group, F16, 1), br.random_rows(b, hkv, n, d, group, F16, 2)
+    for rows, part in (("first", cache[3][:, :, :40]), ("last", cache[3][:, :, -40:]), ("draft", draft[3])):
+        if where in (rows, "all"):
+            part.copy_(part.float() * (9350.0 / 0.45))  # 1039 .. 9350
+            cache[2][:, :, :40] |= 0x88  # codes 8 .. 15: no value past f16's largest
+            cache[2][:, :, -40:] |= 0x88
+            draft[2] |= 0x88
+    q = torch.randn(b, hq, n, d, generator=torch.Generator().manual_seed(3)).to(F16)
+    mask = br.tree_mask(b, n, 4)
+    ops.device_error()
+    got = tree_attention_quant_gqa(q.cuda(), *[t.cuda() for t in cache], *[t.cuda() for t in draft], mask.cuda(),
+                                   n_q_heads=hq, n_kv_heads=hkv, group_size=group)
+    assert ops.device_error() == 0
+    for x in range(b):
+        rows = [torch.cat((c[x], f[x]), 1) for c, f in zip(cache, draft)]
+        seen = torch.ones(n, s + n, dtype=torch.bool)
+        seen[:, s:] = mask[x]
+        _check(got[x], q[x], br.values(*rows[:2], group, d), br.values(*rows[2:], group, d), rows[1], rows[3],
+               seen, s + n)
