@@ -120,11 +120,10 @@ __device__ __forceinline__ void v_scales(uint32_t (&sp)[2], const uint32_t (&vs)
     // f16 scales are operands as they are; those from 2^13 on, whose products with
     // codes f16 does not hold, times 2^-4, and then all others too
     const uint32_t end = V.e == 0 ? 0x7000u : 0x7C00u;
-    bool over = false;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) over = over || (vs[j] & 0x7FFFu) >= end;
-    uint32_t keep[2] = {0xffffffffu, 0xffffffffu};
-    if (__any_sync(0xffffffffu, over)) {
+    sp[0] = prmt(vs[0], vs[1], 0x5410);
+    sp[1] = prmt(vs[2], vs[3], 0x5410);
+    const uint32_t most = __vmaxu2(sp[0] & 0x7FFF7FFFu, sp[1] & 0x7FFF7FFFu);
+    if (__any_sync(0xffffffffu, max(most & 0xFFFFu, most >> 16) >= end)) {
       bool large = false;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
@@ -132,7 +131,7 @@ __device__ __forceinline__ void v_scales(uint32_t (&sp)[2], const uint32_t (&vs)
           large = large || (vs[j] & 0x7FFFu) >= 0x7000u;
         } else {
           big = true;
-          if (draft) keep[j >> 1] &= j & 1 ? 0xffffu : 0xffff0000u;  // rows that see it are marked
+          if (draft) sp[j >> 1] &= j & 1 ? 0xffffu : 0xffff0000u;  // rows that see it are marked
         }
       }
       if (V.e == 0 && __any_sync(0xffffffffu, large)) {
@@ -140,10 +139,9 @@ __device__ __forceinline__ void v_scales(uint32_t (&sp)[2], const uint32_t (&vs)
         rescale(0.0625f);
       }
     }
-#pragma unroll
-    for (int p = 0; p < 2; ++p) {
-      sp[p] = prmt(vs[2 * p], vs[2 * p + 1], 0x5410) & keep[p];
-      if (V.e != 0) sp[p] = tc::hmul2(sp[p], 0x2C002C00u);
+    if (V.e != 0) {
+      sp[0] = tc::hmul2(sp[0], 0x2C002C00u);
+      sp[1] = tc::hmul2(sp[1], 0x2C002C00u);
     }
     return;
   }
@@ -244,9 +242,11 @@ __device__ __forceinline__ void lds_scales(uint32_t (&w)[(NG + 1) / 2], uint32_t
 }
 
 // A operand of 16 (or 8) rows of q, in the column order of the K words, and the
-// factor of rows g and g + 8 from sums to base-2 exponents.  Rows are scaled by a
-// power of two so that their largest element lies in [2^13, 2^14): exact down to
-// 2^-23 of it (bf16: 2^-26), and off by at most 2^-34 of it below that.
+// factor of rows g and g + 8 from sums to base-2 exponents.  bf16 rows are
+// scaled by a power of two so that their largest element lies in
+// [2^13, 2^14): exact down to 2^-26 of it, and off by at most 2^-34 of it below
+// that.  f16 rows are exact below 2^11; with larger elements, down to 2^-10, and off
+// by at most 2^-21 below that.
 template <int D, bool HALF>
 struct Query {
   uint32_t a[D / 16][HALF ? 2 : 4];
@@ -256,14 +256,19 @@ template <int D, bool HALF>
 __device__ __forceinline__ void load_query(Query<D, HALF> &Q, const TreeParams &T, int64_t b, int kvh,
                                            int row0, int rows, int lane) {
   const int g = lane >> 2, t = lane & 3;
+  constexpr int NR = HALF ? 1 : 2;
+  uint4 rows_w[NR][D / 32];  // both rows are on their way before the first is looked at
 #pragma unroll
-  for (int r = 0; r < (HALF ? 1 : 2); ++r) {
+  for (int r = 0; r < NR; ++r) {
     const int row = row0 + g + 8 * r, node = row / T.R, head = kvh * T.R + row - node * T.R;
     const uint16_t *q = static_cast<const uint16_t *>(T.q) + b * T.qs[0] + head * T.qs[1] + node * T.qs[2] + 8 * t;
-    uint4 w[D / 32];
 #pragma unroll
     for (int i = 0; i < D / 32; ++i)
-      w[i] = row < rows ? __ldg(reinterpret_cast<const uint4 *>(q + 32 * i)) : make_uint4(0, 0, 0, 0);
+      rows_w[r][i] = row < rows ? __ldg(reinterpret_cast<const uint4 *>(q + 32 * i)) : make_uint4(0, 0, 0, 0);
+  }
+#pragma unroll
+  for (int r = 0; r < NR; ++r) {
+    const uint4(&w)[D / 32] = rows_w[r];
     Q.c[r] = T.scale_log2;
     const bool bf = T.q_dtype == KV4_BF16;
     uint32_t top = 0;  // largest |q| as bits: magnitudes of either type order like integers
@@ -271,28 +276,41 @@ __device__ __forceinline__ void load_query(Query<D, HALF> &Q, const TreeParams &
     for (int i = 0; i < D / 32; ++i) {
       const uint32_t u[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
 #pragma unroll
-      for (int e = 0; e < 4; ++e) top = max(top, max(u[e] & 0x7FFFu, (u[e] >> 16) & 0x7FFFu));
+      for (int e = 0; e < 4; ++e) top = __vmaxu2(top, u[e] & 0x7FFF7FFFu);
     }
-    top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-    top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-    int ex = 13 - (static_cast<int>(__float_as_uint(bf ? bf16lo_to_f32(top) : f16lo_to_f32(top)) >> 23) - 127);
-    ex = top == 0 ? 0 : min(max(ex, -126), 126);
-    const float up = tc::pow2(ex);
-    Q.c[r] *= tc::pow2(-ex);
+    top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, 2));
+    top = max(top & 0xFFFFu, top >> 16);
+    // pairs 1 and 3 meet codes times 16 (see code_pair)
+    float up = 1.0f;
+    uint32_t even = 0x3C003C00u, odd = 0x2C002C00u;  // 1, 1/16
+    if (bf) {
+      int ex = 13 - (static_cast<int>(top >> 7) - 127);
+      ex = top == 0 ? 0 : min(max(ex, -126), 126);
+      up = tc::pow2(ex);
+      Q.c[r] *= tc::pow2(-ex);
+    } else if (top < 0x6800u) {  // below 2^11: pairs 0 and 2 times 16 instead
+      even = 0x4C004C00u;
+      odd = 0x3C003C00u;
+      Q.c[r] *= 0.0625f;
+    }
 #pragma unroll
     for (int i = 0; i < D / 32; ++i) {
       const uint32_t u[4] = {w[i].x, w[i].y, w[i].z, w[i].w};  // columns 8t .. 8t + 7 of the block
-      float lo[4], hi[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        lo[e] = (bf ? bf16lo_to_f32(u[e]) : f16lo_to_f32(u[e])) * up;
-        hi[e] = (bf ? bf16hi_to_f32(u[e]) : f16hi_to_f32(u[e])) * up;
+      uint32_t p[4];                                          // pairs (0,4) (1,5) (2,6) (3,7)
+      if (bf) {
+        p[0] = pack_f16x2(bf16lo_to_f32(u[0]) * up, bf16lo_to_f32(u[2]) * up);
+        p[1] = pack_f16x2(bf16hi_to_f32(u[0]) * up, bf16hi_to_f32(u[2]) * up);
+        p[2] = pack_f16x2(bf16lo_to_f32(u[1]) * up, bf16lo_to_f32(u[3]) * up);
+        p[3] = pack_f16x2(bf16hi_to_f32(u[1]) * up, bf16hi_to_f32(u[3]) * up);
+      } else {
+        p[0] = tc::hmul2(prmt(u[0], u[2], 0x5410), even);
+        p[1] = prmt(u[0], u[2], 0x7632);
+        p[2] = tc::hmul2(prmt(u[1], u[3], 0x5410), even);
+        p[3] = prmt(u[1], u[3], 0x7632);
       }
-      uint32_t p[4] = {pack_f16x2(lo[0], lo[2]), pack_f16x2(hi[0], hi[2]),  // pairs (0,4) (1,5) (2,6) (3,7)
-                       pack_f16x2(lo[1], lo[3]), pack_f16x2(hi[1], hi[3])};
-      // pairs 1 and 3 meet codes times 16 (see code_pair)
-      p[1] = tc::hmul2(p[1], 0x2C002C00u);
-      p[3] = tc::hmul2(p[3], 0x2C002C00u);
+      p[1] = tc::hmul2(p[1], odd);
+      p[3] = tc::hmul2(p[3], odd);
       // k-step 2i: pairs 0 and 1; k-step 2i + 1: pairs 2 and 3
       if (HALF) {
         Q.a[2 * i][0] = p[0];
