@@ -27,7 +27,7 @@
 // Bound: instructions, about 450 per warp and 16 keys of 128 columns, a third of
 // which take codes apart; memory next.  Measured, 8 KV heads of 128 columns: single
 // tokens of 4 rows, 16 sequences x 4096, 29.5 us (84 MB: 2.8 TB/s, a step in 60 % of
-// the issue slots); 8 nodes x 512 8.9 us with the join, most of it loads that wait
+// the issue slots); 8 nodes x 512 9.1 us with the join, most of it loads that wait
 // for one another; 32 rows x 4096, batch 4, 23 us.
 #include <algorithm>
 

@@ -32,10 +32,10 @@
 // Weights enter the second product rounded to f16, times 2^7 (at most 2^15);
 // their sum is taken before that rounding, in fp32.
 //
-// Bound: the chain scores -> maximum -> weights -> products of a stream, 4900 cycles
+// Bound: the chain scores -> maximum -> weights -> products of a stream, 5000 cycles
 // a tile with both streams at it, where products and exponentials need 2048 each.
-// Measured: 64 nodes x 16K x 64 heads over 8, batch 4, 146 us (770 TFLOP/s); 63 nodes
-// x 4K x 32 heads, batch 8, 52.5 us, of which about 5 pass before the first product.
+// Measured: 64 nodes x 16K x 64 heads over 8, batch 4, 149 us (755 TFLOP/s); 63 nodes
+// x 4K x 32 heads, batch 8, 54 us, of which about 5 pass before the first product.
 #include <algorithm>
 
 #include "branch.cuh"
@@ -838,7 +838,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_tc(const __grid_constant__ Tc
       __shfl_sync(0xffffffffu, *reinterpret_cast<volatile uint32_t *>(smem_raw + SM::MISC), 0);
   const Walk walk{static_cast<uint32_t>(start[0]), start[1], start[2], start[3], start[4], true};
   // 128 * (2 * 96 + 2 * 104 + 80) = 640 * 96 registers.  Measured at 64 nodes x 16K
-  // x 64 heads, batch 4: 146 us, 148 with 104 / 88 / 96; sixteen dequantizing or
+  // x 64 heads, batch 4, when it took 146 us: 148 with 104 / 88 / 96; sixteen dequantizing or
   // sixteen softmax warps (896 threads, two to a row there) spill: 160 and 154.
   if (warp < 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");

@@ -13,7 +13,7 @@
 // weights of every other tile (one such group alone took 4500 cycles a tile,
 // twice what the rest needs), 8-11 dequantize key tiles (loaded two tiles ahead
 // into registers) into two buffers.  All (unit, tile) pairs are cut evenly over
-// the CTAs.  Measured, 256 rows x 16384 keys x 8 heads, batch 2: 46.7 us, where the
+// the CTAs.  Measured, 256 rows x 16384 keys x 8 heads, batch 2: 47.3 us, where the
 // exponentials take 15.7 (16 a cycle and SM) and the products 5; what is left is
 // waiting between the three roles, and a pass of its own for the second 128 rows.
 #include <algorithm>
