@@ -242,9 +242,9 @@ __device__ __forceinline__ uint32_t scales_top(const uint16_t (&x)[N]) {
   }
   return __reduce_max_sync(0xffffffffu, top) | (__all_sync(0xffffffffu, exact) ? 0u : 0x8000u);
 }
-// 2^e, e held within the normal numbers
+// 2^e for e <= 127; 0 below the normal numbers
 __device__ __forceinline__ float pow2(int e) {
-  return __uint_as_float(static_cast<uint32_t>(min(max(e, -126), 127) + 127) << 23);
+  return __uint_as_float(static_cast<uint32_t>(max(e + 127, 0)) << 23);
 }
 // e for the largest usable scale (as bits)
 __device__ __forceinline__ int scale_shift(uint32_t top) {

@@ -225,3 +225,20 @@ def test_large_f16_scales(path, where):
         seen[:, s:] = mask[x]
         _check(got[x], q[x], br.values(*rows[:2], group, d), br.values(*rows[2:], group, d), rows[1], rows[3],
                seen, s + n)
+
+
+@pytest.mark.parametrize("path", [p for p in PATHS if p != "any shape"])
+def test_a_hidden_row_out_of_all_proportion(path):
+    """A drafted row 2^180 larger than the rest takes the bits of the rows beside it, and
+    nothing else: what does not see it stays as small as it was."""
+    from kernels.llama3.tree_attention_quant import tree_attention_quant_gqa
+    b, hq, hkv, n, s, d, group = PATHS[path]
+    cache = [t.cuda() for t in br.random_rows(b, hkv, s, d, group, BF16, 1, 1e-25)]
+    draft = [t.cuda() for t in br.random_rows(b, hkv, n, d, group, BF16, 2, 1e-25)]
+    draft[3][:, :, 1] = 2.0 ** 99
+    q = torch.randn(b, hq, n, d, generator=torch.Generator().manual_seed(3)).to(BF16).cuda()
+    mask = torch.eye(n, dtype=torch.bool, device="cuda")
+    got = tree_attention_quant_gqa(q, *cache, *draft, mask, n_q_heads=hq, n_kv_heads=hkv, group_size=group)
+    others = [i for i in range(n) if i != 1]
+    assert float(got[:, :, others].float().abs().max()) <= 8 * 0.45e-25
+    assert float(got[:, :, 1].float().abs().max()) > 1e20
