@@ -46,8 +46,9 @@ class LayerStore:
     # [B, n_kv, capacity] f32: attention weight each token received so far
     # (``track_mass`` stores only)
     mass_buf: torch.Tensor | None = None
-    # the first ``scored`` tokens were there when an attention last scored the layer
-    scored: int = 0
+    # first of the tokens that came by a path that scores nothing (``note_unscored``)
+    # and that no attention has scored since
+    unscored: int | None = None
 
     @property
     def capacity(self) -> int:
@@ -163,8 +164,14 @@ class Int4KVStore:
             raise ValueError("the store does not track scores (track_mass=True)")
         ops.scored_attention_into(query, layer.views(), self.mass(layer_idx), self.mass(layer_idx),
                                   out, self.group_size, is_causal, self.mass_decay)
-        layer.scored = layer.seq_len
+        layer.unscored = None
         return out
+
+    def note_unscored(self, layer_idx: int, tokens: int) -> None:
+        """The layer's last ``tokens`` tokens came by a path that scores nothing."""
+        layer = self.layer(layer_idx)
+        if layer.mass_buf is not None and tokens > 0 and layer.unscored is None:
+            layer.unscored = layer.seq_len - tokens
 
     def score_window(self, query: torch.Tensor, layer_idx: int) -> None:
         """Score the layer's tokens by the last ``mass_window`` queries of
@@ -185,15 +192,14 @@ class Int4KVStore:
         ``sinks``, the last ``recent`` and the highest scored of the rest, per KV
         head, in token order; returns the kept token numbers
         ``{layer: int32 [B, n_kv, keep]}`` of the layers that were cut.  Refused,
-        with nothing cut, while tokens that no attention has scored since they were
-        appended would be ranked: a prompt under a mask, for instance, which the
-        scoring kernels do not take."""
+        with nothing cut, while tokens would be ranked that came by a path that scores
+        nothing (attention under a mask) and that no attention has scored since."""
         if not 0 <= recent + sinks <= keep or recent < 0 or sinks < 0:
             raise ValueError("keep must be at least recent + sinks, all >= 0")
         kept = {}
         for layer_idx, old in self._layers.items():
-            if old.seq_len > keep and self.mass(layer_idx).shape[2] > old.scored + recent:
-                raise ValueError(f"layer {layer_idx}: the last {old.seq_len - old.scored} tokens have no scores "
+            if old.seq_len > keep and old.unscored is not None and old.seq_len - old.unscored > recent:
+                raise ValueError(f"layer {layer_idx}: the last {old.seq_len - old.unscored} tokens have no scores "
                                  f"(score_window() them, or keep them as recent)")
         for layer_idx, old in self._layers.items():
             if old.seq_len <= keep:
@@ -205,7 +211,7 @@ class Int4KVStore:
             bufs = [torch.empty(b, h, new_cap, t.shape[-1], dtype=t.dtype, device=t.device)
                     for t in (old.k_packed_buf, old.k_scales_buf, old.v_packed_buf, old.v_scales_buf)]
             new = LayerStore(*bufs, seq_len=keep, mass_buf=torch.zeros(b, h, new_cap, device=mass.device),
-                             scored=keep)
+                             unscored=None if old.unscored is None else keep - (old.seq_len - old.unscored))
             index = torch.empty(b, h, keep, dtype=torch.int32, device=mass.device)
             ops.evict_into(mass, old.views(), new.views(), new.mass_buf[:, :, :keep], index,
                            recent, sinks)
@@ -246,7 +252,7 @@ class Int4KVStore:
                     dst[:, :, :n].copy_(src[:, :, :n])
                 if grown.mass_buf is not None:
                     grown.mass_buf[:, :, :n].copy_(layer.mass_buf[:, :, :n])
-                grown.seq_len, grown.scored = n, layer.scored
+                grown.seq_len, grown.unscored = n, layer.unscored
                 layer = grown
                 self._layers[layer_idx] = layer
         return layer
@@ -257,7 +263,8 @@ class Int4KVStore:
         for st in self._layers.values():
             n = max_length if max_length >= 0 else st.seq_len + max_length
             st.seq_len = max(0, min(st.seq_len, n))
-            st.scored = min(st.scored, st.seq_len)
+            if st.unscored is not None and st.unscored >= st.seq_len:
+                st.unscored = None
 
     def reorder(self, beam_idx: torch.Tensor) -> None:
         """Reorder the batch dimension of every layer (beam search)."""

@@ -120,8 +120,8 @@ class QuantizedKVCache:
     def evict(self, keep: int, *, recent: int = 0, sinks: int = 0) -> dict[int, torch.Tensor]:
         """Cut every layer to ``keep`` tokens per KV head: the first ``sinks``, the
         last ``recent`` and the highest scored of the rest; returns the kept token
-        numbers per layer.  Tokens without scores are not ranked: ``ValueError``
-        unless ``recent`` covers them.  ``get_seq_length`` is then the number of tokens held,
+        numbers per layer.  Tokens that came under a mask (or through ``update``)
+        have no scores and are not ranked: ``ValueError`` unless ``recent`` covers them.  ``get_seq_length`` is then the number of tokens held,
         no longer the number seen: pass ``position_ids`` to the model yourself
         (keys keep the rotary positions they were cached with)."""
         return self._store.evict(int(keep), recent=int(recent), sinks=int(sinks))
@@ -146,6 +146,7 @@ class QuantizedKVCache:
         """
         del cache_kwargs
         self._store.append(key_states, value_states, layer_idx)
+        self._store.note_unscored(layer_idx, key_states.shape[2])
         return self.get_dequantized(layer_idx, out_dtype=key_states.dtype)
 
     def get_quantized(

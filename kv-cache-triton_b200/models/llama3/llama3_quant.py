@@ -40,8 +40,7 @@ class _DequantizedCacheView:
         self.cache = cache
 
     def update(self, key_states, value_states, layer_idx, cache_kwargs=None):
-        self.cache.append(key_states, value_states, layer_idx)
-        return self.cache.get_dequantized(layer_idx, out_dtype=key_states.dtype)
+        return self.cache.update(key_states, value_states, layer_idx)
 
 
 class LlamaAttentionQuantized(LlamaAttention):

@@ -6,6 +6,8 @@ from __future__ import annotations
 import pytest
 import torch
 
+import branch_ref as br
+
 pytestmark = pytest.mark.gpu
 
 
@@ -40,30 +42,46 @@ def test_append_attend_scores_by_the_window(chunks, causal):
 
 
 def test_tokens_without_scores_are_not_ranked():
-    from kvint4.cache import Int4KVStore
-    store = Int4KVStore(32, track_mass=True, mass_window=16)
+    from models.llama3.kv_cache import QuantizedKVCache
+    cache = QuantizedKVCache(track_mass=True, mass_window=16)
     q, k, v = _data(200, 1)
-    for layer in (0, 1):
-        store.append(k[:, :, :150], v[:, :, :150], layer)
-    store.score_window(q[:, :, :150], 0)
-    before = [t.clone() for layer in (0, 1) for t in store.layer(layer).views()]
+    for layer in (0, 1):  # update: what a module that knows nothing of the scores calls
+        cache.update(k[:, :, :150], v[:, :, :150], layer)
+    cache.score_window(q[:, :, :150], 0)
+    before = [t.clone() for layer in (0, 1) for t in cache.get_quantized(layer)]
     with pytest.raises(ValueError, match="layer 1.*150 tokens"):
-        store.evict(60, recent=8)
-    for x, y in zip(before, [t for layer in (0, 1) for t in store.layer(layer).views()]):
+        cache.evict(60, recent=8)
+    for x, y in zip(before, [t for layer in (0, 1) for t in cache.get_quantized(layer)]):
         assert torch.equal(x, y)  # layer 0 neither
-    store.score_window(q[:, :, :150], 1)
+    cache.score_window(q[:, :, :150], 1)
     for layer in (0, 1):
-        store.append(k[:, :, 150:], v[:, :, 150:], layer)
+        cache.update(k[:, :, 150:], v[:, :, 150:], layer)
     with pytest.raises(ValueError, match="50 tokens"):
-        store.evict(60, recent=49)
-    assert store.evict(200) == {}
-    store.crop(180)
-    assert set(store.evict(60, recent=30)) == {0, 1}  # the tokens without scores are the recent ones
+        cache.evict(60, recent=49)
+    assert cache.evict(200) == {}
+    cache.crop(180)
+    assert set(cache.evict(60, recent=30)) == {0, 1}  # the tokens without scores are the recent ones
     with pytest.raises(ValueError, match="30 tokens"):
-        store.append(k[:, :, :30], v[:, :, :30], 0)
-        store.evict(40, recent=20)
-    store.crop(60)
-    assert set(store.evict(40)) == {0, 1}
+        cache.evict(40, recent=20)                    # and still have none
+    cache.append(k[:, :, :100], v[:, :, :100], 0)     # (grows the buffers)
+    with pytest.raises(ValueError, match="130 tokens"):
+        cache.evict(70, recent=20)
+    cache.crop(30)
+    assert set(cache.evict(20)) == {0, 1}
+
+
+def test_scores_kept_by_hand():
+    """Rows appended and scored by the user's own calls are ranked by what stands there."""
+    from kernels.llama3.evict import attention_forward_quant_gqa_scored
+    from models.llama3.kv_cache import QuantizedKVCache
+    cache = QuantizedKVCache(track_mass=True)
+    q, k, v = _data(150, 1)
+    cache.append(k, v, 0)
+    attention_forward_quant_gqa_scored(q[:, :, -8:], *cache.get_quantized(0), cache.mass(0), n_q_heads=8,
+                                       n_kv_heads=2, is_causal=True)
+    mass = cache.mass(0).cpu()
+    kept = cache.evict(40, recent=4)[0].cpu().long()
+    assert torch.equal(kept, br.evict_index(mass, 40, 4, 0))
 
 
 def test_a_masked_prompt_is_not_cut_blindly():
