@@ -95,7 +95,7 @@ void written(const at::Tensor &t) {
 struct Overlap {
   struct Step { int64_t by, low, high, least, most; };
   Step s[8];
-  int n = 0, left = 4096;  // places looked at: more only for strides that nest in no way
+  int n = 0, left = 20000;  // places looked at; strides that nest in no way may need more, and pass
   int64_t a_size, b_size;
 
   void add(const at::Tensor &t, int64_t sign) {
@@ -109,7 +109,7 @@ struct Overlap {
     }
   }
   bool reach(int i, int64_t at) {
-    if (--left < 0) return true;
+    if (--left < 0) return false;
     if (i == n) return -a_size < at && at < b_size;
     const Step &k = s[i];
     const int64_t by = k.by, to = k.most - at, from = at - k.least;
