@@ -102,13 +102,14 @@ __global__ void __launch_bounds__(KTHREADS, 4)
   const int64_t ctx = (T.S + 15) & ~int64_t(15);
   const float *in = P.in + b * P.is[0] + kvh * P.is[1];
   float *out = P.out + b * P.os[0] + kvh * P.os[1];
-  float sum[PER];
+  float old[PER], sum[PER];  // the weights are summed before they meet the score, and its rounding
   bool on[PER];
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
     const int64_t slot = slot0 + i * KTHREADS, t = slot < ctx ? slot : T.S + slot - ctx;
     on[i] = slot < ctx ? slot < T.S : t < P.keys;
-    sum[i] = on[i] ? in[t * P.is[2]] * P.decay : 0.0f;  // was there before the attention began
+    old[i] = on[i] ? in[t * P.is[2]] : 0.0f;  // was there before the attention began
+    sum[i] = 0.0f;
   }
   griddep_wait();
   // The first rows' scores are on their way while maxima and sums are joined: 3.7 us
@@ -173,7 +174,7 @@ __global__ void __launch_bounds__(KTHREADS, 4)
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
     const int64_t slot = slot0 + i * KTHREADS, t = slot < ctx ? slot : T.S + slot - ctx;
-    if (on[i]) out[t * P.os[2]] = sum[i];
+    if (on[i]) out[t * P.os[2]] = fmaf(old[i], P.decay, sum[i]);
   }
 }
 
