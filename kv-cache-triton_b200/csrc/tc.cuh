@@ -206,9 +206,9 @@ __device__ __forceinline__ void dequant_word(uint32_t w, uint32_t scale, uint32_
 // A scale of 8 significant bits times a code is exact in f16 while the scale lies
 // in [2^-17, 2^12): f16 steps by 2^-24 at its lower end, and 8 * 2^12 is below its
 // upper.  Scales elsewhere are first multiplied by a power of two 2^e, the same
-// for all scales of a key tile (or of a warp's step), and whatever was
-// multiplied with them by 2^-e in fp32: with the largest brought to [2^10, 2^11),
-// all down to 2^-27 of it are exact.  e = 0 while all lie in that range as they are.
+// for all scales of a key tile (or of a warp's step), and the fp32 sums that they
+// go into by 2^-e: with the largest brought to [2^10, 2^11), all down to 2^-27 of
+// it are exact.  e = 0 while all lie in that range as they are.
 constexpr uint32_t kExactLo = 110u << 7, kExactSpan = 29u << 7;  // bits of 2^-17; of 2^-17 .. 2^12
 constexpr uint32_t kUsableEnd = 227u << 7;                       // 2^100: a larger scale is reported, not used
 constexpr int kMaxShift = 96;

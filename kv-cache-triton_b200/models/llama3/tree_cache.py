@@ -54,6 +54,7 @@ class TreeKVCache:
         # true position of a sequence's next token minus its tokens in the cache
         self.offset = torch.zeros(batch, dtype=torch.int32, device=device)
         self._mask: torch.Tensor | None = None
+        self._nodes = self._draft  # the draft rows of the current tree's nodes (views)
 
     @classmethod
     def from_cache(cls, cache, *, extra: int, max_nodes: int, tokens_seen: int | None = None):
@@ -87,6 +88,8 @@ class TreeKVCache:
             raise ValueError("mask must be bool [N, N] or [B, N, N]")
         if n > self.max_nodes:
             raise ValueError(f"{n} nodes, but the cache was made for {self.max_nodes}")
+        if n != self._nodes[0][0].shape[2]:
+            self._nodes = [[t[:, :, :n] for t in rows] for rows in self._draft]
         self._mask = mask
 
     def positions(self, depth: torch.Tensor) -> torch.Tensor:
@@ -102,7 +105,7 @@ class TreeKVCache:
         n = self._mask.shape[-1]
         if q.shape[2] != n or k.shape[2] != n:
             raise ValueError(f"{q.shape[2]} tokens for a tree of {n} nodes")
-        draft = [t[:, :, :n] for t in self._draft[layer]]
+        draft = self._nodes[layer]
         ops.append_kv(k, v, *draft, 0, self.group_size, self.tie_mode)
         return tree_attention_quant_gqa(q, *self._cache[layer], *draft, self._mask,
                                         n_q_heads=q.shape[1], n_kv_heads=k.shape[1],
@@ -113,9 +116,9 @@ class TreeKVCache:
         ``accepted[b]`` of each row) of the step's tree behind each sequence's context."""
         if self._mask is None:
             raise ValueError("begin() a step first")
-        n, new = self._mask.shape[-1], None
-        for cache, draft in zip(self._cache, self._draft):
-            new = commit_draft_rows(*cache, *[t[:, :, :n] for t in draft], path, accepted, context_lens=self.lens)
+        new = None
+        for cache, draft in zip(self._cache, self._nodes):
+            new = commit_draft_rows(*cache, *draft, path, accepted, context_lens=self.lens)
         self.lens = new
         self._mask = None
 
